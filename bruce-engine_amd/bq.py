@@ -28,6 +28,7 @@ LIB_PATH = os.path.join(HERE, "libbq.so")
 
 BQ_OK, BQ_UNSUPPORTED, BQ_EINVAL, BQ_ETOOBIG = 0, 1, 2, 3
 TYPE_Q5_K, TYPE_Q6_K = 13, 14
+TYPE_F32, TYPE_Q8_0, TYPE_BF16 = 0, 8, 30
 Q5K_BYTES, Q6K_BYTES = 176, 210
 Q8S_BYTES = 272  # Q8_0 logits head: 8 fp16 scales + 256 int8 per (row, 256 values)
 
@@ -43,7 +44,8 @@ EXPORTS = [
     "bq_gemv_norm_fused", "bq_gate_up_silu", "bq_gemm_workspace_bytes", "bq_gemm_workspace_bytes_cus",
     "bq_gemm_b_fused_noalloc",
     "bq_noalloc_scratch_bytes", "bq_decode_enqueue", "bq_decode_graph_create", "bq_decode_graph_launch",
-    "bq_decode_graph_destroy",
+    "bq_decode_graph_destroy", "bq_kv_page_bytes", "bq_append", "bq_kv_read", "bq_attn_workspace_bytes",
+    "bq_attn_decode", "bq_attn_prefill", "bq_attn_hook", "bq_sample_workspace_bytes", "bq_sample",
 ]
 
 
@@ -93,6 +95,43 @@ class DecodeStep(ctypes.Structure):
                 ("vocab", ctypes.c_int), ("logits", ctypes.c_void_p), ("rows", ctypes.c_int),
                 ("x_alt", ctypes.c_void_p), ("xdh", ctypes.c_void_p), ("work", ctypes.c_void_p),
                 ("work_bytes", ctypes.c_size_t)]
+
+
+class KvCacheStruct(ctypes.Structure):
+    """bq_kv_cache (include/bq.h): the paged key-value cache."""
+    _fields_ = [("pages", ctypes.c_void_p), ("table", ctypes.c_void_p), ("type", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("page_tokens", ctypes.c_int),
+                ("n_pages", ctypes.c_int), ("n_seq", ctypes.c_int), ("max_pages", ctypes.c_int)]
+
+
+class AppendArgs(ctypes.Structure):
+    """bq_append_args (include/bq.h)."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("ldq", ctypes.c_int64), ("ldk", ctypes.c_int64), ("ldv", ctypes.c_int64),
+                ("rows", ctypes.c_int), ("q_heads", ctypes.c_int), ("pos", ctypes.c_void_p), ("seq", ctypes.c_void_p),
+                ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("eps", ctypes.c_float),
+                ("rope", ctypes.c_void_p), ("rot", ctypes.c_int), ("n_pos", ctypes.c_int),
+                ("interleaved", ctypes.c_int), ("q_out", ctypes.c_void_p), ("q_type", ctypes.c_int)]
+
+
+class AttnArgs(ctypes.Structure):
+    """bq_attn_args (include/bq.h)."""
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_type", ctypes.c_int), ("out_type", ctypes.c_int),
+                ("ldq", ctypes.c_int64), ("ldo", ctypes.c_int64), ("q_heads", ctypes.c_int), ("n_rows", ctypes.c_int),
+                ("rows", ctypes.c_int), ("row0", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("max_len", ctypes.c_int), ("scale", ctypes.c_float), ("window", ctypes.c_int), ("sinks", ctypes.c_int),
+                ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_size_t)]
+
+
+class AttnBlock(ctypes.Structure):
+    """bq_attn_block (include/bq.h): what the attention hook runs for one block of the step."""
+    _fields_ = [("kv", ctypes.POINTER(KvCacheStruct)), ("append", ctypes.POINTER(AppendArgs)),
+                ("attn", ctypes.POINTER(AttnArgs)), ("prefill", ctypes.c_int)]
+
+
+class AttnPlanStruct(ctypes.Structure):
+    """bq_attn_plan (include/bq.h)."""
+    _fields_ = [("n_blocks", ctypes.c_int), ("blocks", ctypes.POINTER(AttnBlock)), ("status", ctypes.c_int)]
 
 
 _lib = None
@@ -161,6 +200,15 @@ def load(path=LIB_PATH):
         "bq_gguf_kv_str": (I, [P, ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p)]),
         "bq_gguf_read": (I, [P, ctypes.c_int64, P, S, ctypes.c_uint64]),
         "bq_gguf_load": (I, [P, ctypes.c_int64, P, P, P, WP, P]),
+        "bq_kv_page_bytes": (S, [I, I, I, I]),
+        "bq_append": (I, [P, P, P]),
+        "bq_kv_read": (I, [P, P, P, I, P, P, P]),
+        "bq_attn_workspace_bytes": (S, [I, I, I, I, I, I]),
+        "bq_attn_decode": (I, [P, P, P]),
+        "bq_attn_prefill": (I, [P, P, P]),
+        "bq_attn_hook": (None, [P, I, P]),
+        "bq_sample_workspace_bytes": (S, [I, I]),
+        "bq_sample": (I, [P, ctypes.c_int64, I, I, P, P, P, P, P, P, P, S, P]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -552,3 +600,207 @@ class DecodeGraph:
             self.close()
         except Exception:
             pass
+
+
+# ---------------------------------------------------------------- serving operators
+def _type_of(t, what):
+    import torch
+    if t.dtype == torch.float32:
+        return TYPE_F32
+    if t.dtype == torch.bfloat16:
+        return TYPE_BF16
+    raise TypeError(f"{what}: fp32 or bf16, not {t.dtype}")
+
+
+def _expect(t, dtype, shape, what):
+    """A contiguous device tensor of this dtype and shape (or None)."""
+    if t is None:
+        return None
+    if not t.is_cuda or t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous device tensor {dtype} {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _rows_ld(t, width, what):
+    """Row stride of a [rows, width] device tensor whose rows are contiguous."""
+    if not t.is_cuda or t.dim() != 2 or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: device rows of {width} contiguous values, not {tuple(t.shape)}")
+    return t.stride(0) if t.shape[0] > 1 else max(width, t.stride(0))
+
+
+KV_TYPES = {"bf16": TYPE_BF16, "q8": TYPE_Q8_0}
+
+
+def kv_page_bytes(kv_type, kv_heads, head_dim, page_tokens):
+    n = int(load().bq_kv_page_bytes(KV_TYPES[kv_type], kv_heads, head_dim, page_tokens))
+    if n == 0:
+        raise BqError(BQ_UNSUPPORTED, "bq_kv_page_bytes")
+    return n
+
+
+def rope_table(n_pos, rot, base=10000.0, device="cuda"):
+    """fp32 [n_pos, rot]: cosines, then sines, of pos * base^(-2 i / rot), formed in 64 bits."""
+    import torch
+    i = torch.arange(rot // 2, dtype=torch.float64, device=device)
+    a = torch.arange(n_pos, dtype=torch.float64, device=device)[:, None] * base ** (-2.0 * i / rot)
+    return torch.cat([a.cos(), a.sin()], 1).float().contiguous()
+
+
+class KvCache:
+    """The paged key-value cache: pages uint8 [n_pages, kv_page_bytes], table int32 [n_seq, max_pages]."""
+
+    def __init__(self, pages, table, kv_type, kv_heads, head_dim, page_tokens):
+        import torch
+        n = kv_page_bytes(kv_type, kv_heads, head_dim, page_tokens)
+        _expect(pages, torch.uint8, (pages.shape[0], n), "pages")
+        _expect(table, torch.int32, (table.shape[0], table.shape[1]), "table")
+        self.pages, self.table, self.kv_heads, self.head_dim = pages, table, kv_heads, head_dim
+        self.struct = KvCacheStruct(_ptr(pages), _ptr(table), KV_TYPES[kv_type], kv_heads, head_dim, page_tokens,
+                                    pages.shape[0], table.shape[0], table.shape[1])
+        self.ref = ctypes.byref(self.struct)
+        self._read = load().bq_kv_read
+
+    @classmethod
+    def empty(cls, n_pages, table, kv_type, kv_heads, head_dim, page_tokens, device="cuda"):
+        """With pages of its own."""
+        import torch
+        n = kv_page_bytes(kv_type, kv_heads, head_dim, page_tokens)
+        return cls(torch.zeros((n_pages, n), dtype=torch.uint8, device=device), table, kv_type, kv_heads, head_dim,
+                   page_tokens)
+
+    def read(self, pos, k=None, v=None, seq=None):
+        """K and / or V of tokens pos (int32 [rows]) of sequences seq into bf16 [rows, kv_heads * head_dim]."""
+        import torch
+        rows = pos.shape[0]
+        for t, what in ((pos, "pos"), (seq, "seq")):
+            _expect(t, torch.int32, (rows,), what)
+        for t, what in ((k, "k"), (v, "v")):
+            _expect(t, torch.bfloat16, (rows, self.kv_heads * self.head_dim), what)
+        return _check(self._read(self.ref, _ptr(seq), _ptr(pos), rows, _ptr(k), _ptr(v), _stream()), "bq_kv_read")
+
+
+class Append:
+    """bq_append over fixed buffers: q [rows, q_heads * D], k and v [rows, kv_heads * D] fp32 (rows may be
+    strided), pos and seq int32 [rows], q_out fp32 or bf16 [rows, q_heads * D]; rope fp32 [n_pos, rot] as from
+    rope_table (None: no rotation, positions below n_pos)."""
+
+    def __init__(self, kv, q, k, v, pos, q_out, seq=None, q_weight=None, k_weight=None, eps=1e-6, rope=None,
+                 n_pos=None, interleaved=False):
+        import torch
+        rows, D = pos.shape[0], kv.head_dim
+        _expect(pos, torch.int32, (rows,), "pos")
+        _expect(seq, torch.int32, (rows,), "seq")
+        for t, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+            _expect(t, torch.float32, (D,), what)
+        if rope is not None:
+            _expect(rope, torch.float32, tuple(rope.shape), "rope")
+        width = q_out.shape[1]
+        _expect(q_out, q_out.dtype, (rows, width), "q_out")
+        if width % D:
+            raise ValueError("q_out: whole heads")
+        for t, what in ((q, "q"), (k, "k"), (v, "v")):
+            if t.dtype != torch.float32 or t.shape[0] != rows:
+                raise ValueError(f"{what}: fp32 rows, as many as pos has")
+        ld = [_rows_ld(q, width, "q")] + [_rows_ld(t, kv.kv_heads * D, "k, v") for t in (k, v)]
+        rot = 0 if rope is None else rope.shape[1]
+        if n_pos is None:
+            n_pos = (1 << 31) - 1 if rope is None else rope.shape[0]
+        elif rope is not None and n_pos > rope.shape[0]:
+            raise ValueError("n_pos: at most the rows of rope")
+        self.kv, self._keep = kv, (q, k, v, pos, seq, q_weight, k_weight, rope, q_out)
+        self.struct = AppendArgs(_ptr(q), _ptr(k), _ptr(v), *ld, rows, width // D, _ptr(pos), _ptr(seq),
+                                 _ptr(q_weight), _ptr(k_weight), eps, _ptr(rope), rot, n_pos, int(interleaved),
+                                 _ptr(q_out), _type_of(q_out, "q_out"))
+        self._ref, self._run = ctypes.byref(self.struct), load().bq_append
+
+    def run(self):
+        return _check(self._run(self.kv.ref, self._ref, _stream()), "bq_append")
+
+
+class Attention:
+    """bq_attn_decode / bq_attn_prefill over fixed buffers: q and out [n_rows, q_heads * D] fp32 or bf16 (rows
+    may be strided), kv_len int32 [n_seq].  For prefill() of a batch row0 int32 [n_seq + 1], max_rows the most
+    rows a sequence has; for decode() every sequence has n_rows / n_seq rows.  work: a workspace tensor of the
+    caller's, "auto" for one of the object's own, None for none (decode() only)."""
+
+    def __init__(self, kv, q, out, kv_len, scale=None, window=0, sinks=0, max_len=None, row0=None, max_rows=None,
+                 work="auto"):
+        import torch
+        D, n_seq = kv.head_dim, kv.table.shape[0]
+        n_rows, width = q.shape
+        if width % D or out.shape != q.shape:
+            raise ValueError("q and out: rows of whole heads, alike")
+        _expect(kv_len, torch.int32, (n_seq,), "kv_len")
+        _expect(row0, torch.int32, (n_seq + 1,), "row0")
+        P = kv.struct.page_tokens
+        if max_len is None:
+            max_len = kv.table.shape[1] * P
+        if row0 is not None or n_rows == 0:
+            rows = max_rows or n_rows or 1
+        else:
+            rows = n_rows // n_seq
+        L = load()
+        if isinstance(work, str):
+            n = L.bq_attn_workspace_bytes(n_seq, rows, width // D, kv.kv_heads, D, max_len) if row0 is None else 0
+            work = torch.empty(n // 4, dtype=torch.float32, device=q.device) if n else None
+        self.kv, self._keep = kv, (q, out, kv_len, row0, work)
+        self.struct = AttnArgs(_ptr(q), _ptr(out), _type_of(q, "q"), _type_of(out, "out"), _rows_ld(q, width, "q"),
+                               _rows_ld(out, width, "out"), width // D, n_rows, rows, _ptr(row0), _ptr(kv_len), max_len,
+                               D ** -0.5 if scale is None else scale, window, sinks, _ptr(work),
+                               0 if work is None else work.numel() * work.element_size())
+        self._ref, self._decode, self._prefill = ctypes.byref(self.struct), L.bq_attn_decode, L.bq_attn_prefill
+
+    def decode(self):
+        return _check(self._decode(self.kv.ref, self._ref, _stream()), "bq_attn_decode")
+
+    def prefill(self):
+        return _check(self._prefill(self.kv.ref, self._ref, _stream()), "bq_attn_prefill")
+
+
+class AttentionPlan:
+    """The decode step's attention hook over its blocks: blocks[i] None, or (Append, Attention) of block i.
+    install(step) sets step.attention and step.user; check() raises what the hook met."""
+
+    def __init__(self, blocks, prefill=False):
+        self._keep = blocks
+        P = ctypes.pointer
+        self._blocks = (AttnBlock * max(1, len(blocks)))(*[
+            AttnBlock() if b is None else AttnBlock(P(b[1].kv.struct), P(b[0].struct), P(b[1].struct), int(prefill))
+            for b in blocks])
+        self.struct = AttnPlanStruct(len(blocks), self._blocks, BQ_OK)
+
+    def install(self, step):
+        step.attention = ctypes.cast(load().bq_attn_hook, ATTN_HOOK)
+        step.user = ctypes.addressof(self.struct)
+        step._attention_plan = self
+        return step
+
+    def check(self):
+        code, self.struct.status = self.struct.status, BQ_OK
+        return _check(code, "bq_attn_hook")
+
+
+class Sampler:
+    """bq_sample over fixed buffers: logits fp32 [rows, vocab] (rows may be strided), out int32 [rows], u fp32
+    [rows] in [0, 1); temperature, top_p, min_p fp32 [rows] and top_k int32 [rows], or None."""
+
+    def __init__(self, logits, out, u, temperature=None, top_k=None, top_p=None, min_p=None, work=None):
+        import torch
+        rows, vocab = logits.shape
+        if logits.dtype != torch.float32:
+            raise TypeError("logits: fp32")
+        _expect(out, torch.int32, (rows,), "out")
+        _expect(top_k, torch.int32, (rows,), "top_k")
+        for t, what in ((u, "u"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")):
+            _expect(t, torch.float32, (rows,), what)
+        L = load()
+        if work is None:
+            work = torch.empty(int(L.bq_sample_workspace_bytes(rows, vocab)), dtype=torch.uint8, device=logits.device)
+        ld = _rows_ld(logits, vocab, "logits")
+        self._keep = (logits, out, u, temperature, top_k, top_p, min_p, work)
+        self._args = (_ptr(logits), ld, rows, vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(u),
+                      _ptr(out), _ptr(work), work.numel() * work.element_size())
+        self._run = L.bq_sample
+
+    def run(self):
+        return _check(self._run(*self._args, _stream()), "bq_sample")

@@ -1,0 +1,418 @@
+// bq_attn.hip -- attention of 1..8 new tokens per sequence over the paged
+// cache (decode and speculative verify), split over the cache's length.
+//
+//   o = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),  x_j = scale log2(e) q.k_j
+// in one pass over the visible tokens, with a running m.  It reads every
+// visible token's K and V once per 16 query rows, so HBM bandwidth bounds it.
+//
+// A wave takes 32 tokens at a time and 16 query rows of one key-value head
+// (the heads of the group times the new tokens).  Scores are computed
+// transposed, S^T = K Q^T on 16x16x32 MFMA, so a lane holds tokens of one
+// query row; the rows of the two K tiles are dealt so that lane group g holds
+// tokens 8g..8g+7, which is what the second product O^T = V^T P^T takes as its
+// B operand: the softmax weights never leave their lane.  The cache's layout
+// is the A operands' (16 bytes per lane, 256 contiguous bytes per 16 lanes), so
+// K and V go straight from HBM to registers.
+//
+// fp32 precision on bf16 MFMA: K, V (and int8 codes) are exact in bf16; an
+// fp32 q is the sum of three bf16 parts, a softmax weight the sum of two (its
+// error, at most 2^-16 of the weight, is near the sums' own), each with its own MFMA.
+// The matrix pipe is far from busy here, the parts cost no time.
+//
+// The running maximum is kept per query row and only moved when a score passes
+// it by more than 2^8 (kLazy): a weight is then at most 2^8, which fp32 sums
+// carry, and the accumulators are rarely rescaled.
+#include <algorithm>
+
+#include "bq_internal.hpp"
+#include "bq_kv.hpp"
+
+namespace bq {
+
+namespace {
+constexpr int kWaves = 4;          // per workgroup
+constexpr int kRound = 512;        // 32-token steps whose pages are staged at once
+constexpr float kNone = -1e30f;    // the running maximum before any token
+constexpr float kLazy = 8.f;
+
+struct DecodeP {
+    KvView kv;
+    const void* q;
+    void* out;
+    int64_t ldq, ldo;
+    const int32_t* kv_len;
+    float* part;  // [n_seq][tiles][nsplit][16][D], then [..][16][2] (m, l)
+    int64_t ml;   // floats before the (m, l) part
+    int rows, G, tiles, nsplit, max_len, window, sinks, q_bf16, out_bf16;
+    float scale;  // scale * log2(e)
+};
+
+// four int8 codes -> bf16 (exact)
+BQ_DEV u32x2 codes_bf16(uint32_t w) {
+    const float a = (float)(int8_t)w, b = (float)(int8_t)(w >> 8), c = (float)(int8_t)(w >> 16), d = (float)((int32_t)w >> 24);
+    auto hi2 = [](float x, float y) {  // the high halves: small integers are exact in bf16
+        return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
+    };
+    return u32x2{hi2(a, b), hi2(c, d)};
+}
+BQ_DEV bf16x8 codes8(uint32_t lo, uint32_t hi) {
+    const u32x2 a = codes_bf16(lo), b = codes_bf16(hi);
+    return __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
+}
+BQ_DEV f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// sum over the four lane groups that share lane & 15
+BQ_DEV float groups_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+BQ_DEV float groups_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// NQ bf16 parts of q, NP of a softmax weight
+template <int D, int KV, int NQ, int NP>
+__global__ void __launch_bounds__(256, 2) k_attn_decode(DecodeP p) {
+    constexpr int KS = D / 32, DT = D / 16;
+    __shared__ int s_page[kRound * 2];
+    __shared__ __attribute__((aligned(16))) float s_o[kWaves][16][D + 4];
+    __shared__ float s_m[kWaves][16], s_l[kWaves][16], s_mt[16], s_lt[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const KvView& kv = p.kv;
+    const int seq = blockIdx.z, h = blockIdx.y % kv.heads, qt = blockIdx.y / kv.heads;
+    const int len = min(max(p.kv_len[seq], 0), min(p.max_len, kv.max_pages << kv.plog));
+
+    // the lane's query row: new token i, head hg of the group
+    const int M = p.rows * p.G, first = qt * 16, last = min(M, first + 16) - 1;
+    const int r = min(first + c, last), i = r / p.G;
+    const int pos = len - p.rows + i, pfirst = len - p.rows + first / p.G, plast = len - p.rows + last / p.G;
+    bf16x8 q[NQ][KS];
+    {
+        const size_t at = (size_t)(seq * p.rows + i) * p.ldq + (size_t)(h * p.G + r % p.G) * D + 8 * g;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            if constexpr (NQ == 1) {
+                q[0][k] = *(const bf16x8*)((const uint16_t*)p.q + at + 32 * k);
+            } else {
+                float x[8];
+                if (p.q_bf16) {
+                    const bf16x8 b = *(const bf16x8*)((const uint16_t*)p.q + at + 32 * k);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = (float)b[e];
+                } else {
+                    const f32x4 a = *(const f32x4*)((const float*)p.q + at + 32 * k), b = *(const f32x4*)((const float*)p.q + at + 32 * k + 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        const __bf16 t = (__bf16)x[e];
+                        q[n][k][e] = t;
+                        x[e] -= (float)t;
+                    }
+            }
+        }
+    }
+
+    // the tokens any of the tile's rows sees, in 32-token steps: the sinks'
+    // steps [0, ns), then [lo_step, end_step)
+    const int end = plast + 1;
+    const int lo = p.window ? max(0, pfirst - p.window + 1) : 0;
+    const int lo_step = lo >> 5, end_step = end > 0 ? (end + 31) >> 5 : 0;
+    const int ns = p.window ? min(lo_step, (p.sinks + 31) >> 5) : 0;
+    const int n = end > 0 ? ns + end_step - lo_step : 0;
+    const int per = (n + p.nsplit - 1) / p.nsplit;
+    const int v0 = blockIdx.x * per, v1 = min(n, v0 + per);
+
+    f32x4 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = kNone, l = 0.f;
+
+    const bool half_pages = kv.plog == 4;  // a step spans two 16-token pages
+    const int P = kv.P;
+    for (int vr = v0; vr < v1; vr += kRound) {
+        const int cnt = min(kRound, v1 - vr);
+        __syncthreads();
+        for (int e = tid; e < cnt << (half_pages ? 1 : 0); e += 256) {
+            const int v = vr + (half_pages ? e >> 1 : e), ts = v < ns ? v : v - ns + lo_step;
+            s_page[e] = kv_page(kv, seq, ts * 32 + (half_pages ? (e & 1) * 16 : 0));
+        }
+        __syncthreads();
+        for (int w = wave; w < cnt; w += kWaves) {
+            const int v = vr + w, ts = v < ns ? v : v - ns + lo_step, t0 = ts * 32;
+            // keys: lane row c holds token 8 (c / 4) + c % 4 (+ 4 in the second tile); values: tokens 8g..
+            const int gk = c >> 2;
+            const int pk = half_pages ? s_page[2 * w + (gk >> 1)] : s_page[w], pv = half_pages ? s_page[2 * w + (g >> 1)] : s_page[w];
+            const int ib = t0 & (P - 1);  // 0 with 16-token pages
+            const int tk = ib + 8 * (half_pages ? gk & 1 : gk) + (c & 3), tv = ib + 8 * (half_pages ? g & 1 : g);
+            const char* bk = kv.pages + (size_t)max(pk, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
+            const char* bv = kv.pages + (size_t)max(pv, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
+            f32x4 s[2];
+            if constexpr (KV == kKvBf16) {
+                bf16x8 kf[2][KS];
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) kf[t][k] = *(const bf16x8*)(bk + kv_k_unit(P, 4 * k + g, tk + 4 * t));
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int a = NQ - 1; a >= 0; --a) s[t] = mfma16(kf[t][k], q[a][k], s[t]);
+                }
+            } else {
+                u32x4 kf[2][KS / 2], sc[KS];
+#pragma unroll
+                for (int k = 0; k < KS / 2; ++k)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) kf[t][k] = *(const u32x4*)(bk + kv_kq_unit(P, k, g, tk + 4 * t));
+#pragma unroll
+                for (int k = 0; k < KS; ++k) sc[k] = *(const u32x4*)(bv + kv_ks_off(P, D, k, tv));
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const bf16x8 kb = codes8(kf[t][k / 2][2 * (k & 1)], kf[t][k / 2][2 * (k & 1) + 1]);
+                        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int a = NQ - 1; a >= 0; --a) x = mfma16(kb, q[a][k], x);
+                        const uint32_t a = sc[k][2 * t], b = sc[k][2 * t + 1];
+                        s[t] += x * f32x4{as_float(a << 16), as_float(a & 0xFFFF0000u), as_float(b << 16), as_float(b & 0xFFFF0000u)};
+                    }
+                }
+            }
+            // scores of tokens t0 + 8g + 4t + e for the lane's query row
+            const bool edge = t0 + 31 > pfirst || (p.window && t0 <= plast - p.window && t0 + 32 > p.sinks) || __any(pv < 0);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * p.scale;
+            uint32_t seen = 0xFF;  // tokens any row of the tile sees (their values are read)
+            if (edge) {
+                seen = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int t = t0 + 8 * g + e;
+                    const bool me = pv >= 0 && t <= pos && (!p.window || t > pos - p.window || t < p.sinks);
+                    const bool any = pv >= 0 && t < end && (t >= lo || t < p.sinks);
+                    x[e] = me ? x[e] : -INFINITY;
+                    seen |= any ? 1u << e : 0u;
+                }
+            }
+            float mx = x[0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+            if (__any(mx > m + kLazy)) {
+                const float mn = fmaxf(m, groups_max(mx));
+                const float al = __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] *= al;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(x[e] - m);
+                l += x[e];
+            }
+            auto parts = [&](const float (&y)[8], bf16x8 (&pp)[NP]) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float z = y[e];
+#pragma unroll
+                    for (int a = 0; a < NP; ++a) {
+                        const __bf16 t = (__bf16)z;
+                        pp[a][e] = t;
+                        z -= (float)t;
+                    }
+                }
+            };
+            if constexpr (KV == kKvBf16) {
+                bf16x8 vf[DT];
+#pragma unroll
+                for (int d = 0; d < DT; ++d) vf[d] = *(const bf16x8*)(bv + kv_v_unit(P, D, tv >> 3, 16 * d + c));
+                if (edge) {
+                    // what no row sees may hold anything: its products must not
+                    u32x4 mask;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        mask[e] = (seen >> (2 * e) & 1 ? 0xFFFFu : 0u) | (seen >> (2 * e + 1) & 1 ? 0xFFFF0000u : 0u);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) vf[d] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, vf[d]) & mask);
+                }
+                bf16x8 pp[NP];
+                parts(x, pp);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int a = NP - 1; a >= 0; --a) o[d] = mfma16(vf[d], pp[a], o[d]);
+            } else {
+                u32x4 vf[DT / 2], sc[DT / 2];
+#pragma unroll
+                for (int d = 0; d < DT / 2; ++d) vf[d] = *(const u32x4*)(bv + kv_vq_unit(P, D, tv >> 3, d, c));
+#pragma unroll
+                for (int d = 0; d < DT / 2; ++d) sc[d] = *(const u32x4*)(bv + kv_vs_off(P, D, d, tv));
+#pragma unroll
+                for (int d = 0; d < DT / 2; ++d) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float vs = as_float(e & 1 ? sc[d][e >> 1] & 0xFFFF0000u : sc[d][e >> 1] << 16);
+                        y[e] = x[e] * (edge && !(seen >> e & 1) ? 0.f : vs);  // codes are finite, an unseen scale may not be
+                    }
+                    bf16x8 pp[NP];
+                    parts(y, pp);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int a = NP - 1; a >= 0; --a) o[2 * d + u] = mfma16(codes8(vf[d][2 * u], vf[d][2 * u + 1]), pp[a], o[2 * d + u]);
+                }
+            }
+        }
+    }
+
+    // join the waves
+    l = groups_sum(l);
+    if (g == 0) {
+        s_m[wave][c] = m;
+        s_l[wave][c] = l;
+    }
+    __syncthreads();
+    float mt = s_m[0][c], lt = 0.f;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) mt = fmaxf(mt, s_m[w][c]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) lt += s_l[w][c] * __builtin_amdgcn_exp2f(s_m[w][c] - mt);
+    const float f = __builtin_amdgcn_exp2f(m - mt);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *(f32x4*)&s_o[wave][c][16 * d + 4 * g] = o[d] * f;
+    if (wave == 0 && g == 0) {
+        s_mt[c] = mt;
+        s_lt[c] = lt;
+    }
+    __syncthreads();
+    const size_t tile = ((size_t)seq * p.tiles + blockIdx.y) * p.nsplit + blockIdx.x;
+    for (int e = tid; e < 16 * (D / 4); e += 256) {
+        const int row = e / (D / 4), d = e % (D / 4) * 4;
+        if (first + row > last) continue;
+        f32x4 a = *(const f32x4*)&s_o[0][row][d];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) a += *(const f32x4*)&s_o[w][row][d];
+        const float lr = s_lt[row];
+        if (p.nsplit > 1) {
+            *(f32x4*)(p.part + (tile * 16 + row) * D + d) = a;
+            if (d == 0) {
+                p.part[p.ml + (tile * 16 + row) * 2] = s_mt[row];
+                p.part[p.ml + (tile * 16 + row) * 2 + 1] = lr;
+            }
+        } else {
+            const int rr = first + row;
+            const size_t at = (size_t)(seq * p.rows + rr / p.G) * p.ldo + (size_t)(h * p.G + rr % p.G) * D + d;
+            const float inv = lr == 0.f ? 0.f : 1.f / lr;
+            a = a * inv;
+            if (lr == 0.f) a = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (p.out_bf16)
+                *(u32x2*)((uint16_t*)p.out + at) = u32x2{f2bf2(a[0], a[1]), f2bf2(a[2], a[3])};
+            else
+                *(f32x4*)((float*)p.out + at) = a;
+        }
+    }
+}
+
+// joins the splits of one query row: D / 4 lanes per split, the splits dealt
+// over the rest of the workgroup, summed in a fixed order
+template <int D>
+__global__ void __launch_bounds__(256) k_attn_join(DecodeP p) {
+    constexpr int L = D / 4, S = 256 / L;
+    __shared__ __attribute__((aligned(16))) float s_o[S][D];
+    __shared__ float s_l[S], s_mx[4];
+    const int ht = p.kv.heads, tid = threadIdx.x;
+    const int row = blockIdx.x, h = blockIdx.y, seq = blockIdx.z;
+    const size_t tile = ((size_t)seq * p.tiles + (size_t)(row / 16) * ht + h) * p.nsplit;
+    const float* ml = p.part + p.ml;
+    float mt = kNone;
+    for (int s = tid; s < p.nsplit; s += 256) mt = fmaxf(mt, ml[((tile + s) * 16 + row % 16) * 2]);
+    for (int d = 1; d < 64; d <<= 1) mt = fmaxf(mt, __shfl_xor(mt, d, 64));
+    if ((tid & 63) == 0) s_mx[tid >> 6] = mt;
+    __syncthreads();
+    mt = fmaxf(fmaxf(s_mx[0], s_mx[1]), fmaxf(s_mx[2], s_mx[3]));
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    float lt = 0.f;
+#pragma unroll 4
+    for (int s = tid / L; s < p.nsplit; s += S) {
+        const size_t at = (tile + s) * 16 + row % 16;
+        const float l = ml[at * 2 + 1];
+        if (l == 0.f) continue;
+        const float f = __builtin_amdgcn_exp2f(ml[at * 2] - mt);
+        a += *(const f32x4*)(p.part + at * D + tid % L * 4) * f;
+        lt += l * f;
+    }
+    *(f32x4*)&s_o[tid / L][tid % L * 4] = a;
+    if (tid % L == 0) s_l[tid / L] = lt;
+    __syncthreads();
+    if (tid >= L) return;
+    for (int s = 1; s < S; ++s) {
+        a += *(const f32x4*)&s_o[s][tid * 4];
+        lt += s_l[s];
+    }
+    a = lt == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a * (1.f / lt);
+    const size_t at = (size_t)(seq * p.rows + row / p.G) * p.ldo + (size_t)(h * p.G + row % p.G) * D + tid * 4;
+    if (p.out_bf16)
+        *(u32x2*)((uint16_t*)p.out + at) = u32x2{f2bf2(a[0], a[1]), f2bf2(a[2], a[3])};
+    else
+        *(f32x4*)((float*)p.out + at) = a;
+}
+
+template <int D, int KV>
+hipError_t launch_decode_of(const DecodeP& p, hipStream_t st) {
+    const dim3 grid(p.nsplit, p.tiles, p.kv.n_seq);
+    if (p.q_bf16 && p.out_bf16)
+        launch_kernel((k_attn_decode<D, KV, 1, 1>), grid, dim3(256), 0, st, p);
+    else
+        launch_kernel((k_attn_decode<D, KV, 3, 2>), grid, dim3(256), 0, st, p);
+    if (p.nsplit > 1) {
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        launch_kernel((k_attn_join<D>), dim3(p.rows * p.G, p.kv.heads, p.kv.n_seq), dim3(256), 0, st, p);
+    }
+    return hipGetLastError();
+}
+int q_tiles(int rows, int G) { return (rows * G + 15) / 16; }
+}  // namespace
+
+// two workgroups per CU, each wave at least one 32-token step
+int decode_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus) {
+    const int64_t tiles = (int64_t)n_seq * kv_heads * q_tiles(rows, q_heads / kv_heads);
+    const int64_t steps = ((int64_t)max_len + 31) / 32;
+    return (int)std::max<int64_t>(1, std::min<int64_t>((steps + kWaves - 1) / kWaves, 2 * cus / tiles));
+}
+
+size_t decode_part_floats(int n_seq, int rows, int q_heads, int kv_heads, int D) {
+    return (size_t)n_seq * kv_heads * q_tiles(rows, q_heads / kv_heads) * 16 * (D + 2);
+}
+
+hipError_t launch_attn_decode(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st) {
+    DecodeP p;
+    p.kv = kv;
+    p.q = a.q; p.out = a.out; p.ldq = a.ldq; p.ldo = a.ldo; p.kv_len = a.kv_len;
+    p.rows = a.rows; p.G = a.q_heads / kv.heads; p.tiles = kv.heads * q_tiles(p.rows, p.G);
+    p.nsplit = nsplit; p.max_len = a.max_len; p.window = a.window; p.sinks = a.sinks;
+    p.q_bf16 = a.q_type == BQ_TYPE_BF16; p.out_bf16 = a.out_type == BQ_TYPE_BF16;
+    p.scale = a.scale * 1.44269504088896341f;
+    p.part = (float*)a.work;
+    p.ml = (int64_t)kv.n_seq * p.tiles * nsplit * 16 * kv.D;
+    const bool q8 = type == kKvQ8;
+    switch (kv.D) {
+        case 64: return q8 ? launch_decode_of<64, kKvQ8>(p, st) : launch_decode_of<64, kKvBf16>(p, st);
+        case 128: return q8 ? launch_decode_of<128, kKvQ8>(p, st) : launch_decode_of<128, kKvBf16>(p, st);
+        default: return q8 ? launch_decode_of<256, kKvQ8>(p, st) : launch_decode_of<256, kKvBf16>(p, st);
+    }
+}
+
+}  // namespace bq

@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "../../include/bq.h"
+
 namespace bq {
 
 constexpr int kMaxParts = 4;
@@ -130,5 +132,21 @@ constexpr int kNormMaxN = 32768;
 hipError_t launch_norm_q8(int op, float* out, const float* a, const float* b, const float* c,
                           const float* d, int rows, int n, int8_t* xq, float* xd, int32_t* xsum,
                           hipStream_t st);
+
+// the paged cache (bq_kv.hpp); type: KvType
+struct KvView;
+hipError_t launch_append(const KvView& kv, int type, const bq_append_args& a, hipStream_t st);
+hipError_t launch_kv_read(const KvView& kv, int type, const int32_t* seq, const int32_t* pos, int rows, uint16_t* k,
+                          uint16_t* v, hipStream_t st);
+// attention over it.  decode_splits: workgroups a sequence and head's tokens
+// are split over when the workspace allows it
+int decode_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus);
+size_t decode_part_floats(int n_seq, int rows, int q_heads, int kv_heads, int D);  // workspace of one split
+hipError_t launch_attn_decode(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st);
+hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, hipStream_t st);
+
+size_t sample_work_bytes(int rows, int vocab);
+hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, const float* temp, const int32_t* top_k,
+                         const float* top_p, const float* min_p, const float* u, int32_t* out, void* work, hipStream_t st);
 
 }  // namespace bq

@@ -1,0 +1,433 @@
+// bq_sample.hip -- one token per row of logits: temperature, top-k, top-p,
+// min-p, from a given uniform number.
+//
+// Kept tokens are a run of the row sorted by logit, so only the row's head has
+// to be sorted.  Two launches:
+//   k_sample_scan, one workgroup per 8192 logits: reads them once (the floor:
+//     4 bytes a logit), keeps the head of its slice -- every logit not below a
+//     threshold t, the slice's 256 threads' maxima put in order and one of them
+//     taken, which leaves about 768 candidates for the whole row -- and, where
+//     top-p needs the row's mass, its sum of exponentials.
+//   k_sample_pick, one workgroup per row: sorts the candidates, takes their
+//     running mass and cuts it.  All tokens of the row not below the largest t
+//     are among the candidates, so a cut that falls there is exact.  Where it
+//     does not (a flat row, no filter, many equal logits), the row is read
+//     again: radix selection by count and by mass on the ordered bits of the
+//     logit, then of the index, 11 bits at a time.
+// Slices are 256-logit blocks dealt in turn: likely tokens that lie together
+// in the vocabulary spread over the slices.
+// A mass is exp(x) in units of 2^-40 of the first token's, in 64-bit integers:
+// the atomic sums come out the same in any order.  (The row's mass of the scan
+// is a float sum per slice, in a fixed order.)
+#include <algorithm>
+#include <cmath>
+
+#include "bq_device.hpp"
+#include "bq_internal.hpp"
+
+namespace bq {
+
+namespace {
+constexpr int kSlice = 8192;
+constexpr int kMaxCand = 1024;
+constexpr int kWant = 768;  // candidates wanted of a row
+typedef unsigned long long u64;
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any logit
+
+struct SliceInfo {
+    u64 best;      // largest key
+    float t;       // every logit >= t of the slice is a candidate (-inf: all finite ones, +inf: none)
+    float sum;     // of exp((x - max) / temperature), where top-p needs it
+    int count, pad;
+};
+
+struct SampleP {
+    const float* logits;
+    int64_t ld;
+    int vocab, slices, cap, rank;
+    const float* temp;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    const float* u;
+    int32_t* out;
+    SliceInfo* info;
+    u64* cand;
+};
+
+// ordered bits of a logit (-0 as 0, NaN as -inf), and the sort key: larger
+// logits first, then lower indices
+BQ_DEV float clean(float x) { return x == x ? x + 0.f : -INFINITY; }
+BQ_DEV uint32_t ordered(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    return b ^ (b >> 31 ? 0xFFFFFFFFu : 0x80000000u);
+}
+BQ_DEV float unordered(uint32_t o) { return as_float(o ^ (o >> 31 ? 0x80000000u : 0xFFFFFFFFu)); }
+BQ_DEV u64 key_of(float x, int i) { return (u64)ordered(x) << 32 | (0xFFFFFFFFu - (uint32_t)i); }
+BQ_DEV int index_of(u64 key) { return (int)(0xFFFFFFFFu - (uint32_t)key); }
+BQ_DEV u64 mass_of(float x, float mx, float temp) { return (u64)__builtin_rintf(expf((x - mx) / temp) * 0x1p40f); }
+BQ_DEV u64 shfl_xor64(u64 v, int d) {
+    const uint32_t lo = __shfl_xor((uint32_t)v, d, 64), hi = __shfl_xor((uint32_t)(v >> 32), d, 64);
+    return (u64)hi << 32 | lo;
+}
+BQ_DEV u64 shfl_up64(u64 v, int d) {
+    const uint32_t lo = __shfl_up((uint32_t)v, d, 64), hi = __shfl_up((uint32_t)(v >> 32), d, 64);
+    return (u64)hi << 32 | lo;
+}
+
+struct RowRule {
+    float temp, top_p, min_p;
+    int top_k;  // vocab: all
+    bool greedy;
+};
+BQ_DEV RowRule rule_of(const SampleP& p, int row) {
+    RowRule r;
+    r.temp = p.temp ? p.temp[row] : 1.f;
+    r.top_p = p.top_p ? p.top_p[row] : 1.f;
+    r.min_p = p.min_p ? p.min_p[row] : 0.f;
+    const int k = p.top_k ? p.top_k[row] : 0;
+    r.top_k = k > 0 && k < p.vocab ? k : p.vocab;
+    r.greedy = !(r.temp > 0.f) || r.top_k == 1;
+    return r;
+}
+
+__global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
+    constexpr int V = kSlice / 1024;  // 16-byte loads of a thread
+    __shared__ float s_max[256];
+    __shared__ u64 s_best[4];
+    __shared__ float s_sum[4], s_t;
+    __shared__ int s_count;
+    const int tid = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
+    const float* x = p.logits + (size_t)row * p.ld;
+    const RowRule rule = rule_of(p, row);
+    // the slice's k-th run of four waves' blocks: block (4k + wave) * slices + slice
+    float v[V][4];
+    auto at = [&](int k) { return ((4 * k + (tid >> 6)) * p.slices + slice) * 256 + (tid & 63) * 4; };
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int i = at(k);
+        f32x4 a = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (i + 4 <= p.vocab) {
+            a = *(const f32x4u*)(x + i);
+        } else {
+            for (int e = 0; e < 4; ++e)
+                if (i + e < p.vocab) a[e] = x[i + e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[k][e] = clean(a[e]);
+    }
+    u64 best = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const u64 key = key_of(v[k][e], at(k) + e);
+            best = key > best ? key : best;
+        }
+    const float mine = unordered((uint32_t)(best >> 32));
+    s_max[tid] = mine;
+    if (tid == 0) s_count = 0;
+    for (int d = 1; d < 64; d <<= 1) {
+        const u64 o = shfl_xor64(best, d);
+        best = o > best ? o : best;
+    }
+    if ((tid & 63) == 0) s_best[tid >> 6] = best;
+    __syncthreads();
+    best = s_best[0];
+    for (int w = 1; w < 4; ++w) best = s_best[w] > best ? s_best[w] : best;
+    SliceInfo* info = p.info + (size_t)row * p.slices + slice;
+    if (rule.greedy) {
+        if (tid == 0) info->best = best;
+        return;
+    }
+    // the thread whose maximum is the rank-th gives the threshold
+    int ahead = 0;
+    for (int i = 0; i < 256; i += 4) {
+        const f32x4 a = *(const f32x4*)(s_max + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ahead += a[e] > mine || (a[e] == mine && i + e < tid);
+    }
+    if (ahead == p.rank) s_t = mine;
+    float sum = 0.f;
+    if (rule.top_p < 1.f && rule.top_k == p.vocab) {
+        const float mx = unordered((uint32_t)(best >> 32));
+        if (mx > -INFINITY && mx < INFINITY) {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += expf((v[k][e] - mx) / rule.temp);
+        }
+        sum = wave_sum_dpp63(sum);
+        if ((tid & 63) == 63) s_sum[tid >> 6] = sum;
+    }
+    __syncthreads();
+    const float t = s_t;
+    u64* cand = p.cand + ((size_t)row * p.slices + slice) * p.cap;
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (v[k][e] >= t && v[k][e] > -INFINITY) {
+                const int c = atomicAdd(&s_count, 1);
+                if (c < p.cap) cand[c] = key_of(v[k][e], at(k) + e);
+            }
+    __syncthreads();
+    if (tid == 0) {
+        const bool over = s_count > p.cap;
+        info->best = best;
+        info->t = over ? INFINITY : t;
+        info->sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+        info->count = over ? 0 : s_count;
+    }
+}
+
+// exclusive scan over the workgroup's 1024 threads, and the total
+BQ_DEV u64 scan1024(u64 v, u64* red, u64& total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    u64 s = v;
+    for (int d = 1; d < 64; d <<= 1) {
+        const u64 o = shfl_up64(s, d);
+        if (lane >= d) s += o;
+    }
+    __syncthreads();
+    if (lane == 63) red[w] = s;
+    __syncthreads();
+    u64 before = 0;
+    total = 0;
+    for (int i = 0; i < 16; ++i) {
+        if (i < w) before += red[i];
+        total += red[i];
+    }
+    return before + s - v;
+}
+
+// The whole row, by radix selection.
+struct Whole {
+    const float* x;
+    int vocab;
+    float mx, temp;
+    u64* bins;   // [2048]
+    u64* red;    // [16]
+    u64* found;  // [2]: the bin, the mass before it
+
+    // f(key, logit) over the logits above -inf
+    template <typename F>
+    BQ_DEV void each(F f) const {
+        for (int i = threadIdx.x; i < vocab; i += 1024) {
+            const float v = clean(x[i]);
+            if (!(v > -INFINITY)) continue;
+            f(key_of(v, i), v);
+        }
+    }
+
+    // The keys in descending order, each weighing 1 (by_count) or its mass;
+    // the first whose running weight w meets w >= target (or w > target).
+    // Only keys >= low count.  Returns 0 if none does.
+    BQ_DEV u64 select(bool by_count, double target, bool strict, u64 low) const {
+        constexpr int kShift[6] = {53, 42, 32, 21, 10, 0}, kBits[6] = {11, 11, 10, 11, 11, 10};
+        u64 prefix = 0;   // the digits found so far, in place
+        u64 before = 0;   // the weight of larger keys
+        for (int d = 0; d < 6; ++d) {
+            const int sh = kShift[d], nb = 1 << kBits[d];
+            __syncthreads();
+            for (int i = threadIdx.x; i < 2048; i += 1024) bins[i] = 0;
+            if (threadIdx.x == 0) found[0] = ~0ull;
+            __syncthreads();
+            each([&](u64 key, float v) {
+                if (key < low || (d && (key ^ prefix) >> (sh + kBits[d]))) return;
+                const u64 w = by_count ? 1 : mass_of(v, mx, temp);
+                if (w) atomicAdd(&bins[(key >> sh) & (nb - 1)], w);
+            });
+            __syncthreads();
+            // thread i owns the i-th and (i + 1)-th bins from the top
+            const int hi = nb - 1 - 2 * (int)threadIdx.x;
+            const u64 a = hi >= 1 ? bins[hi] : 0, b = hi >= 1 ? bins[hi - 1] : 0;
+            u64 total;
+            const u64 ex = before + scan1024(a + b, red, total);
+            auto meets = [&](u64 w) { return strict ? (double)w > target : (double)w >= target; };
+            if (a && !meets(ex) && meets(ex + a)) {
+                found[0] = hi;
+                found[1] = ex;
+            } else if (b && !meets(ex + a) && meets(ex + a + b)) {
+                found[0] = hi - 1;
+                found[1] = ex + a;
+            }
+            __syncthreads();
+            if (found[0] == ~0ull) return 0;
+            prefix |= found[0] << sh;
+            before = found[1];
+        }
+        return prefix;
+    }
+
+    BQ_DEV u64 mass_from(u64 low) const {
+        u64 s = 0, total;
+        each([&](u64 key, float v) {
+            if (key >= low) s += mass_of(v, mx, temp);
+        });
+        scan1024(s, red, total);
+        return total;
+    }
+};
+
+__global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
+    __shared__ u64 s_key[kMaxCand], s_bins[2048], s_red[16], s_found[2];
+    __shared__ int s_first[129], s_stop;
+    __shared__ u64 s_best;
+    __shared__ float s_t;
+    __shared__ double s_mass;
+    const int tid = threadIdx.x, row = blockIdx.x;
+    const RowRule rule = rule_of(p, row);
+    const SliceInfo* info = p.info + (size_t)row * p.slices;
+    if (tid == 0) {
+        u64 best = 0;
+        for (int s = 0; s < p.slices; ++s) best = info[s].best > best ? info[s].best : best;
+        s_best = best;
+    }
+    __syncthreads();
+    const float mx = unordered((uint32_t)(s_best >> 32));
+    if (rule.greedy || !(mx > -INFINITY) || mx == INFINITY) {
+        // a row of -inf has its largest key at index 0
+        if (tid == 0) p.out[row] = index_of(s_best);
+        return;
+    }
+    const bool need_mass = rule.top_p < 1.f && rule.top_k == p.vocab;
+    if (tid == 0) {
+        int c = 0;
+        float t = -INFINITY;
+        double mass = 0;
+        for (int s = 0; s < p.slices; ++s) {
+            s_first[s] = c;
+            c += info[s].count;
+            t = fmaxf(t, info[s].t);
+            if (need_mass)
+                mass += (double)info[s].sum * (double)expf((unordered((uint32_t)(info[s].best >> 32)) - mx) / rule.temp);
+        }
+        s_first[p.slices] = c;
+        s_t = t;
+        s_mass = mass * 0x1p40;
+        s_stop = kMaxCand + 1;
+    }
+    __syncthreads();
+    const int total = s_first[p.slices];
+    const float t = s_t;
+    const double u = (double)p.u[row];
+    if (total > 0 && total <= kMaxCand) {
+        int n = 64;
+        while (n < total) n <<= 1;
+        u64 key = 0;
+        if (tid < total) {
+            int s = 0;
+            for (int hi = p.slices; hi - s > 1;) {
+                const int mid = (s + hi) / 2;
+                if (s_first[mid] <= tid) s = mid;
+                else hi = mid;
+            }
+            key = p.cand[((size_t)row * p.slices + s) * p.cap + tid - s_first[s]];
+        }
+        // bitonic sort, descending, one key per thread
+        for (int k = 2; k <= n; k <<= 1)
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                u64 o;
+                if (j >= 64) {
+                    __syncthreads();
+                    s_key[tid] = key;
+                    __syncthreads();
+                    o = s_key[tid ^ j];
+                } else {
+                    o = shfl_xor64(key, j);
+                }
+                const bool larger = ((tid & k) == 0) == ((tid & j) == 0);
+                key = larger == (o > key) ? o : key;
+            }
+        const float x = unordered((uint32_t)(key >> 32));
+        const bool in = tid < total;
+        const float e = in ? expf((x - mx) / rule.temp) : 0.f;
+        const u64 w = in ? mass_of(x, mx, rule.temp) : 0;
+        u64 all;
+        const u64 ex = scan1024(w, s_red, all);
+        s_key[tid] = ex + w;
+        // candidates that are the row's largest for sure: those not below t
+        const int sure = __syncthreads_count(in && x >= t);
+        const bool whole = !(t > -INFINITY);
+        // mass of the first top_k
+        const bool k_sure = rule.top_k <= sure;
+        const double z = k_sure ? (double)s_key[rule.top_k - 1] : s_mass;
+        const bool z_known = rule.top_p >= 1.f || k_sure || rule.top_k == p.vocab || whole;
+        const double cut = (double)rule.top_p * (whole && !k_sure ? (double)s_key[total - 1] : z);
+        if (tid <= sure && tid > 0 &&
+            (tid >= rule.top_k || (rule.top_p < 1.f && (double)ex >= cut) || (tid < sure && e < rule.min_p)))
+            atomicMin(&s_stop, tid);
+        __syncthreads();
+        int kept = s_stop;
+        if (kept > kMaxCand && whole) kept = total;
+        if (z_known && kept <= kMaxCand) {
+            const u64 mass = s_key[kept - 1];
+            const double target = u * (double)mass;
+            if (tid < kept && ((double)(ex + w) > target || tid == kept - 1) && (tid == 0 || !((double)ex > target)))
+                p.out[row] = index_of(key);
+            return;
+        }
+    }
+    // the head was not enough
+    Whole r{p.logits + (size_t)row * p.ld, p.vocab, mx, rule.temp, s_bins, s_red, s_found};
+    u64 low = rule.top_k < p.vocab ? r.select(true, (double)rule.top_k, false, 0) : 0;  // 0: fewer finite ones
+    if (rule.top_p < 1.f) {
+        const double z = (double)r.mass_from(low);
+        const u64 at = rule.top_p > 0.f ? r.select(false, (double)rule.top_p * z, false, low) : s_best;
+        low = at > low ? at : low;
+    }
+    if (rule.min_p > 0.f) {
+        // the smallest key whose weight is at least min_p: weights fall with the key
+        u64 least = s_best;
+        r.each([&](u64 key, float v) {
+            if (key < least && expf((v - mx) / rule.temp) >= rule.min_p) least = key;
+        });
+        for (int d = 1; d < 64; d <<= 1) {
+            const u64 o = shfl_xor64(least, d);
+            least = o < least ? o : least;
+        }
+        __syncthreads();
+        if ((tid & 63) == 0) s_red[tid >> 6] = least;
+        __syncthreads();
+        for (int i = 0; i < 16; ++i) least = s_red[i] < least ? s_red[i] : least;
+        low = least > low ? least : low;
+    }
+    const u64 mass = r.mass_from(low);
+    u64 pick = r.select(false, u * (double)mass, true, low);
+    if (pick == 0) {
+        // u = 1: the last key with a weight
+        pick = r.select(false, (double)mass, false, low);
+    }
+    if (tid == 0) p.out[row] = pick ? index_of(pick) : index_of(s_best);
+}
+
+int slices_of(int vocab) { return (vocab + kSlice - 1) / kSlice; }
+int cap_of(int slices) { return std::max(16, 2 * kWant / slices); }
+}  // namespace
+
+size_t sample_work_bytes(int rows, int vocab) {
+    const int s = slices_of(vocab);
+    return (size_t)rows * s * (sizeof(SliceInfo) + (size_t)cap_of(s) * sizeof(u64));
+}
+
+hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, const float* temp, const int32_t* top_k,
+                         const float* top_p, const float* min_p, const float* u, int32_t* out, void* work, hipStream_t st) {
+    SampleP p;
+    p.logits = logits; p.ld = ld; p.vocab = vocab;
+    p.slices = slices_of(vocab);
+    p.cap = cap_of(p.slices);
+    // of the 256 maxima of 32 logits each in random order, the rank-th leaves
+    // about 256 ln(256 / (256 - rank)) logits above it
+    p.rank = std::max(4, std::min(250, (int)(256 * (1 - std::exp(-(double)kWant / p.slices / 256)))));
+    p.temp = temp; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p; p.u = u; p.out = out;
+    p.info = (SliceInfo*)work;
+    p.cand = (u64*)(p.info + (size_t)rows * p.slices);
+    launch_kernel(k_sample_scan, dim3(p.slices, rows), dim3(256), 0, st, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    launch_kernel(k_sample_pick, dim3(rows), dim3(1024), 0, st, p);
+    return hipGetLastError();
+}
+
+}  // namespace bq

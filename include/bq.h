@@ -447,6 +447,144 @@ int bq_decode_graph_create(const bq_decode_step* s, bq_stream_t st, bq_decode_gr
 int bq_decode_graph_launch(const bq_decode_graph* g, bq_stream_t st);  /* one token */
 void bq_decode_graph_destroy(bq_decode_graph* g);
 
+/* ---- serving operators -------------------------------------------------------
+ * What a decode or prompt step needs around the matmuls: the step's keys and
+ * values into a paged cache with the per-head norm and rotation (bq_append),
+ * attention over that cache (bq_attn_decode, bq_attn_prefill), and the next
+ * token from the logits (bq_sample).  Stream-ordered and allocation-free as
+ * every entry point above; positions, lengths and page tables are device
+ * memory, so a captured graph serves every token of a growing sequence.
+ *
+ * The cache.  One page holds page_tokens tokens (16, 32, 64, 128 or 256) of
+ * every key-value head; token t of sequence s lies in page
+ * table[s * max_pages + t / page_tokens].  A table entry outside 0..n_pages-1
+ * is an unmapped page: nothing is written to it and its tokens are not seen.
+ * Per page and head first the keys, then the values (P = page_tokens, D =
+ * head_dim, 64, 128 or 256), in the order the matrix instructions take them:
+ *   BQ_TYPE_BF16  K [D/8][P][8]          V [P/8][D][8]
+ *   BQ_TYPE_Q8_0  K codes [D/64][4][P][2][8]: dim 64c + 32u + 8g + i at [c][g][token][u][i]
+ *                 V codes [P/8][D/32][16][2][8]: token 8t + i, dim 32c + 16u + m at [t][c][m][u][i]
+ *                 K scales bf16 [D/32][P], V scales bf16 [D/32][P]
+ *                 per (token, 32 dims) d = bf16(amax / 127), code = clamp(rint(x / d), -127, 127)
+ * (a bf16 scale keeps fp32's range, so no finite row overflows it).
+ * bq_kv_page_bytes is the size of one page, 0 for a layout that is not handled. */
+enum { BQ_TYPE_F32 = 0, BQ_TYPE_Q8_0 = 8, BQ_TYPE_BF16 = 30 }; /* GGML type ids */
+typedef struct bq_kv_cache {
+    void* pages;                  /* [n_pages][bq_kv_page_bytes], 16-byte aligned */
+    const int32_t* table;         /* device, [n_seq][max_pages] */
+    int type;                     /* BQ_TYPE_BF16 or BQ_TYPE_Q8_0 */
+    int kv_heads, head_dim, page_tokens;
+    int n_pages, n_seq, max_pages;
+} bq_kv_cache;
+size_t bq_kv_page_bytes(int type, int kv_heads, int head_dim, int page_tokens);
+
+/* Rows of the QKV projections into the cache, and the rotated queries.  Per
+ * row r and head, n(x) = x * rsqrt(sum x^2 / D + eps) * weight[D] (weight NULL:
+ * n(x) = x), then the first `rot` values are rotated by the row's position:
+ * with (c, s) = rope[pos[r]][i], rope[pos[r]][rot/2 + i] for i < rot/2,
+ * (a, b) -> (a c - b s, b c + a s) on the pairs (i, i + rot/2), or (2i, 2i + 1)
+ * with interleaved != 0.  Keys and unchanged values go to token pos[r] of
+ * sequence seq[r] (seq NULL: every row to sequence 0); queries to q_out
+ * [rows][q_heads * D] as fp32 or bf16.  q_out may be q itself (fp32, ldq =
+ * q_heads * D).  rot % 8 == 0, 0 <= rot <= D; rope NULL with rot = 0.  A row
+ * whose position is negative or >= n_pos (padding), or whose sequence is not
+ * one of n_seq, is not appended and its queries are zeros; n_pos is the
+ * number of positions allowed also when rot = 0.  Two rows of one call must not name the
+ * same token.  Row strides are in elements, multiples of 4. */
+typedef struct bq_append_args {
+    const float* q; const float* k; const float* v;
+    int64_t ldq, ldk, ldv;
+    int rows, q_heads;
+    const int32_t* pos; const int32_t* seq;
+    const float* q_weight; const float* k_weight;
+    float eps;
+    const float* rope;            /* [n_pos][rot]: rot/2 cosines, then rot/2 sines */
+    int rot, n_pos, interleaved;
+    void* q_out;
+    int q_type;                   /* BQ_TYPE_F32 or BQ_TYPE_BF16 */
+} bq_append_args;
+int bq_append(const bq_kv_cache* kv, const bq_append_args* a, bq_stream_t st);
+/* The cached K and V of `rows` tokens as bf16 rows [rows][kv_heads * D] (either
+ * may be NULL): token pos[r] of sequence seq[r]; zeros where none is mapped. */
+int bq_kv_read(const bq_kv_cache* kv, const int32_t* seq, const int32_t* pos, int rows, uint16_t* k, uint16_t* v,
+               bq_stream_t st);
+
+/* Attention over the cache: out = sum_j softmax_j(scale * q.k_j) v_j per row
+ * and query head (query head h reads key-value head h / (q_heads / kv_heads)),
+ * over the tokens j <= p with window == 0, j > p - window or j < sinks, where
+ * p is the row's position: a sequence of length kv_len[s] (its new rows
+ * included, appended before) whose call has n rows has them at positions
+ * kv_len[s] - n .. kv_len[s] - 1.  A row that sees no token (kv_len 0, a
+ * negative position, unmapped pages) gives zeros.  What the cache holds past
+ * kv_len, or at tokens that no row of the call sees, does not matter (it may
+ * be NaN).  kv_len is clamped to max_len.
+ *   bq_attn_decode: 1..8 rows per sequence (`rows`), rows s * rows ... of q
+ *     and out; products carry fp32 precision (q and the softmax weights as
+ *     sums of bf16 parts) unless q and out are both bf16.  The tokens of a
+ *     sequence are split over workgroups and joined through `work`
+ *     (bq_attn_workspace_bytes for the full split; NULL or less: a smaller
+ *     split or none).  The split follows max_len, which a captured graph
+ *     fixes, not kv_len.
+ *   bq_attn_prefill: a ragged batch, rows row0[s] .. row0[s + 1] - 1 of q and
+ *     out for sequence s (device, [n_seq + 1], non-decreasing, within n_rows;
+ *     NULL: n_seq must be 1 and its rows are all n_rows), at most `rows` each;
+ *     q and the softmax weights enter the products as bf16, sums are fp32.
+ * scale > 0.  q_heads % kv_heads == 0 and q_heads / kv_heads <= 64, else BQ_UNSUPPORTED.
+ * Row strides in elements, multiples of 8. */
+typedef struct bq_attn_args {
+    const void* q; void* out;
+    int q_type, out_type;         /* BQ_TYPE_F32 or BQ_TYPE_BF16 */
+    int64_t ldq, ldo;
+    int q_heads, n_rows;          /* rows of q and out */
+    int rows;                     /* per sequence (prefill: at most) */
+    const int32_t* row0;          /* prefill */
+    const int32_t* kv_len;        /* device, [n_seq] */
+    int max_len;                  /* no kv_len is larger */
+    float scale;
+    int window, sinks;
+    void* work;
+    size_t work_bytes;
+} bq_attn_args;
+size_t bq_attn_workspace_bytes(int n_seq, int rows, int q_heads, int kv_heads, int head_dim, int max_len);
+int bq_attn_decode(const bq_kv_cache* kv, const bq_attn_args* a, bq_stream_t st);
+int bq_attn_prefill(const bq_kv_cache* kv, const bq_attn_args* a, bq_stream_t st);
+
+/* The decode step's attention hook over a list of blocks: set
+ * bq_decode_step.attention = bq_attn_hook and user = a bq_attn_plan whose
+ * blocks[i] belongs to the step's block i (kv NULL: no attention there).  The
+ * hook appends the block's rows and attends, by bq_attn_prefill where
+ * `prefill` is set, else bq_attn_decode.  The hook cannot fail the step, so
+ * the first code that is not BQ_OK stays in `status` (the caller clears it). */
+typedef struct bq_attn_block {
+    const bq_kv_cache* kv;
+    const bq_append_args* append;
+    const bq_attn_args* attn;
+    int prefill;
+} bq_attn_block;
+typedef struct bq_attn_plan {
+    int n_blocks;
+    const bq_attn_block* blocks;
+    int status;
+} bq_attn_plan;
+void bq_attn_hook(void* user, int block, bq_stream_t st);
+
+/* One token per row of logits, from one given uniform number per row.  With
+ * x_i = (logit_i - max) / temperature[r], tokens ordered by logit, ties by the
+ * lower index, kept are the leading tokens that satisfy all of: among the
+ * first top_k (<= 0: all); the mass of those before it, exp(x) summed, is less
+ * than top_p times the mass of the first top_k; exp(x) >= min_p.  The first is
+ * always kept.  The token is the first whose running mass exceeds u[r] times
+ * the kept mass.  temperature <= 0: the first token.  A NaN logit counts as
+ * -inf; -inf is never drawn unless the whole row is (token 0); a +inf logit
+ * makes the row greedy.  temperature, top_k, top_p, min_p: device arrays of
+ * one value per row, or NULL (1, all, 1, 0).  Equal calls give equal tokens.
+ * Rows are ld >= vocab apart, any ld; vocab <= 2^20 (else BQ_UNSUPPORTED).  work: at least
+ * bq_sample_workspace_bytes (else BQ_EINVAL), not shared by calls that overlap. */
+size_t bq_sample_workspace_bytes(int rows, int vocab);
+int bq_sample(const float* logits, int64_t ld, int rows, int vocab, const float* temperature, const int32_t* top_k,
+              const float* top_p, const float* min_p, const float* u, int32_t* out, void* work, size_t work_bytes,
+              bq_stream_t st);
+
 /* ---- tooling ---------------------------------------------------------------
  * No counterpart in the reference (its harnesses bracket launches with
  * cudaEventRecord, tools/gemvbench.cu:360-371).  Times the calling thread's
