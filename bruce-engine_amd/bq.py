@@ -603,6 +603,13 @@ class DecodeGraph:
 
 
 # ---------------------------------------------------------------- serving operators
+def _raw_stream(device):
+    """The current stream of a device as a number (torch.cuda.current_stream builds an object for it)."""
+    import torch
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(device) if get is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def _type_of(t, what):
     import torch
     if t.dtype == torch.float32:
@@ -658,7 +665,7 @@ class KvCache:
         self.struct = KvCacheStruct(_ptr(pages), _ptr(table), KV_TYPES[kv_type], kv_heads, head_dim, page_tokens,
                                     pages.shape[0], table.shape[0], table.shape[1])
         self.ref = ctypes.byref(self.struct)
-        self._read = load().bq_kv_read
+        self._read, self.device = load().bq_kv_read, pages.device.index
 
     @classmethod
     def empty(cls, n_pages, table, kv_type, kv_heads, head_dim, page_tokens, device="cuda"):
@@ -676,7 +683,7 @@ class KvCache:
             _expect(t, torch.int32, (rows,), what)
         for t, what in ((k, "k"), (v, "v")):
             _expect(t, torch.bfloat16, (rows, self.kv_heads * self.head_dim), what)
-        return _check(self._read(self.ref, _ptr(seq), _ptr(pos), rows, _ptr(k), _ptr(v), _stream()), "bq_kv_read")
+        return _check(self._read(self.ref, _ptr(seq), _ptr(pos), rows, _ptr(k), _ptr(v), _raw_stream(self.device)), "bq_kv_read")
 
 
 class Append:
@@ -714,7 +721,7 @@ class Append:
         self._ref, self._run = ctypes.byref(self.struct), load().bq_append
 
     def run(self):
-        return _check(self._run(self.kv.ref, self._ref, _stream()), "bq_append")
+        return _check(self._run(self.kv.ref, self._ref, _raw_stream(self.kv.device)), "bq_append")
 
 
 class Attention:
@@ -751,10 +758,10 @@ class Attention:
         self._ref, self._decode, self._prefill = ctypes.byref(self.struct), L.bq_attn_decode, L.bq_attn_prefill
 
     def decode(self):
-        return _check(self._decode(self.kv.ref, self._ref, _stream()), "bq_attn_decode")
+        return _check(self._decode(self.kv.ref, self._ref, _raw_stream(self.kv.device)), "bq_attn_decode")
 
     def prefill(self):
-        return _check(self._prefill(self.kv.ref, self._ref, _stream()), "bq_attn_prefill")
+        return _check(self._prefill(self.kv.ref, self._ref, _raw_stream(self.kv.device)), "bq_attn_prefill")
 
 
 class AttentionPlan:
@@ -800,7 +807,7 @@ class Sampler:
         self._keep = (logits, out, u, temperature, top_k, top_p, min_p, work)
         self._args = (_ptr(logits), ld, rows, vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(u),
                       _ptr(out), _ptr(work), work.numel() * work.element_size())
-        self._run = L.bq_sample
+        self._run, self._device = L.bq_sample, logits.device.index
 
     def run(self):
-        return _check(self._run(*self._args, _stream()), "bq_sample")
+        return _check(self._run(*self._args, _raw_stream(self._device)), "bq_sample")

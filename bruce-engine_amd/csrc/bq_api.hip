@@ -122,6 +122,7 @@ ScaledCopy& next_scaled_copy() {
 }
 
 int device_cus() { return t_dev ? t_dev->cus : 256; }
+int device_ready() { return ensure_init(); }
 
 int gemv_gate_den_fused(float* y, const void* w_raw, int K, int N, const float* a, const float* den, void* st) {
     if (int r = ensure_init()) return r;

@@ -41,11 +41,36 @@ struct DecodeP {
     void* out;
     int64_t ldq, ldo;
     const int32_t* kv_len;
-    float* part;  // [n_seq][tiles][nsplit][16][D], then [..][16][2] (m, l)
-    int64_t ml;   // floats before the (m, l) part
+    float* part;       // [n_seq][tiles][nsplit][16][D], then [..][16][2] (m, l)
+    int64_t ml;        // floats before the (m, l) part
     int rows, G, tiles, nsplit, max_len, window, sinks, q_bf16, out_bf16;
     float scale;  // scale * log2(e)
 };
+
+// 32-token steps that a tile's rows at positions pfirst..plast see: the
+// sinks' [0, ns), then [lo_step, lo_step + n - ns)
+struct Steps {
+    int lo, lo_step, ns, n;
+};
+BQ_DEV Steps steps_of(const DecodeP& p, int pfirst, int plast) {
+    Steps s;
+    s.lo = p.window ? max(0, pfirst - p.window + 1) : 0;
+    s.lo_step = s.lo >> 5;
+    s.ns = p.window ? min(s.lo_step, (p.sinks + 31) >> 5) : 0;
+    s.n = plast < 0 ? 0 : s.ns + ((plast + 32) >> 5) - s.lo_step;
+    return s;
+}
+BQ_DEV int length_of(const DecodeP& p, int seq) {
+    return min(max(p.kv_len[seq], 0), min(p.max_len, p.kv.max_pages << p.kv.plog));
+}
+
+BQ_DEV void store4(const DecodeP& p, size_t at, f32x4 a) {
+    if (p.out_bf16)
+        *(u32x2*)((uint16_t*)p.out + at) = u32x2{f2bf2(a[0], a[1]), f2bf2(a[2], a[3])};
+    else
+        *(f32x4*)((float*)p.out + at) = a;
+}
+BQ_DEV f32x4 over(f32x4 a, float l) { return l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a * (1.f / l); }
 
 // four int8 codes -> bf16 (exact)
 BQ_DEV u32x2 codes_bf16(uint32_t w) {
@@ -73,20 +98,20 @@ BQ_DEV float groups_sum(float v) {
 
 // NQ bf16 parts of q, NP of a softmax weight
 template <int D, int KV, int NQ, int NP>
-__global__ void __launch_bounds__(256, 2) k_attn_decode(DecodeP p) {
+__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p) {
     constexpr int KS = D / 32, DT = D / 16;
     __shared__ int s_page[kRound * 2];
-    __shared__ __attribute__((aligned(16))) float s_o[kWaves][16][D + 4];
+    __shared__ __attribute__((aligned16)) float s_o[kWaves][16][D + 4];
     __shared__ float s_m[kWaves][16], s_l[kWaves][16], s_mt[16], s_lt[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const KvView& kv = p.kv;
     const int seq = blockIdx.z, h = blockIdx.y % kv.heads, qt = blockIdx.y / kv.heads;
-    const int len = min(max(p.kv_len[seq], 0), min(p.max_len, kv.max_pages << kv.plog));
+    const int len = length_of(p, seq);
 
-    // the lane's query row: new token i, head hg of the group
+    // the lane's query row: new token i, head r % G of the group
     const int M = p.rows * p.G, first = qt * 16, last = min(M, first + 16) - 1;
-    const int r = min(first + c, last), i = r / p.G;
-    const int pos = len - p.rows + i, pfirst = len - p.rows + first / p.G, plast = len - p.rows + last / p.G;
+    const int pfirst = len - p.rows + first / p.G, plast = len - p.rows + last / p.G;
+    const int r = min(first + c, last), i = r / p.G, pos = len - p.rows + i;
     bf16x8 q[NQ][KS];
     {
         const size_t at = (size_t)(seq * p.rows + i) * p.ldq + (size_t)(h * p.G + r % p.G) * D + 8 * g;
@@ -109,23 +134,18 @@ __global__ void __launch_bounds__(256, 2) k_attn_decode(DecodeP p) {
                 for (int e = 0; e < 8; ++e)
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) {
-                        const __bf16 t = (__bf16)x[e];
-                        q[n][k][e] = t;
-                        x[e] -= (float)t;
+                        const __bf16 y = (__bf16)x[e];
+                        q[n][k][e] = y;
+                        x[e] -= (float)y;
                     }
             }
         }
     }
 
-    // the tokens any of the tile's rows sees, in 32-token steps: the sinks'
-    // steps [0, ns), then [lo_step, end_step)
-    const int end = plast + 1;
-    const int lo = p.window ? max(0, pfirst - p.window + 1) : 0;
-    const int lo_step = lo >> 5, end_step = end > 0 ? (end + 31) >> 5 : 0;
-    const int ns = p.window ? min(lo_step, (p.sinks + 31) >> 5) : 0;
-    const int n = end > 0 ? ns + end_step - lo_step : 0;
+    const Steps st = steps_of(p, pfirst, plast);
+    const int end = plast + 1, lo = st.lo, n = st.n;
     const int per = (n + p.nsplit - 1) / p.nsplit;
-    const int v0 = blockIdx.x * per, v1 = min(n, v0 + per);
+    const int v0 = min(n, (int)blockIdx.x * per), v1 = min(n, v0 + per);
 
     f32x4 o[DT];
 #pragma unroll
@@ -138,12 +158,12 @@ __global__ void __launch_bounds__(256, 2) k_attn_decode(DecodeP p) {
         const int cnt = min(kRound, v1 - vr);
         __syncthreads();
         for (int e = tid; e < cnt << (half_pages ? 1 : 0); e += 256) {
-            const int v = vr + (half_pages ? e >> 1 : e), ts = v < ns ? v : v - ns + lo_step;
+            const int v = vr + (half_pages ? e >> 1 : e), ts = v < st.ns ? v : v - st.ns + st.lo_step;
             s_page[e] = kv_page(kv, seq, ts * 32 + (half_pages ? (e & 1) * 16 : 0));
         }
         __syncthreads();
         for (int w = wave; w < cnt; w += kWaves) {
-            const int v = vr + w, ts = v < ns ? v : v - ns + lo_step, t0 = ts * 32;
+            const int v = vr + w, ts = v < st.ns ? v : v - st.ns + st.lo_step, t0 = ts * 32;
             // keys: lane row c holds token 8 (c / 4) + c % 4 (+ 4 in the second tile); values: tokens 8g..
             const int gk = c >> 2;
             const int pk = half_pages ? s_page[2 * w + (gk >> 1)] : s_page[w], pv = half_pages ? s_page[2 * w + (g >> 1)] : s_page[w];
@@ -151,58 +171,78 @@ __global__ void __launch_bounds__(256, 2) k_attn_decode(DecodeP p) {
             const int tk = ib + 8 * (half_pages ? gk & 1 : gk) + (c & 3), tv = ib + 8 * (half_pages ? g & 1 : g);
             const char* bk = kv.pages + (size_t)max(pk, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
             const char* bv = kv.pages + (size_t)max(pv, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
-            f32x4 s[2];
-            if constexpr (KV == kKvBf16) {
-                bf16x8 kf[2][KS];
+            // every load of the step first: the values' arrive during the scores
+            constexpr bool Q8 = KV == kKvQ8;
+            u32x4 kf[2][Q8 ? KS / 2 : KS], vf[Q8 ? DT / 2 : DT], ksc[Q8 ? KS : 1], vsc[Q8 ? KS : 1];
+            if constexpr (!Q8) {
 #pragma unroll
                 for (int k = 0; k < KS; ++k)
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) kf[t][k] = *(const bf16x8*)(bk + kv_k_unit(P, 4 * k + g, tk + 4 * t));
+                    for (int t = 0; t < 2; ++t) kf[t][k] = *(const u32x4*)(bk + kv_k_unit(P, 4 * k + g, tk + 4 * t));
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < KS; ++k)
-#pragma unroll
-                        for (int a = NQ - 1; a >= 0; --a) s[t] = mfma16(kf[t][k], q[a][k], s[t]);
-                }
+                for (int d = 0; d < DT; ++d) vf[d] = *(const u32x4*)(bv + kv_v_unit(P, D, tv >> 3, 16 * d + c));
             } else {
-                u32x4 kf[2][KS / 2], sc[KS];
 #pragma unroll
                 for (int k = 0; k < KS / 2; ++k)
 #pragma unroll
                     for (int t = 0; t < 2; ++t) kf[t][k] = *(const u32x4*)(bk + kv_kq_unit(P, k, g, tk + 4 * t));
 #pragma unroll
-                for (int k = 0; k < KS; ++k) sc[k] = *(const u32x4*)(bv + kv_ks_off(P, D, k, tv));
+                for (int k = 0; k < KS; ++k) ksc[k] = *(const u32x4*)(bv + kv_ks_off(P, D, k, tv));
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int d = 0; d < DT / 2; ++d) vf[d] = *(const u32x4*)(bv + kv_vq_unit(P, D, tv >> 3, d, c));
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) {
-                        const bf16x8 kb = codes8(kf[t][k / 2][2 * (k & 1)], kf[t][k / 2][2 * (k & 1) + 1]);
+                for (int d = 0; d < DT / 2; ++d) vsc[d] = *(const u32x4*)(bv + kv_vs_off(P, D, d, tv));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    if constexpr (!Q8) {
+                        const bf16x8 kb = __builtin_bit_cast(bf16x8, kf[y][k]);
+#pragma unroll
+                        for (int a = NQ - 1; a >= 0; --a) s[y] = mfma16(kb, q[a][k], s[y]);
+                    } else {
+                        const bf16x8 kb = codes8(kf[y][k / 2][2 * (k & 1)], kf[y][k / 2][2 * (k & 1) + 1]);
+                        const uint32_t a0 = ksc[k][2 * y], a1 = ksc[k][2 * y + 1];
+                        const f32x4 sc = {as_float(a0 << 16), as_float(a0 & 0xFFFF0000u), as_float(a1 << 16), as_float(a1 & 0xFFFF0000u)};
                         f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int a = NQ - 1; a >= 0; --a) x = mfma16(kb, q[a][k], x);
-                        const uint32_t a = sc[k][2 * t], b = sc[k][2 * t + 1];
-                        s[t] += x * f32x4{as_float(a << 16), as_float(a & 0xFFFF0000u), as_float(b << 16), as_float(b & 0xFFFF0000u)};
+                        s[y] += x * sc;
                     }
                 }
-            }
-            // scores of tokens t0 + 8g + 4t + e for the lane's query row
+            // scores of tokens t0 + 8g + 4y + e for the lane's query rows
             const bool edge = t0 + 31 > pfirst || (p.window && t0 <= plast - p.window && t0 + 32 > p.sinks) || __any(pv < 0);
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * p.scale;
-            uint32_t seen = 0xFF;  // tokens any row of the tile sees (their values are read)
+            uint32_t seen = 0xFF;  // tokens any row of the tiles sees (their values are read)
             if (edge) {
                 seen = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int t = t0 + 8 * g + e;
-                    const bool me = pv >= 0 && t <= pos && (!p.window || t > pos - p.window || t < p.sinks);
-                    const bool any = pv >= 0 && t < end && (t >= lo || t < p.sinks);
-                    x[e] = me ? x[e] : -INFINITY;
+                    const int tok = t0 + 8 * g + e;
+                    const bool any = pv >= 0 && tok < end && (tok >= lo || tok < p.sinks);
                     seen |= any ? 1u << e : 0u;
+                }
+                // what no row sees may hold anything: its products must not
+                if constexpr (!Q8) {
+                    u32x4 mask;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        mask[e] = (seen >> (2 * e) & 1 ? 0xFFFFu : 0u) | (seen >> (2 * e + 1) & 1 ? 0xFFFF0000u : 0u);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) vf[d] &= mask;
+                }
+            }
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * p.scale;
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int tok = t0 + 8 * g + e;
+                    const bool me = pv >= 0 && tok <= pos && (!p.window || tok > pos - p.window || tok < p.sinks);
+                    x[e] = me ? x[e] : -INFINITY;
                 }
             }
             float mx = x[0];
@@ -227,51 +267,34 @@ __global__ void __launch_bounds__(256, 2) k_attn_decode(DecodeP p) {
                     float z = y[e];
 #pragma unroll
                     for (int a = 0; a < NP; ++a) {
-                        const __bf16 t = (__bf16)z;
-                        pp[a][e] = t;
-                        z -= (float)t;
+                        const __bf16 w = (__bf16)z;
+                        pp[a][e] = w;
+                        z -= (float)w;
                     }
                 }
             };
-            if constexpr (KV == kKvBf16) {
-                bf16x8 vf[DT];
-#pragma unroll
-                for (int d = 0; d < DT; ++d) vf[d] = *(const bf16x8*)(bv + kv_v_unit(P, D, tv >> 3, 16 * d + c));
-                if (edge) {
-                    // what no row sees may hold anything: its products must not
-                    u32x4 mask;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        mask[e] = (seen >> (2 * e) & 1 ? 0xFFFFu : 0u) | (seen >> (2 * e + 1) & 1 ? 0xFFFF0000u : 0u);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) vf[d] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, vf[d]) & mask);
-                }
-                bf16x8 pp[NP];
+            bf16x8 pp[NP];
+            if constexpr (!Q8) {
                 parts(x, pp);
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int a = NP - 1; a >= 0; --a) o[d] = mfma16(vf[d], pp[a], o[d]);
+                    for (int a = NP - 1; a >= 0; --a) o[d] = mfma16(__builtin_bit_cast(bf16x8, vf[d]), pp[a], o[d]);
             } else {
-                u32x4 vf[DT / 2], sc[DT / 2];
-#pragma unroll
-                for (int d = 0; d < DT / 2; ++d) vf[d] = *(const u32x4*)(bv + kv_vq_unit(P, D, tv >> 3, d, c));
-#pragma unroll
-                for (int d = 0; d < DT / 2; ++d) sc[d] = *(const u32x4*)(bv + kv_vs_off(P, D, d, tv));
 #pragma unroll
                 for (int d = 0; d < DT / 2; ++d) {
                     float y[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float vs = as_float(e & 1 ? sc[d][e >> 1] & 0xFFFF0000u : sc[d][e >> 1] << 16);
+                        const float vs = as_float(e & 1 ? vsc[d][e >> 1] & 0xFFFF0000u : vsc[d][e >> 1] << 16);
                         y[e] = x[e] * (edge && !(seen >> e & 1) ? 0.f : vs);  // codes are finite, an unseen scale may not be
                     }
-                    bf16x8 pp[NP];
                     parts(y, pp);
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int a = NP - 1; a >= 0; --a) o[2 * d + u] = mfma16(codes8(vf[d][2 * u], vf[d][2 * u + 1]), pp[a], o[2 * d + u]);
+                        for (int a = NP - 1; a >= 0; --a)
+                            o[2 * d + u] = mfma16(codes8(vf[d][2 * u], vf[d][2 * u + 1]), pp[a], o[2 * d + u]);
                 }
             }
         }
@@ -297,60 +320,50 @@ __global__ void __launch_bounds__(256, 2) k_attn_decode(DecodeP p) {
         s_lt[c] = lt;
     }
     __syncthreads();
-    const size_t tile = ((size_t)seq * p.tiles + blockIdx.y) * p.nsplit + blockIdx.x;
+    const size_t piece = ((size_t)seq * p.tiles + blockIdx.y) * p.nsplit + blockIdx.x;
     for (int e = tid; e < 16 * (D / 4); e += 256) {
-        const int row = e / (D / 4), d = e % (D / 4) * 4;
-        if (first + row > last) continue;
+        const int row = e / (D / 4), d = e % (D / 4) * 4, r = first + row;
+        if (r > last) continue;
         f32x4 a = *(const f32x4*)&s_o[0][row][d];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) a += *(const f32x4*)&s_o[w][row][d];
-        const float lr = s_lt[row];
         if (p.nsplit > 1) {
-            *(f32x4*)(p.part + (tile * 16 + row) * D + d) = a;
+            const size_t at = piece * 16 + row;
+            *(f32x4*)(p.part + at * D + d) = a;
             if (d == 0) {
-                p.part[p.ml + (tile * 16 + row) * 2] = s_mt[row];
-                p.part[p.ml + (tile * 16 + row) * 2 + 1] = lr;
+                p.part[p.ml + at * 2] = s_mt[row];
+                p.part[p.ml + at * 2 + 1] = s_lt[row];
             }
         } else {
-            const int rr = first + row;
-            const size_t at = (size_t)(seq * p.rows + rr / p.G) * p.ldo + (size_t)(h * p.G + rr % p.G) * D + d;
-            const float inv = lr == 0.f ? 0.f : 1.f / lr;
-            a = a * inv;
-            if (lr == 0.f) a = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (p.out_bf16)
-                *(u32x2*)((uint16_t*)p.out + at) = u32x2{f2bf2(a[0], a[1]), f2bf2(a[2], a[3])};
-            else
-                *(f32x4*)((float*)p.out + at) = a;
+            store4(p, (size_t)(seq * p.rows + r / p.G) * p.ldo + (size_t)(h * p.G + r % p.G) * D + d, over(a, s_lt[row]));
         }
     }
 }
 
-// joins the splits of one query row: D / 4 lanes per split, the splits dealt
-// over the rest of the workgroup, summed in a fixed order
-template <int D>
-__global__ void __launch_bounds__(256) k_attn_join(DecodeP p) {
-    constexpr int L = D / 4, S = 256 / L;
-    __shared__ __attribute__((aligned(16))) float s_o[S][D];
-    __shared__ float s_l[S], s_mx[4];
+// joins the pieces of one query row: D / 4 lanes per piece, the pieces dealt
+// over the rest of the workgroup's T lanes, in a fixed order
+template <int D, int T>
+__global__ void __launch_bounds__(T) k_attn_join(DecodeP p) {
+    constexpr int L = D / 4, S = T / L;
+    __shared__ __attribute__((aligned16)) float s_o[S][D];
+    __shared__ float s_l[S], s_mx[T / 64];
     const int ht = p.kv.heads, tid = threadIdx.x;
     const int row = blockIdx.x, h = blockIdx.y, seq = blockIdx.z;
-    const size_t tile = ((size_t)seq * p.tiles + (size_t)(row / 16) * ht + h) * p.nsplit;
-    const float* ml = p.part + p.ml;
+    const size_t tile = (size_t)seq * p.tiles + (size_t)(row / 16) * ht + h, at0 = tile * p.nsplit * 16 + row % 16;
+    const float* ml = p.part + p.ml + at0 * 2;
     float mt = kNone;
-    for (int s = tid; s < p.nsplit; s += 256) mt = fmaxf(mt, ml[((tile + s) * 16 + row % 16) * 2]);
+    for (int s = tid; s < p.nsplit; s += T) mt = fmaxf(mt, ml[s * 32]);
     for (int d = 1; d < 64; d <<= 1) mt = fmaxf(mt, __shfl_xor(mt, d, 64));
     if ((tid & 63) == 0) s_mx[tid >> 6] = mt;
     __syncthreads();
-    mt = fmaxf(fmaxf(s_mx[0], s_mx[1]), fmaxf(s_mx[2], s_mx[3]));
+    for (int w = 0; w < T / 64; ++w) mt = fmaxf(mt, s_mx[w]);
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
     float lt = 0.f;
 #pragma unroll 4
     for (int s = tid / L; s < p.nsplit; s += S) {
-        const size_t at = (tile + s) * 16 + row % 16;
-        const float l = ml[at * 2 + 1];
-        if (l == 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(ml[at * 2] - mt);
-        a += *(const f32x4*)(p.part + at * D + tid % L * 4) * f;
+        const float l = ml[s * 32 + 1];
+        const float f = __builtin_amdgcn_exp2f(ml[s * 32] - mt);
+        a += *(const f32x4*)(p.part + (at0 + (size_t)s * 16) * D + tid % L * 4) * f;
         lt += l * f;
     }
     *(f32x4*)&s_o[tid / L][tid % L * 4] = a;
@@ -361,12 +374,7 @@ __global__ void __launch_bounds__(256) k_attn_join(DecodeP p) {
         a += *(const f32x4*)&s_o[s][tid * 4];
         lt += s_l[s];
     }
-    a = lt == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a * (1.f / lt);
-    const size_t at = (size_t)(seq * p.rows + row / p.G) * p.ldo + (size_t)(h * p.G + row % p.G) * D + tid * 4;
-    if (p.out_bf16)
-        *(u32x2*)((uint16_t*)p.out + at) = u32x2{f2bf2(a[0], a[1]), f2bf2(a[2], a[3])};
-    else
-        *(f32x4*)((float*)p.out + at) = a;
+    store4(p, (size_t)(seq * p.rows + row / p.G) * p.ldo + (size_t)(h * p.G + row % p.G) * D + tid * 4, over(a, lt));
 }
 
 template <int D, int KV>
@@ -379,14 +387,24 @@ hipError_t launch_decode_of(const DecodeP& p, hipStream_t st) {
     if (p.nsplit > 1) {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        launch_kernel((k_attn_join<D>), dim3(p.rows * p.G, p.kv.heads, p.kv.n_seq), dim3(256), 0, st, p);
+        // more than 32 pieces keep 1024 lanes busy; fewer leave them idle
+        const dim3 rows(p.rows * p.G, p.kv.heads, p.kv.n_seq);
+        if (p.nsplit > 32)
+            launch_kernel((k_attn_join<D, 1024>), rows, dim3(1024), 0, st, p);
+        else
+            launch_kernel((k_attn_join<D, 256>), rows, dim3(256), 0, st, p);
     }
     return hipGetLastError();
 }
+// 16-row tiles of a key-value head's query rows, each a workgroup of its own:
+// a wave with two tiles on the same tokens reads them once, but half as many
+// waves read (8 sequences x 8 rows of 8 heads over 9001 tokens: 49 us with two,
+// 43 us with one)
 int q_tiles(int rows, int G) { return (rows * G + 15) / 16; }
 }  // namespace
 
-// two workgroups per CU, each wave at least one 32-token step
+// Pieces that one sequence's tokens are cut into: two workgroups per CU, each
+// wave at least one 32-token step
 int decode_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus) {
     const int64_t tiles = (int64_t)n_seq * kv_heads * q_tiles(rows, q_heads / kv_heads);
     const int64_t steps = ((int64_t)max_len + 31) / 32;

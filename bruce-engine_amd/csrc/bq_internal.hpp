@@ -58,6 +58,8 @@ ScaledCopy& next_scaled_copy();
 int gemv_gate_den_fused(float* y, const void* w_raw, int K, int N, const float* a, const float* den, void* st);
 // CU count of the current device (set by the entry point's init; 256 before any)
 int device_cus();
+// that init by itself: BQ_OK, or the code to return
+int device_ready();
 
 template <typename F, typename... Args>
 inline void launch_kernel(F kernel, dim3 grid, dim3 block, size_t lds, hipStream_t st, Args... args) {
@@ -141,7 +143,7 @@ hipError_t launch_kv_read(const KvView& kv, int type, const int32_t* seq, const 
 // attention over it.  decode_splits: workgroups a sequence and head's tokens
 // are split over when the workspace allows it
 int decode_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus);
-size_t decode_part_floats(int n_seq, int rows, int q_heads, int kv_heads, int D);  // workspace of one split
+size_t decode_part_floats(int n_seq, int rows, int q_heads, int kv_heads, int D);  // workspace of one piece each
 hipError_t launch_attn_decode(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st);
 hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, hipStream_t st);
 

@@ -18,7 +18,7 @@
 namespace bq {
 
 namespace {
-constexpr int kRowsPerBlock = 16;
+constexpr int kFewRows = 1024;
 
 struct AppendP {
     KvView kv;
@@ -51,14 +51,14 @@ BQ_DEV bool quad_offsets(const AppendP& p, int j, int& oa, int& ob) {
     return false;
 }
 
-// the lane's quads of one head: loaded, normed (w != NULL), rotated (turn)
+// the lane's quads of one head, normed (w != NULL) and rotated (turn)
 template <int D>
-BQ_DEV void load_head(const AppendP& p, const float* src, const float* w, bool live, bool turn, int pos, int oa, int ob,
-                      int j, f32x4& a, f32x4& b) {
-    a = b = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (live) {
-        a = *(const f32x4*)(src + oa);
-        b = *(const f32x4*)(src + ob);
+BQ_DEV void norm_turn(const AppendP& p, const float* w, bool turn, int pos, int oa, int ob, int j, f32x4& a, f32x4& b) {
+    f32x4 c, s;
+    if (turn) {
+        const float* cs = p.rope + (size_t)pos * p.rot + 4 * j;
+        c = *(const f32x4*)cs;
+        s = *(const f32x4*)(cs + p.rot / 2);
     }
     if (w) {
         float ss = 0.f;
@@ -71,9 +71,7 @@ BQ_DEV void load_head(const AppendP& p, const float* src, const float* w, bool l
         a = a * k * wa;
         b = b * k * wb;
     }
-    if (turn && live) {
-        const float* cs = p.rope + (size_t)pos * p.rot + 4 * j;
-        const f32x4 c = *(const f32x4*)cs, s = *(const f32x4*)(cs + p.rot / 2);
+    if (turn) {
         if (p.interleaved) {
             const f32x4 x = a, y = b;
             a = f32x4{x[0] * c[0] - x[1] * s[0], x[1] * c[0] + x[0] * s[0], x[2] * c[1] - x[3] * s[1], x[3] * c[1] + x[2] * s[1]};
@@ -98,11 +96,10 @@ BQ_DEV uint32_t code_of(float x, float inv) {
     return (uint32_t)(int)rintf(c) & 0xFF;
 }
 
-template <int D, int KV>
+template <int D, int KV, int R>
 __global__ void __launch_bounds__(256) k_append(AppendP p) {
     constexpr int L = D / 8;          // lanes of a head
     constexpr int UPB = 256 / L;      // heads a workgroup takes at a time
-    constexpr int R = kRowsPerBlock;
     constexpr int PD = D + 4;
     __shared__ __attribute__((aligned(16))) float rowv[2][R][PD];
     __shared__ int s_page[R], s_tok[R], s_run[R];
@@ -114,12 +111,13 @@ __global__ void __launch_bounds__(256) k_append(AppendP p) {
     if ((int)blockIdx.x >= p.kv_blocks) {  // queries
         const int64_t unit = (int64_t)(blockIdx.x - p.kv_blocks) * UPB + u;
         const int row = (int)(unit / p.q_heads), h = (int)(unit % p.q_heads);
-        const bool in = row < p.rows;
-        const int pos = in ? p.pos[row] : -1;
-        const bool live = in && pos >= 0 && pos < p.n_pos && (p.seq ? (unsigned)p.seq[row] < (unsigned)p.kv.n_seq : true);
-        f32x4 a, b;
-        load_head<D>(p, p.x[0] + (in ? row : 0) * p.ld[0] + (size_t)h * D, p.w[0], live, turn, pos, oa, ob, j, a, b);
-        if (!in) return;
+        if (row >= p.rows) return;  // all lanes of a head together
+        const float* src = p.x[0] + row * p.ld[0] + (size_t)h * D;
+        f32x4 a = *(const f32x4*)(src + oa), b = *(const f32x4*)(src + ob);
+        const int pos = p.pos[row];
+        const bool live = pos >= 0 && pos < p.n_pos && (p.seq ? (unsigned)p.seq[row] < (unsigned)p.kv.n_seq : true);
+        norm_turn<D>(p, p.w[0], turn && live, pos, oa, ob, j, a, b);
+        if (!live) a = b = f32x4{0.f, 0.f, 0.f, 0.f};
         const size_t o = ((size_t)row * p.q_heads + h) * D;
         if (p.q_bf16) {
             uint16_t* q = (uint16_t*)p.q_out + o;
@@ -136,6 +134,19 @@ __global__ void __launch_bounds__(256) k_append(AppendP p) {
     // keys and values: R rows of one head
     const KvView& kv = p.kv;
     const int h = blockIdx.x % kv.heads, r0 = (int)(blockIdx.x / kv.heads) * R;
+    // rows 0..R-1 of keys, then of values, before the pages they go to are known
+    constexpr int N = (2 * R + UPB - 1) / UPB;
+    f32x4 xa[N], xb[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const int i = u + e * UPB, which = i / R, row = r0 + i % R;
+        xa[e] = xb[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (i < 2 * R && row < p.rows) {
+            const float* src = p.x[1 + which] + row * p.ld[1 + which] + (size_t)h * D;
+            xa[e] = *(const f32x4*)(src + oa);
+            xb[e] = *(const f32x4*)(src + ob);
+        }
+    }
     if (tid < R) {
         const int row = r0 + tid;
         int page = -1, tok = -1;
@@ -158,15 +169,16 @@ __global__ void __launch_bounds__(256) k_append(AppendP p) {
         }
         s_run[tid] = run;
     }
-    for (int i = u; i < 2 * R; i += UPB) {
-        const int which = i / R, r = i % R;
-        const bool live = s_page[r] >= 0;
-        const int pos = live ? p.pos[r0 + r] : 0;
-        f32x4 a, b;
-        load_head<D>(p, p.x[1 + which] + (live ? r0 + r : 0) * p.ld[1 + which] + (size_t)h * D, which ? nullptr : p.w[1], live,
-                     turn && which == 0, pos, oa, ob, j, a, b);
-        *(f32x4*)&rowv[which][r][oa] = a;
-        *(f32x4*)&rowv[which][r][ob] = b;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const int i = u + e * UPB, which = i / R, r = i % R;
+        if (i >= 2 * R) break;
+        if (which == 0) {
+            const int pos = r0 + r < p.rows ? p.pos[r0 + r] : -1;
+            norm_turn<D>(p, p.w[1], turn && pos >= 0 && pos < p.n_pos, pos, oa, ob, j, xa[e], xb[e]);
+        }
+        *(f32x4*)&rowv[which][r][oa] = xa[e];
+        *(f32x4*)&rowv[which][r][ob] = xb[e];
     }
     __syncthreads();
     auto head_at = [&](int r) { return kv.pages + (size_t)s_page[r] * kv.page_bytes + (size_t)h * kv.head_bytes; };
@@ -288,10 +300,20 @@ __global__ void __launch_bounds__(256) k_kv_read(KvView kv, const int32_t* seq, 
 }
 
 template <int D, int KV>
-hipError_t launch_append_of(const AppendP& p, hipStream_t st) {
+hipError_t launch_append_of(AppendP p, hipStream_t st) {
     constexpr int upb = 256 / (D / 8);
     const int64_t qb = ((int64_t)p.rows * p.q_heads + upb - 1) / upb;
-    launch_kernel((k_append<D, KV>), dim3((uint32_t)(p.kv_blocks + qb)), dim3(256), 0, st, p);
+    // 16 rows of a head per workgroup make whole units of a prompt's values;
+    // four end sooner where the GPU is not full (32 + 2 x 4 heads of 128, rows
+    // of 16 / of 4 per workgroup: 1 row 4.8 / 4.0 us, 256 rows 7.4 / 4.8,
+    // 2048 rows 14.1 / 16.5, 8192 rows 50 / 52)
+    const bool few = p.rows <= kFewRows;
+    p.kv_blocks = (p.rows + (few ? 3 : 15)) / (few ? 4 : 16) * p.kv.heads;
+    const dim3 grid((uint32_t)(p.kv_blocks + qb));
+    if (few)
+        launch_kernel((k_append<D, KV, 4>), grid, dim3(256), 0, st, p);
+    else
+        launch_kernel((k_append<D, KV, 16>), grid, dim3(256), 0, st, p);
     return hipGetLastError();
 }
 }  // namespace
@@ -305,7 +327,6 @@ hipError_t launch_append(const KvView& kv, int type, const bq_append_args& a, hi
     p.pos = a.pos; p.seq = a.seq; p.rope = a.rope; p.q_out = a.q_out; p.eps = a.eps;
     p.rows = a.rows; p.q_heads = a.q_heads; p.rot = a.rot; p.n_pos = a.n_pos; p.interleaved = a.interleaved != 0;
     p.q_bf16 = a.q_type == BQ_TYPE_BF16;
-    p.kv_blocks = (a.rows + kRowsPerBlock - 1) / kRowsPerBlock * kv.heads;
     const bool q8 = type == kKvQ8;
     switch (kv.D) {
         case 64: return q8 ? launch_append_of<64, kKvQ8>(p, st) : launch_append_of<64, kKvBf16>(p, st);

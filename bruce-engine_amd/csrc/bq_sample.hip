@@ -3,11 +3,11 @@
 //
 // Kept tokens are a run of the row sorted by logit, so only the row's head has
 // to be sorted.  Two launches:
-//   k_sample_scan, one workgroup per 8192 logits: reads them once (the floor:
+//   k_sample_scan, one workgroup per 4096 logits: reads them once (the floor:
 //     4 bytes a logit), keeps the head of its slice -- every logit not below a
-//     threshold t, the slice's 256 threads' maxima put in order and one of them
-//     taken, which leaves about 768 candidates for the whole row -- and, where
-//     top-p needs the row's mass, its sum of exponentials.
+//     threshold t, taken from the lanes' maxima in order, which leaves about 448
+//     candidates for the whole row -- and, where top-p needs the row's mass, its
+//     sum of exponentials.
 //   k_sample_pick, one workgroup per row: sorts the candidates, takes their
 //     running mass and cuts it.  All tokens of the row not below the largest t
 //     are among the candidates, so a cut that falls there is exact.  Where it
@@ -28,9 +28,10 @@
 namespace bq {
 
 namespace {
-constexpr int kSlice = 8192;
+constexpr int kSlice = 4096;
+constexpr int kMaxSlices = 256;
 constexpr int kMaxCand = 1024;
-constexpr int kWant = 768;  // candidates wanted of a row
+constexpr int kWant = 448;  // candidates wanted of a row
 typedef unsigned long long u64;
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any logit
 
@@ -75,6 +76,34 @@ BQ_DEV u64 shfl_up64(u64 v, int d) {
     return (u64)hi << 32 | lo;
 }
 
+// the value of lane ^ J (J < 64), without LDS
+template <int J>
+BQ_DEV uint32_t lane_xor(uint32_t v) {
+    if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false);  // quad_perm [1,0,3,2]
+    if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);  // quad_perm [2,3,0,1]
+    if constexpr (J == 4) {  // row_half_mirror is ^7, quad_perm [3,2,1,0] ^3
+        return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, false), 0x1B, 0xF, 0xF, false);
+    }
+    if constexpr (J == 8) {  // row_mirror is ^15
+        return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, false), 0x141, 0xF, 0xF, false);
+    }
+    if constexpr (J == 16) {  // both rows of a pair: [0] holds the even rows' values, [1] the odd rows'
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? r[0] : r[1];
+    }
+    if constexpr (J == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return threadIdx.x & 32 ? r[0] : r[1];
+    }
+}
+// one exchange of a bitonic network: the larger of the pair stays in the lower lane if `down`
+template <int J>
+BQ_DEV u64 exchange(u64 key, bool down) {
+    const u64 o = (u64)lane_xor<J>((uint32_t)(key >> 32)) << 32 | lane_xor<J>((uint32_t)key);
+    const bool larger = down == ((threadIdx.x & J) == 0);
+    return larger == (o > key) ? o : key;
+}
+
 struct RowRule {
     float temp, top_p, min_p;
     int top_k;  // vocab: all
@@ -91,18 +120,25 @@ BQ_DEV RowRule rule_of(const SampleP& p, int row) {
     return r;
 }
 
+// the wave's maximum, in every lane
+BQ_DEV float wave_max(float v) {
+    v = fmaxf(v, dpp_f<0xB1, 0xF, true>(v));   // quad_perm [1,0,3,2]
+    v = fmaxf(v, dpp_f<0x4E, 0xF, true>(v));   // quad_perm [2,3,0,1]
+    v = fmaxf(v, dpp_f<0x141, 0xF, true>(v));  // row_half_mirror
+    v = fmaxf(v, dpp_f<0x140, 0xF, true>(v));  // row_mirror
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
 __global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
     constexpr int V = kSlice / 1024;  // 16-byte loads of a thread
-    __shared__ float s_max[256];
-    __shared__ u64 s_best[4];
-    __shared__ float s_sum[4], s_t;
-    __shared__ int s_count;
-    const int tid = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
+    __shared__ float s_max[4], s_t[4], s_sum[4];
+    __shared__ int s_count[4], s_at[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slice = blockIdx.x, row = blockIdx.y;
     const float* x = p.logits + (size_t)row * p.ld;
-    const RowRule rule = rule_of(p, row);
     // the slice's k-th run of four waves' blocks: block (4k + wave) * slices + slice
     float v[V][4];
-    auto at = [&](int k) { return ((4 * k + (tid >> 6)) * p.slices + slice) * 256 + (tid & 63) * 4; };
+    auto at = [&](int k) { return ((4 * k + wave) * p.slices + slice) * 256 + lane * 4; };
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         const int i = at(k);
@@ -116,68 +152,84 @@ __global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[k][e] = clean(a[e]);
     }
-    u64 best = 0;
+    const RowRule rule = rule_of(p, row);
+    float mine = v[0][0];
 #pragma unroll
     for (int k = 0; k < V; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const u64 key = key_of(v[k][e], at(k) + e);
-            best = key > best ? key : best;
-        }
-    const float mine = unordered((uint32_t)(best >> 32));
-    s_max[tid] = mine;
-    if (tid == 0) s_count = 0;
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = shfl_xor64(best, d);
-        best = o > best ? o : best;
-    }
-    if ((tid & 63) == 0) s_best[tid >> 6] = best;
-    __syncthreads();
-    best = s_best[0];
-    for (int w = 1; w < 4; ++w) best = s_best[w] > best ? s_best[w] : best;
-    SliceInfo* info = p.info + (size_t)row * p.slices + slice;
-    if (rule.greedy) {
-        if (tid == 0) info->best = best;
-        return;
-    }
-    // the thread whose maximum is the rank-th gives the threshold
-    int ahead = 0;
-    for (int i = 0; i < 256; i += 4) {
-        const f32x4 a = *(const f32x4*)(s_max + i);
+        for (int e = 0; e < 4; ++e) mine = fmaxf(mine, v[k][e]);
+    // the wave's threshold: the largest 16-bit prefix of the ordered bits that
+    // more than `rank` of its lanes' maxima reach (a lower value than the
+    // maximum itself is as good)
+    uint32_t cut = 0;
+    const uint32_t om = ordered(mine);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ahead += a[e] > mine || (a[e] == mine && i + e < tid);
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t c = cut | 1u << bit;
+        if (__popcll(__ballot(om >= c)) > p.rank) cut = c;
     }
-    if (ahead == p.rank) s_t = mine;
-    float sum = 0.f;
+    const float wmax = wave_max(mine);
+    if (lane == 0) {
+        s_t[wave] = cut < 0x00800000u ? -INFINITY : unordered(cut);  // below the lowest finite logit: all of them
+        s_max[wave] = wmax;
+    }
+    __syncthreads();
+    const float mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    const float t = fmaxf(fmaxf(s_t[0], s_t[1]), fmaxf(s_t[2], s_t[3]));
+    const float least = fmaxf(t, -3.402823466e38f);  // -inf is no candidate
+    int count = 0, first = 0x7FFFFFFF;
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) count += __popcll(__ballot(v[k][e] >= least));
+    if (__any(mine == mx)) {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (v[k][e] == mx) first = min(first, at(k) + e);
+        for (int d = 1; d < 64; d <<= 1) first = min(first, __shfl_xor(first, d, 64));
+    }
+    if (lane == 0) {
+        s_count[wave] = count;
+        s_at[wave] = first;
+    }
     if (rule.top_p < 1.f && rule.top_k == p.vocab) {
-        const float mx = unordered((uint32_t)(best >> 32));
+        float sum = 0.f;
         if (mx > -INFINITY && mx < INFINITY) {
+            const float inv = 1.44269504088896341f / rule.temp;
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum += expf((v[k][e] - mx) / rule.temp);
+                for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f((v[k][e] - mx) * inv);
         }
         sum = wave_sum_dpp63(sum);
-        if ((tid & 63) == 63) s_sum[tid >> 6] = sum;
+        if (lane == 63) s_sum[wave] = sum;
     }
     __syncthreads();
-    const float t = s_t;
-    u64* cand = p.cand + ((size_t)row * p.slices + slice) * p.cap;
+    const int total = s_count[0] + s_count[1] + s_count[2] + s_count[3];
+    const bool over = total > p.cap;
+    if (!over && !rule.greedy) {
+        u64* cand = p.cand + ((size_t)row * p.slices + slice) * p.cap;
+        for (int w = 0; w < wave; ++w) cand += s_count[w];
 #pragma unroll
-    for (int k = 0; k < V; ++k)
+        for (int k = 0; k < V; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (v[k][e] >= t && v[k][e] > -INFINITY) {
-                const int c = atomicAdd(&s_count, 1);
-                if (c < p.cap) cand[c] = key_of(v[k][e], at(k) + e);
+            for (int e = 0; e < 4; ++e) {
+                const bool in = v[k][e] >= least;
+                const u64 mask = __ballot(in);
+                if (mask == 0) continue;
+                if (in) cand[__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] =
+                    key_of(v[k][e], at(k) + e);
+                cand += __popcll(mask);
             }
-    __syncthreads();
+    }
     if (tid == 0) {
-        const bool over = s_count > p.cap;
-        info->best = best;
+        SliceInfo* info = p.info + (size_t)row * p.slices + slice;
+        info->best = key_of(mx, min(min(s_at[0], s_at[1]), min(s_at[2], s_at[3])));
         info->t = over ? INFINITY : t;
         info->sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-        info->count = over ? 0 : s_count;
+        info->count = over ? 0 : total;
     }
 }
 
@@ -272,17 +324,52 @@ struct Whole {
 
 __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
     __shared__ u64 s_key[kMaxCand], s_bins[2048], s_red[16], s_found[2];
-    __shared__ int s_first[129], s_stop;
+    __shared__ int s_first[kMaxSlices + 1], s_stop;
     __shared__ u64 s_best;
     __shared__ float s_t;
     __shared__ double s_mass;
     const int tid = threadIdx.x, row = blockIdx.x;
     const RowRule rule = rule_of(p, row);
     const SliceInfo* info = p.info + (size_t)row * p.slices;
-    if (tid == 0) {
+    if (tid < 64) {
+        // four slices a lane: the largest key, the largest threshold, where each slice's candidates begin
+        constexpr int N = kMaxSlices / 64;
+        SliceInfo in[N];
+        int c[N], all = 0;
         u64 best = 0;
-        for (int s = 0; s < p.slices; ++s) best = info[s].best > best ? info[s].best : best;
-        s_best = best;
+        float t = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            in[i] = SliceInfo{0, -INFINITY, 0.f, 0, 0};
+            if (N * tid + i < p.slices) in[i] = info[N * tid + i];
+            c[i] = all;
+            all += in[i].count;
+            best = in[i].best > best ? in[i].best : best;
+            t = fmaxf(t, in[i].t);
+        }
+        int before = all;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(before, d, 64);
+            if (tid >= d) before += o;
+            const u64 k = shfl_xor64(best, d);
+            best = k > best ? k : best;
+        }
+        t = wave_max(t);
+        const float mx = unordered((uint32_t)(best >> 32));
+        double mass = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (N * tid + i <= p.slices) s_first[N * tid + i] = before - all + c[i];
+            if (in[i].sum > 0.f) mass += (double)in[i].sum * (double)expf((unordered((uint32_t)(in[i].best >> 32)) - mx) / rule.temp);
+        }
+        for (int d = 1; d < 64; d <<= 1) mass += __shfl_xor(mass, d, 64);
+        if (tid == 63) s_first[p.slices] = before;
+        if (tid == 0) {
+            s_best = best;
+            s_t = t;
+            s_mass = mass * 0x1p40;
+            s_stop = kMaxCand + 1;
+        }
     }
     __syncthreads();
     const float mx = unordered((uint32_t)(s_best >> 32));
@@ -291,24 +378,6 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
         if (tid == 0) p.out[row] = index_of(s_best);
         return;
     }
-    const bool need_mass = rule.top_p < 1.f && rule.top_k == p.vocab;
-    if (tid == 0) {
-        int c = 0;
-        float t = -INFINITY;
-        double mass = 0;
-        for (int s = 0; s < p.slices; ++s) {
-            s_first[s] = c;
-            c += info[s].count;
-            t = fmaxf(t, info[s].t);
-            if (need_mass)
-                mass += (double)info[s].sum * (double)expf((unordered((uint32_t)(info[s].best >> 32)) - mx) / rule.temp);
-        }
-        s_first[p.slices] = c;
-        s_t = t;
-        s_mass = mass * 0x1p40;
-        s_stop = kMaxCand + 1;
-    }
-    __syncthreads();
     const int total = s_first[p.slices];
     const float t = s_t;
     const double u = (double)p.u[row];
@@ -326,20 +395,24 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
             key = p.cand[((size_t)row * p.slices + s) * p.cap + tid - s_first[s]];
         }
         // bitonic sort, descending, one key per thread
-        for (int k = 2; k <= n; k <<= 1)
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                u64 o;
-                if (j >= 64) {
-                    __syncthreads();
-                    s_key[tid] = key;
-                    __syncthreads();
-                    o = s_key[tid ^ j];
-                } else {
-                    o = shfl_xor64(key, j);
-                }
-                const bool larger = ((tid & k) == 0) == ((tid & j) == 0);
+        for (int k = 2; k <= n; k <<= 1) {
+            const bool down = (tid & k) == 0;
+            for (int j = k >> 1; j >= 64; j >>= 1) {
+                __syncthreads();
+                s_key[tid] = key;
+                __syncthreads();
+                const u64 o = s_key[tid ^ j];
+                const bool larger = down == ((tid & j) == 0);
                 key = larger == (o > key) ? o : key;
             }
+            if (tid >= n) continue;  // whole waves
+            if (k >= 64) key = exchange<32>(key, down);
+            if (k >= 32) key = exchange<16>(key, down);
+            if (k >= 16) key = exchange<8>(key, down);
+            if (k >= 8) key = exchange<4>(key, down);
+            if (k >= 4) key = exchange<2>(key, down);
+            key = exchange<1>(key, down);
+        }
         const float x = unordered((uint32_t)(key >> 32));
         const bool in = tid < total;
         const float e = in ? expf((x - mx) / rule.temp) : 0.f;
@@ -417,9 +490,10 @@ hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, c
     p.logits = logits; p.ld = ld; p.vocab = vocab;
     p.slices = slices_of(vocab);
     p.cap = cap_of(p.slices);
-    // of the 256 maxima of 32 logits each in random order, the rank-th leaves
-    // about 256 ln(256 / (256 - rank)) logits above it
-    p.rank = std::max(4, std::min(250, (int)(256 * (1 - std::exp(-(double)kWant / p.slices / 256)))));
+    // each wave's threshold is one of its 64 lanes' maxima of 16 logits: the
+    // rank-th leaves about 64 ln(64 / (64 - rank)) of its 1024 above it; the
+    // slice takes the largest of four
+    p.rank = std::max(2, std::min(62, (int)(64 * (1 - std::exp(-(double)kWant / p.slices / 256)))));
     p.temp = temp; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p; p.u = u; p.out = out;
     p.info = (SliceInfo*)work;
     p.cand = (u64*)(p.info + (size_t)rows * p.slices);

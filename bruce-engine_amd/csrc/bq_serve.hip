@@ -69,7 +69,7 @@ size_t bq_kv_page_bytes(int type, int kv_heads, int head_dim, int page_tokens) {
 }
 
 int bq_append(const bq_kv_cache* c, const bq_append_args* a, bq_stream_t st) {
-    if (int r = bq_init()) return r;
+    if (int r = device_ready()) return r;
     KvView kv;
     int type;
     if (int r = view_of(c, kv, type)) return r;
@@ -87,7 +87,7 @@ int bq_append(const bq_kv_cache* c, const bq_append_args* a, bq_stream_t st) {
 }
 
 int bq_kv_read(const bq_kv_cache* c, const int32_t* seq, const int32_t* pos, int rows, uint16_t* k, uint16_t* v, bq_stream_t st) {
-    if (int r = bq_init()) return r;
+    if (int r = device_ready()) return r;
     KvView kv;
     int type;
     if (int r = view_of(c, kv, type)) return r;
@@ -99,14 +99,14 @@ int bq_kv_read(const bq_kv_cache* c, const int32_t* seq, const int32_t* pos, int
 
 size_t bq_attn_workspace_bytes(int n_seq, int rows, int q_heads, int kv_heads, int head_dim, int max_len) {
     if (n_seq <= 0 || rows < 1 || rows > BQ_MAX_ROWS || kv_heads <= 0 || q_heads % kv_heads != 0 || q_heads <= 0 || head_dim <= 0 ||
-        max_len < 0 || bq_init() != BQ_OK)
+        max_len < 0 || device_ready() != BQ_OK)
         return 0;
     const int n = decode_splits(n_seq, rows, q_heads, kv_heads, max_len, device_cus());
     return n > 1 ? n * decode_part_floats(n_seq, rows, q_heads, kv_heads, head_dim) * sizeof(float) : 0;
 }
 
 int bq_attn_decode(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t st) {
-    if (int r = bq_init()) return r;
+    if (int r = device_ready()) return r;
     KvView kv;
     int type;
     if (int r = view_of(c, kv, type)) return r;
@@ -123,7 +123,7 @@ int bq_attn_decode(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t s
 }
 
 int bq_attn_prefill(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t st) {
-    if (int r = bq_init()) return r;
+    if (int r = device_ready()) return r;
     KvView kv;
     int type;
     if (int r = view_of(c, kv, type)) return r;
@@ -156,7 +156,7 @@ size_t bq_sample_workspace_bytes(int rows, int vocab) {
 
 int bq_sample(const float* logits, int64_t ld, int rows, int vocab, const float* temperature, const int32_t* top_k, const float* top_p,
               const float* min_p, const float* u, int32_t* out, void* work, size_t work_bytes, bq_stream_t st) {
-    if (int r = bq_init()) return r;
+    if (int r = device_ready()) return r;
     if (rows < 0 || vocab <= 0 || ld < vocab) return BQ_EINVAL;
     if (vocab > (1 << 20) || rows > 65535) return BQ_UNSUPPORTED;
     if (rows == 0) return BQ_OK;
