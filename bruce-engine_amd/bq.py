@@ -45,7 +45,7 @@ EXPORTS = [
     "bq_gemm_b_fused_noalloc",
     "bq_noalloc_scratch_bytes", "bq_decode_enqueue", "bq_decode_graph_create", "bq_decode_graph_launch",
     "bq_decode_graph_destroy", "bq_kv_page_bytes", "bq_append", "bq_kv_read", "bq_attn_workspace_bytes",
-    "bq_attn_decode", "bq_attn_prefill", "bq_attn_hook", "bq_sample_workspace_bytes", "bq_sample",
+    "bq_attn_prefill_workspace_bytes", "bq_attn_decode", "bq_attn_prefill", "bq_attn_hook", "bq_sample_workspace_bytes", "bq_sample",
 ]
 
 
@@ -204,6 +204,7 @@ def load(path=LIB_PATH):
         "bq_append": (I, [P, P, P]),
         "bq_kv_read": (I, [P, P, P, I, P, P, P]),
         "bq_attn_workspace_bytes": (S, [I, I, I, I, I, I]),
+        "bq_attn_prefill_workspace_bytes": (S, [I] * 7),
         "bq_attn_decode": (I, [P, P, P]),
         "bq_attn_prefill": (I, [P, P, P]),
         "bq_attn_hook": (None, [P, I, P]),
@@ -728,7 +729,7 @@ class Attention:
     """bq_attn_decode / bq_attn_prefill over fixed buffers: q and out [n_rows, q_heads * D] fp32 or bf16 (rows
     may be strided), kv_len int32 [n_seq].  For prefill() of a batch row0 int32 [n_seq + 1], max_rows the most
     rows a sequence has; for decode() every sequence has n_rows / n_seq rows.  work: a workspace tensor of the
-    caller's, "auto" for one of the object's own, None for none (decode() only)."""
+    caller's, "auto" for one of the object's own, None for none (no split)."""
 
     def __init__(self, kv, q, out, kv_len, scale=None, window=0, sinks=0, max_len=None, row0=None, max_rows=None,
                  work="auto"):
@@ -748,7 +749,12 @@ class Attention:
             rows = n_rows // n_seq
         L = load()
         if isinstance(work, str):
-            n = L.bq_attn_workspace_bytes(n_seq, rows, width // D, kv.kv_heads, D, max_len) if row0 is None else 0
+            # without row0 the object serves decode() and, for one sequence, prefill()
+            n = 0
+            if row0 is None:
+                n = L.bq_attn_workspace_bytes(n_seq, rows, width // D, kv.kv_heads, D, max_len)
+            if row0 is not None or n_seq == 1:
+                n = max(n, L.bq_attn_prefill_workspace_bytes(n_seq, rows, n_rows, width // D, kv.kv_heads, D, max_len))
             work = torch.empty(n // 4, dtype=torch.float32, device=q.device) if n else None
         self.kv, self._keep = kv, (q, out, kv_len, row0, work)
         self.struct = AttnArgs(_ptr(q), _ptr(out), _type_of(q, "q"), _type_of(out, "out"), _rows_ld(q, width, "q"),

@@ -13,7 +13,12 @@
 // stay in their lane, rounded to bf16 (at most 2^-8 of a weight, as the queries are;
 // sums and statistics are fp32).  K and V are in the A operands' order in the
 // cache already, so a tile is copied to LDS as it lies (direct to LDS for
-// bf16; q8 is dequantized to bf16 on the way) while the one before is computed.
+// bf16; q8 is dequantized on the way) while the one before is computed.
+// Over a q8 cache the score product is fp16: a code times its scale and an
+// fp32 query need more than bf16's 8 bits (rounding both to bf16 moves an
+// output by 0.5% of its length at scores of a few units, fp16 by what the
+// weights' rounding does); each token and each query row is divided by a power
+// of two first, which keeps fp32's range.
 #include <algorithm>
 
 #include "bq_internal.hpp"
@@ -22,8 +27,8 @@
 namespace bq {
 
 namespace {
-constexpr int kBM = 128;         // query rows of a workgroup
 constexpr int kBN = 64;          // tokens of a tile
+constexpr int kPiece = 8;        // tiles of a piece at least, where the tokens are split
 constexpr float kNone = -1e30f;  // the running maximum before any token
 constexpr float kLazy = 8.f;     // it moves when a score passes it by more (log2)
 
@@ -34,50 +39,120 @@ struct PrefillP {
     int64_t ldq, ldo;
     const int32_t* row0;
     const int32_t* kv_len;
-    int G, n_rows, max_rows, max_len, window, sinks, q_bf16, out_bf16;
+    float* part;  // nsplit > 1: [nsplit][n_rows][q_heads][D], then [..][2] (m, l)
+    int64_t ml;   // floats before the (m, l) part
+    int G, q_heads, n_rows, max_rows, max_len, window, sinks, q_bf16, out_bf16, nsplit;
     float scale;  // scale * log2(e)
 };
 
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+BQ_DEV float pow2(int e) { return as_float((uint32_t)(e + 127) << 23); }                              // |e| <= 126
+BQ_DEV int ilogb2(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 0xFF) - 127; }  // of a normal x
+
 BQ_DEV f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
-// 16 bytes per lane straight to LDS at lds + 16 * lane (m0: see bq_gemm.hip's dma16)
+BQ_DEV f32x16 mfma32h(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// 16 bytes per lane straight to LDS at lds + 16 * lane (m0: see bq_gemm.hip's
+// dma16), from a lane's own address or from a wave's base + 16 * lane
 BQ_DEV void copy_lds(const void* src, const void* lds) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
     asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(m0) : "m0", "memory");
 }
+BQ_DEV void copy_lds_row(const void* base, uint32_t off, const void* lds) {
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(m0) : "m0", "memory");
+}
 
+// four int8 codes times their scales -> bf16
 BQ_DEV u32x2 dequant4(uint32_t w, float a, float b, float c, float d) {
     return u32x2{f2bf2((float)(int8_t)w * a, (float)(int8_t)(w >> 8) * b),
                  f2bf2((float)(int8_t)(w >> 16) * c, (float)((int32_t)w >> 24) * d)};
 }
+// four int8 codes times one fp16 scale: a byte c ^ 0x80 under the exponent of
+// 1024 is 1024 + 128 + c, exactly
+BQ_DEV u32x2 dequant4h(uint32_t w, f16x2 scale) {
+    w ^= 0x80808080u;
+    const f16x2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+    const f16x2 lo = (__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - bias) * scale;
+    const f16x2 hi = (__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - bias) * scale;
+    return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
 
-template <int D, int KV>
-__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_prefill(PrefillP p) {
-    constexpr int KS = D / 16, DT = D / 32;
+// four values of a row (zeros where the row saw nothing: l is 0)
+BQ_DEV void store4(const PrefillP& p, size_t at, f32x4 y, float l) {
+    if (l == 0.f) y = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (p.out_bf16)
+        *(u32x2*)((uint16_t*)p.out + at) = u32x2{f2bf2(y[0], y[1]), f2bf2(y[2], y[3])};
+    else
+        *(f32x4*)((float*)p.out + at) = y;
+}
+
+template <int D, int KV, int W>
+__global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_attn_prefill(PrefillP p) {
+    constexpr int KS = D / 16, DT = D / 32, BM = 32 * W, T = 64 * W;
+    constexpr bool Q8 = KV == kKvQ8;
+    constexpr int NU = D / 8 / W;                      // 1 KiB units of K (and of V) that a wave copies
+    constexpr int NQ8 = D / 64 * 4 / W > 0 ? D / 64 * 4 / W : 1;  // q8 units of a thread
     __shared__ __attribute__((aligned(16))) char s_k[2][kBN * D * 2], s_v[2][kBN * D * 2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, hf = lane >> 5;
+    __shared__ __attribute__((aligned(16))) float s_mul[2][kBN];  // q8: what a token's scores are multiplied by
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hf = lane >> 5;
     const KvView& kv = p.kv;
-    const int seq = blockIdx.z, h = blockIdx.y, P = kv.P;
+    const int seq = blockIdx.z / p.nsplit, split = blockIdx.z % p.nsplit, h = blockIdx.x, P = kv.P;
     const int b0 = p.row0 ? p.row0[seq] : 0, b1 = p.row0 ? p.row0[seq + 1] : p.n_rows;
     // a sequence's rows, kept inside the buffers whatever row0 holds
     const int base = min(max(b0, 0), p.n_rows), rows = min(min(max(b1, 0), p.n_rows) - base, p.max_rows);
-    const int M = rows * p.G, first = (int)(gridDim.x - 1 - blockIdx.x) * kBM;
+    const int M = rows * p.G, first = (int)(gridDim.y - 1 - blockIdx.y) * BM;
     if (rows <= 0 || first >= M) return;
     const int len = min(max(p.kv_len[seq], 0), min(p.max_len, kv.max_pages << kv.plog));
-    const int last = min(M, first + kBM) - 1;
+    const int last = min(M, first + BM) - 1;
     const int r = min(first + wave * 32 + c, last), i = r / p.G;
     const int pos = len - rows + i, pfirst = len - rows + first / p.G, plast = len - rows + last / p.G;
     const size_t qat = (size_t)(base + i) * p.ldq + (size_t)(h * p.G + r % p.G) * D;
 
-    bf16x8 q[KS];
+    // the query row's operand: bf16; over a q8 cache fp16 of the row divided by
+    // a power of two, which comes back in `scale`
+    u32x4 q[KS];
+    float scale = p.scale;
+    if constexpr (!Q8) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-        if (p.q_bf16) {
-            q[k] = *(const bf16x8*)((const uint16_t*)p.q + qat + 16 * k + 8 * hf);
-        } else {
-            const float* x = (const float*)p.q + qat + 16 * k + 8 * hf;
-            const f32x4 a = *(const f32x4*)x, b = *(const f32x4*)(x + 4);
-            q[k] = __builtin_bit_cast(bf16x8, u32x4{f2bf2(a[0], a[1]), f2bf2(a[2], a[3]), f2bf2(b[0], b[1]), f2bf2(b[2], b[3])});
+        for (int k = 0; k < KS; ++k) {
+            if (p.q_bf16) {
+                q[k] = *(const u32x4*)((const uint16_t*)p.q + qat + 16 * k + 8 * hf);
+            } else {
+                const float* x = (const float*)p.q + qat + 16 * k + 8 * hf;
+                const f32x4 a = *(const f32x4*)x, b = *(const f32x4*)(x + 4);
+                q[k] = u32x4{f2bf2(a[0], a[1]), f2bf2(a[2], a[3]), f2bf2(b[0], b[1]), f2bf2(b[2], b[3])};
+            }
+        }
+    } else {
+        f32x4 x[KS][2];
+        float amax = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            if (p.q_bf16) {
+                const u32x4 b = *(const u32x4*)((const uint16_t*)p.q + qat + 16 * k + 8 * hf);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[k][e >> 2][e & 3] = as_float(e & 1 ? b[e >> 1] & 0xFFFF0000u : b[e >> 1] << 16);
+            } else {
+                const float* y = (const float*)p.q + qat + 16 * k + 8 * hf;
+                x[k][0] = *(const f32x4*)y;
+                x[k][1] = *(const f32x4*)(y + 4);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[k][e >> 2][e & 3]));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+        const int ex = max(-100, min(100, ilogb2(amax) - 4));  // the largest value in [16, 32)
+        const float down = pow2(-ex);
+        scale *= pow2(ex);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            f16x8 y;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = (_Float16)(x[k][e >> 2][e & 3] * down);
+            q[k] = __builtin_bit_cast(u32x4, y);
         }
     }
 
@@ -86,58 +161,89 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_prefill(PrefillP
     const int lo = p.window ? max(0, pfirst - p.window + 1) : 0;
     const int lo_t = lo / kBN, end_t = end > 0 ? (end + kBN - 1) / kBN : 0;
     const int ns = p.window ? min(lo_t, (p.sinks + kBN - 1) / kBN) : 0;
-    const int n = end > 0 ? ns + end_t - lo_t : 0;
+    const int all = end > 0 ? ns + end_t - lo_t : 0;
+    // this workgroup's share of them: v0 .. n - 1
+    const int per = p.nsplit > 1 ? max(kPiece, (all + p.nsplit - 1) / p.nsplit) : all;
+    const int v0 = min(all, split * per), n = min(all, v0 + per);
     auto tile0 = [&](int v) { return (v < ns ? v : v - ns + lo_t) * kBN; };
 
     // staging.  pid: the page of token tile0 + lane (-1: none)
-    u32x4 rk[D / 64], rv[D / 64], rvs[D / 64];
+    u32x4 rk[NQ8], rv[NQ8], rvs[NQ8];
     uint16_t rks[D / 32];
     auto page_at = [&](int v) { return v < n ? kv_page(kv, seq, tile0(v) + lane) : -1; };
     auto fetch = [&](int v, int pid, int buf) {
         const int t0 = tile0(v) & (P - 1);  // token of the page where the tile starts (0 for pages below a tile)
         const int tk = (t0 + lane) & (P - 1);
-        const char* kb = kv.pages + (size_t)max(pid, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
-        if constexpr (KV == kKvBf16) {
+        const char* head = kv.pages + (size_t)h * kv.head_bytes;
+        if constexpr (!Q8) {
+            const char* kl = s_k[buf] + wave * 1024;
+            const char* vl = s_v[buf] + wave * 1024;
+            if (P >= kBN) {  // one page: rows of 1 KiB at addresses of the wave
+                const char* pg = head + (int64_t)max(__builtin_amdgcn_readfirstlane(pid), 0) * kv.page_bytes + 16 * t0;
+                const char* kb = pg + wave * (P * 16);
+                const char* vb = pg + P * D * 2 + (2 * D - 16) * t0 + wave * 1024;
 #pragma unroll
-            for (int e = 0; e < D / 32; ++e) {  // 8 dims of the tile's tokens
-                const int ch = wave + 4 * e;
-                copy_lds(kb + kv_k_unit(P, ch, tk), s_k[buf] + ch * 1024);
-            }
+                for (int e = 0; e < NU; ++e)  // 8 dims of the tile's tokens
+                    copy_lds_row(kb, 16 * lane + e * (W * 16) * P, kl + e * (W * 1024));
 #pragma unroll
-            for (int e = 0; e < D / 32; ++e) {  // 64 dims of 8 tokens
-                const int unit = wave + 4 * e, t8 = unit / (D / 64), d = unit % (D / 64) * 64 + lane;
-                const int pv = max(__shfl(pid, 8 * t8, 64), 0);
-                const char* vb = kv.pages + (size_t)pv * kv.page_bytes + (size_t)h * kv.head_bytes;
-                copy_lds(vb + kv_v_unit(P, D, ((t0 + 8 * t8) & (P - 1)) >> 3, d), s_v[buf] + unit * 1024);
+                for (int e = 0; e < NU; ++e)  // 64 dims of 8 tokens
+                    copy_lds_row(vb, 16 * lane + e * (W * 1024), vl + e * (W * 1024));
+            } else {
+                const char* kb = head + (int64_t)max(pid, 0) * kv.page_bytes + 16 * tk + wave * (P * 16);
+#pragma unroll
+                for (int e = 0; e < NU; ++e) copy_lds(kb + e * (W * 16) * P, kl + e * (W * 1024));
+#pragma unroll
+                for (int e = 0; e < NU; ++e) {
+                    const int unit = wave + W * e, t8 = unit / (D / 64), d = unit % (D / 64) * 64;
+                    const char* vb = head + (int64_t)max(__builtin_amdgcn_readlane(pid, 8 * t8), 0) * kv.page_bytes;
+                    copy_lds_row(vb + kv_v_unit(P, D, ((8 * t8) & (P - 1)) >> 3, d), 16 * lane, vl + e * (W * 1024));
+                }
             }
         } else {
+            const char* kb = head + (int64_t)max(pid, 0) * kv.page_bytes;
 #pragma unroll
-            for (int e = 0; e < D / 64; ++e) rk[e] = *(const u32x4*)(kb + kv_kq_unit(P, e, wave, tk));
+            for (int e = 0; e < NQ8; ++e) {
+                const int u = wave + W * e;  // unit (c, g) of the lane's token
+                if (u < D / 16) rk[e] = *(const u32x4*)(kb + kv_kq_unit(P, u >> 2, u & 3, tk));
+            }
 #pragma unroll
             for (int e = 0; e < D / 32; ++e) rks[e] = *(const uint16_t*)(kb + kv_ks_off(P, D, e, tk));
 #pragma unroll
-            for (int e = 0; e < D / 64; ++e) {
-                const int u = tid + 256 * e, m = u % 16, cc = u / 16 % (D / 32), t8 = u / (D / 2);
-                const int pv = max(__shfl(pid, 8 * t8, 64), 0), tv = (t0 + 8 * t8) & (P - 1);
-                const char* vb = kv.pages + (size_t)pv * kv.page_bytes + (size_t)h * kv.head_bytes;
-                rv[e] = *(const u32x4*)(vb + kv_vq_unit(P, D, tv >> 3, cc, m));
-                rvs[e] = *(const u32x4*)(vb + kv_vs_off(P, D, cc, tv));
+            for (int e = 0; e < NQ8; ++e) {
+                const int u = tid + T * e, m = u % 16, cc = u / 16 % (D / 32), t8 = u / (D / 2);
+                if (t8 < kBN / 8) {
+                    const int pv = max(__shfl(pid, 8 * t8, 64), 0), tv = (t0 + 8 * t8) & (P - 1);
+                    const char* vb = head + (int64_t)pv * kv.page_bytes;
+                    rv[e] = *(const u32x4*)(vb + kv_vq_unit(P, D, tv >> 3, cc, m));
+                    rvs[e] = *(const u32x4*)(vb + kv_vs_off(P, D, cc, tv));
+                }
             }
         }
     };
-    auto land = [&](int buf) {  // q8: the fetched tile as bf16
-        if constexpr (KV == kKvQ8) {
+    auto land = [&](int buf) {  // q8: the fetched tile, keys as fp16 over a power of two of their token, values as bf16
+        if constexpr (Q8) {
+            uint32_t top = 0;
 #pragma unroll
-            for (int e = 0; e < D / 64; ++e)
+            for (int e = 0; e < D / 32; ++e) top = max(top, (uint32_t)rks[e]);
+            const int ex = max(-100, min(100, (int)(top >> 7) - 127));
+            const float down = pow2(-ex);
+            if (wave == 0) s_mul[buf][lane] = pow2(ex);
+#pragma unroll
+            for (int e = 0; e < NQ8; ++e) {
+                const int u = wave + W * e, cc = u >> 2, g = u & 3;
+                if (u >= D / 16) break;
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const float s = bf2f(rks[2 * e + k]);
-                    const u32x2 a = dequant4(rk[e][2 * k], s, s, s, s), b = dequant4(rk[e][2 * k + 1], s, s, s, s);
-                    *(u32x4*)(s_k[buf] + ((8 * e + 4 * k + wave) * kBN + lane) * 16) = u32x4{a[0], a[1], b[0], b[1]};
+                    const _Float16 sh = (_Float16)(bf2f(rks[2 * cc + k]) * down);
+                    const f16x2 s = {sh, sh};
+                    const u32x2 a = dequant4h(rk[e][2 * k], s), b = dequant4h(rk[e][2 * k + 1], s);
+                    *(u32x4*)(s_k[buf] + ((8 * cc + 4 * k + g) * kBN + lane) * 16) = u32x4{a[0], a[1], b[0], b[1]};
                 }
+            }
 #pragma unroll
-            for (int e = 0; e < D / 64; ++e) {
-                const int u = tid + 256 * e, m = u % 16, cc = u / 16 % (D / 32), t8 = u / (D / 2);
+            for (int e = 0; e < NQ8; ++e) {
+                const int u = tid + T * e, m = u % 16, cc = u / 16 % (D / 32), t8 = u / (D / 2);
+                if (t8 >= kBN / 8) break;
                 float s[8];
 #pragma unroll
                 for (int x = 0; x < 8; ++x) s[x] = as_float(x & 1 ? rvs[e][x >> 1] & 0xFFFF0000u : rvs[e][x >> 1] << 16);
@@ -159,45 +265,80 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_prefill(PrefillP
     // K row of the lane in the score product (see above)
     const int krow = 16 * (c >> 4) + 8 * (c >> 2 & 1) + 4 * (c >> 3 & 1) + (c & 3);
 
-    int pid = page_at(0), pid_next = page_at(1);
-    if (n > 0) fetch(0, pid, 0);
-    if (n > 0) land(0);
-    for (int v = 0; v < n; ++v) {
-        const int buf = v & 1, t0 = tile0(v);
+    int pid = page_at(v0), pid_next = page_at(v0 + 1);
+    if (v0 < n) {
+        fetch(v0, pid, 0);
+        land(0);
+    }
+    for (int v = v0; v < n; ++v) {
+        const int buf = (v - v0) & 1, t0 = tile0(v);
         const uint64_t bad = __ballot(pid < 0);
         BQ_WAIT_VM(0);
         __syncthreads();
         pid = pid_next;
         if (v + 1 < n) fetch(v + 1, pid, buf ^ 1);
         pid_next = page_at(v + 2);
-
+        const char* kp = s_k[buf] + (hf * kBN + krow) * 16;
+        const char* vp = s_v[buf] + (hf * D + c) * 16;
+        // the wave that is on the matrix pipe goes first: its partner on the SIMD
+        // (another workgroup's) then has the vector pipe while it waits for results
+        if constexpr (!Q8) __builtin_amdgcn_s_setprio(1);
         f32x16 s[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
-                s[t] = mfma32(*(const bf16x8*)(s_k[buf] + ((2 * k + hf) * kBN + 32 * t + krow) * 16), q[k], s[t]);
-        }
-        const bool edge = bad != 0 || t0 + kBN - 1 > pfirst || (p.window && t0 <= plast - p.window && t0 + kBN > p.sinks);
+            for (int t = 0; t < 2; ++t) {
+                const u32x4 kf = *(const u32x4*)(kp + (2 * k * kBN + 32 * t) * 16);
+                if constexpr (Q8)
+                    s[t] = mfma32h(__builtin_bit_cast(f16x8, kf), __builtin_bit_cast(f16x8, q[k]), s[t]);
+                else
+                    s[t] = mfma32(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, q[k]), s[t]);
+            }
+        if constexpr (!Q8) __builtin_amdgcn_s_setprio(0);
         // s[t][8u + e]: token t0 + 32t + 16u + 8hf + e
-        if (edge) {
+        if constexpr (Q8) {
+            const float* mp = s_mul[buf] + 8 * hf;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+                const f32x4 y = *(const f32x4*)(mp + 32 * (e >> 4) + 16 * (e >> 3 & 1) + (e & 4));
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s[e >> 4][(e & 15) + x] *= y[x];
+            }
+        }
+        if (bad != 0 || t0 + kBN - 1 > pfirst || (p.window && t0 <= plast - p.window && t0 + kBN > p.sinks)) {
+            // at an edge of what the rows see
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int at = 32 * t + 16 * (e >> 3) + 8 * hf + (e & 7), tok = t0 + at;
-                    const bool me = !(bad >> at & 1) && tok <= pos && (!p.window || tok > pos - p.window || tok < p.sinks);
+                    const bool me = (!(bad >> at & 1)) & (tok <= pos) & ((!p.window) | (tok > pos - p.window) | (tok < p.sinks));
                     s[t][e] = me ? s[t][e] : -INFINITY;
                 }
+            if (bad != 0 || t0 + kBN > end || t0 < lo) {
+                // values that no row sees may hold anything: their products must not
+                for (int u = tid; u < D * (kBN / 8); u += T) {
+                    u32x4 mask;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int at = u / D * 8 + e, tok = t0 + at;
+                        const bool any = (!(bad >> at & 1)) & (tok < end) & ((tok >= lo) | (tok < p.sinks));
+                        const uint32_t keep = any ? (e & 1 ? 0xFFFF0000u : 0xFFFFu) : 0u;
+                        mask[e >> 1] = e & 1 ? mask[e >> 1] | keep : keep;
+                    }
+                    *(u32x4*)(s_v[buf] + u * 16) &= mask;
+                }
+                __syncthreads();
+            }
         }
         float mx = s[0][0];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
-        mx *= p.scale;
+        mx *= scale;
         if (__any(mx > m + kLazy)) {
             const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
             const float al = __builtin_amdgcn_exp2f(m - mn);
@@ -206,73 +347,103 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_prefill(PrefillP
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= al;
         }
-        bf16x8 pp[4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * u + e], p.scale, -m));
-                    l += x[e];
-                }
-                pp[2 * t + u] = __builtin_bit_cast(bf16x8, u32x4{f2bf2(x[0], x[1]), f2bf2(x[2], x[3]), f2bf2(x[4], x[5]), f2bf2(x[6], x[7])});
-            }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            u32x4 mask = {~0u, ~0u, ~0u, ~0u};
-            if (edge) {
-                // what no row sees may hold anything: its products must not
+            float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int at = 16 * u + 8 * hf + e, tok = t0 + at;
-                    const bool any = !(bad >> at & 1) && tok < end && (tok >= lo || tok < p.sinks);
-                    if (!any) mask[e >> 1] &= e & 1 ? 0xFFFFu : 0xFFFF0000u;
-                }
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][8 * (u & 1) + e], scale, -m));
+                l += x[e];
             }
+            const bf16x8 pp = __builtin_bit_cast(bf16x8, u32x4{f2bf2(x[0], x[1]), f2bf2(x[2], x[3]), f2bf2(x[4], x[5]), f2bf2(x[6], x[7])});
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                u32x4 vf = *(const u32x4*)(s_v[buf] + ((2 * u + hf) * D + 32 * d + c) * 16);
-                if (edge) vf &= mask;
-                o[d] = mfma32(__builtin_bit_cast(bf16x8, vf), pp[u], o[d]);
-            }
+            for (int d = 0; d < DT; ++d) o[d] = mfma32(*(const bf16x8*)(vp + (2 * u * D + 32 * d) * 16), pp, o[d]);
         }
         if (v + 1 < n) land(buf ^ 1);
     }
 
     l += __shfl_xor(l, 32, 64);
     if (first + wave * 32 + c > last) return;
+    if (p.nsplit > 1) {
+        const size_t to = ((size_t)split * p.n_rows + base + i) * p.q_heads + h * p.G + r % p.G;
+        if (hf == 0) *(u32x2*)(p.part + p.ml + to * 2) = u32x2{__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, l)};
+        if (v0 >= n) return;  // l is 0: the row is not read
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                *(f32x4*)(p.part + to * D + 32 * d + 8 * b + 4 * hf) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+        return;
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const size_t at = (size_t)(base + i) * p.ldo + (size_t)(h * p.G + r % p.G) * D;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {  // dims 32d + 8b + 4hf ..
-            f32x4 y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = l == 0.f ? 0.f : o[d][4 * b + e] * inv;
-            const size_t to = at + 32 * d + 8 * b + 4 * hf;
-            if (p.out_bf16)
-                *(u32x2*)((uint16_t*)p.out + to) = u32x2{f2bf2(y[0], y[1]), f2bf2(y[2], y[3])};
-            else
-                *(f32x4*)((float*)p.out + to) = y;
-        }
+        for (int b = 0; b < 4; ++b)  // dims 32d + 8b + 4hf ..
+            store4(p, at + 32 * d + 8 * b + 4 * hf, f32x4{o[d][4 * b] * inv, o[d][4 * b + 1] * inv, o[d][4 * b + 2] * inv, o[d][4 * b + 3] * inv}, l);
 }
+
+// joins the pieces of the rows, in their order: a lane has 4 dims of one row and head
+template <int D>
+__global__ void __launch_bounds__(256) k_attn_prefill_join(PrefillP p) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, at = e / (D / 4), rows = (int64_t)p.n_rows * p.q_heads;
+    if (at >= rows) return;
+    const int row = (int)(at / p.q_heads), head = (int)(at % p.q_heads), d = (int)(e % (D / 4)) * 4;
+    if (p.row0) {  // rows of no sequence have no pieces
+        bool mine = false;
+        for (int s = 0; s < p.kv.n_seq; ++s) {
+            const int b = min(max(p.row0[s], 0), p.n_rows);
+            mine |= row >= b && row < min(p.row0[s + 1], b + p.max_rows);
+        }
+        if (!mine) return;
+    }
+    float mt = kNone;
+    for (int s = 0; s < p.nsplit; ++s) mt = fmaxf(mt, p.part[p.ml + (s * rows + at) * 2]);
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (int s = 0; s < p.nsplit; ++s) {
+        const float ls = p.part[p.ml + (s * rows + at) * 2 + 1];
+        if (ls == 0.f) continue;
+        const float f = __builtin_amdgcn_exp2f(p.part[p.ml + (s * rows + at) * 2] - mt);
+        a += *(const f32x4*)(p.part + (s * rows + at) * D + d) * f;
+        l += ls * f;
+    }
+    store4(p, (size_t)row * p.ldo + (size_t)head * D + d, a * (l == 0.f ? 0.f : 1.f / l), l);
+}
+
+constexpr int kW = 4;  // waves of a workgroup
 
 template <int D, int KV>
 hipError_t launch_of(const PrefillP& p, hipStream_t st) {
-    const int64_t tiles = ((int64_t)p.max_rows * p.G + kBM - 1) / kBM;
-    launch_kernel((k_attn_prefill<D, KV>), dim3((uint32_t)tiles, p.kv.heads, p.kv.n_seq), dim3(256), 0, st, p);
-    return hipGetLastError();
+    const int64_t tiles = ((int64_t)p.max_rows * p.G + 32 * kW - 1) / (32 * kW);
+    launch_kernel((k_attn_prefill<D, KV, kW>), dim3(p.kv.heads, (uint32_t)tiles, p.kv.n_seq * p.nsplit), dim3(64 * kW), 0, st, p);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && p.nsplit > 1) {
+        const int64_t n = (int64_t)p.n_rows * p.q_heads * (D / 4);
+        launch_kernel((k_attn_prefill_join<D>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, p);
+        e = hipGetLastError();
+    }
+    return e;
 }
 }  // namespace
 
-hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, hipStream_t st) {
+// Pieces that the tokens of a sequence are cut into: where the row tiles leave
+// workgroup slots (two per CU) free, as many pieces as fill them, of kPiece
+// tiles at least.
+int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus) {
+    const int64_t tiles = ((int64_t)rows * (q_heads / kv_heads) + 32 * kW - 1) / (32 * kW) * n_seq * kv_heads;
+    const int64_t steps = ((int64_t)max_len + kBN - 1) / kBN;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(steps / kPiece, 2 * cus / tiles));
+}
+size_t prefill_part_floats(int n_rows, int q_heads, int D) { return (size_t)n_rows * q_heads * (D + 2); }
+
+hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st) {
     PrefillP p;
     p.kv = kv;
     p.q = a.q; p.out = a.out; p.ldq = a.ldq; p.ldo = a.ldo; p.row0 = a.row0; p.kv_len = a.kv_len;
-    p.G = a.q_heads / kv.heads; p.n_rows = a.n_rows; p.max_rows = std::min(a.rows, a.n_rows); p.max_len = a.max_len;
+    p.nsplit = nsplit; p.part = (float*)a.work; p.ml = (int64_t)nsplit * a.n_rows * a.q_heads * kv.D;
+    p.q_heads = a.q_heads; p.G = a.q_heads / kv.heads; p.n_rows = a.n_rows; p.max_rows = std::min(a.rows, a.n_rows); p.max_len = a.max_len;
     p.window = a.window; p.sinks = a.sinks;
     p.q_bf16 = a.q_type == BQ_TYPE_BF16; p.out_bf16 = a.out_type == BQ_TYPE_BF16;
     p.scale = a.scale * 1.44269504088896341f;

@@ -145,7 +145,9 @@ hipError_t launch_kv_read(const KvView& kv, int type, const int32_t* seq, const 
 int decode_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus);
 size_t decode_part_floats(int n_seq, int rows, int q_heads, int kv_heads, int D);  // workspace of one piece each
 hipError_t launch_attn_decode(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st);
-hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, hipStream_t st);
+int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus);
+size_t prefill_part_floats(int n_rows, int q_heads, int D);
+hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st);
 
 size_t sample_work_bytes(int rows, int vocab);
 hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, const float* temp, const int32_t* top_k,

@@ -105,6 +105,14 @@ size_t bq_attn_workspace_bytes(int n_seq, int rows, int q_heads, int kv_heads, i
     return n > 1 ? n * decode_part_floats(n_seq, rows, q_heads, kv_heads, head_dim) * sizeof(float) : 0;
 }
 
+size_t bq_attn_prefill_workspace_bytes(int n_seq, int rows, int n_rows, int q_heads, int kv_heads, int head_dim, int max_len) {
+    if (n_seq <= 0 || rows < 1 || n_rows < 1 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0 ||
+        max_len < 0 || device_ready() != BQ_OK)
+        return 0;
+    const int n = prefill_splits(n_seq, std::min(rows, n_rows), q_heads, kv_heads, max_len, device_cus());
+    return n > 1 ? n * prefill_part_floats(n_rows, q_heads, head_dim) * sizeof(float) : 0;
+}
+
 int bq_attn_decode(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t st) {
     if (int r = device_ready()) return r;
     KvView kv;
@@ -133,7 +141,13 @@ int bq_attn_prefill(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t 
     if (!a.row0 && (kv.n_seq != 1 || a.rows != a.n_rows)) return BQ_EINVAL;
     if (a.n_rows == 0) return BQ_OK;
     if ((int64_t)a.rows * (a.q_heads / kv.heads) > INT32_MAX / 2) return BQ_UNSUPPORTED;
-    return from_hip(launch_attn_prefill(kv, type, a, (hipStream_t)st));
+    if (!al16(a.work) || (a.work_bytes && !a.work)) return BQ_EINVAL;
+    int n = prefill_splits(kv.n_seq, std::min(a.rows, a.n_rows), a.q_heads, kv.heads, a.max_len, device_cus());
+    const size_t part = prefill_part_floats(a.n_rows, a.q_heads, kv.D) * sizeof(float);
+    n = (int)std::min<size_t>(n, std::max<size_t>(1, a.work_bytes / part));
+    // (sequence, piece) is one grid dimension
+    n = std::max(1, std::min(n, 65535 / kv.n_seq));
+    return from_hip(launch_attn_prefill(kv, type, a, n, (hipStream_t)st));
 }
 
 void bq_attn_hook(void* user, int block, bq_stream_t st) {

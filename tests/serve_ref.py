@@ -32,6 +32,26 @@ def quant(x):
     return (g * inv[..., None]).round().clamp(-127, 127).to(torch.int8).reshape(x.shape), d
 
 
+def power(x):
+    """2^e of the largest magnitude over the last dimension, in [1, 2) 2^e."""
+    m = x.abs().amax(-1, keepdim=True).double()
+    return torch.where(m > 0, torch.exp2(torch.floor(torch.log2(m.clamp(min=1e-300)))), torch.ones((), dtype=torch.float64))
+
+
+def half_keys(codes, scales):
+    """q8 keys rounded to fp16 (fp64 out): a token's scales over the power of two of its largest are rounded
+    to fp16, and so are their products with the codes."""
+    p = power(scales.float())
+    s = (scales.double() / p).half().repeat_interleave(32, -1)
+    return (codes.double() * s.double()).half().double() * p
+
+
+def half_rows(q):
+    """Query rows [.., D] rounded to fp16 over a power of two of their largest value."""
+    p = power(q.float()) / 16
+    return (q.double() / p).half().double() * p
+
+
 class Pages:
     """A cache built on the CPU: every byte that holds no token of a sequence is NaN (bf16 pages and q8
     scales) or an extreme code, so a kernel that lets one count gives NaN."""
@@ -49,6 +69,7 @@ class Pages:
         self.table = torch.from_numpy(self.rng.permutation(self.n_pages)[: n_seq * max_pages].reshape(n_seq, max_pages)
                                       .astype(np.int32))
         self.k, self.v = {}, {}
+        self.kh = {}  # keys as the prefill attention's products take them
 
     def put(self, seq, k, v):
         """Tokens 0..n-1 of sequence seq: k and v fp32 [n, H, D]; what the cache then stands for is kept (fp64)."""
@@ -60,10 +81,14 @@ class Pages:
         for value, x, keep in ((0, k, self.k), (1, v, self.v)):
             if self.kv == "bf16":
                 x = bf16(x)
+                if not value:
+                    self.kh[seq] = x.double()
                 self.raw.view(torch.bfloat16)[page, h, addr_bf16(P, D, t % P, d, value)] = x
                 keep[seq] = x.double()
             else:
                 c, s = quant(x)
+                if not value:
+                    self.kh[seq] = half_keys(c, s)
                 code, scale = addr_q8(P, D, t % P, d, value)
                 self.raw.view(torch.int8)[page, h, code] = c
                 sd = s.repeat_interleave(32, -1)

@@ -11,7 +11,8 @@ and denominator once each):
     twice: below 2^-19 A each way.  tol = 2^-16 + 2^-18 A.
   bf16 weights (prefill; decode with bf16 in and out): 2^-8 of a weight instead
     of 2^-16, and 2^-8 of a bf16 output: tol = 2^-7 (1 + 2^-6) + 2^-18 A.
-Prefill takes q (and q8 values) as bf16: the reference rounds them the same.
+Prefill takes q as bf16, and over a q8 cache q and keys as fp16 over a power of
+two of their row, values as bf16: the reference rounds them the same.
 """
 import ctypes
 
@@ -169,7 +170,8 @@ def _prefill(bq, kv, rows, past, Hq, H, D, P, qt, ot, window=0, sinks=0, seed=1,
     if pad:
         assert torch.isnan(out[:, Hq * D:]).all()
     got = out[:, : Hq * D].cpu().double().reshape(total, Hq, D)
-    qr = R.bf16(q).double().reshape(total, Hq, D)
+    qr = q.float().reshape(total, Hq, D)
+    qr = R.bf16(qr).double() if kv == "bf16" else R.half_rows(qr)
     first = 0
     for s, (r, T) in enumerate(zip(rows, lens)):
         hidden = torch.zeros(T, dtype=torch.bool)
@@ -177,7 +179,7 @@ def _prefill(bq, kv, rows, past, Hq, H, D, P, qt, ot, window=0, sinks=0, seed=1,
             if hs == s:
                 hidden[p * P:(p + 1) * P] = True
         if r:
-            k, v = (R.bf16(x[s]).double() for x in (pages.k, pages.v))
+            k, v = pages.kh[s], R.bf16(pages.v[s]).double()
             ref = R.attention(qr[first: first + r], k, v, torch.arange(T - r, T), D ** -0.5, window, sinks, hidden)
             _check(got[first: first + r], *ref, False, f"prefill seq {s}: {r} rows of {T} tokens")
         first += r

@@ -32,7 +32,8 @@ class _Watch:
 
     def __init__(self, G, c, model, n_seq):
         self.c, self.L = c, model.layers[-1]
-        self.k, self.v = [[] for _ in range(n_seq)], [[] for _ in range(n_seq)]
+        # what the cache stands for, and what the prefill attention's products make of it
+        self.k, self.v, self.kh, self.vh = ([[] for _ in range(n_seq)] for _ in range(4))
 
     def check(self, step, g, seqs, positions, fine):
         c = self.c
@@ -42,22 +43,22 @@ class _Watch:
         pos = torch.tensor(positions)
         q, k, v = R.append(*x, pos, rope, c.head_dim, self.L["q_weight"].cpu().double(), self.L["k_weight"].cpu().double(), 1e-6, False)
         if not fine:
-            q = R.bf16(q).double()
+            q = R.bf16(q).double() if c.kv_type == "bf16" else R.half_rows(R.bf16(q).float())
         for r, (s, p) in enumerate(zip(seqs, positions)):
-            for keep, t in ((self.k, k), (self.v, v)):
+            for keep, coarse, t in ((self.k, self.kh, k), (self.v, self.vh, v)):
                 t = t[r: r + 1]
                 if c.kv_type == "bf16":
-                    t = R.bf16(t).double()
+                    t = rounded = R.bf16(t).double()
                 else:
                     codes, d = R.quant(t.float())
                     t = codes.double() * d.double().repeat_interleave(32, -1)
-                if not fine:
-                    t = R.bf16(t).double()
+                    rounded = R.half_keys(codes, d) if coarse is self.kh else R.bf16(t).double()
                 assert len(keep[s]) == p
                 keep[s].append(t)
+                coarse[s].append(rounded)
         got = step.attn_out.cpu().double().reshape(step.rows, c.q_heads, c.head_dim)
         for r, (s, p) in enumerate(zip(seqs, positions)):
-            ks, vs = torch.cat(self.k[s][: p + 1]), torch.cat(self.v[s][: p + 1])
+            ks, vs = (torch.cat(x[s][: p + 1]) for x in ((self.k, self.v) if fine else (self.kh, self.vh)))
             ref, bound, A = R.attention(q[r: r + 1], ks, vs, [p], c.head_dim ** -0.5, c.window, c.sinks)
             tol = (2.0 ** -16 if fine else 2.0 ** -8) + 2.0 ** -18 * A[..., None] + 2.0 ** -7
             err = (got[r: r + 1] - ref).abs()
