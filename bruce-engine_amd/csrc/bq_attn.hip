@@ -14,10 +14,13 @@
 // is the A operands' (16 bytes per lane, 256 contiguous bytes per 16 lanes), so
 // K and V go straight from HBM to registers.
 //
-// fp32 precision on bf16 MFMA: K, V (and int8 codes) are exact in bf16; an
-// fp32 q is the sum of three bf16 parts, a softmax weight the sum of two (its
-// error, at most 2^-16 of the weight, is near the sums' own), each with its own MFMA.
-// The matrix pipe is far from busy here, the parts cost no time.
+// fp32 precision on 16-bit MFMA: K, V and int8 codes are exact in bf16, the
+// codes in fp16 too.  Over a bf16 cache q and the softmax weights are sums of
+// three bf16 parts (all 24 bits).  Over a q8 cache q is two fp16 parts of the
+// row over a power of two (2^-22 of its largest value), a weight times a
+// token's value scale two bf16 parts (2^-16 of it: a third costs 13% here,
+// where the vector pipe is busy unpacking; over bf16 it costs 1%).  Every part
+// has its own MFMA: the matrix pipe is far from busy.
 //
 // The running maximum is kept per query row and only moved when a score passes
 // it by more than 2^8 (kLazy): a weight is then at most 2^8, which fp32 sums
@@ -84,6 +87,13 @@ BQ_DEV bf16x8 codes8(uint32_t lo, uint32_t hi) {
     const u32x2 a = codes_bf16(lo), b = codes_bf16(hi);
     return __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
 }
+BQ_DEV f16x8 codes8h(uint32_t lo, uint32_t hi) {
+    f16x2 v[4];
+    codes_f16(lo, v[0], v[1]);
+    codes_f16(hi, v[2], v[3]);
+    return f16x8{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
+}
+BQ_DEV f32x4 mfma16h(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 BQ_DEV f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
 // sum over the four lane groups that share lane & 15
@@ -96,7 +106,7 @@ BQ_DEV float groups_sum(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
-// NQ bf16 parts of q, NP of a softmax weight
+// NQ parts of q, NP of a softmax weight
 template <int D, int KV, int NQ, int NP>
 __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p) {
     constexpr int KS = D / 32, DT = D / 16;
@@ -112,33 +122,63 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p
     const int M = p.rows * p.G, first = qt * 16, last = min(M, first + 16) - 1;
     const int pfirst = len - p.rows + first / p.G, plast = len - p.rows + last / p.G;
     const int r = min(first + c, last), i = r / p.G, pos = len - p.rows + i;
-    bf16x8 q[NQ][KS];
+    constexpr bool Q8 = KV == kKvQ8;
+    u32x4 q[NQ][KS];
+    float scale = p.scale;
     {
         const size_t at = (size_t)(seq * p.rows + i) * p.ldq + (size_t)(h * p.G + r % p.G) * D + 8 * g;
+        if constexpr (!Q8 && NQ == 1) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            if constexpr (NQ == 1) {
-                q[0][k] = *(const bf16x8*)((const uint16_t*)p.q + at + 32 * k);
-            } else {
-                float x[8];
+            for (int k = 0; k < KS; ++k) q[0][k] = *(const u32x4*)((const uint16_t*)p.q + at + 32 * k);
+        } else {
+            float x[KS][8], amax = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
                 if (p.q_bf16) {
-                    const bf16x8 b = *(const bf16x8*)((const uint16_t*)p.q + at + 32 * k);
+                    const u32x4 b = *(const u32x4*)((const uint16_t*)p.q + at + 32 * k);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = (float)b[e];
+                    for (int e = 0; e < 8; ++e) x[k][e] = as_float(e & 1 ? b[e >> 1] & 0xFFFF0000u : b[e >> 1] << 16);
                 } else {
                     const f32x4 a = *(const f32x4*)((const float*)p.q + at + 32 * k), b = *(const f32x4*)((const float*)p.q + at + 32 * k + 4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
+                    for (int e = 0; e < 4; ++e) x[k][e] = a[e], x[k][4 + e] = b[e];
                 }
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) {
-                        const __bf16 y = (__bf16)x[e];
-                        q[n][k][e] = y;
-                        x[e] -= (float)y;
-                    }
             }
+            if constexpr (Q8) {  // the row's largest value to [16, 32)
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[k][e]));
+                const int ex = max(-100, min(100, ilogb2(groups_max(amax)) - 4));
+                const float down = pow2(-ex);
+                scale *= pow2(ex);
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[k][e] *= down;
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    if constexpr (Q8) {
+                        f16x8 y;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            y[e] = (_Float16)x[k][e];
+                            x[k][e] -= (float)y[e];
+                        }
+                        q[n][k] = __builtin_bit_cast(u32x4, y);
+                    } else {
+                        bf16x8 y;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            y[e] = (__bf16)x[k][e];
+                            x[k][e] -= (float)y[e];
+                        }
+                        q[n][k] = __builtin_bit_cast(u32x4, y);
+                    }
+                }
         }
     }
 
@@ -172,7 +212,6 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p
             const char* bk = kv.pages + (size_t)max(pk, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
             const char* bv = kv.pages + (size_t)max(pv, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
             // every load of the step first: the values' arrive during the scores
-            constexpr bool Q8 = KV == kKvQ8;
             u32x4 kf[2][Q8 ? KS / 2 : KS], vf[Q8 ? DT / 2 : DT], ksc[Q8 ? KS : 1], vsc[Q8 ? KS : 1];
             if constexpr (!Q8) {
 #pragma unroll
@@ -202,14 +241,14 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p
                     if constexpr (!Q8) {
                         const bf16x8 kb = __builtin_bit_cast(bf16x8, kf[y][k]);
 #pragma unroll
-                        for (int a = NQ - 1; a >= 0; --a) s[y] = mfma16(kb, q[a][k], s[y]);
+                        for (int a = NQ - 1; a >= 0; --a) s[y] = mfma16(kb, __builtin_bit_cast(bf16x8, q[a][k]), s[y]);
                     } else {
-                        const bf16x8 kb = codes8(kf[y][k / 2][2 * (k & 1)], kf[y][k / 2][2 * (k & 1) + 1]);
+                        const f16x8 kb = codes8h(kf[y][k / 2][2 * (k & 1)], kf[y][k / 2][2 * (k & 1) + 1]);
                         const uint32_t a0 = ksc[k][2 * y], a1 = ksc[k][2 * y + 1];
                         const f32x4 sc = {as_float(a0 << 16), as_float(a0 & 0xFFFF0000u), as_float(a1 << 16), as_float(a1 & 0xFFFF0000u)};
                         f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int a = NQ - 1; a >= 0; --a) x = mfma16(kb, q[a][k], x);
+                        for (int a = NQ - 1; a >= 0; --a) x = mfma16h(kb, __builtin_bit_cast(f16x8, q[a][k]), x);
                         s[y] += x * sc;
                     }
                 }
@@ -236,7 +275,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p
             }
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * p.scale;
+            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * scale;
             if (edge) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -383,7 +422,7 @@ hipError_t launch_decode_of(const DecodeP& p, hipStream_t st) {
     if (p.q_bf16 && p.out_bf16)
         launch_kernel((k_attn_decode<D, KV, 1, 1>), grid, dim3(256), 0, st, p);
     else
-        launch_kernel((k_attn_decode<D, KV, 3, 2>), grid, dim3(256), 0, st, p);
+        launch_kernel((k_attn_decode<D, KV, KV == kKvQ8 ? 2 : 3, KV == kKvQ8 ? 2 : 3>), grid, dim3(256), 0, st, p);
     if (p.nsplit > 1) {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;

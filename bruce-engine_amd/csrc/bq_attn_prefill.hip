@@ -45,11 +45,6 @@ struct PrefillP {
     float scale;  // scale * log2(e)
 };
 
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-BQ_DEV float pow2(int e) { return as_float((uint32_t)(e + 127) << 23); }                              // |e| <= 126
-BQ_DEV int ilogb2(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 0xFF) - 127; }  // of a normal x
-
 BQ_DEV f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 BQ_DEV f32x16 mfma32h(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
@@ -70,14 +65,11 @@ BQ_DEV u32x2 dequant4(uint32_t w, float a, float b, float c, float d) {
     return u32x2{f2bf2((float)(int8_t)w * a, (float)(int8_t)(w >> 8) * b),
                  f2bf2((float)(int8_t)(w >> 16) * c, (float)((int32_t)w >> 24) * d)};
 }
-// four int8 codes times one fp16 scale: a byte c ^ 0x80 under the exponent of
-// 1024 is 1024 + 128 + c, exactly
+// four int8 codes times one fp16 scale
 BQ_DEV u32x2 dequant4h(uint32_t w, f16x2 scale) {
-    w ^= 0x80808080u;
-    const f16x2 bias = {(_Float16)1152.f, (_Float16)1152.f};
-    const f16x2 lo = (__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - bias) * scale;
-    const f16x2 hi = (__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - bias) * scale;
-    return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+    f16x2 lo, hi;
+    codes_f16(w, lo, hi);
+    return u32x2{__builtin_bit_cast(uint32_t, lo * scale), __builtin_bit_cast(uint32_t, hi * scale)};
 }
 
 // four values of a row (zeros where the row saw nothing: l is 0)

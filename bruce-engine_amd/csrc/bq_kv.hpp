@@ -38,6 +38,20 @@ BQ_DEV int kv_vq_unit(int P, int D, int t8, int c, int m) { return P * D + ((t8 
 BQ_DEV int kv_ks_off(int P, int D, int c, int t) { return 2 * P * D + (c * P + t) * 2; }
 BQ_DEV int kv_vs_off(int P, int D, int c, int t) { return 2 * P * D + (D / 32 * P + c * P + t) * 2; }
 
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+BQ_DEV float pow2(int e) { return as_float((uint32_t)(e + 127) << 23); }                           // |e| <= 126
+BQ_DEV int ilogb2(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 0xFF) - 127; }  // of a normal x
+
+// four int8 codes -> fp16: a byte c ^ 0x80 under the exponent of 1024 is
+// 1024 + 128 + c, exactly
+BQ_DEV void codes_f16(uint32_t w, f16x2& lo, f16x2& hi) {
+    w ^= 0x80808080u;
+    const f16x2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+    lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - bias;
+    hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - bias;
+}
+
 BQ_DEV uint16_t f2bf(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 BQ_DEV float bf2f(uint16_t b) { return as_float((uint32_t)b << 16); }
 BQ_DEV uint32_t f2bf2(float a, float b) {
