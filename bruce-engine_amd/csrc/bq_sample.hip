@@ -5,15 +5,14 @@
 // to be sorted.  Two launches:
 //   k_sample_scan, one workgroup per 4096 logits: reads them once (the floor:
 //     4 bytes a logit), keeps the head of its slice -- every logit not below a
-//     threshold t, taken from the lanes' maxima in order, which leaves about 448
+//     threshold t, taken from the lanes' maxima in order, which leaves about 400
 //     candidates for the whole row -- and, where top-p needs the row's mass, its
 //     sum of exponentials.
 //   k_sample_pick, one workgroup per row: sorts the candidates, takes their
 //     running mass and cuts it.  All tokens of the row not below the largest t
 //     are among the candidates, so a cut that falls there is exact.  Where it
-//     does not (a flat row, no filter, many equal logits), the row is read
-//     again: radix selection by count and by mass on the ordered bits of the
-//     logit, then of the index, 11 bits at a time.
+//     does not (a flat row, no filter, hundreds of tokens kept), the row is read
+//     again, two or three times (struct Whole).
 // Slices are 256-logit blocks dealt in turn: likely tokens that lie together
 // in the vocabulary spread over the slices.
 // A mass is exp(x) in units of 2^-40 of the first token's, in 64-bit integers:
@@ -31,7 +30,7 @@ namespace {
 constexpr int kSlice = 4096;
 constexpr int kMaxSlices = 256;
 constexpr int kMaxCand = 1024;
-constexpr int kWant = 448;  // candidates wanted of a row
+constexpr int kWant = 384;  // candidates wanted of a row
 typedef unsigned long long u64;
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any logit
 
@@ -66,7 +65,7 @@ BQ_DEV uint32_t ordered(float x) {
 BQ_DEV float unordered(uint32_t o) { return as_float(o ^ (o >> 31 ? 0x80000000u : 0xFFFFFFFFu)); }
 BQ_DEV u64 key_of(float x, int i) { return (u64)ordered(x) << 32 | (0xFFFFFFFFu - (uint32_t)i); }
 BQ_DEV int index_of(u64 key) { return (int)(0xFFFFFFFFu - (uint32_t)key); }
-BQ_DEV u64 mass_of(float x, float mx, float temp) { return (u64)__builtin_rintf(expf((x - mx) / temp) * 0x1p40f); }
+BQ_DEV u64 mass(float e) { return (u64)__builtin_rintf(e * 0x1p40f); }
 BQ_DEV u64 shfl_xor64(u64 v, int d) {
     const uint32_t lo = __shfl_xor((uint32_t)v, d, 64), hi = __shfl_xor((uint32_t)(v >> 32), d, 64);
     return (u64)hi << 32 | lo;
@@ -175,7 +174,8 @@ __global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
     }
     __syncthreads();
     const float mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-    const float t = fmaxf(fmaxf(s_t[0], s_t[1]), fmaxf(s_t[2], s_t[3]));
+    // (any threshold is right; the waves' mean is the steadiest)
+    const float t = (s_t[0] + s_t[1]) * 0.25f + (s_t[2] + s_t[3]) * 0.25f;
     const float least = fmaxf(t, -3.402823466e38f);  // -inf is no candidate
     int count = 0, first = 0x7FFFFFFF;
 #pragma unroll
@@ -253,28 +253,146 @@ BQ_DEV u64 scan1024(u64 v, u64* red, u64& total) {
     return before + s - v;
 }
 
-// The whole row, by radix selection.
+// bitonic sort, descending, of one key per thread; keys past thread n - 1 (a
+// power of two >= 64) are zeros
+BQ_DEV u64 sort_keys(u64 key, int n, u64* s_key) {
+    const int tid = threadIdx.x;
+    int turn = 0;
+    __syncthreads();
+    for (int k = 2; k <= n; k <<= 1) {
+        const bool down = (tid & k) == 0;
+        for (int j = k >> 1; j >= 64; j >>= 1) {
+            // two buffers in turn: one barrier an exchange
+            u64* at = s_key + (turn ^= 1) * kMaxCand;
+            at[tid] = key;
+            __syncthreads();
+            const u64 o = at[tid ^ j];
+            const bool larger = down == ((tid & j) == 0);
+            key = larger == (o > key) ? o : key;
+        }
+        if (tid >= n) continue;  // whole waves
+        if (k >= 64) key = exchange<32>(key, down);
+        if (k >= 32) key = exchange<16>(key, down);
+        if (k >= 16) key = exchange<8>(key, down);
+        if (k >= 8) key = exchange<4>(key, down);
+        if (k >= 4) key = exchange<2>(key, down);
+        key = exchange<1>(key, down);
+    }
+    return key;
+}
+
+// The whole row.  A cut is found in two readings: the weights (1 each, or the
+// masses) in 2048 even bins between the first logit and the last one whose mass
+// counts, then the keys of the bin that the cut falls into, sorted.  Where one
+// bin holds more than 1024 keys (many equal logits), by radix selection on the
+// ordered bits of the logit, then of the index.
 struct Whole {
     const float* x;
     int vocab;
-    float mx, temp;
+    float mx, to_log2, per_bin;  // log2(e) / temperature; bins per unit of logit
     u64* bins;   // [2048]
+    u64* keys;   // [2 kMaxCand]
     u64* red;    // [16]
-    u64* found;  // [2]: the bin, the mass before it
+    u64* found;  // [3]
 
     // f(key, logit) over the logits above -inf
     template <typename F>
     BQ_DEV void each(F f) const {
-        for (int i = threadIdx.x; i < vocab; i += 1024) {
-            const float v = clean(x[i]);
-            if (!(v > -INFINITY)) continue;
-            f(key_of(v, i), v);
+        constexpr int N = 4;  // loads in flight
+        for (int i0 = 4 * threadIdx.x; i0 < vocab; i0 += 4096 * N) {
+            f32x4 a[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int i = i0 + 4096 * k;
+                a[k] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (i + 4 <= vocab) {
+                    a[k] = *(const f32x4u*)(x + i);
+                } else {
+                    for (int e = 0; e < 4; ++e)
+                        if (i + e < vocab) a[k][e] = x[i + e];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float v = clean(a[k][e]);
+                    if (v > -INFINITY) f(key_of(v, i0 + 4096 * k + e), v);
+                }
         }
     }
+    BQ_DEV u64 mass_of(float v) const { return mass(__builtin_amdgcn_exp2f((v - mx) * to_log2)); }
+    BQ_DEV u64 weight(bool by_count, float v) const { return by_count ? 1 : mass_of(v); }
+    BQ_DEV int bin_of(float v) const { return (int)fminf((mx - v) * per_bin, 2047.f); }  // rises as v falls
 
-    // The keys in descending order, each weighing 1 (by_count) or its mass;
-    // the first whose running weight w meets w >= target (or w > target).
-    // Only keys >= low count.  Returns 0 if none does.
+    // weights of the keys >= low into the bins
+    BQ_DEV void fill(bool by_count, u64 low) const {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2048; i += 1024) bins[i] = 0;
+        __syncthreads();
+        each([&](u64 key, float v) {
+            if (key < low) return;
+            const u64 w = weight(by_count, v);
+            if (w) atomicAdd(&bins[bin_of(v)], w);
+        });
+        __syncthreads();
+    }
+    BQ_DEV u64 filled() const {  // their sum
+        u64 total;
+        scan1024(bins[2 * threadIdx.x] + bins[2 * threadIdx.x + 1], red, total);
+        return total;
+    }
+
+    // With the bins filled from the same keys: the first key in descending
+    // order whose running weight meets w >= target (or w > target), and that
+    // weight.  0 if none does; `many` where the bin holds too many.
+    BQ_DEV u64 locate(bool by_count, double target, bool strict, u64 low, u64& upto, bool& many) const {
+        const int tid = threadIdx.x;
+        auto meets = [&](u64 w) { return strict ? (double)w > target : (double)w >= target; };
+        if (tid == 0) found[0] = ~0ull, found[2] = 0;
+        __syncthreads();
+        const u64 a = bins[2 * tid], b = bins[2 * tid + 1];
+        u64 total;
+        const u64 ex = scan1024(a + b, red, total);
+        if (a && !meets(ex) && meets(ex + a)) {
+            found[0] = 2 * tid;
+            found[1] = ex;
+        } else if (b && !meets(ex + a) && meets(ex + a + b)) {
+            found[0] = 2 * tid + 1;
+            found[1] = ex + a;
+        }
+        __syncthreads();
+        const u64 bin = found[0], before = found[1];
+        if (bin == ~0ull) return 0;
+        each([&](u64 key, float v) {
+            if (key < low || bin_of(v) != (int)bin) return;
+            const u64 c = atomicAdd(&found[2], 1ull);
+            if (c < kMaxCand) keys[c] = key;
+        });
+        __syncthreads();
+        const int count = (int)found[2];
+        if (count > kMaxCand) {
+            many = true;
+            return 0;
+        }
+        int n = 64;
+        while (n < count) n <<= 1;
+        u64 key = tid < count ? keys[tid] : 0;
+        key = sort_keys(key, n, keys);
+        const u64 w = tid < count ? weight(by_count, unordered((uint32_t)(key >> 32))) : 0;
+        const u64 at = before + scan1024(w, red, total);
+        if (tid == 0) found[0] = 0;
+        __syncthreads();
+        if (w && !meets(at) && meets(at + w)) {
+            found[0] = key;
+            found[1] = at + w;
+        }
+        __syncthreads();
+        upto = found[1];
+        return found[0];
+    }
+
+    // the same by radix selection
     BQ_DEV u64 select(bool by_count, double target, bool strict, u64 low) const {
         constexpr int kShift[6] = {53, 42, 32, 21, 10, 0}, kBits[6] = {11, 11, 10, 11, 11, 10};
         u64 prefix = 0;   // the digits found so far, in place
@@ -287,7 +405,7 @@ struct Whole {
             __syncthreads();
             each([&](u64 key, float v) {
                 if (key < low || (d && (key ^ prefix) >> (sh + kBits[d]))) return;
-                const u64 w = by_count ? 1 : mass_of(v, mx, temp);
+                const u64 w = weight(by_count, v);
                 if (w) atomicAdd(&bins[(key >> sh) & (nb - 1)], w);
             });
             __syncthreads();
@@ -311,11 +429,22 @@ struct Whole {
         }
         return prefix;
     }
+    // either; bins must be filled from the keys >= low
+    BQ_DEV u64 cut(bool by_count, double target, bool strict, u64 low, u64& upto) const {
+        bool many = false;
+        u64 key = per_bin > 0.f ? locate(by_count, target, strict, low, upto, many) : 0;
+        if (many || !(per_bin > 0.f)) {
+            key = select(by_count, target, strict, low);
+            fill(by_count, low);  // it used the bins
+            if (key && !by_count) upto = mass_from(key);
+        }
+        return key;
+    }
 
     BQ_DEV u64 mass_from(u64 low) const {
         u64 s = 0, total;
         each([&](u64 key, float v) {
-            if (key >= low) s += mass_of(v, mx, temp);
+            if (key >= low) s += mass_of(v);
         });
         scan1024(s, red, total);
         return total;
@@ -323,13 +452,14 @@ struct Whole {
 };
 
 __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
-    __shared__ u64 s_key[kMaxCand], s_bins[2048], s_red[16], s_found[2];
-    __shared__ int s_first[kMaxSlices + 1], s_stop;
+    __shared__ u64 s_key[2 * kMaxCand], s_bins[2048], s_red[16], s_found[3];
+    __shared__ int s_first[kMaxSlices + 1], s_wave[16];
     __shared__ u64 s_best;
-    __shared__ float s_t;
+    __shared__ float s_t, s_least[16];
     __shared__ double s_mass;
     const int tid = threadIdx.x, row = blockIdx.x;
     const RowRule rule = rule_of(p, row);
+    const double u = (double)p.u[row];
     const SliceInfo* info = p.info + (size_t)row * p.slices;
     if (tid < 64) {
         // four slices a lane: the largest key, the largest threshold, where each slice's candidates begin
@@ -368,7 +498,6 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
             s_best = best;
             s_t = t;
             s_mass = mass * 0x1p40;
-            s_stop = kMaxCand + 1;
         }
     }
     __syncthreads();
@@ -380,7 +509,6 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
     }
     const int total = s_first[p.slices];
     const float t = s_t;
-    const double u = (double)p.u[row];
     if (total > 0 && total <= kMaxCand) {
         int n = 64;
         while (n < total) n <<= 1;
@@ -394,29 +522,11 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
             }
             key = p.cand[((size_t)row * p.slices + s) * p.cap + tid - s_first[s]];
         }
-        // bitonic sort, descending, one key per thread
-        for (int k = 2; k <= n; k <<= 1) {
-            const bool down = (tid & k) == 0;
-            for (int j = k >> 1; j >= 64; j >>= 1) {
-                __syncthreads();
-                s_key[tid] = key;
-                __syncthreads();
-                const u64 o = s_key[tid ^ j];
-                const bool larger = down == ((tid & j) == 0);
-                key = larger == (o > key) ? o : key;
-            }
-            if (tid >= n) continue;  // whole waves
-            if (k >= 64) key = exchange<32>(key, down);
-            if (k >= 32) key = exchange<16>(key, down);
-            if (k >= 16) key = exchange<8>(key, down);
-            if (k >= 8) key = exchange<4>(key, down);
-            if (k >= 4) key = exchange<2>(key, down);
-            key = exchange<1>(key, down);
-        }
+        key = sort_keys(key, n, s_key);
         const float x = unordered((uint32_t)(key >> 32));
         const bool in = tid < total;
         const float e = in ? expf((x - mx) / rule.temp) : 0.f;
-        const u64 w = in ? mass_of(x, mx, rule.temp) : 0;
+        const u64 w = mass(e);
         u64 all;
         const u64 ex = scan1024(w, s_red, all);
         s_key[tid] = ex + w;
@@ -428,27 +538,46 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
         const double z = k_sure ? (double)s_key[rule.top_k - 1] : s_mass;
         const bool z_known = rule.top_p >= 1.f || k_sure || rule.top_k == p.vocab || whole;
         const double cut = (double)rule.top_p * (whole && !k_sure ? (double)s_key[total - 1] : z);
-        if (tid <= sure && tid > 0 &&
-            (tid >= rule.top_k || (rule.top_p < 1.f && (double)ex >= cut) || (tid < sure && e < rule.min_p)))
-            atomicMin(&s_stop, tid);
+        const bool stop = tid <= sure && tid > 0 &&
+                          (tid >= rule.top_k || (rule.top_p < 1.f && (double)ex >= cut) || (tid < sure && e < rule.min_p));
+        const u64 stops = __ballot(stop);
+        if ((tid & 63) == 0) s_wave[tid >> 6] = stops ? tid + __builtin_ctzll(stops) : kMaxCand + 1;
         __syncthreads();
-        int kept = s_stop;
+        int kept = kMaxCand + 1;
+#pragma unroll
+        for (int i = 15; i >= 0; --i) kept = min(kept, s_wave[i]);
         if (kept > kMaxCand && whole) kept = total;
         if (z_known && kept <= kMaxCand) {
-            const u64 mass = s_key[kept - 1];
-            const double target = u * (double)mass;
+            const double target = u * (double)s_key[kept - 1];
             if (tid < kept && ((double)(ex + w) > target || tid == kept - 1) && (tid == 0 || !((double)ex > target)))
                 p.out[row] = index_of(key);
             return;
         }
     }
-    // the head was not enough
-    Whole r{p.logits + (size_t)row * p.ld, p.vocab, mx, rule.temp, s_bins, s_red, s_found};
-    u64 low = rule.top_k < p.vocab ? r.select(true, (double)rule.top_k, false, 0) : 0;  // 0: fewer finite ones
+    // the head was not enough: the whole row
+    Whole r{p.logits + (size_t)row * p.ld, p.vocab, mx, 1.44269504088896341f / rule.temp, 0.f, s_bins, s_key, s_red, s_found};
+    float last = INFINITY;
+    r.each([&](u64, float v) { last = fminf(last, v); });
+    last = -wave_max(-last);
+    if ((tid & 63) == 0) s_least[tid >> 6] = last;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) last = fminf(last, s_least[i]);
+    const float range = fminf(mx - last, 32.f * rule.temp);  // e^-32 is below half a unit of mass
+    r.per_bin = range > 0.f ? 2047.f / range : 0.f;
+    u64 low = 0, kept = 0;  // the keys kept are >= low, of mass `kept`
+    if (rule.top_k < p.vocab) {
+        r.fill(true, 0);
+        low = r.cut(true, (double)rule.top_k, false, 0, kept);  // 0: fewer finite ones
+    }
+    r.fill(false, low);
+    kept = r.filled();
+    // from here on only the kept mass changes: the bins serve every cut
+    const u64 from = low;
     if (rule.top_p < 1.f) {
-        const double z = (double)r.mass_from(low);
-        const u64 at = rule.top_p > 0.f ? r.select(false, (double)rule.top_p * z, false, low) : s_best;
-        low = at > low ? at : low;
+        u64 upto = 0;
+        const u64 at = rule.top_p > 0.f ? r.cut(false, (double)rule.top_p * (double)kept, false, from, upto) : s_best;
+        if (!(rule.top_p > 0.f)) upto = mass(1.f);
+        if (at) low = at, kept = upto;
     }
     if (rule.min_p > 0.f) {
         // the smallest key whose weight is at least min_p: weights fall with the key
@@ -464,14 +593,11 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
         if ((tid & 63) == 0) s_red[tid >> 6] = least;
         __syncthreads();
         for (int i = 0; i < 16; ++i) least = s_red[i] < least ? s_red[i] : least;
-        low = least > low ? least : low;
+        if (least > low) low = least, kept = r.mass_from(low);
     }
-    const u64 mass = r.mass_from(low);
-    u64 pick = r.select(false, u * (double)mass, true, low);
-    if (pick == 0) {
-        // u = 1: the last key with a weight
-        pick = r.select(false, (double)mass, false, low);
-    }
+    u64 upto;
+    u64 pick = r.cut(false, u * (double)kept, true, from, upto);
+    if (pick < low) pick = r.cut(false, (double)kept, false, from, upto);  // u = 1: the last kept key with a mass
     if (tid == 0) p.out[row] = pick ? index_of(pick) : index_of(s_best);
 }
 
