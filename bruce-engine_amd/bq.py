@@ -204,7 +204,7 @@ def load(path=LIB_PATH):
         "bq_append": (I, [P, P, P]),
         "bq_kv_read": (I, [P, P, P, I, P, P, P]),
         "bq_attn_workspace_bytes": (S, [I, I, I, I, I, I]),
-        "bq_attn_prefill_workspace_bytes": (S, [I] * 7),
+        "bq_attn_prefill_workspace_bytes": (S, [I] * 8),
         "bq_attn_decode": (I, [P, P, P]),
         "bq_attn_prefill": (I, [P, P, P]),
         "bq_attn_hook": (None, [P, I, P]),
@@ -754,7 +754,8 @@ class Attention:
             if row0 is None:
                 n = L.bq_attn_workspace_bytes(n_seq, rows, width // D, kv.kv_heads, D, max_len)
             if row0 is not None or n_seq == 1:
-                n = max(n, L.bq_attn_prefill_workspace_bytes(n_seq, rows, n_rows, width // D, kv.kv_heads, D, max_len))
+                n = max(n, L.bq_attn_prefill_workspace_bytes(kv.struct.type, n_seq, rows, n_rows, width // D,
+                                                              kv.kv_heads, D, max_len))
             work = torch.empty(n // 4, dtype=torch.float32, device=q.device) if n else None
         self.kv, self._keep = kv, (q, out, kv_len, row0, work)
         self.struct = AttnArgs(_ptr(q), _ptr(out), _type_of(q, "q"), _type_of(out, "out"), _rows_ld(q, width, "q"),

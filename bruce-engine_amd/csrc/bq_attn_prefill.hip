@@ -28,6 +28,11 @@ namespace bq {
 
 namespace {
 constexpr int kBN = 64;          // tokens of a tile
+// a q8 cache's tiles turned into the products' operands ahead of the attention:
+// fp16 keys and bf16 values as they lie in LDS, what the tokens' scores are
+// multiplied by, and the mask of unmapped tokens
+constexpr int kKvStaged = 2;
+constexpr int64_t tile_record(int D) { return 4 * kBN * D + 512; }
 constexpr int kPiece = 8;        // tiles of a piece at least, where the tokens are split
 constexpr float kNone = -1e30f;  // the running maximum before any token
 constexpr float kLazy = 8.f;     // it moves when a score passes it by more (log2)
@@ -41,6 +46,8 @@ struct PrefillP {
     const int32_t* kv_len;
     float* part;  // nsplit > 1: [nsplit][n_rows][q_heads][D], then [..][2] (m, l)
     int64_t ml;   // floats before the (m, l) part
+    char* stage;  // kKvStaged: [n_seq][heads][stage_tiles] records of a tile
+    int stage_tiles;
     int G, q_heads, n_rows, max_rows, max_len, window, sinks, q_bf16, out_bf16, nsplit;
     float scale;  // scale * log2(e)
 };
@@ -81,10 +88,80 @@ BQ_DEV void store4(const PrefillP& p, size_t at, f32x4 y, float l) {
         *(f32x4*)((float*)p.out + at) = y;
 }
 
-template <int D, int KV, int W>
-__global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_attn_prefill(PrefillP p) {
-    constexpr int KS = D / 16, DT = D / 32, BM = 32 * W, T = 64 * W;
-    constexpr bool Q8 = KV == kKvQ8;
+// 2^e of a q8 token's largest key scale, from its bf16 bits
+BQ_DEV int key_power(uint32_t top) { return max(-100, min(100, (int)(top >> 7) - 127)); }
+// 16 key codes (dims 64c + 8g.. and 64c + 32 + 8g..) times two scales over the token's power of two
+BQ_DEV u32x4 half_keys(u32x4 codes, int k, uint16_t scale, float down) {
+    const _Float16 sh = (_Float16)(bf2f(scale) * down);
+    const u32x2 a = dequant4h(codes[2 * k], f16x2{sh, sh}), b = dequant4h(codes[2 * k + 1], f16x2{sh, sh});
+    return u32x4{a[0], a[1], b[0], b[1]};
+}
+// 8 tokens' codes of a value's dim times their scales
+BQ_DEV u32x4 bf16_values(u32x4 codes, int k, u32x4 scales) {
+    float y[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) y[x] = as_float(x & 1 ? scales[x >> 1] & 0xFFFF0000u : scales[x >> 1] << 16);
+    const u32x2 a = dequant4(codes[2 * k], y[0], y[1], y[2], y[3]), b = dequant4(codes[2 * k + 1], y[4], y[5], y[6], y[7]);
+    return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// One 64-token tile of one head into its record.  Every row tile of a prompt
+// reads the tile again: converting it there each time costs as many vector
+// instructions as the softmax, so it is done once, in a launch of its own, where
+// there are enough row tiles (kStageRows).
+template <int D>
+__global__ void __launch_bounds__(256) k_stage_q8(PrefillP p) {
+    const KvView& kv = p.kv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tile = blockIdx.x, h = blockIdx.y, seq = blockIdx.z, P = kv.P;
+    const int b0 = p.row0 ? p.row0[seq] : 0, b1 = p.row0 ? p.row0[seq + 1] : p.n_rows;
+    const int base = min(max(b0, 0), p.n_rows), rows = min(min(max(b1, 0), p.n_rows) - base, p.max_rows);
+    const int len = min(max(p.kv_len[seq], 0), min(p.max_len, kv.max_pages << kv.plog));
+    const int t0 = tile * kBN;
+    if (rows <= 0 || t0 >= len) return;
+    if (p.window && t0 + kBN <= len - rows - p.window + 1 && t0 >= p.sinks) return;  // no row sees it
+    char* rec = p.stage + (((size_t)seq * kv.heads + h) * p.stage_tiles + tile) * tile_record(D);
+    const int pid = t0 + lane < len ? kv_page(kv, seq, t0 + lane) : -1, tk = (t0 + lane) & (P - 1);
+    const char* head = kv.pages + (size_t)h * kv.head_bytes;
+    const char* kb = head + (int64_t)max(pid, 0) * kv.page_bytes;
+    uint16_t ks[D / 32];
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+        ks[e] = *(const uint16_t*)(kb + kv_ks_off(P, D, e, tk));
+        top = max(top, (uint32_t)ks[e]);
+    }
+    const int ex = key_power(top);
+    const uint64_t bad = __ballot(pid < 0);
+    if (wave == 0) {
+        float* tail = (float*)(rec + 4 * kBN * D);
+        tail[lane] = pow2(ex);
+        if (lane == 0) *(uint64_t*)(tail + kBN) = bad;
+    }
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+        const int u = wave + 4 * e, cc = u >> 2, g = u & 3;
+        const u32x4 codes = *(const u32x4*)(kb + kv_kq_unit(P, cc, g, tk));
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            *(u32x4*)(rec + ((8 * cc + 4 * k + g) * kBN + lane) * 16) = half_keys(codes, k, ks[2 * cc + k], pow2(-ex));
+    }
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+        const int u = tid + 256 * e, m = u % 16, cc = u / 16 % (D / 32), t8 = u / (D / 2), tv = (t0 + 8 * t8) & (P - 1);
+        const char* vb = head + (int64_t)max(__shfl(pid, 8 * t8, 64), 0) * kv.page_bytes;
+        const u32x4 codes = *(const u32x4*)(vb + kv_vq_unit(P, D, tv >> 3, cc, m)), sc = *(const u32x4*)(vb + kv_vs_off(P, D, cc, tv));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) *(u32x4*)(rec + 2 * kBN * D + (t8 * D + 32 * cc + 16 * k + m) * 16) = bf16_values(codes, k, sc);
+    }
+}
+
+// KT = 2: two waves share 32 query rows, each with half of a tile's tokens, and
+// join at the end; a workgroup then has 64 rows and a tile takes half as long.
+template <int D, int KV, int W, int KT>
+__global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) k_attn_prefill(PrefillP p) {
+    constexpr int KS = D / 16, DT = D / 32, BM = 32 * W / KT, T = 64 * W;
+    constexpr int NT = 2 / KT;                         // 32-token parts of a tile that a wave takes
+    constexpr bool Q8 = KV == kKvQ8, STAGED = KV == kKvStaged, HALF = KV != kKvBf16;  // HALF: fp16 scores
     constexpr int NU = D / 8 / W;                      // 1 KiB units of K (and of V) that a wave copies
     constexpr int NQ8 = D / 64 * 4 / W > 0 ? D / 64 * 4 / W : 1;  // q8 units of a thread
     __shared__ __attribute__((aligned(16))) char s_k[2][kBN * D * 2], s_v[2][kBN * D * 2];
@@ -99,7 +176,8 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_att
     if (rows <= 0 || first >= M) return;
     const int len = min(max(p.kv_len[seq], 0), min(p.max_len, kv.max_pages << kv.plog));
     const int last = min(M, first + BM) - 1;
-    const int r = min(first + wave * 32 + c, last), i = r / p.G;
+    const int group = wave / KT, part = wave % KT, row32 = group * 32 + c;
+    const int r = min(first + row32, last), i = r / p.G;
     const int pos = len - rows + i, pfirst = len - rows + first / p.G, plast = len - rows + last / p.G;
     const size_t qat = (size_t)(base + i) * p.ldq + (size_t)(h * p.G + r % p.G) * D;
 
@@ -107,7 +185,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_att
     // a power of two, which comes back in `scale`
     u32x4 q[KS];
     float scale = p.scale;
-    if constexpr (!Q8) {
+    if constexpr (!HALF) {
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             if (p.q_bf16) {
@@ -162,12 +240,29 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_att
     // staging.  pid: the page of token tile0 + lane (-1: none)
     u32x4 rk[NQ8], rv[NQ8], rvs[NQ8];
     uint16_t rks[D / 32];
-    auto page_at = [&](int v) { return v < n ? kv_page(kv, seq, tile0(v) + lane) : -1; };
+    auto page_at = [&](int v) {
+        if (v >= n) return -1;
+        if constexpr (STAGED) {  // the record's mask stands for the pages
+            const uint64_t mask = *(const uint64_t*)(p.stage + (((size_t)seq * kv.heads + h) * p.stage_tiles + tile0(v) / kBN) * tile_record(D) + 4 * kBN * D + 4 * kBN);
+            return mask >> lane & 1 ? -1 : 0;
+        } else {
+            return kv_page(kv, seq, tile0(v) + lane);
+        }
+    };
     auto fetch = [&](int v, int pid, int buf) {
         const int t0 = tile0(v) & (P - 1);  // token of the page where the tile starts (0 for pages below a tile)
         const int tk = (t0 + lane) & (P - 1);
         const char* head = kv.pages + (size_t)h * kv.head_bytes;
-        if constexpr (!Q8) {
+        if constexpr (STAGED) {
+            const char* rec = p.stage + (((size_t)seq * kv.heads + h) * p.stage_tiles + tile0(v) / kBN) * tile_record(D);
+#pragma unroll
+            for (int e = 0; e < NU; ++e)
+                copy_lds_row(rec + wave * 1024, 16 * lane + e * (W * 1024), s_k[buf] + wave * 1024 + e * (W * 1024));
+#pragma unroll
+            for (int e = 0; e < NU; ++e)
+                copy_lds_row(rec + 2 * kBN * D + wave * 1024, 16 * lane + e * (W * 1024), s_v[buf] + wave * 1024 + e * (W * 1024));
+            if (wave == 0 && lane < 16) copy_lds_row(rec + 4 * kBN * D, 16 * lane, s_mul[buf]);
+        } else if constexpr (!Q8) {
             const char* kl = s_k[buf] + wave * 1024;
             const char* vl = s_v[buf] + wave * 1024;
             if (P >= kBN) {  // one page: rows of 1 KiB at addresses of the wave
@@ -217,7 +312,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_att
             uint32_t top = 0;
 #pragma unroll
             for (int e = 0; e < D / 32; ++e) top = max(top, (uint32_t)rks[e]);
-            const int ex = max(-100, min(100, (int)(top >> 7) - 127));
+            const int ex = key_power(top);
             const float down = pow2(-ex);
             if (wave == 0) s_mul[buf][lane] = pow2(ex);
 #pragma unroll
@@ -225,25 +320,15 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_att
                 const int u = wave + W * e, cc = u >> 2, g = u & 3;
                 if (u >= D / 16) break;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const _Float16 sh = (_Float16)(bf2f(rks[2 * cc + k]) * down);
-                    const f16x2 s = {sh, sh};
-                    const u32x2 a = dequant4h(rk[e][2 * k], s), b = dequant4h(rk[e][2 * k + 1], s);
-                    *(u32x4*)(s_k[buf] + ((8 * cc + 4 * k + g) * kBN + lane) * 16) = u32x4{a[0], a[1], b[0], b[1]};
-                }
+                for (int k = 0; k < 2; ++k)
+                    *(u32x4*)(s_k[buf] + ((8 * cc + 4 * k + g) * kBN + lane) * 16) = half_keys(rk[e], k, rks[2 * cc + k], down);
             }
 #pragma unroll
             for (int e = 0; e < NQ8; ++e) {
                 const int u = tid + T * e, m = u % 16, cc = u / 16 % (D / 32), t8 = u / (D / 2);
                 if (t8 >= kBN / 8) break;
-                float s[8];
 #pragma unroll
-                for (int x = 0; x < 8; ++x) s[x] = as_float(x & 1 ? rvs[e][x >> 1] & 0xFFFF0000u : rvs[e][x >> 1] << 16);
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const u32x2 a = dequant4(rv[e][2 * k], s[0], s[1], s[2], s[3]), b = dequant4(rv[e][2 * k + 1], s[4], s[5], s[6], s[7]);
-                    *(u32x4*)(s_v[buf] + (t8 * D + 32 * cc + 16 * k + m) * 16) = u32x4{a[0], a[1], b[0], b[1]};
-                }
+                for (int k = 0; k < 2; ++k) *(u32x4*)(s_v[buf] + (t8 * D + 32 * cc + 16 * k + m) * 16) = bf16_values(rv[e], k, rvs[e]);
             }
         }
     };
@@ -270,30 +355,32 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_att
         pid = pid_next;
         if (v + 1 < n) fetch(v + 1, pid, buf ^ 1);
         pid_next = page_at(v + 2);
-        const char* kp = s_k[buf] + (hf * kBN + krow) * 16;
-        const char* vp = s_v[buf] + (hf * D + c) * 16;
+        const char* kp = s_k[buf] + (hf * kBN + 32 * NT * part + krow) * 16;
+        const char* vp = s_v[buf] + ((4 * NT * part + hf) * D + c) * 16;
         // the wave that is on the matrix pipe goes first: its partner on the SIMD
         // (another workgroup's) then has the vector pipe while it waits for results
         if constexpr (!Q8) __builtin_amdgcn_s_setprio(1);
-        f32x16 s[2];
+        f32x16 s[NT];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0.f;
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < NT; ++t) {
                 const u32x4 kf = *(const u32x4*)(kp + (2 * k * kBN + 32 * t) * 16);
-                if constexpr (Q8)
+                if constexpr (HALF)
                     s[t] = mfma32h(__builtin_bit_cast(f16x8, kf), __builtin_bit_cast(f16x8, q[k]), s[t]);
                 else
                     s[t] = mfma32(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, q[k]), s[t]);
             }
         if constexpr (!Q8) __builtin_amdgcn_s_setprio(0);
-        // s[t][8u + e]: token t0 + 32t + 16u + 8hf + e
-        if constexpr (Q8) {
-            const float* mp = s_mul[buf] + 8 * hf;
+        // s[t][8u + e]: token t0 + 32 (NT part + t) + 16u + 8hf + e
+        if constexpr (HALF) {
+            const float* mp = s_mul[buf] + 32 * NT * part + 8 * hf;
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
+            for (int e = 0; e < 16 * NT; e += 4) {
                 const f32x4 y = *(const f32x4*)(mp + 32 * (e >> 4) + 16 * (e >> 3 & 1) + (e & 4));
 #pragma unroll
                 for (int x = 0; x < 4; ++x) s[e >> 4][(e & 15) + x] *= y[x];
@@ -302,10 +389,10 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_att
         if (bad != 0 || t0 + kBN - 1 > pfirst || (p.window && t0 <= plast - p.window && t0 + kBN > p.sinks)) {
             // at an edge of what the rows see
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int at = 32 * t + 16 * (e >> 3) + 8 * hf + (e & 7), tok = t0 + at;
+                    const int at = 32 * (NT * part + t) + 16 * (e >> 3) + 8 * hf + (e & 7), tok = t0 + at;
                     const bool me = (!(bad >> at & 1)) & (tok <= pos) & ((!p.window) | (tok > pos - p.window) | (tok < p.sinks));
                     s[t][e] = me ? s[t][e] : -INFINITY;
                 }
@@ -327,7 +414,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_att
         }
         float mx = s[0][0];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
         mx *= scale;
@@ -340,7 +427,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_att
             for (int d = 0; d < DT; ++d) o[d] *= al;
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < 2 * NT; ++u) {
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -355,7 +442,31 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? (W == 4 ? 2 : 1) : 1) k_att
     }
 
     l += __shfl_xor(l, 32, 64);
-    if (first + wave * 32 + c > last) return;
+    if constexpr (KT == 2) {
+        // the second part's sums to the first, through the key buffers
+        float* so = (float*)s_k + group * (DT * 16 * 64) + lane;
+        float* sm = (float*)s_v + group * 128 + lane;
+        __syncthreads();
+        if (part == 1) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) so[(16 * d + e) * 64] = o[d][e];
+            sm[0] = m;
+            sm[64] = l;
+        }
+        __syncthreads();
+        if (part == 1) return;
+        const float mt = fmaxf(m, sm[0]);
+        const float fa = __builtin_amdgcn_exp2f(m - mt), fb = __builtin_amdgcn_exp2f(sm[0] - mt);
+        l = l * fa + sm[64] * fb;
+        m = mt;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = o[d][e] * fa + so[(16 * d + e) * 64] * fb;
+    }
+    if (first + row32 > last) return;
     if (p.nsplit > 1) {
         const size_t to = ((size_t)split * p.n_rows + base + i) * p.q_heads + h * p.G + r % p.G;
         if (hf == 0) *(u32x2*)(p.part + p.ml + to * 2) = u32x2{__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, l)};
@@ -405,18 +516,41 @@ __global__ void __launch_bounds__(256) k_attn_prefill_join(PrefillP p) {
 }
 
 constexpr int kW = 4;  // waves of a workgroup
+// 512 rows of 32 + 4 heads over 4000 tokens 84 us converting on the way, 66
+// ahead; 128 rows 39 and 41, 64 rows 31 and 37
+constexpr int kStageRows = 2048;
+
+// Row tiles of 32 kW rows; of half that, shared by pairs of waves, where the
+// launch would leave CUs without a workgroup, or with one where the tokens are
+// not split (512 rows: 19.7 us with whole tiles, 16.4 with half ones; 1500 rows
+// 47 / 40; 512 rows over 4000 tokens in four pieces 59 / 78)
+bool half_tiles(int64_t tiles, int nsplit, int cus) { return nsplit == 1 ? tiles <= 2 * cus : tiles * nsplit <= cus; }
 
 template <int D, int KV>
-hipError_t launch_of(const PrefillP& p, hipStream_t st) {
-    const int64_t tiles = ((int64_t)p.max_rows * p.G + 32 * kW - 1) / (32 * kW);
-    launch_kernel((k_attn_prefill<D, KV, kW>), dim3(p.kv.heads, (uint32_t)tiles, p.kv.n_seq * p.nsplit), dim3(64 * kW), 0, st, p);
-    hipError_t e = hipGetLastError();
+hipError_t launch_of(const PrefillP& p, int cus, hipStream_t st) {
+    const int64_t rows = (int64_t)p.max_rows * p.G;
+    const int64_t tiles = (rows + 32 * kW - 1) / (32 * kW), halves = (rows + 16 * kW - 1) / (16 * kW);
+    hipError_t e = hipSuccess;
+    if constexpr (KV == kKvStaged) {
+        launch_kernel((k_stage_q8<D>), dim3(p.stage_tiles, p.kv.heads, p.kv.n_seq), dim3(256), 0, st, p);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    if (half_tiles(tiles * p.kv.heads * p.kv.n_seq, p.nsplit, cus))
+        launch_kernel((k_attn_prefill<D, KV, kW, 2>), dim3(p.kv.heads, (uint32_t)halves, p.kv.n_seq * p.nsplit), dim3(64 * kW), 0, st, p);
+    else
+        launch_kernel((k_attn_prefill<D, KV, kW, 1>), dim3(p.kv.heads, (uint32_t)tiles, p.kv.n_seq * p.nsplit), dim3(64 * kW), 0, st, p);
+    e = hipGetLastError();
     if (e == hipSuccess && p.nsplit > 1) {
         const int64_t n = (int64_t)p.n_rows * p.q_heads * (D / 4);
         launch_kernel((k_attn_prefill_join<D>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, p);
         e = hipGetLastError();
     }
     return e;
+}
+template <int D>
+hipError_t launch_d(const PrefillP& p, int type, int cus, hipStream_t st) {
+    if (type == kKvBf16) return launch_of<D, kKvBf16>(p, cus, st);
+    return p.stage ? launch_of<D, kKvStaged>(p, cus, st) : launch_of<D, kKvQ8>(p, cus, st);
 }
 }  // namespace
 
@@ -430,20 +564,29 @@ int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, 
 }
 size_t prefill_part_floats(int n_rows, int q_heads, int D) { return (size_t)n_rows * q_heads * (D + 2); }
 
-hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st) {
+// Bytes of a q8 cache's converted tiles, 0 where they are converted as they are
+// read: below kStageRows rows of a head group, or beyond 1 GiB.
+size_t prefill_stage_bytes(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int max_len) {
+    if (type != kKvQ8 || (int64_t)rows * (q_heads / kv_heads) < kStageRows) return 0;
+    const size_t n = (size_t)n_seq * kv_heads * ((max_len + kBN - 1) / kBN) * tile_record(D);
+    return n <= (size_t)1 << 30 ? n : 0;
+}
+
+hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, size_t stage_bytes, int nsplit, int cus, hipStream_t st) {
     PrefillP p;
     p.kv = kv;
     p.q = a.q; p.out = a.out; p.ldq = a.ldq; p.ldo = a.ldo; p.row0 = a.row0; p.kv_len = a.kv_len;
-    p.nsplit = nsplit; p.part = (float*)a.work; p.ml = (int64_t)nsplit * a.n_rows * a.q_heads * kv.D;
+    p.stage = stage_bytes ? (char*)a.work : nullptr;
+    p.stage_tiles = (a.max_len + kBN - 1) / kBN;
+    p.nsplit = nsplit; p.part = (float*)((char*)a.work + stage_bytes); p.ml = (int64_t)nsplit * a.n_rows * a.q_heads * kv.D;
     p.q_heads = a.q_heads; p.G = a.q_heads / kv.heads; p.n_rows = a.n_rows; p.max_rows = std::min(a.rows, a.n_rows); p.max_len = a.max_len;
     p.window = a.window; p.sinks = a.sinks;
     p.q_bf16 = a.q_type == BQ_TYPE_BF16; p.out_bf16 = a.out_type == BQ_TYPE_BF16;
     p.scale = a.scale * 1.44269504088896341f;
-    const bool q8 = type == kKvQ8;
     switch (kv.D) {
-        case 64: return q8 ? launch_of<64, kKvQ8>(p, st) : launch_of<64, kKvBf16>(p, st);
-        case 128: return q8 ? launch_of<128, kKvQ8>(p, st) : launch_of<128, kKvBf16>(p, st);
-        default: return q8 ? launch_of<256, kKvQ8>(p, st) : launch_of<256, kKvBf16>(p, st);
+        case 64: return launch_d<64>(p, type, cus, st);
+        case 128: return launch_d<128>(p, type, cus, st);
+        default: return launch_d<256>(p, type, cus, st);
     }
 }
 

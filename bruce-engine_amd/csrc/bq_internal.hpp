@@ -147,7 +147,10 @@ size_t decode_part_floats(int n_seq, int rows, int q_heads, int kv_heads, int D)
 hipError_t launch_attn_decode(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st);
 int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus);
 size_t prefill_part_floats(int n_rows, int q_heads, int D);
-hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st);
+size_t prefill_stage_bytes(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int max_len);
+// work: stage_bytes of converted tiles (0: none), then the pieces
+hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, size_t stage_bytes, int nsplit, int cus,
+                               hipStream_t st);
 
 size_t sample_work_bytes(int rows, int vocab);
 hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, const float* temp, const int32_t* top_k,

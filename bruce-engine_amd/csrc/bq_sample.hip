@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
         }
     }
     // the head was not enough: the whole row
-    Whole r{p.logits + (size_t)row * p.ld, p.vocab, mx, 1.44269504088896341f / rule.temp, 0.f, s_bins, s_key, s_red, s_found};
+    Whole r{p.logits + (size_t)row * p.ld, p.vocab, mx, fminf(1.44269504088896341f / rule.temp, 3e38f), 0.f, s_bins, s_key, s_red, s_found};
     float last = INFINITY;
     r.each([&](u64, float v) { last = fminf(last, v); });
     last = -wave_max(-last);

@@ -105,12 +105,14 @@ size_t bq_attn_workspace_bytes(int n_seq, int rows, int q_heads, int kv_heads, i
     return n > 1 ? n * decode_part_floats(n_seq, rows, q_heads, kv_heads, head_dim) * sizeof(float) : 0;
 }
 
-size_t bq_attn_prefill_workspace_bytes(int n_seq, int rows, int n_rows, int q_heads, int kv_heads, int head_dim, int max_len) {
+size_t bq_attn_prefill_workspace_bytes(int type, int n_seq, int rows, int n_rows, int q_heads, int kv_heads, int head_dim, int max_len) {
     if (n_seq <= 0 || rows < 1 || n_rows < 1 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0 ||
         max_len < 0 || device_ready() != BQ_OK)
         return 0;
     const int n = prefill_splits(n_seq, std::min(rows, n_rows), q_heads, kv_heads, max_len, device_cus());
-    return n > 1 ? n * prefill_part_floats(n_rows, q_heads, head_dim) * sizeof(float) : 0;
+    const size_t parts = n > 1 ? n * prefill_part_floats(n_rows, q_heads, head_dim) * sizeof(float) : 0;
+    return parts + prefill_stage_bytes(type == BQ_TYPE_Q8_0 ? kKvQ8 : kKvBf16, n_seq, std::min(rows, n_rows), q_heads, kv_heads,
+                                       head_dim, max_len);
 }
 
 int bq_attn_decode(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t st) {
@@ -142,12 +144,15 @@ int bq_attn_prefill(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t 
     if (a.n_rows == 0) return BQ_OK;
     if ((int64_t)a.rows * (a.q_heads / kv.heads) > INT32_MAX / 2) return BQ_UNSUPPORTED;
     if (!al16(a.work) || (a.work_bytes && !a.work)) return BQ_EINVAL;
+    // the converted tiles first, the pieces in what is left
+    size_t stage = prefill_stage_bytes(type, kv.n_seq, std::min(a.rows, a.n_rows), a.q_heads, kv.heads, kv.D, a.max_len);
+    if (stage > a.work_bytes) stage = 0;
     int n = prefill_splits(kv.n_seq, std::min(a.rows, a.n_rows), a.q_heads, kv.heads, a.max_len, device_cus());
     const size_t part = prefill_part_floats(a.n_rows, a.q_heads, kv.D) * sizeof(float);
-    n = (int)std::min<size_t>(n, std::max<size_t>(1, a.work_bytes / part));
+    n = (int)std::min<size_t>(n, std::max<size_t>(1, (a.work_bytes - stage) / part));
     // (sequence, piece) is one grid dimension
     n = std::max(1, std::min(n, 65535 / kv.n_seq));
-    return from_hip(launch_attn_prefill(kv, type, a, n, (hipStream_t)st));
+    return from_hip(launch_attn_prefill(kv, type, a, stage, n, device_cus(), (hipStream_t)st));
 }
 
 void bq_attn_hook(void* user, int block, bq_stream_t st) {

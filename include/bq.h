@@ -532,8 +532,9 @@ int bq_kv_read(const bq_kv_cache* kv, const int32_t* seq, const int32_t* pos, in
  *     q and the softmax weights enter the products as bf16; over a q8 cache q
  *     and the keys as fp16 (each row over a power of two of its own, so the
  *     range stays fp32's) and the values as bf16.  Sums are fp32.  A few rows
- *     over many tokens are split over workgroups too (work:
- *     bq_attn_prefill_workspace_bytes, or less as above).
+ *     over many tokens are split over workgroups too, and many rows over a q8
+ *     cache convert its tokens once, into work (bq_attn_prefill_workspace_bytes;
+ *     with less, or NULL, a smaller split and conversion on the way).
  * scale > 0.  q_heads % kv_heads == 0 and q_heads / kv_heads <= 64, else BQ_UNSUPPORTED.
  * Row strides in elements, multiples of 8. */
 typedef struct bq_attn_args {
@@ -551,8 +552,8 @@ typedef struct bq_attn_args {
     size_t work_bytes;
 } bq_attn_args;
 size_t bq_attn_workspace_bytes(int n_seq, int rows, int q_heads, int kv_heads, int head_dim, int max_len);
-/* for a ragged batch of at most `rows` rows a sequence, n_rows in all */
-size_t bq_attn_prefill_workspace_bytes(int n_seq, int rows, int n_rows, int q_heads, int kv_heads, int head_dim,
+/* for a ragged batch of at most `rows` rows a sequence, n_rows in all, over a cache of this type */
+size_t bq_attn_prefill_workspace_bytes(int type, int n_seq, int rows, int n_rows, int q_heads, int kv_heads, int head_dim,
                                        int max_len);
 int bq_attn_decode(const bq_kv_cache* kv, const bq_attn_args* a, bq_stream_t st);
 int bq_attn_prefill(const bq_kv_cache* kv, const bq_attn_args* a, bq_stream_t st);

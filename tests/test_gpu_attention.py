@@ -148,7 +148,8 @@ def test_decode_clamps_length(bq):
             _check(got[s], *ref, True, f"clamped {max_len} seq {s}")
 
 
-def _prefill(bq, kv, rows, past, Hq, H, D, P, qt, ot, window=0, sinks=0, seed=1, holes=(), pad=0, max_rows=None):
+def _prefill(bq, kv, rows, past, Hq, H, D, P, qt, ot, window=0, sinks=0, seed=1, holes=(), pad=0, max_rows=None,
+             work="auto"):
     n = len(rows)
     lens = [a + b for a, b in zip(rows, past)]
     pages = R.Pages(kv, H, D, P, n, max(1, (max(lens) + P - 1) // P + 1), seed)
@@ -165,7 +166,7 @@ def _prefill(bq, kv, rows, past, Hq, H, D, P, qt, ot, window=0, sinks=0, seed=1,
     out = torch.full((total, Hq * D + pad), float("nan"), dtype=DT[ot], device="cuda")
     row0 = torch.tensor(np.concatenate([[0], np.cumsum(rows)]), dtype=torch.int32, device="cuda")
     bq.Attention(cache, gq[:, : Hq * D], out[:, : Hq * D], torch.tensor(lens, dtype=torch.int32, device="cuda"),
-                 window=window, sinks=sinks, row0=row0, max_rows=max_rows or max(rows)).prefill()
+                 window=window, sinks=sinks, row0=row0, max_rows=max_rows or max(rows), work=work).prefill()
     torch.cuda.synchronize()
     if pad:
         assert torch.isnan(out[:, Hq * D:]).all()
@@ -208,6 +209,25 @@ def test_prefill_window_and_sinks(bq, kv, window, sinks):
 def test_prefill_unmapped_pages_and_wide_bound(bq):
     _prefill(bq, "bf16", [60, 20], [100, 12], 8, 2, 128, 16, "bf16", "bf16", seed=6, holes=[(0, 0), (0, 6), (1, 0), (1, 1)])
     _prefill(bq, "q8", [60, 20], [100, 12], 8, 2, 64, 64, "bf16", "bf16", seed=6, holes=[(0, 1)], max_rows=400)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "q8"])
+@pytest.mark.parametrize("D,Hq,H,P", [(64, 4, 4, 16), (128, 8, 2, 64), (256, 6, 2, 32)])
+def test_prefill_split(bq, kv, D, Hq, H, P):
+    """Few rows over many tokens: pieces and their join, without a workspace, and with room for two pieces."""
+    for work in ("auto", None, torch.empty(2 * 50 * Hq * (D + 2) + 9, device="cuda")):
+        _prefill(bq, kv, [40, 0, 9, 1], [1500, 3, 700, 0], Hq, H, D, P, "bf16", "bf16", seed=D, work=work)
+    _prefill(bq, kv, [33], [2100], Hq, H, D, P, "f32", "f32", 1300, 70, seed=D + 1)
+    _prefill(bq, kv, [33, 12], [1900, 800], Hq, H, D, P, "bf16", "bf16", seed=D + 2, holes=[(0, 0), (0, 9), (1, 4)])
+
+
+@pytest.mark.parametrize("D,Hq,H,P", [(64, 8, 1, 16), (128, 16, 2, 64), (256, 8, 1, 32), (128, 8, 1, 256)])
+def test_prefill_many_rows_over_q8(bq, D, Hq, H, P):
+    """Enough rows for the q8 tiles to be converted ahead; without the workspace they are converted on the way."""
+    for work in ("auto", None):
+        _prefill(bq, "q8", [260, 5, 0], [100, 400, 7], Hq, H, D, P, "bf16", "bf16", seed=D, work=work)
+    _prefill(bq, "q8", [270], [150], Hq, H, D, P, "f32", "f32", 90, 20, seed=D + 1)
+    _prefill(bq, "q8", [256, 40], [130, 60], Hq, H, D, P, "bf16", "bf16", seed=D + 2, holes=[(0, 0), (1, 0)])
 
 
 def test_prefill_one_sequence_without_row0(bq):
