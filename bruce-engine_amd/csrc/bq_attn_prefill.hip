@@ -52,6 +52,13 @@ struct PrefillP {
     float scale;  // scale * log2(e)
 };
 
+// a sequence's rows of q and out, kept inside the buffers whatever row0 holds
+BQ_DEV void rows_of(const PrefillP& p, int seq, int& base, int& rows) {
+    const int b0 = p.row0 ? p.row0[seq] : 0, b1 = p.row0 ? p.row0[seq + 1] : p.n_rows;
+    base = min(max(b0, 0), p.n_rows);
+    rows = min(min(max(b1, 0), p.n_rows) - base, p.max_rows);
+}
+
 BQ_DEV f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 BQ_DEV f32x16 mfma32h(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
@@ -113,8 +120,8 @@ template <int D>
 __global__ void __launch_bounds__(256) k_stage_q8(PrefillP p) {
     const KvView& kv = p.kv;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tile = blockIdx.x, h = blockIdx.y, seq = blockIdx.z, P = kv.P;
-    const int b0 = p.row0 ? p.row0[seq] : 0, b1 = p.row0 ? p.row0[seq + 1] : p.n_rows;
-    const int base = min(max(b0, 0), p.n_rows), rows = min(min(max(b1, 0), p.n_rows) - base, p.max_rows);
+    int base, rows;
+    rows_of(p, seq, base, rows);
     const int len = min(max(p.kv_len[seq], 0), min(p.max_len, kv.max_pages << kv.plog));
     const int t0 = tile * kBN;
     if (rows <= 0 || t0 >= len) return;
@@ -169,9 +176,8 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) k_attn_prefill(Prefi
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hf = lane >> 5;
     const KvView& kv = p.kv;
     const int seq = blockIdx.z / p.nsplit, split = blockIdx.z % p.nsplit, h = blockIdx.x, P = kv.P;
-    const int b0 = p.row0 ? p.row0[seq] : 0, b1 = p.row0 ? p.row0[seq + 1] : p.n_rows;
-    // a sequence's rows, kept inside the buffers whatever row0 holds
-    const int base = min(max(b0, 0), p.n_rows), rows = min(min(max(b1, 0), p.n_rows) - base, p.max_rows);
+    int base, rows;
+    rows_of(p, seq, base, rows);
     const int M = rows * p.G, first = (int)(gridDim.y - 1 - blockIdx.y) * BM;
     if (rows <= 0 || first >= M) return;
     const int len = min(max(p.kv_len[seq], 0), min(p.max_len, kv.max_pages << kv.plog));
@@ -490,17 +496,12 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) k_attn_prefill(Prefi
 // joins the pieces of the rows, in their order: a lane has 4 dims of one row and head
 template <int D>
 __global__ void __launch_bounds__(256) k_attn_prefill_join(PrefillP p) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, at = e / (D / 4), rows = (int64_t)p.n_rows * p.q_heads;
-    if (at >= rows) return;
+    int base, count;
+    rows_of(p, blockIdx.y, base, count);
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, in = e / (D / 4), rows = (int64_t)p.n_rows * p.q_heads;
+    if (in >= (int64_t)count * p.q_heads) return;
+    const int64_t at = (int64_t)base * p.q_heads + in;
     const int row = (int)(at / p.q_heads), head = (int)(at % p.q_heads), d = (int)(e % (D / 4)) * 4;
-    if (p.row0) {  // rows of no sequence have no pieces
-        bool mine = false;
-        for (int s = 0; s < p.kv.n_seq; ++s) {
-            const int b = min(max(p.row0[s], 0), p.n_rows);
-            mine |= row >= b && row < min(p.row0[s + 1], b + p.max_rows);
-        }
-        if (!mine) return;
-    }
     float mt = kNone;
     for (int s = 0; s < p.nsplit; ++s) mt = fmaxf(mt, p.part[p.ml + (s * rows + at) * 2]);
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
@@ -541,8 +542,8 @@ hipError_t launch_of(const PrefillP& p, int cus, hipStream_t st) {
         launch_kernel((k_attn_prefill<D, KV, kW, 1>), dim3(p.kv.heads, (uint32_t)tiles, p.kv.n_seq * p.nsplit), dim3(64 * kW), 0, st, p);
     e = hipGetLastError();
     if (e == hipSuccess && p.nsplit > 1) {
-        const int64_t n = (int64_t)p.n_rows * p.q_heads * (D / 4);
-        launch_kernel((k_attn_prefill_join<D>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, p);
+        const int64_t n = (int64_t)p.max_rows * p.q_heads * (D / 4);
+        launch_kernel((k_attn_prefill_join<D>), dim3((uint32_t)((n + 255) / 256), p.kv.n_seq), dim3(256), 0, st, p);
         e = hipGetLastError();
     }
     return e;
