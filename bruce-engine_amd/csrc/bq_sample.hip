@@ -174,8 +174,10 @@ __global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
     }
     __syncthreads();
     const float mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-    // (any threshold is right; the waves' mean is the steadiest)
-    const float t = (s_t[0] + s_t[1]) * 0.25f + (s_t[2] + s_t[3]) * 0.25f;
+    // any threshold is right; the mean of the middle two is steadiest (one wave
+    // may hold several of the row's likeliest tokens)
+    const float t = 0.5f * fmaxf(fminf(s_t[0], s_t[1]), fminf(s_t[2], s_t[3])) +
+                    0.5f * fminf(fmaxf(s_t[0], s_t[1]), fmaxf(s_t[2], s_t[3]));
     const float least = fmaxf(t, -3.402823466e38f);  // -inf is no candidate
     int count = 0, first = 0x7FFFFFFF;
 #pragma unroll
@@ -453,7 +455,7 @@ struct Whole {
 
 __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
     __shared__ u64 s_key[2 * kMaxCand], s_bins[2048], s_red[16], s_found[3];
-    __shared__ int s_first[kMaxSlices + 1], s_wave[16];
+    __shared__ int s_first[kMaxSlices + 1], s_wave[32];
     __shared__ u64 s_best;
     __shared__ float s_t, s_least[16];
     __shared__ double s_mass;
@@ -533,21 +535,34 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
         // candidates that are the row's largest for sure: those not below t
         const int sure = __syncthreads_count(in && x >= t);
         const bool whole = !(t > -INFINITY);
-        // mass of the first top_k
+        // mass of the first top_k; where t cuts them off, its bounds: the others
+        // have at most the mass of a logit t each
         const bool k_sure = rule.top_k <= sure;
-        const double z = k_sure ? (double)s_key[rule.top_k - 1] : s_mass;
-        const bool z_known = rule.top_p >= 1.f || k_sure || rule.top_k == p.vocab || whole;
-        const double cut = (double)rule.top_p * (whole && !k_sure ? (double)s_key[total - 1] : z);
-        const bool stop = tid <= sure && tid > 0 &&
-                          (tid >= rule.top_k || (rule.top_p < 1.f && (double)ex >= cut) || (tid < sure && e < rule.min_p));
-        const u64 stops = __ballot(stop);
-        if ((tid & 63) == 0) s_wave[tid >> 6] = stops ? tid + __builtin_ctzll(stops) : kMaxCand + 1;
+        const float e_t = sure > 0 ? expf((t - mx) / rule.temp) : 1.f;
+        double z = k_sure ? (double)s_key[rule.top_k - 1] : whole ? (double)s_key[total - 1] : s_mass, z_most = z;
+        if (!k_sure && !whole && rule.top_k < p.vocab) {
+            z = sure > 0 ? (double)s_key[sure - 1] : 0.;
+            z_most = z + (double)(rule.top_k - sure) * (double)mass(e_t);
+        }
+        const bool cuts = rule.top_p < 1.f;
+        const double cut = (double)rule.top_p * z, cut_most = (double)rule.top_p * z_most;
+        const bool at = tid > 0 && tid <= sure;
+        const bool stop = at && (tid >= rule.top_k || (tid < sure ? e : e_t) < rule.min_p);
+        const u64 stops = __ballot(stop || (at && cuts && (double)ex >= cut));
+        const u64 stops_most = __ballot(stop || (at && cuts && (double)ex >= cut_most));
+        if ((tid & 63) == 0) {
+            s_wave[tid >> 6] = stops ? tid + __builtin_ctzll(stops) : kMaxCand + 1;
+            s_wave[16 + (tid >> 6)] = stops_most ? tid + __builtin_ctzll(stops_most) : kMaxCand + 1;
+        }
         __syncthreads();
-        int kept = kMaxCand + 1;
+        int kept = kMaxCand + 1, kept_most = kMaxCand + 1;
 #pragma unroll
-        for (int i = 15; i >= 0; --i) kept = min(kept, s_wave[i]);
-        if (kept > kMaxCand && whole) kept = total;
-        if (z_known && kept <= kMaxCand) {
+        for (int i = 0; i < 16; ++i) {
+            kept = min(kept, s_wave[i]);
+            kept_most = min(kept_most, s_wave[16 + i]);
+        }
+        if (whole) kept = min(kept, total), kept_most = min(kept_most, total);
+        if (kept <= kMaxCand && kept == kept_most) {
             const double target = u * (double)s_key[kept - 1];
             if (tid < kept && ((double)(ex + w) > target || tid == kept - 1) && (tid == 0 || !((double)ex > target)))
                 p.out[row] = index_of(key);
@@ -602,7 +617,9 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
 }
 
 int slices_of(int vocab) { return (vocab + kSlice - 1) / kSlice; }
-int cap_of(int slices) { return std::max(16, 2 * kWant / slices); }
+// room for a slice's candidates: 64 or four times those wanted of it, so that
+// few rows have a slice that overflows (a row's 1024 bound them all the same)
+int cap_of(int slices) { return std::max(64, std::min(kMaxCand, 4 * kWant / slices)); }
 }  // namespace
 
 size_t sample_work_bytes(int rows, int vocab) {
@@ -617,8 +634,7 @@ hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, c
     p.slices = slices_of(vocab);
     p.cap = cap_of(p.slices);
     // each wave's threshold is one of its 64 lanes' maxima of 16 logits: the
-    // rank-th leaves about 64 ln(64 / (64 - rank)) of its 1024 above it; the
-    // slice takes the largest of four
+    // rank-th leaves about 64 ln(64 / (64 - rank)) of its 1024 above it
     p.rank = std::max(2, std::min(62, (int)(64 * (1 - std::exp(-(double)kWant / p.slices / 256)))));
     p.temp = temp; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p; p.u = u; p.out = out;
     p.info = (SliceInfo*)work;

@@ -87,6 +87,23 @@ def test_flat_rows(bq, flat):
             assert abs(got[1] - 300) <= 1
 
 
+@pytest.mark.parametrize("vocab", [5000, 76721, 131072])
+def test_cuts_near_the_end_of_the_head(bq, vocab):
+    """Likely tokens bunched in neighbouring indices, and top-k, top-p and min-p that fall before, at and behind
+    the last logit that the scan can vouch for (a hundred or two of the row)."""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((6, vocab)).astype(np.float32) * 1.5
+    for r in range(6):
+        n = 8 * (r + 1)
+        at = int(rng.integers(0, vocab - 200))
+        x[r, at + rng.choice(200, n, replace=False)] += rng.uniform(4, 12, n).astype(np.float32)
+    print(f"sample cuts vocab {vocab}", flush=True)
+    for k in (12, 47, 100, 160, 250, 400, 0):
+        for p, mp, t in ((1.0, 0.0, 0.8), (0.9, 0.0, 1.0), (0.97, 0.0, 2.0), (0.9999, 0.0, 1.0), (1.0, 1e-4, 1.0), (0.95, 3e-3, 2.0)):
+            u = rng.random(6).astype(np.float32)
+            _check(bq, x, u, t, k, p, mp)
+
+
 def test_unusual_logits(bq):
     inf, nan = np.inf, np.nan
     vocab = 9000
