@@ -44,7 +44,7 @@ struct SliceInfo {
 struct SampleP {
     const float* logits;
     int64_t ld;
-    int vocab, slices, cap, rank;
+    int vocab, slices, cap_log, rank;  // a slice has room for 2^cap_log candidates
     const float* temp;
     const int32_t* top_k;
     const float* top_p;
@@ -70,9 +70,20 @@ BQ_DEV u64 shfl_xor64(u64 v, int d) {
     const uint32_t lo = __shfl_xor((uint32_t)v, d, 64), hi = __shfl_xor((uint32_t)(v >> 32), d, 64);
     return (u64)hi << 32 | lo;
 }
-BQ_DEV u64 shfl_up64(u64 v, int d) {
-    const uint32_t lo = __shfl_up((uint32_t)v, d, 64), hi = __shfl_up((uint32_t)(v >> 32), d, 64);
-    return (u64)hi << 32 | lo;
+// the wave's inclusive sums
+template <int CTRL, int ROWS>
+BQ_DEV u64 plus_dpp(u64 v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)v, CTRL, ROWS, 0xF, ROWS == 0xF);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), CTRL, ROWS, 0xF, ROWS == 0xF);
+    return v + ((u64)hi << 32 | lo);
+}
+BQ_DEV u64 wave_scan64(u64 v) {
+    v = plus_dpp<0x111, 0xF>(v);   // row_shr:1
+    v = plus_dpp<0x112, 0xF>(v);   // row_shr:2
+    v = plus_dpp<0x114, 0xF>(v);   // row_shr:4
+    v = plus_dpp<0x118, 0xF>(v);   // row_shr:8
+    v = plus_dpp<0x142, 0xA>(v);   // row_bcast:15 into rows 1, 3
+    return plus_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2, 3
 }
 
 // the value of lane ^ J (J < 64), without LDS
@@ -83,9 +94,7 @@ BQ_DEV uint32_t lane_xor(uint32_t v) {
     if constexpr (J == 4) {  // row_half_mirror is ^7, quad_perm [3,2,1,0] ^3
         return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, false), 0x1B, 0xF, 0xF, false);
     }
-    if constexpr (J == 8) {  // row_mirror is ^15
-        return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, false), 0x141, 0xF, 0xF, false);
-    }
+    if constexpr (J == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, false);  // row_ror:8
     if constexpr (J == 16) {  // both rows of a pair: [0] holds the even rows' values, [1] the odd rows'
         const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
         return threadIdx.x & 16 ? r[0] : r[1];
@@ -127,6 +136,15 @@ BQ_DEV float wave_max(float v) {
     v = fmaxf(v, dpp_f<0x140, 0xF, true>(v));  // row_mirror
     v = fmaxf(v, __shfl_xor(v, 16, 64));
     return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
+BQ_DEV u64 larger(u64 a, u64 b) { return a > b ? a : b; }
+template <int J>
+BQ_DEV u64 larger_xor(u64 v) {
+    return larger(v, (u64)lane_xor<J>((uint32_t)(v >> 32)) << 32 | lane_xor<J>((uint32_t)v));
+}
+BQ_DEV u64 wave_max64(u64 v) {
+    return larger_xor<32>(larger_xor<16>(larger_xor<8>(larger_xor<4>(larger_xor<2>(larger_xor<1>(v))))));
 }
 
 __global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
@@ -210,9 +228,9 @@ __global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
     }
     __syncthreads();
     const int total = s_count[0] + s_count[1] + s_count[2] + s_count[3];
-    const bool over = total > p.cap;
+    const bool over = total > 1 << p.cap_log;
     if (!over && !rule.greedy) {
-        u64* cand = p.cand + ((size_t)row * p.slices + slice) * p.cap;
+        u64* cand = p.cand + (((size_t)row * p.slices + slice) << p.cap_log);
         for (int w = 0; w < wave; ++w) cand += s_count[w];
 #pragma unroll
         for (int k = 0; k < V; ++k)
@@ -238,11 +256,7 @@ __global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
 // exclusive scan over the workgroup's 1024 threads, and the total
 BQ_DEV u64 scan1024(u64 v, u64* red, u64& total) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    u64 s = v;
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = shfl_up64(s, d);
-        if (lane >= d) s += o;
-    }
+    const u64 s = wave_scan64(v);
     __syncthreads();
     if (lane == 63) red[w] = s;
     __syncthreads();
@@ -453,53 +467,116 @@ struct Whole {
     }
 };
 
+// The token of a row whose largest logits are sorted, by one wave: its lanes
+// have E each, key[] and masses weight[] in descending order, `total` of them,
+// all not below t.  -1: the cut may lie behind them.
+constexpr u64 kBelow = 1ull << 63;  // of a weight: its token is less likely than min_p allows
+template <int E>
+BQ_DEV int decide(const SampleP& p, const RowRule& rule, const u64* key, u64* weight, int total, float mx, float t, double row_mass,
+                  double u) {
+    const int i0 = threadIdx.x * E;
+    constexpr int kNone = kMaxCand + 1;
+    u64 upto[E], sum = 0;
+    int below = kNone;
+#pragma unroll
+    for (int e = E - 1; e >= 0; --e) {
+        const u64 w = weight[i0 + e];
+        upto[e] = w & ~kBelow;
+        if (w & kBelow) below = i0 + e;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) upto[e] = sum += upto[e];
+    const u64 before = wave_scan64(sum) - sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) weight[i0 + e] = upto[e] += before;  // read by the other lanes
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const double all = (double)weight[total - 1];
+    // mass of the first top_k; where t cuts them off, its bounds: the others
+    // have at most the mass of a logit t each
+    const bool whole = !(t > -INFINITY), cuts = rule.top_p < 1.f;
+    const float e_t = expf((t - mx) / rule.temp);
+    double z = rule.top_k <= total ? (double)weight[rule.top_k - 1] : whole ? all : row_mass, z_most = z;
+    if (rule.top_k > total && !whole && rule.top_k < p.vocab) {
+        z = all;
+        z_most = all + (double)(rule.top_k - total) * (double)mass(e_t);
+    }
+    const double cut = (double)rule.top_p * z, cut_most = (double)rule.top_p * z_most;
+    // the first index that a rule shuts out, with either
+    auto first_of = [&](int mine) {
+        const u64 any = __ballot(mine < kNone);
+        return any ? __builtin_amdgcn_readlane(mine, __builtin_ctzll(any)) : kNone;
+    };
+    int stop = kNone, stop_most = kNone;
+#pragma unroll
+    for (int e = E - 1; e >= 0; --e) {
+        const int i = i0 + e;
+        if (i == 0 || i >= total) continue;
+        const double ex = (double)(e ? upto[e - 1] : before);
+        if (i >= rule.top_k || i >= below || (cuts && ex >= cut)) stop = i;
+        if (i >= rule.top_k || i >= below || (cuts && ex >= cut_most)) stop_most = i;
+    }
+    int kept = first_of(stop), kept_most = first_of(stop_most);
+    const bool end = whole || total >= rule.top_k || e_t < rule.min_p;  // nothing behind them is kept
+    if (kept == kNone && (end || (cuts && all >= cut))) kept = total;
+    if (kept_most == kNone && (end || (cuts && all >= cut_most))) kept_most = total;
+    if (kept == kNone || kept != kept_most) return -1;
+    const double target = u * (double)weight[kept - 1];
+    int at = kNone;
+#pragma unroll
+    for (int e = E - 1; e >= 0; --e) {
+        const int i = i0 + e;
+        if (i < kept && ((double)upto[e] > target || i == kept - 1)) at = i;
+    }
+    return index_of(key[first_of(at)]);
+}
+
 __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
     __shared__ u64 s_key[2 * kMaxCand], s_bins[2048], s_red[16], s_found[3];
-    __shared__ int s_first[kMaxSlices + 1], s_wave[32];
+    __shared__ int s_count[kMaxSlices], s_total, s_pick;
     __shared__ u64 s_best;
     __shared__ float s_t, s_least[16];
-    __shared__ double s_mass;
     const int tid = threadIdx.x, row = blockIdx.x;
     const RowRule rule = rule_of(p, row);
     const double u = (double)p.u[row];
     const SliceInfo* info = p.info + (size_t)row * p.slices;
+    // two slots a thread are read beside the counts that say which of them hold
+    // a candidate: all of them up to 32 slices
+    const int slots = p.slices << p.cap_log;
+    const u64* cand = p.cand + (size_t)row * slots;
+    const u64 slot0 = tid < slots ? cand[tid] : 0, slot1 = tid + 1024 < slots ? cand[tid + 1024] : 0;
+    double row_mass = 0;  // wave 0's
     if (tid < 64) {
-        // four slices a lane: the largest key, the largest threshold, where each slice's candidates begin
+        // four slices a lane: the largest key, the largest threshold, the mass
         constexpr int N = kMaxSlices / 64;
         SliceInfo in[N];
-        int c[N], all = 0;
         u64 best = 0;
         float t = -INFINITY;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             in[i] = SliceInfo{0, -INFINITY, 0.f, 0, 0};
-            if (N * tid + i < p.slices) in[i] = info[N * tid + i];
-            c[i] = all;
-            all += in[i].count;
-            best = in[i].best > best ? in[i].best : best;
-            t = fmaxf(t, in[i].t);
+            if (64 * i + tid < p.slices) in[i] = info[64 * i + tid];
         }
-        int before = all;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(before, d, 64);
-            if (tid >= d) before += o;
-            const u64 k = shfl_xor64(best, d);
-            best = k > best ? k : best;
-        }
-        t = wave_max(t);
-        const float mx = unordered((uint32_t)(best >> 32));
-        double mass = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (N * tid + i <= p.slices) s_first[N * tid + i] = before - all + c[i];
-            if (in[i].sum > 0.f) mass += (double)in[i].sum * (double)expf((unordered((uint32_t)(in[i].best >> 32)) - mx) / rule.temp);
+            if (64 * i + tid < p.slices) s_count[64 * i + tid] = in[i].count;
+            best = larger(best, in[i].best);
+            t = fmaxf(t, in[i].t);
         }
-        for (int d = 1; d < 64; d <<= 1) mass += __shfl_xor(mass, d, 64);
-        if (tid == 63) s_first[p.slices] = before;
+        best = wave_max64(best);
+        t = wave_max(t);
+        if (rule.top_p < 1.f && rule.top_k == p.vocab) {
+            const float mx = unordered((uint32_t)(best >> 32));
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (in[i].sum > 0.f)
+                    row_mass += (double)in[i].sum * (double)expf((unordered((uint32_t)(in[i].best >> 32)) - mx) / rule.temp);
+            for (int d = 1; d < 64; d <<= 1) row_mass += __shfl_xor(row_mass, d, 64);
+            row_mass *= 0x1p40;
+        }
         if (tid == 0) {
             s_best = best;
             s_t = t;
-            s_mass = mass * 0x1p40;
+            s_total = 0;
         }
     }
     __syncthreads();
@@ -509,65 +586,52 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
         if (tid == 0) p.out[row] = index_of(s_best);
         return;
     }
-    const int total = s_first[p.slices];
+    // the candidates not below t, the row's largest logits for sure (in any order: they are sorted)
     const float t = s_t;
+    const uint32_t least = ordered(t);
+    auto take = [&](int at, u64 key) {
+        const bool is = at < slots && (at & ((1 << p.cap_log) - 1)) < s_count[at >> p.cap_log] && (uint32_t)(key >> 32) >= least;
+        const u64 mask = __ballot(is);
+        if (mask == 0) return;
+        int to = 0;
+        if ((tid & 63) == 0) to = atomicAdd(&s_total, __popcll(mask));
+        to = __builtin_amdgcn_readfirstlane(to) + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+        if (is && to < kMaxCand) s_key[to] = key;
+    };
+    take(tid, slot0);
+    take(tid + 1024, slot1);
+    for (int at = tid + 2048; at - tid < slots; at += 2048) {
+        const u64 a = at < slots ? cand[at] : 0, b = at + 1024 < slots ? cand[at + 1024] : 0;
+        take(at, a);
+        take(at + 1024, b);
+    }
+    __syncthreads();
+    const int total = s_total;
     if (total > 0 && total <= kMaxCand) {
         int n = 64;
         while (n < total) n <<= 1;
-        u64 key = 0;
-        if (tid < total) {
-            int s = 0;
-            for (int hi = p.slices; hi - s > 1;) {
-                const int mid = (s + hi) / 2;
-                if (s_first[mid] <= tid) s = mid;
-                else hi = mid;
-            }
-            key = p.cand[((size_t)row * p.slices + s) * p.cap + tid - s_first[s]];
-        }
-        key = sort_keys(key, n, s_key);
-        const float x = unordered((uint32_t)(key >> 32));
-        const bool in = tid < total;
-        const float e = in ? expf((x - mx) / rule.temp) : 0.f;
-        const u64 w = mass(e);
-        u64 all;
-        const u64 ex = scan1024(w, s_red, all);
-        s_key[tid] = ex + w;
-        // candidates that are the row's largest for sure: those not below t
-        const int sure = __syncthreads_count(in && x >= t);
-        const bool whole = !(t > -INFINITY);
-        // mass of the first top_k; where t cuts them off, its bounds: the others
-        // have at most the mass of a logit t each
-        const bool k_sure = rule.top_k <= sure;
-        const float e_t = sure > 0 ? expf((t - mx) / rule.temp) : 1.f;
-        double z = k_sure ? (double)s_key[rule.top_k - 1] : whole ? (double)s_key[total - 1] : s_mass, z_most = z;
-        if (!k_sure && !whole && rule.top_k < p.vocab) {
-            z = sure > 0 ? (double)s_key[sure - 1] : 0.;
-            z_most = z + (double)(rule.top_k - sure) * (double)mass(e_t);
-        }
-        const bool cuts = rule.top_p < 1.f;
-        const double cut = (double)rule.top_p * z, cut_most = (double)rule.top_p * z_most;
-        const bool at = tid > 0 && tid <= sure;
-        const bool stop = at && (tid >= rule.top_k || (tid < sure ? e : e_t) < rule.min_p);
-        const u64 stops = __ballot(stop || (at && cuts && (double)ex >= cut));
-        const u64 stops_most = __ballot(stop || (at && cuts && (double)ex >= cut_most));
-        if ((tid & 63) == 0) {
-            s_wave[tid >> 6] = stops ? tid + __builtin_ctzll(stops) : kMaxCand + 1;
-            s_wave[16 + (tid >> 6)] = stops_most ? tid + __builtin_ctzll(stops_most) : kMaxCand + 1;
+        const u64 key = sort_keys(tid < total ? s_key[tid] : 0, n, s_key);
+        u64 *const keys = s_bins + kMaxCand, *const weights = s_bins;
+        if (tid < n) {
+            const float e = tid < total ? expf((unordered((uint32_t)(key >> 32)) - mx) / rule.temp) : 0.f;
+            keys[tid] = key;
+            weights[tid] = mass(e) | (e < rule.min_p ? kBelow : 0);
         }
         __syncthreads();
-        int kept = kMaxCand + 1, kept_most = kMaxCand + 1;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            kept = min(kept, s_wave[i]);
-            kept_most = min(kept_most, s_wave[16 + i]);
+        if (tid < 64) {
+            int pick;
+            if (n == 64) pick = decide<1>(p, rule, keys, weights, total, mx, t, row_mass, u);
+            else if (n == 128) pick = decide<2>(p, rule, keys, weights, total, mx, t, row_mass, u);
+            else if (n == 256) pick = decide<4>(p, rule, keys, weights, total, mx, t, row_mass, u);
+            else if (n == 512) pick = decide<8>(p, rule, keys, weights, total, mx, t, row_mass, u);
+            else pick = decide<16>(p, rule, keys, weights, total, mx, t, row_mass, u);
+            if (tid == 0) {
+                s_pick = pick;
+                if (pick >= 0) p.out[row] = pick;
+            }
         }
-        if (whole) kept = min(kept, total), kept_most = min(kept_most, total);
-        if (kept <= kMaxCand && kept == kept_most) {
-            const double target = u * (double)s_key[kept - 1];
-            if (tid < kept && ((double)(ex + w) > target || tid == kept - 1) && (tid == 0 || !((double)ex > target)))
-                p.out[row] = index_of(key);
-            return;
-        }
+        __syncthreads();
+        if (s_pick >= 0) return;
     }
     // the head was not enough: the whole row
     Whole r{p.logits + (size_t)row * p.ld, p.vocab, mx, fminf(1.44269504088896341f / rule.temp, 3e38f), 0.f, s_bins, s_key, s_red, s_found};
@@ -617,14 +681,18 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
 }
 
 int slices_of(int vocab) { return (vocab + kSlice - 1) / kSlice; }
-// room for a slice's candidates: 64 or four times those wanted of it, so that
-// few rows have a slice that overflows (a row's 1024 bound them all the same)
-int cap_of(int slices) { return std::max(64, std::min(kMaxCand, 4 * kWant / slices)); }
+// room for a slice's candidates: 64, or three times those wanted of it, so that
+// few rows have a slice that overflows
+int cap_log_of(int slices) {
+    int n = 6;
+    while (1 << n < std::min(kMaxCand, 3 * kWant / slices)) ++n;
+    return n;
+}
 }  // namespace
 
 size_t sample_work_bytes(int rows, int vocab) {
     const int s = slices_of(vocab);
-    return (size_t)rows * s * (sizeof(SliceInfo) + (size_t)cap_of(s) * sizeof(u64));
+    return (size_t)rows * s * (sizeof(SliceInfo) + (sizeof(u64) << cap_log_of(s)));
 }
 
 hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, const float* temp, const int32_t* top_k,
@@ -632,7 +700,7 @@ hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, c
     SampleP p;
     p.logits = logits; p.ld = ld; p.vocab = vocab;
     p.slices = slices_of(vocab);
-    p.cap = cap_of(p.slices);
+    p.cap_log = cap_log_of(p.slices);
     // each wave's threshold is one of its 64 lanes' maxima of 16 logits: the
     // rank-th leaves about 64 ln(64 / (64 - rank)) of its 1024 above it
     p.rank = std::max(2, std::min(62, (int)(64 * (1 - std::exp(-(double)kWant / p.slices / 256)))));
