@@ -77,6 +77,14 @@ BQ_DEV u64 plus_dpp(u64 v) {
     const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), CTRL, ROWS, 0xF, ROWS == 0xF);
     return v + ((u64)hi << 32 | lo);
 }
+BQ_DEV int wave_scan32(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+}
 BQ_DEV u64 wave_scan64(u64 v) {
     v = plus_dpp<0x111, 0xF>(v);   // row_shr:1
     v = plus_dpp<0x112, 0xF>(v);   // row_shr:2
@@ -530,9 +538,10 @@ BQ_DEV int decide(const SampleP& p, const RowRule& rule, const u64* key, u64* we
     return index_of(key[first_of(at)]);
 }
 
+constexpr int kBins = 1024, kManyKeys = 32;
 __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
     __shared__ u64 s_key[2 * kMaxCand], s_bins[2048], s_red[16], s_found[3];
-    __shared__ int s_count[kMaxSlices], s_total, s_pick;
+    __shared__ int s_count[kMaxSlices], s_sum[16], s_total, s_pick, s_many;
     __shared__ u64 s_best;
     __shared__ float s_t, s_least[16];
     const int tid = threadIdx.x, row = blockIdx.x;
@@ -543,7 +552,9 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
     // a candidate: all of them up to 32 slices
     const int slots = p.slices << p.cap_log;
     const u64* cand = p.cand + (size_t)row * slots;
-    const u64 slot0 = tid < slots ? cand[tid] : 0, slot1 = tid + 1024 < slots ? cand[tid + 1024] : 0;
+    u64 k0 = tid < slots ? cand[tid] : 0, k1 = tid + 1024 < slots ? cand[tid + 1024] : 0;
+    int *const count = (int*)s_bins, *const start = count + kBins;  // of a bin's keys
+    count[tid] = 0;
     double row_mass = 0;  // wave 0's
     if (tid < 64) {
         // four slices a lane: the largest key, the largest threshold, the mass
@@ -576,7 +587,7 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
         if (tid == 0) {
             s_best = best;
             s_t = t;
-            s_total = 0;
+            s_total = s_many = 0;
         }
     }
     __syncthreads();
@@ -589,33 +600,88 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
     // the candidates not below t, the row's largest logits for sure (in any order: they are sorted)
     const float t = s_t;
     const uint32_t least = ordered(t);
-    auto take = [&](int at, u64 key) {
-        const bool is = at < slots && (at & ((1 << p.cap_log) - 1)) < s_count[at >> p.cap_log] && (uint32_t)(key >> 32) >= least;
-        const u64 mask = __ballot(is);
-        if (mask == 0) return;
-        int to = 0;
-        if ((tid & 63) == 0) to = atomicAdd(&s_total, __popcll(mask));
-        to = __builtin_amdgcn_readfirstlane(to) + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-        if (is && to < kMaxCand) s_key[to] = key;
+    auto sure = [&](int at, u64 key) {
+        return at < slots && (at & ((1 << p.cap_log) - 1)) < s_count[at >> p.cap_log] && (uint32_t)(key >> 32) >= least;
     };
-    take(tid, slot0);
-    take(tid + 1024, slot1);
-    for (int at = tid + 2048; at - tid < slots; at += 2048) {
-        const u64 a = at < slots ? cand[at] : 0, b = at + 1024 < slots ? cand[at + 1024] : 0;
-        take(at, a);
-        take(at + 1024, b);
+    bool in0 = sure(tid, k0), in1 = sure(tid + 1024, k1);
+    int lost = 0;
+    if (slots > 2048) {  // packed: one a thread
+        auto take = [&](bool is, u64 key) {
+            const u64 mask = __ballot(is);
+            if (mask == 0) return;
+            int to = 0;
+            if ((tid & 63) == 0) to = atomicAdd(&s_total, __popcll(mask));
+            to = __builtin_amdgcn_readfirstlane(to) +
+                 __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+            if (is && to < kMaxCand) s_key[to] = key;
+        };
+        take(in0, k0);
+        take(in1, k1);
+        for (int at = tid + 2048; at - tid < slots; at += 2048) {
+            const u64 a = at < slots ? cand[at] : 0, b = at + 1024 < slots ? cand[at + 1024] : 0;
+            take(sure(at, a), a);
+            take(sure(at + 1024, b), b);
+        }
+        __syncthreads();
+        lost = max(0, s_total - kMaxCand);
+        in0 = tid < s_total;
+        in1 = false;
+        if (in0) k0 = s_key[tid];
     }
+    // Sorted by bins of their distance to t, even in its logarithm (most lie
+    // near t): a key's place is where its bin starts plus its larger ones there.
+    const float per = 1.f / (mx - t);
+    const bool even = t > -INFINITY && per > 0.f && per < INFINITY;
+    auto bin_of = [&](u64 key) {  // of the least key: 0x382
+        const float d = (unordered((uint32_t)(key >> 32)) - t) * per + 0x1p-7f;
+        return even ? 0x382 - min(max((__builtin_bit_cast(int, d) - 0x3C000000) >> 16, 0), 0x382) : 0;
+    };
+    const int b0 = in0 ? bin_of(k0) : 0, b1 = in1 ? bin_of(k1) : 0;
+    const int at0 = in0 ? atomicAdd(&count[b0], 1) : 0, at1 = in1 ? atomicAdd(&count[b1], 1) : 0;
     __syncthreads();
+    {
+        const int c = count[tid], w = tid >> 6;
+        const int upto = wave_scan32(c);
+        if ((tid & 63) == 63) s_sum[w] = upto;
+        if (c > kManyKeys) s_many = 1;
+        __syncthreads();
+        int before = 0, all = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            before += i < w ? s_sum[i] : 0;
+            all += s_sum[i];
+        }
+        start[tid] = before + upto - c;
+        if (tid == 0) s_total = all + lost;
+        __syncthreads();
+    }
     const int total = s_total;
     if (total > 0 && total <= kMaxCand) {
+        if (in0) s_key[start[b0] + at0] = k0;
+        if (in1) s_key[start[b1] + at1] = k1;
+        __syncthreads();
         int n = 64;
         while (n < total) n <<= 1;
-        const u64 key = sort_keys(tid < total ? s_key[tid] : 0, n, s_key);
-        u64 *const keys = s_bins + kMaxCand, *const weights = s_bins;
+        u64 *const keys = s_key + kMaxCand, *const weights = s_bins + kMaxCand;
+        auto put = [&](int to, u64 key) {
+            const float e = key ? expf((unordered((uint32_t)(key >> 32)) - mx) / rule.temp) : 0.f;
+            keys[to] = key;
+            weights[to] = mass(e) | (e < rule.min_p ? kBelow : 0);
+        };
+        u64 key = tid < total ? s_key[tid] : 0;
+        int to = tid;
+        if (s_many) {
+            key = sort_keys(key, n, s_key);
+            __syncthreads();
+        } else if (tid < total) {
+            const int b = bin_of(key), c = count[b], from = start[b];
+            to = from;
+            for (int i = 0; i < c; ++i) to += s_key[from + i] > key;
+        }
         if (tid < n) {
             const float e = tid < total ? expf((unordered((uint32_t)(key >> 32)) - mx) / rule.temp) : 0.f;
-            keys[tid] = key;
-            weights[tid] = mass(e) | (e < rule.min_p ? kBelow : 0);
+            keys[to] = key;
+            weights[to] = mass(e) | (e < rule.min_p ? kBelow : 0);
         }
         __syncthreads();
         if (tid < 64) {
