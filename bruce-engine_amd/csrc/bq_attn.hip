@@ -442,12 +442,21 @@ hipError_t launch_decode_of(const DecodeP& p, hipStream_t st) {
 int q_tiles(int rows, int G) { return (rows * G + 15) / 16; }
 }  // namespace
 
-// Pieces that one sequence's tokens are cut into: two workgroups per CU, each
-// wave at least one 32-token step
-int decode_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus) {
+// Pieces that the `len` tokens of a sequence that its rows see are cut into: two
+// workgroups per CU, each wave at least one 32-token step.  A few steps are not
+// cut, as the join is a launch of its own (2.5 us) and a step costs what its
+// bytes do, a q8 one twice that: 512 tokens of bf16 D 128 take 7.8 us whole and
+// 8.3 in four pieces, 777 10.9 and 8.4; D 64 5.7 / 7.5 and 8.1 / 8.1; D 256 11.5
+// / 10.6; q8 D 128, 256 tokens 7.5 / 8.9, 512 10.8 / 9.1
+int decode_splits(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int64_t len, int cus) {
     const int64_t tiles = (int64_t)n_seq * kv_heads * q_tiles(rows, q_heads / kv_heads);
-    const int64_t steps = ((int64_t)max_len + 31) / 32;
-    return (int)std::max<int64_t>(1, std::min<int64_t>((steps + kWaves - 1) / kWaves, 2 * cus / tiles));
+    const int64_t each = ((len + 31) / 32 + kWaves - 1) / kWaves;  // steps of a wave
+    if (each * D * (type == kKvQ8 ? 2 : 1) <= 512) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(each, 2 * cus / tiles));
+}
+// the tokens in the steps that a window and its sinks reach
+int64_t decode_reach(int rows, int window, int sinks, int max_len) {
+    return window ? std::min<int64_t>(max_len, (int64_t)window + rows + 30 + ((int64_t)sinks + 31) / 32 * 32) : max_len;
 }
 
 size_t decode_part_floats(int n_seq, int rows, int q_heads, int kv_heads, int D) {

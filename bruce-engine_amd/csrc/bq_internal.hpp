@@ -142,7 +142,8 @@ hipError_t launch_kv_read(const KvView& kv, int type, const int32_t* seq, const 
                           uint16_t* v, hipStream_t st);
 // attention over it.  decode_splits: workgroups a sequence and head's tokens
 // are split over when the workspace allows it
-int decode_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus);
+int decode_splits(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int64_t len, int cus);
+int64_t decode_reach(int rows, int window, int sinks, int max_len);
 size_t decode_part_floats(int n_seq, int rows, int q_heads, int kv_heads, int D);  // workspace of one piece each
 hipError_t launch_attn_decode(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st);
 int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus);

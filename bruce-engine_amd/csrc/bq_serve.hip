@@ -101,7 +101,8 @@ size_t bq_attn_workspace_bytes(int n_seq, int rows, int q_heads, int kv_heads, i
     if (n_seq <= 0 || rows < 1 || rows > BQ_MAX_ROWS || kv_heads <= 0 || q_heads % kv_heads != 0 || q_heads <= 0 || head_dim <= 0 ||
         max_len < 0 || device_ready() != BQ_OK)
         return 0;
-    const int n = decode_splits(n_seq, rows, q_heads, kv_heads, max_len, device_cus());
+    // of either type: a q8 cache's tokens are cut earlier
+    const int n = decode_splits(kKvQ8, n_seq, rows, q_heads, kv_heads, head_dim, max_len, device_cus());
     return n > 1 ? n * decode_part_floats(n_seq, rows, q_heads, kv_heads, head_dim) * sizeof(float) : 0;
 }
 
@@ -126,7 +127,7 @@ int bq_attn_decode(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t s
     if (a.row0 || (int64_t)kv.n_seq * a.rows != a.n_rows) return BQ_EINVAL;
     if (a.rows > BQ_MAX_ROWS) return BQ_UNSUPPORTED;
     if (!al16(a.work) || (a.work_bytes && !a.work)) return BQ_EINVAL;
-    int n = decode_splits(kv.n_seq, a.rows, a.q_heads, kv.heads, a.max_len, device_cus());
+    int n = decode_splits(type, kv.n_seq, a.rows, a.q_heads, kv.heads, kv.D, decode_reach(a.rows, a.window, a.sinks, a.max_len), device_cus());
     const size_t part = decode_part_floats(kv.n_seq, a.rows, a.q_heads, kv.heads, kv.D) * sizeof(float);
     n = (int)std::min<size_t>(n, std::max<size_t>(1, a.work_bytes / part));
     return from_hip(launch_attn_decode(kv, type, a, n, (hipStream_t)st));

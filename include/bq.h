@@ -524,8 +524,8 @@ int bq_kv_read(const bq_kv_cache* kv, const int32_t* seq, const int32_t* pos, in
  *     sequence are split over workgroups and joined through `work`
  *     (bq_attn_workspace_bytes for the full split; NULL or less: a smaller
  *     split or none).  Calls that share a workspace must be ordered.  The
- *     number of pieces follows max_len, which a captured graph fixes; their
- *     bounds follow kv_len.
+ *     number of pieces follows max_len (what a window lets the rows see of it),
+ *     which a captured graph fixes; their bounds follow kv_len.
  *   bq_attn_prefill: a ragged batch, rows row0[s] .. row0[s + 1] - 1 of q and
  *     out for sequence s (device, [n_seq + 1], non-decreasing, within n_rows;
  *     NULL: n_seq must be 1 and its rows are all n_rows), at most `rows` each;

@@ -115,6 +115,18 @@ def test_decode_split_long(bq):
     _decode(bq, "q8", [66000], 1, 2, 1, 64, 16, "f32", "f32", seed=4, work=None)
 
 
+@pytest.mark.parametrize("kv", ["bf16", "q8"])
+@pytest.mark.parametrize("D,Hq,H,P", [(64, 6, 2, 16), (128, 16, 2, 64), (256, 3, 1, 32)])
+def test_decode_split_shapes(bq, kv, D, Hq, H, P):
+    """Pieces and their join at each head width: several new tokens, windows wider than a piece, unmapped pages,
+    sequences that fill only the first piece or none."""
+    lens = [1500, 1, 0, 1090, 33]
+    _decode(bq, kv, lens, 1, Hq, H, D, P, "f32", "f32", seed=D + 2)
+    _decode(bq, kv, lens, 5, Hq, H, D, P, "bf16", "bf16", seed=D + 3)
+    _decode(bq, kv, lens, 3, Hq, H, D, P, "f32", "bf16", 1200, 40, seed=D + 4)
+    _decode(bq, kv, lens, 1, Hq, H, D, P, "f32", "f32", seed=D + 5, holes=[(0, 0), (0, 12), (3, 9)])
+
+
 def test_decode_peaked_scores(bq):
     """Scores tens apart: the running maximum moves often; and far below the first ones."""
     for kv in ("bf16", "q8"):
