@@ -558,10 +558,14 @@ hipError_t launch_d(const PrefillP& p, int type, int cus, hipStream_t st) {
 // Pieces that the tokens of a sequence are cut into: where the row tiles leave
 // workgroup slots (two per CU) free, as many pieces as fill them, of kPiece
 // tiles at least.
-int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int max_len, int cus) {
+int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int64_t len, int cus) {
     const int64_t tiles = ((int64_t)rows * (q_heads / kv_heads) + 32 * kW - 1) / (32 * kW) * n_seq * kv_heads;
-    const int64_t steps = ((int64_t)max_len + kBN - 1) / kBN;
+    const int64_t steps = (len + kBN - 1) / kBN;
     return (int)std::max<int64_t>(1, std::min<int64_t>(steps / kPiece, 2 * cus / tiles));
+}
+// the tokens in the tiles that a window and its sinks let a row tile reach
+int64_t prefill_reach(int window, int sinks, int max_len) {
+    return window ? std::min<int64_t>(max_len, (int64_t)window + 32 * kW + kBN + ((int64_t)sinks + kBN - 1) / kBN * kBN) : max_len;
 }
 size_t prefill_part_floats(int n_rows, int q_heads, int D) { return (size_t)n_rows * q_heads * (D + 2); }
 

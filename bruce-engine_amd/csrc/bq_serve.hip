@@ -148,7 +148,7 @@ int bq_attn_prefill(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t 
     // the converted tiles first, the pieces in what is left
     size_t stage = prefill_stage_bytes(type, kv.n_seq, std::min(a.rows, a.n_rows), a.q_heads, kv.heads, kv.D, a.max_len);
     if (stage > a.work_bytes) stage = 0;
-    int n = prefill_splits(kv.n_seq, std::min(a.rows, a.n_rows), a.q_heads, kv.heads, a.max_len, device_cus());
+    int n = prefill_splits(kv.n_seq, std::min(a.rows, a.n_rows), a.q_heads, kv.heads, prefill_reach(a.window, a.sinks, a.max_len), device_cus());
     const size_t part = prefill_part_floats(a.n_rows, a.q_heads, kv.D) * sizeof(float);
     n = (int)std::min<size_t>(n, std::max<size_t>(1, (a.work_bytes - stage) / part));
     // (sequence, piece) is one grid dimension
