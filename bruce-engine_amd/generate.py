@@ -168,13 +168,15 @@ class Generator:
         self.gen = torch.Generator(device="cuda").manual_seed(seed)
 
     def prefill(self, s, prompt, chunk=512):
-        """Runs prompt (int32 device tensor) of sequence s in chunks; returns the last token's logits [vocab]."""
+        """Runs prompt (int32 device tensor) of sequence s in even chunks of at most `chunk` tokens; returns the last
+        token's logits [vocab].  (Even, as a few tokens left over would take the decode path, which rounds otherwise.)"""
         import torch
         c, done = self.model.c, 0
         row = self.table[s: s + 1].contiguous()
         views = [bq.KvCache(k.pages, row, c.kv_type, c.kv_heads, c.head_dim, c.page_tokens) for k in self.caches]
         while done < len(prompt):
-            n = min(chunk, len(prompt) - done)
+            left = len(prompt) - done
+            n = -(-left // -(-left // chunk))
             pos = torch.arange(done, done + n, dtype=torch.int32, device="cuda")
             step = Step(self.model, views, self.rope, n, pos, torch.tensor([done + n], dtype=torch.int32, device="cuda"), False)
             logits = step.run(prompt[done: done + n])
