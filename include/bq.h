@@ -534,7 +534,8 @@ int bq_kv_read(const bq_kv_cache* kv, const int32_t* seq, const int32_t* pos, in
  *     range stays fp32's) and the values as bf16.  Sums are fp32.  A few rows
  *     over many tokens are split over workgroups too, and many rows over a q8
  *     cache convert its tokens once, into work (bq_attn_prefill_workspace_bytes;
- *     with less, or NULL, a smaller split and conversion on the way).
+ *     with less, or NULL, a smaller split and conversion on the way), with
+ *     values and weights in fp16 then (64 tokens' values over a power of two).
  * scale > 0.  q_heads % kv_heads == 0 and q_heads / kv_heads <= 64, else BQ_UNSUPPORTED.
  * Row strides in elements, multiples of 8. */
 typedef struct bq_attn_args {

@@ -321,3 +321,28 @@ def test_refusals(bq):
         bq.Attention(cache, q[:, : 4 * D], out, lens.long())
     with pytest.raises(TypeError):
         bq.Attention(cache, q[:, : 4 * D].half(), out, lens)
+
+
+@pytest.mark.parametrize("powers", [(0, 0, 0, 0), (-30, -30, -30, -30), (12, 12, 12, 12), (0, 14, -25, 3), (40, 10, -10, -40)])
+def test_prefill_many_rows_over_q8_value_ranges(bq, powers):
+    """Values of every size, 64 tokens to a power of two: converted tiles keep fp32's range, and their products
+    with the weights are fp16's where they are bf16's otherwise."""
+    D, Hq, H, P, T = 128, 16, 2, 32, 256
+    pages = R.Pages("q8", H, D, P, 1, T // P, 3)
+    k, v = _normal(41, T, H, D), _normal(42, T, H, D)
+    for i, p in enumerate(powers):
+        v[64 * i: 64 * (i + 1)] *= 2.0 ** p
+    pages.put(0, k, v)
+    q = _normal(43, T, Hq * D) * 2
+    out = torch.empty((T, Hq * D), device="cuda")
+    att = bq.Attention(pages.cache(bq), q.cuda(), out, torch.tensor([T], dtype=torch.int32, device="cuda"))
+    assert att.struct.work_bytes > 0
+    att.prefill()
+    got = out.cpu().double().reshape(T, Hq, D)
+    ref, bound, A = R.attention(R.half_rows(q.reshape(T, Hq, D)), pages.kh[0], pages.v[0], torch.arange(T), D ** -0.5)
+    # a value's and a weight's rounding to fp16: 2^-11 of a term each at most, or 2^-25 of the tile's range
+    # (values up to 2^16, weights up to 2^15); fp32 sums as in the other tests
+    tol = 2.0 ** -9 + 2.0 ** -18 * A[..., None]
+    ratio = ((got - ref).abs() / (tol * bound).clamp(min=1e-300)).max().item()
+    print(f"  {powers}: worst error / tolerance {ratio:.3f}", flush=True)
+    assert ratio <= 1
