@@ -6,13 +6,13 @@
 //   k_sample_scan, one workgroup per 4096 logits: reads them once (the floor:
 //     4 bytes a logit), keeps the head of its slice -- every logit not below a
 //     threshold t, taken from the lanes' maxima in order, which leaves about 400
-//     candidates for the whole row -- and, where top-p needs the row's mass, its
-//     sum of exponentials.
+//     candidates for the whole row -- and, where no top-k bounds it, its sum of
+//     exponentials.
 //   k_sample_pick, one workgroup per row: takes the candidates not below the
 //     largest t, which are the row's largest logits for sure, puts them in order
 //     and cuts their running mass.  A cut that falls among them is exact.  Where it
-//     does not (a flat row, no filter, hundreds of tokens kept), the row is read
-//     again, two or three times (struct Whole).
+//     does not (a flat row, hundreds of tokens kept, no filter and a draw behind
+//     them), the row is read again, two or three times (struct Whole).
 // Bounds: one row is latency, two launches and the pick's chain of loads, LDS
 // and barriers (131072 logits 8.9 us: scan 3.9, pick 5); many rows the reading
 // of the logits (64 rows of 131072 with top-p 15.8 us, 34 MB at 2.1 TB/s over both
@@ -41,7 +41,7 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows s
 struct SliceInfo {
     u64 best;      // largest key
     float t;       // every logit >= t of the slice is a candidate (-inf: all finite ones, +inf: none)
-    float sum;     // of exp((x - max) / temperature), where top-p needs it
+    float sum;     // of exp((x - max) / temperature), where top-k does not bound the row
     int count, pad;
 };
 
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
         s_count[wave] = count;
         s_at[wave] = first;
     }
-    if (rule.top_p < 1.f && rule.top_k == p.vocab) {
+    if (rule.top_k == p.vocab && !rule.greedy) {
         float sum = 0.f;
         if (mx > -INFINITY && mx < INFINITY) {
             const float inv = 1.44269504088896341f / rule.temp;
@@ -531,8 +531,13 @@ BQ_DEV int decide(const SampleP& p, const RowRule& rule, const u64* key, u64* we
     const bool end = whole || total >= rule.top_k || e_t < rule.min_p;  // nothing behind them is kept
     if (kept == kNone && (end || (cuts && all >= cut))) kept = total;
     if (kept_most == kNone && (end || (cuts && all >= cut_most))) kept_most = total;
-    if (kept == kNone || kept != kept_most) return -1;
-    const double target = u * (double)weight[kept - 1];
+    double target = u * row_mass;
+    if (kept == kNone && rule.top_k == p.vocab && !cuts && !(rule.min_p > 0.f) && target < all) {
+        kept = total;  // the whole row is kept, and the draw falls among these
+    } else {
+        if (kept == kNone || kept != kept_most) return -1;
+        target = u * (double)weight[kept - 1];
+    }
     int at = kNone;
 #pragma unroll
     for (int e = E - 1; e >= 0; --e) {
@@ -579,7 +584,7 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
         }
         best = wave_max64(best);
         t = wave_max(t);
-        if (rule.top_p < 1.f && rule.top_k == p.vocab) {
+        if (rule.top_k == p.vocab) {
             const float mx = unordered((uint32_t)(best >> 32));
 #pragma unroll
             for (int i = 0; i < N; ++i)

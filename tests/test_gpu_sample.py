@@ -104,6 +104,17 @@ def test_cuts_near_the_end_of_the_head(bq, vocab):
             _check(bq, x, u, t, k, p, mp)
 
 
+@pytest.mark.parametrize("vocab", [700, 76721, 262148])
+def test_no_filter(bq, vocab):
+    """Temperature alone: draws among the likeliest tokens and far behind them, over a peaked and a flat row."""
+    x = _peaked(vocab + 1, 12, vocab)
+    x[6:] = np.random.default_rng(vocab).standard_normal((6, vocab)).astype(np.float32)
+    u = np.array([0.0, 0.2, 0.6, 0.95, 0.99999, np.float32(1) - np.float32(2) ** -24] * 2, np.float32)
+    print(f"sample unfiltered vocab {vocab}", flush=True)
+    for t in (0.3, 1.0, 2.5):
+        _check(bq, x, u, t)
+
+
 def test_unusual_logits(bq):
     inf, nan = np.inf, np.nan
     vocab = 9000
