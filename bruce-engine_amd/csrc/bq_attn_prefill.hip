@@ -594,7 +594,11 @@ constexpr int kStageRows = 2048;
 // launch would leave CUs without a workgroup, or with one where the tokens are
 // not split (512 rows: 19.7 us with whole tiles, 16.4 with half ones; 1500 rows
 // 47 / 40; 512 rows over 4000 tokens in four pieces 59 / 78)
-bool half_tiles(int64_t tiles, int nsplit, int cus) { return nsplit == 1 ? tiles <= 2 * cus : tiles * nsplit <= cus; }
+bool half_tiles(int64_t tiles, int nsplit, int slots) { return nsplit == 1 ? tiles <= slots : tiles * nsplit <= slots / 2; }
+// workgroups that the chip holds at once: two tile buffers are 64 KiB at D 128,
+// 128 KiB at D 256 (counted as two there, 256 rows over 4000 tokens took 88 us
+// instead of 74, 1000 rows 70 instead of 54)
+int slots_of(int D, int cus) { return D <= 128 ? 2 * cus : cus; }
 
 template <int D, int KV>
 hipError_t launch_of(const PrefillP& p, int cus, hipStream_t st) {
@@ -605,7 +609,7 @@ hipError_t launch_of(const PrefillP& p, int cus, hipStream_t st) {
         launch_kernel((k_stage_q8<D>), dim3(p.stage_tiles, p.kv.heads, p.kv.n_seq), dim3(256), 0, st, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    if (half_tiles(tiles * p.kv.heads * p.kv.n_seq, p.nsplit, cus))
+    if (half_tiles(tiles * p.kv.heads * p.kv.n_seq, p.nsplit, slots_of(D, cus)))
         launch_kernel((k_attn_prefill<D, KV, kW, 2>), dim3(p.kv.heads, (uint32_t)halves, p.kv.n_seq * p.nsplit), dim3(64 * kW), 0, st, p);
     else
         launch_kernel((k_attn_prefill<D, KV, kW, 1>), dim3(p.kv.heads, (uint32_t)tiles, p.kv.n_seq * p.nsplit), dim3(64 * kW), 0, st, p);
@@ -625,12 +629,12 @@ hipError_t launch_d(const PrefillP& p, int type, int cus, hipStream_t st) {
 }  // namespace
 
 // Pieces that the tokens of a sequence are cut into: where the row tiles leave
-// workgroup slots (two per CU) free, as many pieces as fill them, of kPiece
+// workgroup slots free, as many pieces as fill them, of kPiece
 // tiles at least.
-int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int64_t len, int cus) {
+int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int D, int64_t len, int cus) {
     const int64_t tiles = ((int64_t)rows * (q_heads / kv_heads) + 32 * kW - 1) / (32 * kW) * n_seq * kv_heads;
     const int64_t steps = (len + kBN - 1) / kBN;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(steps / kPiece, 2 * cus / tiles));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(steps / kPiece, slots_of(D, cus) / tiles));
 }
 // the tokens in the tiles that a window and its sinks let a row tile reach
 int64_t prefill_reach(int window, int sinks, int max_len) {

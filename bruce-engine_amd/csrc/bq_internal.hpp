@@ -146,7 +146,7 @@ int decode_splits(int type, int n_seq, int rows, int q_heads, int kv_heads, int 
 int64_t decode_reach(int rows, int window, int sinks, int max_len);
 size_t decode_part_floats(int n_seq, int rows, int q_heads, int kv_heads, int D);  // workspace of one piece each
 hipError_t launch_attn_decode(const KvView& kv, int type, const bq_attn_args& a, int nsplit, hipStream_t st);
-int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int64_t len, int cus);
+int prefill_splits(int n_seq, int rows, int q_heads, int kv_heads, int D, int64_t len, int cus);
 int64_t prefill_reach(int window, int sinks, int max_len);
 size_t prefill_part_floats(int n_rows, int q_heads, int D);
 size_t prefill_stage_bytes(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int max_len);

@@ -110,7 +110,7 @@ size_t bq_attn_prefill_workspace_bytes(int type, int n_seq, int rows, int n_rows
     if (n_seq <= 0 || rows < 1 || n_rows < 1 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0 ||
         max_len < 0 || device_ready() != BQ_OK)
         return 0;
-    const int n = prefill_splits(n_seq, std::min(rows, n_rows), q_heads, kv_heads, max_len, device_cus());
+    const int n = prefill_splits(n_seq, std::min(rows, n_rows), q_heads, kv_heads, head_dim, max_len, device_cus());
     const size_t parts = n > 1 ? n * prefill_part_floats(n_rows, q_heads, head_dim) * sizeof(float) : 0;
     return parts + prefill_stage_bytes(type == BQ_TYPE_Q8_0 ? kKvQ8 : kKvBf16, n_seq, std::min(rows, n_rows), q_heads, kv_heads,
                                        head_dim, max_len);
@@ -148,7 +148,7 @@ int bq_attn_prefill(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t 
     // the converted tiles first, the pieces in what is left
     size_t stage = prefill_stage_bytes(type, kv.n_seq, std::min(a.rows, a.n_rows), a.q_heads, kv.heads, kv.D, a.max_len);
     if (stage > a.work_bytes) stage = 0;
-    int n = prefill_splits(kv.n_seq, std::min(a.rows, a.n_rows), a.q_heads, kv.heads, prefill_reach(a.window, a.sinks, a.max_len), device_cus());
+    int n = prefill_splits(kv.n_seq, std::min(a.rows, a.n_rows), a.q_heads, kv.heads, kv.D, prefill_reach(a.window, a.sinks, a.max_len), device_cus());
     const size_t part = prefill_part_floats(a.n_rows, a.q_heads, kv.D) * sizeof(float);
     n = (int)std::min<size_t>(n, std::max<size_t>(1, (a.work_bytes - stage) / part));
     // (sequence, piece) is one grid dimension
