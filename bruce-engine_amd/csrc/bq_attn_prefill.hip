@@ -590,11 +590,15 @@ constexpr int kW = 4;  // waves of a workgroup
 // ahead; 128 rows 39 and 41, 64 rows 31 and 37
 constexpr int kStageRows = 2048;
 
-// Row tiles of 32 kW rows; of half that, shared by pairs of waves, where the
-// launch would leave CUs without a workgroup, or with one where the tokens are
-// not split (512 rows: 19.7 us with whole tiles, 16.4 with half ones; 1500 rows
-// 47 / 40; 512 rows over 4000 tokens in four pieces 59 / 78)
-bool half_tiles(int64_t tiles, int nsplit, int slots) { return nsplit == 1 ? tiles <= slots : tiles * nsplit <= slots / 2; }
+// Row tiles of 32 kW rows; of half that, shared by pairs of waves, where those
+// fit the chip at once (512 rows: 19.7 us with whole tiles, 16.4 with half ones;
+// 512 rows over 4000 tokens in four pieces, which do not, 59 / 78) or, where the
+// tokens are not split and are several tiles, almost (the shorter rows' workgroups
+// end early: 1500 rows 47 / 40, 700 rows of D 256 44 / 36; 6 x 105 rows of D 256,
+// two tiles of tokens, 24 / 34)
+bool half_tiles(int64_t tiles, int nsplit, int64_t steps, int slots) {
+    return tiles * nsplit <= slots / 2 || (nsplit == 1 && tiles <= slots && steps >= kPiece);
+}
 // workgroups that the chip holds at once: two tile buffers are 64 KiB at D 128,
 // 128 KiB at D 256 (counted as two there, 256 rows over 4000 tokens took 88 us
 // instead of 74, 1000 rows 70 instead of 54)
@@ -609,7 +613,7 @@ hipError_t launch_of(const PrefillP& p, int cus, hipStream_t st) {
         launch_kernel((k_stage_q8<D>), dim3(p.stage_tiles, p.kv.heads, p.kv.n_seq), dim3(256), 0, st, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    if (half_tiles(tiles * p.kv.heads * p.kv.n_seq, p.nsplit, slots_of(D, cus)))
+    if (half_tiles(tiles * p.kv.heads * p.kv.n_seq, p.nsplit, prefill_reach(p.window, p.sinks, p.max_len) / kBN, slots_of(D, cus)))
         launch_kernel((k_attn_prefill<D, KV, kW, 2>), dim3(p.kv.heads, (uint32_t)halves, p.kv.n_seq * p.nsplit), dim3(64 * kW), 0, st, p);
     else
         launch_kernel((k_attn_prefill<D, KV, kW, 1>), dim3(p.kv.heads, (uint32_t)tiles, p.kv.n_seq * p.nsplit), dim3(64 * kW), 0, st, p);
