@@ -530,12 +530,14 @@ int bq_kv_read(const bq_kv_cache* kv, const int32_t* seq, const int32_t* pos, in
  *     out for sequence s (device, [n_seq + 1], non-decreasing, within n_rows;
  *     NULL: n_seq must be 1 and its rows are all n_rows), at most `rows` each;
  *     q and the softmax weights enter the products as bf16; over a q8 cache q
- *     and the keys as fp16 (each row over a power of two of its own, so the
- *     range stays fp32's) and the values as bf16.  Sums are fp32.  A few rows
+ *     and the keys as fp16 (each row over a power of two of its own: 2^-11 of
+ *     the row's largest value) and the values as bf16.  Sums are fp32.  A few rows
  *     over many tokens are split over workgroups too, and many rows over a q8
  *     cache convert its tokens once, into work (bq_attn_prefill_workspace_bytes;
  *     with less, or NULL, a smaller split and conversion on the way), with
- *     values and weights in fp16 then (64 tokens' values over a power of two).
+ *     values and weights in fp16 then; rows that see a value whose scale is not
+ *     0 or 2^-18 <= scale < 2 take the codes as they are and weights times scales
+ *     in two bf16 parts instead (any size, 2.5 times as long).
  * scale > 0.  q_heads % kv_heads == 0 and q_heads / kv_heads <= 64, else BQ_UNSUPPORTED.
  * Row strides in elements, multiples of 8. */
 typedef struct bq_attn_args {
