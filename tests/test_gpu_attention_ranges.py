@@ -128,3 +128,45 @@ def test_odd_sizes_behind_masks(bq, window, sinks, D, P):
             ok = ((got[first: first + r] - ref).abs() <= tol * bound).all()
             assert torch.isfinite(got[first: first + r]).all() and ok, (s, r, T)
             first += r
+
+
+def _one_hot(bq, kv, rows, q, k, v, what, prefill):
+    """`rows` rows after T - rows tokens, whose scores are so far apart that each row's softmax is one token."""
+    T, H, D = k.shape
+    P, Hq = 32, q.shape[1] // D
+    pages = R.Pages(kv, H, D, P, 1, (T + P - 1) // P, 5)
+    pages.put(0, k, v)
+    out = torch.empty((rows, Hq * D), device="cuda")
+    att = bq.Attention(pages.cache(bq), q.cuda(), out, torch.tensor([T], dtype=torch.int32, device="cuda"))
+    att.prefill() if prefill else att.decode()
+    got = out.cpu().double().reshape(rows, Hq, D)
+    q = q.reshape(rows, Hq, D)
+    if prefill:
+        q = R.bf16(q).double() if kv == "bf16" else R.half_rows(q)
+    keys = pages.kh[0] if prefill else pages.k[0]
+    scale = D ** -0.5
+    ref, bound, A = R.attention(q.double(), keys, pages.v[0], torch.arange(T - rows, T), scale)
+    s = scale * torch.einsum("rhd,thd->rht", q.double(), keys.repeat_interleave(Hq // H, 1))
+    s.masked_fill_(torch.arange(T)[None, None] > torch.arange(T - rows, T)[:, None, None], -torch.inf)
+    top = s.topk(2, -1).values
+    assert ((top[..., 0] - top[..., 1])[1:] > 2.0 ** -18 * A[1:] + 100).all(), "the test's scores are too close"
+    print(f"  {what}: finite {bool(torch.isfinite(got).all())}", flush=True)
+    assert torch.isfinite(got).all(), what
+    assert ((got - ref).abs() <= 2.0 ** -7 * bound)[1:].all(), what
+
+
+@pytest.mark.parametrize("kv", ["bf16", "q8"])
+@pytest.mark.parametrize("rows,prefill", [(300, True), (40, True), (5, False)])
+@pytest.mark.parametrize("size,sign", [(1e4, 1), (1e4, -1), (1e6, 1), (1e6, -1), (1e8, 1), (1e8, -1), (1e16, 1)])
+def test_scores_of_any_size(bq, kv, rows, prefill, size, sign):
+    """Scores of 1e7 to 1e31, all a row's tokens on the same side of 0, still choose the largest."""
+    T, D, Hq = max(rows, 150), 128, 8
+    k, v, q = _normal(91, T, 1, D), _normal(92, T, 1, D), _normal(93, rows, Hq * D)
+    # one dim decides, in a group of its own: 64 steps to a power of two, in a random order
+    step = torch.randperm(T, generator=torch.Generator().manual_seed(1))
+    k[:, 0, :32] = 0
+    q.reshape(rows, Hq, D)[:, :, :32] = 0
+    k[:, 0, 0] = sign * size * (1 + (step % 64).float() / 64) * 2.0 ** (step // 64 - 3).float()
+    k[:, 0, 32:] *= 1e-3
+    q.reshape(rows, Hq, D)[:, :, 0] = size * (1 + 2.0 ** -4 * torch.arange(Hq))
+    _one_hot(bq, kv, rows, q, k, v, f"{kv} {rows} rows, scores {sign} * {size:.0e}^2", prefill)
