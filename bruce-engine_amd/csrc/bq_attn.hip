@@ -40,7 +40,7 @@ namespace bq {
 namespace {
 constexpr int kWaves = 4;          // per workgroup
 constexpr int kRound = 512;        // 32-token steps whose pages are staged at once
-constexpr float kNone = -1e30f;    // the running maximum before any token
+constexpr float kNone = -3.402823466e38f;  // the running maximum before any token
 constexpr float kLazy = 8.f;
 
 struct DecodeP {

@@ -49,7 +49,7 @@ constexpr int kKvStaged = 2;
 constexpr int kKvCodes = 3;
 constexpr int64_t tile_record(int D) { return 4 * kBN * D + 512; }
 constexpr int kPiece = 8;        // tiles of a piece at least, where the tokens are split
-constexpr float kNone = -1e30f;  // the running maximum before any token
+constexpr float kNone = -3.402823466e38f;  // the running maximum before any token
 constexpr float kLazy = 8.f;     // it moves when a score passes it by more (log2)
 
 struct PrefillP {

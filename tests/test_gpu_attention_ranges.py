@@ -170,3 +170,10 @@ def test_scores_of_any_size(bq, kv, rows, prefill, size, sign):
     k[:, 0, 32:] *= 1e-3
     q.reshape(rows, Hq, D)[:, :, 0] = size * (1 + 2.0 ** -4 * torch.arange(Hq))
     _one_hot(bq, kv, rows, q, k, v, f"{kv} {rows} rows, scores {sign} * {size:.0e}^2", prefill)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "q8"])
+@pytest.mark.parametrize("rows,prefill", [(300, True), (40, True), (5, False)])
+def test_scores_far_below_zero(bq, kv, rows, prefill):
+    """Scores of -1e31: rows that see tokens are not rows that see none."""
+    test_scores_of_any_size(bq, kv, rows, prefill, 1e16, -1)
