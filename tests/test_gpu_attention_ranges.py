@@ -177,3 +177,22 @@ def test_scores_of_any_size(bq, kv, rows, prefill, size, sign):
 def test_scores_far_below_zero(bq, kv, rows, prefill):
     """Scores of -1e31: rows that see tokens are not rows that see none."""
     test_scores_of_any_size(bq, kv, rows, prefill, 1e16, -1)
+
+
+@pytest.mark.parametrize("rows,prefill", [(300, True), (40, True), (5, False)])
+def test_zero_queries_with_a_tiny_scale(bq, rows, prefill):
+    """Equal scores of 0, whatever the scale: the mean of what each row sees."""
+    T, D, Hq, P = max(rows, 150), 128, 8, 32
+    k, v = _normal(94, T, 1, D), _normal(95, T, 1, D)
+    for kv in ("bf16", "q8"):
+        pages = R.Pages(kv, 1, D, P, 1, (T + P - 1) // P, 5)
+        pages.put(0, k, v)
+        out = torch.empty((rows, Hq * D), device="cuda")
+        att = bq.Attention(pages.cache(bq), torch.zeros((rows, Hq * D), device="cuda"), out,
+                           torch.tensor([T], dtype=torch.int32, device="cuda"), scale=1e-20)
+        att.prefill() if prefill else att.decode()
+        got = out.cpu().double().reshape(rows, Hq, D)
+        ref, bound, _ = R.attention(torch.zeros((rows, Hq, D), dtype=torch.float64), pages.k[0], pages.v[0],
+                                    torch.arange(T - rows, T), 1e-20)
+        assert torch.isfinite(got).all(), kv
+        assert ((got - ref).abs() <= 2.0 ** -7 * (1 + 2.0 ** -6) * bound).all(), kv
