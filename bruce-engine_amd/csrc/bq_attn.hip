@@ -149,12 +149,12 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p
                     for (int e = 0; e < 4; ++e) x[k][e] = a[e], x[k][4 + e] = b[e];
                 }
             }
-            if constexpr (Q8) {  // the row's largest value to [16, 32)
+            if constexpr (Q8) {  // the row's largest value to [16, 32), but for rows of 2^-122 and less
 #pragma unroll
                 for (int k = 0; k < KS; ++k)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[k][e]));
-                const int ex = max(-100, min(100, ilogb2(groups_max(amax)) - 4));
+                const int ex = max(-126, min(126, ilogb2(groups_max(amax)) - 4));
                 const float down = pow2(-ex);
                 scale *= pow2(ex);
 #pragma unroll

@@ -111,7 +111,7 @@ BQ_DEV void store4(const PrefillP& p, size_t at, f32x4 y, float l) {
 }
 
 // 2^e of a q8 token's largest key scale, from its bf16 bits
-BQ_DEV int key_power(uint32_t top) { return max(-100, min(100, (int)(top >> 7) - 127)); }
+BQ_DEV int key_power(uint32_t top) { return max(-126, min(126, (int)(top >> 7) - 127)); }
 // 16 key codes (dims 64c + 8g.. and 64c + 32 + 8g..) times two scales over the token's power of two
 BQ_DEV u32x4 half_keys(u32x4 codes, int k, uint16_t scale, float down) {
     const _Float16 sh = (_Float16)(bf2f(scale) * down);

@@ -196,3 +196,23 @@ def test_zero_queries_with_a_tiny_scale(bq, rows, prefill):
                                     torch.arange(T - rows, T), 1e-20)
         assert torch.isfinite(got).all(), kv
         assert ((got - ref).abs() <= 2.0 ** -7 * (1 + 2.0 ** -6) * bound).all(), kv
+
+
+@pytest.mark.parametrize("power", [-118, -60, 60, 100])
+def test_keys_and_queries_of_opposite_size(bq, power):
+    """Keys times 2^power and queries divided by it: the same scores."""
+    T, D, Hq = 300, 128, 8
+    k, v, q = _normal(96, T, 1, D), _normal(97, T, 1, D), _normal(98, T, Hq * D)
+    for rows, prefill in ((300, True), (40, True), (5, False)):
+        pages = R.Pages("q8", 1, D, 32, 1, (T + 31) // 32, 5)
+        pages.put(0, k * 2.0 ** power, v)
+        x = q[:rows] * 2.0 ** -power
+        out = torch.empty((rows, Hq * D), device="cuda")
+        att = bq.Attention(pages.cache(bq), x.cuda(), out, torch.tensor([T], dtype=torch.int32, device="cuda"))
+        att.prefill() if prefill else att.decode()
+        got = out.cpu().double().reshape(rows, Hq, D)
+        xr = R.half_rows(x.reshape(rows, Hq, D)) if prefill else x.double().reshape(rows, Hq, D)
+        ref, bound, A = R.attention(xr, (pages.kh if prefill else pages.k)[0], pages.v[0], torch.arange(T - rows, T), D ** -0.5)
+        tol = (2.0 ** -7 * (1 + 2.0 ** -6) if prefill else 2.0 ** -16) + 2.0 ** -18 * A[..., None]
+        assert torch.isfinite(got).all(), (power, rows)
+        assert ((got - ref).abs() <= tol * bound).all(), (power, rows)
