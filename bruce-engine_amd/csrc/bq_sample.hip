@@ -377,6 +377,7 @@ struct Whole {
     BQ_DEV u64 locate(bool by_count, double target, bool strict, u64 low, u64& upto, bool& many) const {
         const int tid = threadIdx.x;
         auto meets = [&](u64 w) { return strict ? (double)w > target : (double)w >= target; };
+        __syncthreads();  // found[] of a call before has been read by every wave
         if (tid == 0) found[0] = ~0ull, found[2] = 0;
         __syncthreads();
         const u64 a = bins[2 * tid], b = bins[2 * tid + 1];
