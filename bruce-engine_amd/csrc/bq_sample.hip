@@ -229,11 +229,12 @@ __global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
     if (rule.top_k == p.vocab && !rule.greedy) {
         float sum = 0.f;
         if (mx > -INFINITY && mx < INFINITY) {
-            const float inv = 1.44269504088896341f / rule.temp;
+            // finite, and -inf has no mass where it is 0
+            const float inv = fminf(1.44269504088896341f / rule.temp, 3e38f);
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f((v[k][e] - mx) * inv);
+                for (int e = 0; e < 4; ++e) sum += v[k][e] > -INFINITY ? __builtin_amdgcn_exp2f((v[k][e] - mx) * inv) : 0.f;
         }
         sum = wave_sum_dpp63(sum);
         if (lane == 63) s_sum[wave] = sum;
