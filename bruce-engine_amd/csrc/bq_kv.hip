@@ -89,7 +89,8 @@ BQ_DEV void norm_turn(const AppendP& p, const float* w, bool turn, int pos, int 
     }
 }
 
-// 1 / d of a bf16 scale (0 for an all-zero group); codes of two values and more below
+// 1 / d of a bf16 scale (0 for an all-zero group, and for one that holds a NaN or an
+// infinity, which stay in the scale)
 BQ_DEV float scale_of(float amax, uint16_t& bits) {
     bits = f2bf(amax * (1.f / 127.f));
     const float d = bf2f(bits);
@@ -212,14 +213,15 @@ __global__ void __launch_bounds__(256) k_append(AppendP p) {
     } else {
         for (int i = tid; i < R * D / 16; i += 256) {  // scale of (key or value, row, 32 dims)
             const int r = i % R, c = i / R % (D / 32), which = i / (R * (D / 32));
-            float amax = 0.f;
+            uint32_t amax = 0;  // the largest magnitude's bits: a NaN's are above all others
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const f32x4 x = *(const f32x4*)&rowv[which][r][32 * c + 4 * e];
-                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+                const u32x4 x = *(const u32x4*)&rowv[which][r][32 * c + 4 * e];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) amax = max(amax, x[k] & 0x7FFFFFFFu);
             }
             uint16_t bits;
-            const float inv = scale_of(amax, bits);
+            const float inv = scale_of(as_float(amax), bits);
             s_inv[which][r][c] = inv;
             if (s_page[r] >= 0)
                 *(uint16_t*)(head_at(r) + (which ? kv_vs_off(P, D, c, s_tok[r]) : kv_ks_off(P, D, c, s_tok[r]))) = bits;

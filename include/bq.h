@@ -466,7 +466,8 @@ void bq_decode_graph_destroy(bq_decode_graph* g);
  *                 V codes [P/8][D/32][16][2][8]: token 8t + i, dim 32c + 16u + m at [t][c][m][u][i]
  *                 K scales bf16 [D/32][P], V scales bf16 [D/32][P]
  *                 per (token, 32 dims) d = bf16(amax / 127), code = clamp(rint(x / d), -127, 127)
- * (a bf16 scale keeps fp32's range, so no finite row overflows it).
+ * (a bf16 scale keeps fp32's range, so no finite row overflows it; a NaN or an
+ * infinity among the 32 values makes the scale one).
  * bq_kv_page_bytes is the size of one page, 0 for a layout that is not handled. */
 enum { BQ_TYPE_F32 = 0, BQ_TYPE_Q8_0 = 8, BQ_TYPE_BF16 = 30 }; /* GGML type ids */
 typedef struct bq_kv_cache {
