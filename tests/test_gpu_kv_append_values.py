@@ -1,12 +1,45 @@
-"""bq_append of rows whose values are not numbers or very small
-(values: test_gpu_kv_append.py)."""
+"""bq_append of long prompts, and of rows whose values are not numbers or very small
+(reference and tolerances: test_gpu_kv_append.py)."""
 import pytest
 import torch
 
 import serve_ref as R
-from test_gpu_kv_append import _rows
+from test_gpu_kv_append import _rows, test_append_matches_reference as _matches
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kv", ["bf16", "q8"])
+@pytest.mark.parametrize("rows,n_seq,kind,Hq,H,D,P,rot,inter,norm", [
+    (1025, 4, "run", 3, 2, 64, 16, 64, False, True),
+    (1100, 5, "run", 5, 1, 128, 64, 128, False, True),
+    (1030, 4, "run", 2, 2, 256, 128, 128, True, False),
+    (1040, 5, "mixed", 2, 1, 128, 32, 64, False, True),
+])
+def test_prompts_match_reference(bq, kv, rows, n_seq, kind, Hq, H, D, P, rot, inter, norm):
+    """Past 1024 rows a workgroup takes 16 rows of a head and stores 8 neighbouring tokens of a value as one unit."""
+    _matches(bq, kv, rows, n_seq, kind, Hq, H, D, P, rot, inter, norm)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "q8"])
+@pytest.mark.parametrize("D,P", [(64, 16), (128, 64), (256, 256)])
+def test_prompt_equals_its_pieces(bq, kv, D, P):
+    """A prompt in one call and in calls of a few rows gives the same pages and queries, bit for bit."""
+    H, Hq, rows, at = 2, 4, 1500, 5
+    g = _rows(D, rows, (Hq + 2 * H) * D).cuda()
+    pos = torch.arange(at, at + rows, dtype=torch.int32, device="cuda")
+    rope = bq.rope_table(at + rows, D)
+    table = torch.arange((at + rows + P - 1) // P, dtype=torch.int32, device="cuda").flip(0)[None].contiguous()
+    cut, made = (Hq * D, (Hq + H) * D), []
+    for step in (rows, 700, 33):
+        cache = bq.KvCache.empty(table.shape[1], table, kv, H, D, P)
+        q = torch.empty((rows, Hq * D), device="cuda")
+        for a in range(0, rows, step):
+            x = g[a: a + step]
+            bq.Append(cache, x[:, : cut[0]], x[:, cut[0]: cut[1]], x[:, cut[1]:], pos[a: a + step], q[a: a + step], rope=rope).run()
+        made.append((cache.pages, q))
+    for pages, q in made[1:]:
+        assert torch.equal(pages, made[0][0]) and torch.equal(q, made[0][1])
 
 
 def _append_raw(bq, kv, k, v, P=32):
