@@ -90,16 +90,16 @@ BQ_DEV void norm_turn(const AppendP& p, const float* w, bool turn, int pos, int 
 }
 
 // 1 / d of a bf16 scale (0 for an all-zero group, and for one that holds a NaN or an
-// infinity, which stay in the scale)
+// infinity, which stay in the scale).  Below 2^-120 it may pass fp32's range: then
+// minus 1 / (2^24 d), against which the values are taken times -2^24.
 BQ_DEV float scale_of(float amax, uint16_t& bits) {
     bits = f2bf(amax * (1.f / 127.f));
     const float d = bf2f(bits);
-    return d > 0.f ? 1.f / d : 0.f;
+    return d >= 0x1p-120f ? 1.f / d : d > 0.f ? -1.f / (d * 0x1p24f) : 0.f;
 }
 BQ_DEV uint32_t code_of(float x, float inv) {
-    // fmed3 after the product: a NaN (0 * inf of a denormal scale) becomes a bound, so 0 is kept apart
-    const float c = x == 0.f ? 0.f : __builtin_amdgcn_fmed3f(x * inv, -127.f, 127.f);
-    return (uint32_t)(int)rintf(c) & 0xFF;
+    const float y = inv < 0.f ? x * -0x1p24f : x;
+    return (uint32_t)(int)rintf(__builtin_amdgcn_fmed3f(y * inv, -127.f, 127.f)) & 0xFF;
 }
 
 template <int D, int KV, int R>

@@ -74,3 +74,24 @@ def test_what_is_no_number_stays_none(bq, kv, rows, bad):
             assert not torch.isfinite(clean[1][which][r, c]), (which, r, c, clean[1][which][r, c])
             same[r, c // 32 * 32: c // 32 * 32 + 32] = False
         assert torch.equal(clean[0][which][same], clean[1][which][same])
+
+
+@pytest.mark.parametrize("rows", [12, 1100])
+@pytest.mark.parametrize("size", [1e-30, 1e-35, 1e-36, 1e-37, 4e-38])
+def test_codes_of_tiny_values(bq, rows, size):
+    """Codes are taken against the stored scale where its reciprocal passes fp32's range, too."""
+    H, D, P = 1, 64, 32
+    k, v = (_rows(s, rows, D) * size for s in (5, 6))
+    cache, _ = _append_raw(bq, "q8", k, v, P)
+    raw = cache.pages.cpu().reshape(cache.pages.shape[0], H, -1)
+    t, d = torch.arange(rows)[:, None], torch.arange(D)[None]
+    page = cache.table.cpu()[0][torch.arange(rows) // P].long()[:, None]
+    for value, x in ((0, k), (1, v)):
+        code, sc = R.addr_q8(P, D, t % P, d, value)
+        c = raw.view(torch.int8)[page, 0, code].double()
+        s = raw.view(torch.bfloat16)[page, 0, sc // 2].double()
+        amax = x.double().reshape(rows, -1, 32).abs().amax(-1).repeat_interleave(32, -1)
+        # bf16: half a step of 8 bits, or of 2^-133
+        assert ((s - amax / 127).abs() <= torch.clamp(2.0 ** -8 * amax / 127, min=2.0 ** -134) * (1 + 2.0 ** -10)).all()
+        want = torch.where(s > 0, (x.double() / s.clamp(min=2.0 ** -140)), torch.zeros(())).clamp(-127, 127)
+        assert ((c - want).abs() <= 0.5 + 2.0 ** -10).all(), (size, (c - want).abs().max())
