@@ -27,6 +27,8 @@ CFLAGS = [
     # MFMA results in VGPRs (not AGPRs): the epilogues read every accumulator
     "-mllvm", "-amdgpu-mfma-vgpr-form=1",
     "-Wno-unused-command-line-argument",
+    # an attribute that the compiler does not know (an alignment spelt wrongly) ends the build
+    "-Werror=unknown-attributes",
 ]
 
 

@@ -116,7 +116,7 @@ template <int D, int KV, int NQ, int NP>
 __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p) {
     constexpr int KS = D / 32, DT = D / 16;
     __shared__ int s_page[kRound * 2];
-    __shared__ __attribute__((aligned16)) float s_o[kWaves][16][D + 4];
+    __shared__ __attribute__((aligned(16))) float s_o[kWaves][16][D + 4];
     __shared__ float s_m[kWaves][16], s_l[kWaves][16], s_mt[16], s_lt[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const KvView& kv = p.kv;
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p
 template <int D, int T>
 __global__ void __launch_bounds__(T) k_attn_join(DecodeP p) {
     constexpr int L = D / 4, S = T / L;
-    __shared__ __attribute__((aligned16)) float s_o[S][D];
+    __shared__ __attribute__((aligned(16))) float s_o[S][D];
     __shared__ float s_l[S], s_mx[T / 64];
     const int ht = p.kv.heads, tid = threadIdx.x;
     const int row = blockIdx.x, h = blockIdx.y, seq = blockIdx.z;
