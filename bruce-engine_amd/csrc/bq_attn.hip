@@ -101,7 +101,7 @@ BQ_DEV f16x8 codes8h(uint32_t lo, uint32_t hi) {
 BQ_DEV f32x4 mfma16h(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 BQ_DEV f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// sum over the four lane groups that share lane & 15
+// largest and sum over the four lane groups that share lane & 15
 BQ_DEV float groups_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16, 64));
     return fmaxf(v, __shfl_xor(v, 32, 64));

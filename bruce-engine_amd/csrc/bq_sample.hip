@@ -674,11 +674,6 @@ __global__ void __launch_bounds__(1024) k_sample_pick(SampleP p) {
         int n = 64;
         while (n < total) n <<= 1;
         u64 *const keys = s_key + kMaxCand, *const weights = s_bins + kMaxCand;
-        auto put = [&](int to, u64 key) {
-            const float e = key ? expf((unordered((uint32_t)(key >> 32)) - mx) / rule.temp) : 0.f;
-            keys[to] = key;
-            weights[to] = mass(e) | (e < rule.min_p ? kBelow : 0);
-        };
         u64 key = tid < total ? s_key[tid] : 0;
         int to = tid;
         if (s_many) {
