@@ -323,7 +323,7 @@ size_t prefill_part_floats(int n_rows, int q_heads, int D) { return (size_t)n_ro
 // read: below kStageRows rows of a head group, or beyond 1 GiB.
 size_t prefill_stage_bytes(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int max_len) {
     if (type != kKvQ8 || (int64_t)rows * (q_heads / kv_heads) < kStageRows) return 0;
-    const size_t n = (size_t)n_seq * kv_heads * ((max_len + kBN - 1) / kBN) * tile_record(D);
+    const size_t n = (size_t)n_seq * kv_heads * (((int64_t)max_len + kBN - 1) / kBN) * tile_record(D);
     return n <= (size_t)1 << 30 ? n : 0;
 }
 

@@ -36,9 +36,9 @@ int view_of(const bq_kv_cache* c, KvView& v, int& type) {
     v.plog = __builtin_ctz((unsigned)c->page_tokens);
     v.n_pages = c->n_pages;
     v.n_seq = c->n_seq;
-    // token indices are 32-bit: a longer table row is never reached (kv_page
-    // strides by the true row length)
-    if (c->max_pages > (INT32_MAX >> v.plog)) return BQ_UNSUPPORTED;
+    // token indices are 32-bit, and a tile's end is one past its last token: room for
+    // one tile (and the tokens of a window's last step) above the longest sequence
+    if (c->max_pages > ((INT32_MAX - 127) >> v.plog)) return BQ_UNSUPPORTED;
     v.max_pages = c->max_pages;
     type = c->type == BQ_TYPE_BF16 ? kKvBf16 : kKvQ8;
     return BQ_OK;

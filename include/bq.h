@@ -468,7 +468,8 @@ void bq_decode_graph_destroy(bq_decode_graph* g);
  *                 per (token, 32 dims) d = bf16(amax / 127), code = clamp(rint(x / d), -127, 127)
  * (a bf16 scale keeps fp32's range, so no finite row overflows it; a NaN or an
  * infinity among the 32 values makes the scale one).
- * bq_kv_page_bytes is the size of one page, 0 for a layout that is not handled. */
+ * bq_kv_page_bytes is the size of one page, 0 for a layout that is not handled.
+ * A table row reaches at most 2^31 - 128 tokens (else BQ_UNSUPPORTED). */
 enum { BQ_TYPE_F32 = 0, BQ_TYPE_Q8_0 = 8, BQ_TYPE_BF16 = 30 }; /* GGML type ids */
 typedef struct bq_kv_cache {
     void* pages;                  /* [n_pages][bq_kv_page_bytes], 16-byte aligned */
