@@ -611,6 +611,22 @@ def _raw_stream(device):
     return get(device) if get is not None else torch.cuda.current_stream(device).cuda_stream
 
 
+def _on(device, f, *args):
+    """f(*args, stream) on the current stream of a device, which is made the current one for the call."""
+    import torch
+    if torch.cuda.current_device() == device:
+        return f(*args, _raw_stream(device))
+    with torch.cuda.device(device):
+        return f(*args, _raw_stream(device))
+
+
+def _one_device(device, **tensors):
+    """ValueError unless every tensor (or None) lies on this device."""
+    for what, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: on {device}, not {t.device}")
+
+
 def _type_of(t, what):
     import torch
     if t.dtype == torch.float32:
@@ -662,6 +678,7 @@ class KvCache:
         n = kv_page_bytes(kv_type, kv_heads, head_dim, page_tokens)
         _expect(pages, torch.uint8, (pages.shape[0], n), "pages")
         _expect(table, torch.int32, (table.shape[0], table.shape[1]), "table")
+        _one_device(pages.device, table=table)
         self.pages, self.table, self.kv_heads, self.head_dim = pages, table, kv_heads, head_dim
         self.struct = KvCacheStruct(_ptr(pages), _ptr(table), KV_TYPES[kv_type], kv_heads, head_dim, page_tokens,
                                     pages.shape[0], table.shape[0], table.shape[1])
@@ -684,7 +701,8 @@ class KvCache:
             _expect(t, torch.int32, (rows,), what)
         for t, what in ((k, "k"), (v, "v")):
             _expect(t, torch.bfloat16, (rows, self.kv_heads * self.head_dim), what)
-        return _check(self._read(self.ref, _ptr(seq), _ptr(pos), rows, _ptr(k), _ptr(v), _raw_stream(self.device)), "bq_kv_read")
+        _one_device(self.pages.device, pos=pos, seq=seq, k=k, v=v)
+        return _check(_on(self.device, self._read, self.ref, _ptr(seq), _ptr(pos), rows, _ptr(k), _ptr(v)), "bq_kv_read")
 
 
 class Append:
@@ -710,6 +728,7 @@ class Append:
             if t.dtype != torch.float32 or t.shape[0] != rows:
                 raise ValueError(f"{what}: fp32 rows, as many as pos has")
         ld = [_rows_ld(q, width, "q")] + [_rows_ld(t, kv.kv_heads * D, "k, v") for t in (k, v)]
+        _one_device(kv.pages.device, q=q, k=k, v=v, pos=pos, seq=seq, q_weight=q_weight, k_weight=k_weight, rope=rope, q_out=q_out)
         rot = 0 if rope is None else rope.shape[1]
         if n_pos is None:
             n_pos = (1 << 31) - 1 if rope is None else rope.shape[0]
@@ -722,7 +741,7 @@ class Append:
         self._ref, self._run = ctypes.byref(self.struct), load().bq_append
 
     def run(self):
-        return _check(self._run(self.kv.ref, self._ref, _raw_stream(self.kv.device)), "bq_append")
+        return _check(_on(self.kv.device, self._run, self.kv.ref, self._ref), "bq_append")
 
 
 class Attention:
@@ -740,6 +759,7 @@ class Attention:
             raise ValueError("q and out: rows of whole heads, alike")
         _expect(kv_len, torch.int32, (n_seq,), "kv_len")
         _expect(row0, torch.int32, (n_seq + 1,), "row0")
+        _one_device(kv.pages.device, q=q, out=out, kv_len=kv_len, row0=row0)
         P = kv.struct.page_tokens
         if max_len is None:
             max_len = kv.table.shape[1] * P
@@ -757,6 +777,7 @@ class Attention:
                 n = max(n, L.bq_attn_prefill_workspace_bytes(kv.struct.type, n_seq, rows, n_rows, width // D,
                                                               kv.kv_heads, D, max_len))
             work = torch.empty(n // 4, dtype=torch.float32, device=q.device) if n else None
+        _one_device(q.device, work=work)
         self.kv, self._keep = kv, (q, out, kv_len, row0, work)
         self.struct = AttnArgs(_ptr(q), _ptr(out), _type_of(q, "q"), _type_of(out, "out"), _rows_ld(q, width, "q"),
                                _rows_ld(out, width, "out"), width // D, n_rows, rows, _ptr(row0), _ptr(kv_len), max_len,
@@ -765,10 +786,10 @@ class Attention:
         self._ref, self._decode, self._prefill = ctypes.byref(self.struct), L.bq_attn_decode, L.bq_attn_prefill
 
     def decode(self):
-        return _check(self._decode(self.kv.ref, self._ref, _raw_stream(self.kv.device)), "bq_attn_decode")
+        return _check(_on(self.kv.device, self._decode, self.kv.ref, self._ref), "bq_attn_decode")
 
     def prefill(self):
-        return _check(self._prefill(self.kv.ref, self._ref, _raw_stream(self.kv.device)), "bq_attn_prefill")
+        return _check(_on(self.kv.device, self._prefill, self.kv.ref, self._ref), "bq_attn_prefill")
 
 
 class AttentionPlan:
@@ -807,9 +828,11 @@ class Sampler:
         _expect(top_k, torch.int32, (rows,), "top_k")
         for t, what in ((u, "u"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")):
             _expect(t, torch.float32, (rows,), what)
+        _one_device(logits.device, out=out, u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         L = load()
         if work is None:
             work = torch.empty(int(L.bq_sample_workspace_bytes(rows, vocab)), dtype=torch.uint8, device=logits.device)
+        _one_device(logits.device, work=work)
         ld = _rows_ld(logits, vocab, "logits")
         self._keep = (logits, out, u, temperature, top_k, top_p, min_p, work)
         self._args = (_ptr(logits), ld, rows, vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(u),
@@ -817,4 +840,4 @@ class Sampler:
         self._run, self._device = L.bq_sample, logits.device.index
 
     def run(self):
-        return _check(self._run(*self._args, _raw_stream(self._device)), "bq_sample")
+        return _check(_on(self._device, self._run, *self._args), "bq_sample")
