@@ -627,6 +627,13 @@ def _one_device(device, **tensors):
             raise ValueError(f"{what}: on {device}, not {t.device}")
 
 
+def _work_of(work, device):
+    """A caller's workspace (or None): its bytes have to be there, and on the device."""
+    if work is not None and (not work.is_cuda or work.device != device or not work.is_contiguous()):
+        raise ValueError(f"work: a contiguous tensor on {device}")
+    return work
+
+
 def _type_of(t, what):
     import torch
     if t.dtype == torch.float32:
@@ -777,7 +784,7 @@ class Attention:
                 n = max(n, L.bq_attn_prefill_workspace_bytes(kv.struct.type, n_seq, rows, n_rows, width // D,
                                                               kv.kv_heads, D, max_len))
             work = torch.empty(n // 4, dtype=torch.float32, device=q.device) if n else None
-        _one_device(q.device, work=work)
+        _work_of(work, q.device)
         self.kv, self._keep = kv, (q, out, kv_len, row0, work)
         self.struct = AttnArgs(_ptr(q), _ptr(out), _type_of(q, "q"), _type_of(out, "out"), _rows_ld(q, width, "q"),
                                _rows_ld(out, width, "out"), width // D, n_rows, rows, _ptr(row0), _ptr(kv_len), max_len,
@@ -832,7 +839,7 @@ class Sampler:
         L = load()
         if work is None:
             work = torch.empty(int(L.bq_sample_workspace_bytes(rows, vocab)), dtype=torch.uint8, device=logits.device)
-        _one_device(logits.device, work=work)
+        _work_of(work, logits.device)
         ld = _rows_ld(logits, vocab, "logits")
         self._keep = (logits, out, u, temperature, top_k, top_p, min_p, work)
         self._args = (_ptr(logits), ld, rows, vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(u),

@@ -72,6 +72,13 @@ def test_tensors_of_another_device(op):
         _cache(Fake(I, 1, 2, index=1))
 
 
+def test_workspaces_that_are_not_there():
+    """A strided or expanded workspace has fewer bytes in a row than its elements say."""
+    for op in ("attention", "sampler"):
+        with pytest.raises(ValueError):
+            _make(op, "work", contiguous=False)
+
+
 @pytest.mark.parametrize("current", [0, 1])
 def test_calls_go_to_the_tensors_device(monkeypatch, current):
     """The launch, not only the stream, is the tensors' device's, whichever is current; the current one comes back."""
