@@ -604,18 +604,22 @@ class DecodeGraph:
 
 
 # ---------------------------------------------------------------- serving operators
-def _raw_stream(device):
-    """The current stream of a device as a number (torch.cuda.current_stream builds an object for it)."""
-    import torch
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return get(device) if get is not None else torch.cuda.current_stream(device).cuda_stream
+# the current device, and a device's current stream as a number (torch.cuda's own functions check and build
+# more, and a call of an operator takes a few microseconds)
+_current = _raw_stream = None
+
+
+def _bind_device():
+    global _current, _raw_stream
+    if _current is None:
+        import torch
+        _current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda d: torch.cuda.current_stream(d).cuda_stream)
 
 
 def _on(device, f, *args):
-    """f(*args, stream) on the current stream of a device, which is made the current one for the call."""
+    """f(*args, stream) on the current stream of a device that is not the current one."""
     import torch
-    if torch.cuda.current_device() == device:
-        return f(*args, _raw_stream(device))
     with torch.cuda.device(device):
         return f(*args, _raw_stream(device))
 
@@ -691,6 +695,7 @@ class KvCache:
                                     pages.shape[0], table.shape[0], table.shape[1])
         self.ref = ctypes.byref(self.struct)
         self._read, self.device = load().bq_kv_read, pages.device.index
+        _bind_device()
 
     @classmethod
     def empty(cls, n_pages, table, kv_type, kv_heads, head_dim, page_tokens, device="cuda"):
@@ -709,7 +714,8 @@ class KvCache:
         for t, what in ((k, "k"), (v, "v")):
             _expect(t, torch.bfloat16, (rows, self.kv_heads * self.head_dim), what)
         _one_device(self.pages.device, pos=pos, seq=seq, k=k, v=v)
-        return _check(_on(self.device, self._read, self.ref, _ptr(seq), _ptr(pos), rows, _ptr(k), _ptr(v)), "bq_kv_read")
+        args, d = (self.ref, _ptr(seq), _ptr(pos), rows, _ptr(k), _ptr(v)), self.device
+        return _check(self._read(*args, _raw_stream(d)) if _current() == d else _on(d, self._read, *args), "bq_kv_read")
 
 
 class Append:
@@ -748,7 +754,8 @@ class Append:
         self._ref, self._run = ctypes.byref(self.struct), load().bq_append
 
     def run(self):
-        return _check(_on(self.kv.device, self._run, self.kv.ref, self._ref), "bq_append")
+        kv, d = self.kv.ref, self.kv.device
+        return _check(self._run(kv, self._ref, _raw_stream(d)) if _current() == d else _on(d, self._run, kv, self._ref), "bq_append")
 
 
 class Attention:
@@ -793,10 +800,14 @@ class Attention:
         self._ref, self._decode, self._prefill = ctypes.byref(self.struct), L.bq_attn_decode, L.bq_attn_prefill
 
     def decode(self):
-        return _check(_on(self.kv.device, self._decode, self.kv.ref, self._ref), "bq_attn_decode")
+        return self._call(self._decode, "bq_attn_decode")
 
     def prefill(self):
-        return _check(_on(self.kv.device, self._prefill, self.kv.ref, self._ref), "bq_attn_prefill")
+        return self._call(self._prefill, "bq_attn_prefill")
+
+    def _call(self, f, what):
+        kv, d = self.kv.ref, self.kv.device
+        return _check(f(kv, self._ref, _raw_stream(d)) if _current() == d else _on(d, f, kv, self._ref), what)
 
 
 class AttentionPlan:
@@ -845,6 +856,8 @@ class Sampler:
         self._args = (_ptr(logits), ld, rows, vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(u),
                       _ptr(out), _ptr(work), work.numel() * work.element_size())
         self._run, self._device = L.bq_sample, logits.device.index
+        _bind_device()
 
     def run(self):
-        return _check(_on(self._device, self._run, *self._args), "bq_sample")
+        d = self._device
+        return _check(self._run(*self._args, _raw_stream(d)) if _current() == d else _on(d, self._run, *self._args), "bq_sample")

@@ -89,7 +89,8 @@ def test_calls_go_to_the_tensors_device(monkeypatch, current):
         before, now[0] = now[0], d
         yield
         now[0] = before
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    bq._bind_device()
+    monkeypatch.setattr(bq, "_current", lambda: now[0])
     monkeypatch.setattr(torch.cuda, "device", device)
     monkeypatch.setattr(bq, "_raw_stream", lambda d: 1000 + d)
     call = lambda *a: seen.append((now[0], a[-1])) or 0
