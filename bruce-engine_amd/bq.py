@@ -762,7 +762,8 @@ class Attention:
     """bq_attn_decode / bq_attn_prefill over fixed buffers: q and out [n_rows, q_heads * D] fp32 or bf16 (rows
     may be strided), kv_len int32 [n_seq].  For prefill() of a batch row0 int32 [n_seq + 1], max_rows the most
     rows a sequence has; for decode() every sequence has n_rows / n_seq rows.  work: a workspace tensor of the
-    caller's, "auto" for one of the object's own, None for none (no split)."""
+    caller's, "auto" for one of the object's own (its `work`, which other objects may share if their calls are
+    ordered), None for none (no split)."""
 
     def __init__(self, kv, q, out, kv_len, scale=None, window=0, sinks=0, max_len=None, row0=None, max_rows=None,
                  work="auto"):
@@ -792,7 +793,7 @@ class Attention:
                                                               kv.kv_heads, D, max_len))
             work = torch.empty(n // 4, dtype=torch.float32, device=q.device) if n else None
         _work_of(work, q.device)
-        self.kv, self._keep = kv, (q, out, kv_len, row0, work)
+        self.kv, self.work, self._keep = kv, work, (q, out, kv_len, row0)
         self.struct = AttnArgs(_ptr(q), _ptr(out), _type_of(q, "q"), _type_of(out, "out"), _rows_ld(q, width, "q"),
                                _rows_ld(out, width, "out"), width // D, n_rows, rows, _ptr(row0), _ptr(kv_len), max_len,
                                D ** -0.5 if scale is None else scale, window, sinks, _ptr(work),

@@ -78,9 +78,10 @@ class Model:
 
 class Step:
     """A decode step over `rows` rows of the model: buffers, the attention plan over `caches`, and run().  decode:
-    row r is the next token of sequence r; otherwise the rows are a chunk of the only sequence of the caches."""
+    row r is the next token of sequence r; otherwise the rows are a chunk of the only sequence of the caches.
+    max_len: the most tokens a sequence has in any run (it sizes the attention's workspace and its pieces)."""
 
-    def __init__(self, model, caches, rope, rows, pos, kv_len, decode):
+    def __init__(self, model, caches, rope, rows, pos, kv_len, max_len, decode):
         import torch
         c, self.model, self.rows = model.c, model, rows
         f32 = lambda *s: torch.zeros(s, device="cuda")
@@ -100,6 +101,7 @@ class Step:
         work = torch.empty(8 << 20, dtype=torch.float32, device="cuda")
         P, ptr = ctypes.pointer, lambda t: t.data_ptr()
         blocks, plan, keep = [], [], []
+        attn_work = "auto"  # the layers run one after another: the first one's serves all
         for cache, L in zip(caches, model.layers):
             qkv = (bq.Weight * 4)(*L["qkv"])
             outs = (ctypes.c_void_p * 4)(*[ptr(t) for t in self.qkv])
@@ -110,7 +112,10 @@ class Step:
             blocks.append(b)
             append = bq.Append(cache, self.qkv[0], self.qkv[1], self.qkv[3], pos, self.q, seq=seq, q_weight=L["q_weight"],
                                k_weight=L["k_weight"], rope=rope)
-            plan.append((append, bq.Attention(cache, self.q, self.attn_out, kv_len, window=c.window, sinks=c.sinks)))
+            attention = bq.Attention(cache, self.q, self.attn_out, kv_len, window=c.window, sinks=c.sinks, max_len=max_len,
+                                     work=attn_work)
+            attn_work = attention.work
+            plan.append((append, attention))
             b = bq.DecodeBlock()
             b.kind, b.alpha, b.gate, b.up, b.down = bq.BLOCK_FFN, ptr(L["alpha_f"]), P(L["gate"]), P(L["up"]), P(L["down"])
             b.s_gate, b.s_up, b.n_ff = ptr(L["s_gate"]), ptr(L["s_up"]), c.n_ff
@@ -162,7 +167,7 @@ class Generator:
         self.length = torch.zeros(n_seq, dtype=torch.int32, device="cuda")   # tokens cached per sequence
         self.pos = torch.zeros(n_seq, dtype=torch.int32, device="cuda")      # of the decode step's rows
         self.kv_len = torch.zeros(n_seq, dtype=torch.int32, device="cuda")
-        self.step = Step(model, self.caches, self.rope, n_seq, self.pos, self.kv_len, True)
+        self.step = Step(model, self.caches, self.rope, n_seq, self.pos, self.kv_len, max_len, True)
         self.tokens = torch.zeros(n_seq, dtype=torch.int32, device="cuda")
         self.u = torch.zeros(n_seq, device="cuda")
         self.gen = torch.Generator(device="cuda").manual_seed(seed)
@@ -178,7 +183,8 @@ class Generator:
             left = len(prompt) - done
             n = -(-left // -(-left // chunk))
             pos = torch.arange(done, done + n, dtype=torch.int32, device="cuda")
-            step = Step(self.model, views, self.rope, n, pos, torch.tensor([done + n], dtype=torch.int32, device="cuda"), False)
+            step = Step(self.model, views, self.rope, n, pos, torch.tensor([done + n], dtype=torch.int32, device="cuda"),
+                        done + n, False)
             logits = step.run(prompt[done: done + n])
             done += n
         self.length[s] = len(prompt)
