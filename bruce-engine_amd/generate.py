@@ -168,6 +168,7 @@ class Generator:
         self.pos = torch.zeros(n_seq, dtype=torch.int32, device="cuda")      # of the decode step's rows
         self.kv_len = torch.zeros(n_seq, dtype=torch.int32, device="cuda")
         self.step = Step(model, self.caches, self.rope, n_seq, self.pos, self.kv_len, max_len, True)
+        self.used = [0] * n_seq                                              # of max_len tokens, on the host
         self.tokens = torch.zeros(n_seq, dtype=torch.int32, device="cuda")
         self.u = torch.zeros(n_seq, device="cuda")
         self.gen = torch.Generator(device="cuda").manual_seed(seed)
@@ -177,6 +178,8 @@ class Generator:
         token's logits [vocab].  (Even, as a few tokens left over would take the decode path, which rounds otherwise.)"""
         import torch
         c, done = self.model.c, 0
+        if len(prompt) > self.max_len:
+            raise ValueError(f"a prompt of {len(prompt)} tokens: the caches have room for {self.max_len}")
         row = self.table[s: s + 1].contiguous()
         views = [bq.KvCache(k.pages, row, c.kv_type, c.kv_heads, c.head_dim, c.page_tokens) for k in self.caches]
         while done < len(prompt):
@@ -187,7 +190,7 @@ class Generator:
                         done + n, False)
             logits = step.run(prompt[done: done + n])
             done += n
-        self.length[s] = len(prompt)
+        self.length[s] = self.used[s] = len(prompt)
         return logits[-1]
 
     def set_sampling(self, temperature=0.8, top_k=40, top_p=0.95, min_p=0.0):
@@ -204,6 +207,9 @@ class Generator:
 
     def decode(self):
         """One more token of every sequence, from self.tokens into self.tokens."""
+        if max(self.used) >= self.max_len:
+            raise ValueError(f"a sequence has its {self.max_len} tokens: the caches have no room for another")
+        self.used = [n + 1 for n in self.used]
         self.pos.copy_(self.length)
         self.length += 1
         self.kv_len.copy_(self.length)

@@ -45,3 +45,21 @@ def test_layers_share_a_workspace_of_the_tokens_size(bq):
     # the same tokens: the same workspace and the same logits, whatever the caches have room for
     assert got[0][0] == got[1][0]
     assert torch.equal(got[0][1], got[1][1])
+
+
+def test_full_caches_are_an_error(bq):
+    import generate as G
+    c = _config(G)
+    g = G.Generator(G.Model(c, 6), 2, 20)
+    g.set_sampling()
+    gen = torch.Generator().manual_seed(2)
+    with pytest.raises(ValueError):
+        g.prefill(0, torch.randint(0, c.vocab, (21,), generator=gen).int().cuda())
+    for s, n in ((0, 5), (1, 18)):
+        g.first(s, g.prefill(s, torch.randint(0, c.vocab, (n,), generator=gen).int().cuda()))
+    g.decode()
+    g.decode()
+    tokens, length = g.tokens.clone(), g.length.tolist()
+    with pytest.raises(ValueError):
+        g.decode()
+    assert g.length.tolist() == length == [7, 20] and torch.equal(g.tokens, tokens)
