@@ -229,12 +229,18 @@ __global__ void __launch_bounds__(256) k_sample_scan(SampleP p) {
     if (rule.top_k == p.vocab && !rule.greedy) {
         float sum = 0.f;
         if (mx > -INFINITY && mx < INFINITY) {
-            // finite, and -inf has no mass where it is 0
-            const float inv = fminf(1.44269504088896341f / rule.temp, 3e38f);
+            const float inv = fminf(1.44269504088896341f / rule.temp, 3e38f);  // finite: 0 * inf is no mass
+            if (inv > 0.f) {
 #pragma unroll
-            for (int k = 0; k < V; ++k)
+                for (int k = 0; k < V; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum += v[k][e] > -INFINITY ? __builtin_amdgcn_exp2f((v[k][e] - mx) * inv) : 0.f;
+                    for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f((v[k][e] - mx) * inv);
+            } else {  // an infinite temperature: the tokens above -inf
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum += v[k][e] > -INFINITY ? 1.f : 0.f;
+            }
         }
         sum = wave_sum_dpp63(sum);
         if (lane == 63) s_sum[wave] = sum;
