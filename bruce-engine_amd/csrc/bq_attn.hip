@@ -448,7 +448,9 @@ int q_tiles(int rows, int G) { return (rows * G + 15) / 16; }
 }  // namespace
 
 // Pieces that the `len` tokens of a sequence that its rows see are cut into: two
-// workgroups per CU, each wave at least one 32-token step.  A few steps are not
+// workgroups per CU, each wave at least one 32-token step.  (At D 256 one fits a CU
+// in all forms but a bf16 cache's with bf16 in and out, so the pieces of a long
+// sequence run in two rounds there.)  A few steps are not
 // cut, as the join is a launch of its own (2.5 us) and a step costs what its
 // bytes do, a q8 one twice that: 512 tokens of bf16 D 128 take 7.8 us whole and
 // 8.3 in four pieces, 777 10.9 and 8.4; D 64 5.7 / 7.5 and 8.1 / 8.1; D 256 11.5

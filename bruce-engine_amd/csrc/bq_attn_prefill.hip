@@ -27,11 +27,13 @@
 //
 // Few rows over many tokens are split over workgroups (prefill_splits) and joined
 // in the pieces' order; a short chunk halves the row tiles (half_tiles).
-// Measured (32 heads of 128 over 4, bf16): 8192 rows 555 us, 990 TFLOP/s of the
-// 1187 that a large library product reaches; 512 rows 15.4 us, where the launch,
-// the first tile's latency (page, then K and V) and the epilogue are most of it.
-// Five ragged chunks of up to 700 rows over a q8 cache, window 2048: 175 us for
-// 77.7 GFLOP; the 584 row tiles fill 512 slots once and then 72 of them again.
+// Measured (32 heads of 128 over 4, bf16): 8192 rows 557 us, 986 TFLOP/s of the
+// 1187 that a large library product reaches; 512 rows 15.7 us, eight dependent tiles
+// on half of the workgroup slots, the launch, the first tile's latency (page, then K
+// and V) and the epilogue.
+// Five ragged chunks of up to 700 rows over a q8 cache, window 2048: 180 us for
+// 77.7 GFLOP; the 584 row tiles fill 512 slots once and then 72 of them again (and
+// are not split, as prefill_splits counts n_seq times the longest chunk: 880).
 #include <algorithm>
 
 #include "bq_internal.hpp"

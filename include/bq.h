@@ -521,8 +521,10 @@ int bq_kv_read(const bq_kv_cache* kv, const int32_t* seq, const int32_t* pos, in
  * kv_len, or at tokens that no row of the call sees, does not matter (it may
  * be NaN).  kv_len is clamped to max_len.
  *   bq_attn_decode: 1..8 rows per sequence (`rows`), rows s * rows ... of q
- *     and out; products carry fp32 precision (q and the softmax weights as
- *     sums of bf16 parts) unless q and out are both bf16.  The tokens of a
+ *     and out.  Unless q and out are both bf16 (one part each then), over a bf16
+ *     cache q and the softmax weights are three bf16 parts (fp32's 24 bits); over a
+ *     q8 cache q is two fp16 parts (2^-22 of the row's largest value) and a weight
+ *     times a value's scale two bf16 parts (2^-16 of each term).  The tokens of a
  *     sequence are split over workgroups and joined through `work`
  *     (bq_attn_workspace_bytes for the full split; NULL or less: a smaller
  *     split or none).  Calls that share a workspace must be ordered.  The
@@ -539,7 +541,8 @@ int bq_kv_read(const bq_kv_cache* kv, const int32_t* seq, const int32_t* pos, in
  *     with less, or NULL, a smaller split and conversion on the way), with
  *     values and weights in fp16 then; rows that see a value whose scale is not
  *     0 or 2^-18 <= scale < 2 take the codes as they are and weights times scales
- *     in two bf16 parts instead (any size, 2.5 times as long).
+ *     in two bf16 parts instead (any size, 2.5 times as long).  Tiles of more than
+ *     1 GiB are converted on the way whatever work holds.
  * scale > 0.  q_heads % kv_heads == 0 and q_heads / kv_heads <= 64, else BQ_UNSUPPORTED.
  * Row strides in elements, multiples of 8. */
 typedef struct bq_attn_args {
