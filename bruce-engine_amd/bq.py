@@ -45,7 +45,8 @@ EXPORTS = [
     "bq_gemm_b_fused_noalloc",
     "bq_noalloc_scratch_bytes", "bq_decode_enqueue", "bq_decode_graph_create", "bq_decode_graph_launch",
     "bq_decode_graph_destroy", "bq_kv_page_bytes", "bq_append", "bq_kv_read", "bq_attn_workspace_bytes",
-    "bq_attn_prefill_workspace_bytes", "bq_attn_decode", "bq_attn_prefill", "bq_attn_hook", "bq_sample_workspace_bytes", "bq_sample",
+    "bq_attn_prefill_workspace_bytes", "bq_attn_decode", "bq_attn_prefill", "bq_attn_shared_workspace_bytes",
+    "bq_attn_decode_shared", "bq_attn_hook", "bq_sample_workspace_bytes", "bq_sample",
 ]
 
 
@@ -123,10 +124,15 @@ class AttnArgs(ctypes.Structure):
                 ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_size_t)]
 
 
+class AttnPrefix(ctypes.Structure):
+    """bq_attn_prefix (include/bq.h): groups of sequences that share their first tokens."""
+    _fields_ = [("group0", ctypes.c_void_p), ("len", ctypes.c_void_p), ("n_groups", ctypes.c_int), ("max_len", ctypes.c_int)]
+
+
 class AttnBlock(ctypes.Structure):
     """bq_attn_block (include/bq.h): what the attention hook runs for one block of the step."""
     _fields_ = [("kv", ctypes.POINTER(KvCacheStruct)), ("append", ctypes.POINTER(AppendArgs)),
-                ("attn", ctypes.POINTER(AttnArgs)), ("prefill", ctypes.c_int)]
+                ("attn", ctypes.POINTER(AttnArgs)), ("prefill", ctypes.c_int), ("shared", ctypes.POINTER(AttnPrefix))]
 
 
 class AttnPlanStruct(ctypes.Structure):
@@ -207,6 +213,8 @@ def load(path=LIB_PATH):
         "bq_attn_prefill_workspace_bytes": (S, [I] * 8),
         "bq_attn_decode": (I, [P, P, P]),
         "bq_attn_prefill": (I, [P, P, P]),
+        "bq_attn_shared_workspace_bytes": (S, [I] * 8),
+        "bq_attn_decode_shared": (I, [P, P, P, P]),
         "bq_attn_hook": (None, [P, I, P]),
         "bq_sample_workspace_bytes": (S, [I, I]),
         "bq_sample": (I, [P, ctypes.c_int64, I, I, P, P, P, P, P, P, P, S, P]),
@@ -811,15 +819,55 @@ class Attention:
         return _check(f(kv, self._ref, _raw_stream(d)) if _current() == d else _on(d, f, kv, self._ref), what)
 
 
+class SharedAttention:
+    """bq_attn_decode_shared over fixed buffers: q, out and kv_len as Attention's for decode() (rows = n_rows /
+    n_seq); group0 int32 [n_groups + 1], prefix_len int32 [n_groups], max_prefix the most tokens that a group
+    shares.  work: a workspace tensor of the caller's, or "auto"."""
+
+    def __init__(self, kv, q, out, kv_len, group0, prefix_len, scale=None, window=0, sinks=0, max_len=None, max_prefix=None,
+                 work="auto"):
+        import torch
+        D, n_seq = kv.head_dim, kv.table.shape[0]
+        n_rows, width = q.shape
+        if width % D or out.shape != q.shape:
+            raise ValueError("q and out: rows of whole heads, alike")
+        n_groups = prefix_len.shape[0]
+        _expect(kv_len, torch.int32, (n_seq,), "kv_len")
+        _expect(prefix_len, torch.int32, (n_groups,), "prefix_len")
+        _expect(group0, torch.int32, (n_groups + 1,), "group0")
+        _one_device(kv.pages.device, q=q, out=out, kv_len=kv_len, group0=group0, prefix_len=prefix_len)
+        room = kv.table.shape[1] * kv.struct.page_tokens
+        max_len = room if max_len is None else max_len
+        max_prefix = max_len if max_prefix is None else max_prefix
+        L, rows = load(), n_rows // n_seq
+        if isinstance(work, str):
+            n = L.bq_attn_shared_workspace_bytes(n_seq, rows, width // D, kv.kv_heads, D, min(max_len, room), n_groups, max_prefix)
+            work = torch.empty(n // 4, dtype=torch.float32, device=q.device)
+        _work_of(work, q.device)
+        self.kv, self.work, self._keep = kv, work, (q, out, kv_len, group0, prefix_len)
+        self.struct = AttnArgs(_ptr(q), _ptr(out), _type_of(q, "q"), _type_of(out, "out"), _rows_ld(q, width, "q"),
+                               _rows_ld(out, width, "out"), width // D, n_rows, rows, None, _ptr(kv_len), max_len,
+                               D ** -0.5 if scale is None else scale, window, sinks, _ptr(work),
+                               0 if work is None else work.numel() * work.element_size())
+        self.prefix = AttnPrefix(_ptr(group0), _ptr(prefix_len), n_groups, max_prefix)
+        self._args, self._run = (ctypes.byref(self.struct), ctypes.byref(self.prefix)), L.bq_attn_decode_shared
+
+    def run(self):
+        kv, d = self.kv.ref, self.kv.device
+        return _check(self._run(kv, *self._args, _raw_stream(d)) if _current() == d else _on(d, self._run, kv, *self._args),
+                      "bq_attn_decode_shared")
+
+
 class AttentionPlan:
-    """The decode step's attention hook over its blocks: blocks[i] None, or (Append, Attention) of block i.
+    """The decode step's attention hook over its blocks: blocks[i] None, or (Append, Attention or SharedAttention) of block i.
     install(step) sets step.attention and step.user; check() raises what the hook met."""
 
     def __init__(self, blocks, prefill=False):
         self._keep = blocks
         P = ctypes.pointer
         self._blocks = (AttnBlock * max(1, len(blocks)))(*[
-            AttnBlock() if b is None else AttnBlock(P(b[1].kv.struct), P(b[0].struct), P(b[1].struct), int(prefill))
+            AttnBlock() if b is None else AttnBlock(P(b[1].kv.struct), P(b[0].struct), P(b[1].struct), int(prefill),
+                                                    P(b[1].prefix) if isinstance(b[1], SharedAttention) else None)
             for b in blocks])
         self.struct = AttnPlanStruct(len(blocks), self._blocks, BQ_OK)
 

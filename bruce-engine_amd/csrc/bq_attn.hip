@@ -32,17 +32,12 @@
 // one of 777 8.4 us, two launches and a chain of loads (length, page, K and V).
 #include <algorithm>
 
+#include "bq_attn_dev.hpp"
 #include "bq_internal.hpp"
-#include "bq_kv.hpp"
 
 namespace bq {
 
 namespace {
-constexpr int kWaves = 4;          // per workgroup
-constexpr int kRound = 512;        // 32-token steps whose pages are staged at once
-constexpr float kNone = -3.402823466e38f;  // the running maximum before any token
-constexpr float kLazy = 8.f;
-
 struct DecodeP {
     KvView kv;
     const void* q;
@@ -55,13 +50,10 @@ struct DecodeP {
     float scale;  // scale * log2(e)
 };
 
-// 32-token steps that a tile's rows at positions pfirst..plast see: the
-// sinks' [0, ns), then [lo_step, lo_step + n - ns)
-struct Steps {
-    int lo, lo_step, ns, n;
-};
+// the steps that a tile's rows at positions pfirst..plast see
 BQ_DEV Steps steps_of(const DecodeP& p, int pfirst, int plast) {
     Steps s;
+    s.b = 0;
     s.lo = p.window ? max(0, pfirst - p.window + 1) : 0;
     s.lo_step = s.lo >> 5;
     s.ns = p.window ? min(s.lo_step, (p.sinks + 31) >> 5) : 0;
@@ -80,37 +72,6 @@ BQ_DEV void store4(const DecodeP& p, size_t at, f32x4 a) {
 }
 BQ_DEV f32x4 over(f32x4 a, float l) { return l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a * (1.f / l); }
 
-// four int8 codes -> bf16 (exact)
-BQ_DEV u32x2 codes_bf16(uint32_t w) {
-    const float a = (float)(int8_t)w, b = (float)(int8_t)(w >> 8), c = (float)(int8_t)(w >> 16), d = (float)((int32_t)w >> 24);
-    auto hi2 = [](float x, float y) {  // the high halves: small integers are exact in bf16
-        return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
-    };
-    return u32x2{hi2(a, b), hi2(c, d)};
-}
-BQ_DEV bf16x8 codes8(uint32_t lo, uint32_t hi) {
-    const u32x2 a = codes_bf16(lo), b = codes_bf16(hi);
-    return __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
-}
-BQ_DEV f16x8 codes8h(uint32_t lo, uint32_t hi) {
-    f16x2 v[4];
-    codes_f16(lo, v[0], v[1]);
-    codes_f16(hi, v[2], v[3]);
-    return f16x8{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
-}
-BQ_DEV f32x4 mfma16h(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-BQ_DEV f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-
-// largest and sum over the four lane groups that share lane & 15
-BQ_DEV float groups_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
-}
-BQ_DEV float groups_sum(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
-}
-
 // NQ parts of q, NP of a softmax weight
 template <int D, int KV, int NQ, int NP>
 __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p) {
@@ -127,243 +88,14 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_decode(DecodeP p
     const int M = p.rows * p.G, first = qt * 16, last = min(M, first + 16) - 1;
     const int pfirst = len - p.rows + first / p.G, plast = len - p.rows + last / p.G;
     const int r = min(first + c, last), i = r / p.G, pos = len - p.rows + i;
-    constexpr bool Q8 = KV == kKvQ8;
-    u32x4 q[NQ][KS];
-    float scale = p.scale;
-    {
-        const size_t at = (size_t)(seq * p.rows + i) * p.ldq + (size_t)(h * p.G + r % p.G) * D + 8 * g;
-        if constexpr (!Q8 && NQ == 1) {
-#pragma unroll
-            for (int k = 0; k < KS; ++k) q[0][k] = *(const u32x4*)((const uint16_t*)p.q + at + 32 * k);
-        } else {
-            float x[KS][8], amax = 0.f;
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                if (p.q_bf16) {
-                    const u32x4 b = *(const u32x4*)((const uint16_t*)p.q + at + 32 * k);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[k][e] = as_float(e & 1 ? b[e >> 1] & 0xFFFF0000u : b[e >> 1] << 16);
-                } else {
-                    const f32x4 a = *(const f32x4*)((const float*)p.q + at + 32 * k), b = *(const f32x4*)((const float*)p.q + at + 32 * k + 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[k][e] = a[e], x[k][4 + e] = b[e];
-                }
-            }
-            if constexpr (Q8) {  // the row's largest value to [16, 32), but for rows of 2^-122 and less
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[k][e]));
-                const int ex = max(-126, min(126, ilogb2(groups_max(amax)) - 4));
-                const float down = pow2(-ex);
-                scale *= pow2(ex);
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[k][e] *= down;
-            }
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    if constexpr (Q8) {
-                        f16x8 y;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            y[e] = (_Float16)x[k][e];
-                            x[k][e] -= (float)y[e];
-                        }
-                        q[n][k] = __builtin_bit_cast(u32x4, y);
-                    } else {
-                        bf16x8 y;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            y[e] = (__bf16)x[k][e];
-                            x[k][e] -= (float)y[e];
-                        }
-                        q[n][k] = __builtin_bit_cast(u32x4, y);
-                    }
-                }
-        }
-    }
-
+    const size_t qat = (size_t)(seq * p.rows + i) * p.ldq + (size_t)(h * p.G + r % p.G) * D;
     const Steps st = steps_of(p, pfirst, plast);
     const int end = plast + 1, lo = st.lo, n = st.n;
     const int per = (n + p.nsplit - 1) / p.nsplit;
     const int v0 = min(n, (int)blockIdx.x * per), v1 = min(n, v0 + per);
-
-    f32x4 o[DT];
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = kNone, l = 0.f;
-
-    const bool half_pages = kv.plog == 4;  // a step spans two 16-token pages
-    const int P = kv.P;
-    for (int vr = v0; vr < v1; vr += kRound) {
-        const int cnt = min(kRound, v1 - vr);
-        __syncthreads();
-        for (int e = tid; e < cnt << (half_pages ? 1 : 0); e += 256) {
-            const int v = vr + (half_pages ? e >> 1 : e), ts = v < st.ns ? v : v - st.ns + st.lo_step;
-            s_page[e] = kv_page(kv, seq, ts * 32 + (half_pages ? (e & 1) * 16 : 0));
-        }
-        __syncthreads();
-        for (int w = wave; w < cnt; w += kWaves) {
-            const int v = vr + w, ts = v < st.ns ? v : v - st.ns + st.lo_step, t0 = ts * 32;
-            // keys: lane row c holds token 8 (c / 4) + c % 4 (+ 4 in the second tile); values: tokens 8g..
-            const int gk = c >> 2;
-            const int pk = half_pages ? s_page[2 * w + (gk >> 1)] : s_page[w], pv = half_pages ? s_page[2 * w + (g >> 1)] : s_page[w];
-            const int ib = t0 & (P - 1);  // 0 with 16-token pages
-            const int tk = ib + 8 * (half_pages ? gk & 1 : gk) + (c & 3), tv = ib + 8 * (half_pages ? g & 1 : g);
-            const char* bk = kv.pages + (size_t)max(pk, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
-            const char* bv = kv.pages + (size_t)max(pv, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
-            // every load of the step first: the values' arrive during the scores
-            u32x4 kf[2][Q8 ? KS / 2 : KS], vf[Q8 ? DT / 2 : DT], ksc[Q8 ? KS : 1], vsc[Q8 ? KS : 1];
-            if constexpr (!Q8) {
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) kf[t][k] = *(const u32x4*)(bk + kv_k_unit(P, 4 * k + g, tk + 4 * t));
-#pragma unroll
-                for (int d = 0; d < DT; ++d) vf[d] = *(const u32x4*)(bv + kv_v_unit(P, D, tv >> 3, 16 * d + c));
-            } else {
-#pragma unroll
-                for (int k = 0; k < KS / 2; ++k)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) kf[t][k] = *(const u32x4*)(bk + kv_kq_unit(P, k, g, tk + 4 * t));
-#pragma unroll
-                for (int k = 0; k < KS; ++k) ksc[k] = *(const u32x4*)(bv + kv_ks_off(P, D, k, tv));
-#pragma unroll
-                for (int d = 0; d < DT / 2; ++d) vf[d] = *(const u32x4*)(bv + kv_vq_unit(P, D, tv >> 3, d, c));
-#pragma unroll
-                for (int d = 0; d < DT / 2; ++d) vsc[d] = *(const u32x4*)(bv + kv_vs_off(P, D, d, tv));
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    if constexpr (!Q8) {
-                        const bf16x8 kb = __builtin_bit_cast(bf16x8, kf[y][k]);
-#pragma unroll
-                        for (int a = NQ - 1; a >= 0; --a) s[y] = mfma16(kb, __builtin_bit_cast(bf16x8, q[a][k]), s[y]);
-                    } else {
-                        const f16x8 kb = codes8h(kf[y][k / 2][2 * (k & 1)], kf[y][k / 2][2 * (k & 1) + 1]);
-                        const uint32_t a0 = ksc[k][2 * y], a1 = ksc[k][2 * y + 1];
-                        const f32x4 sc = {as_float(a0 << 16), as_float(a0 & 0xFFFF0000u), as_float(a1 << 16), as_float(a1 & 0xFFFF0000u)};
-                        f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int a = NQ - 1; a >= 0; --a) x = mfma16h(kb, __builtin_bit_cast(f16x8, q[a][k]), x);
-                        s[y] += x * sc;
-                    }
-                }
-            // scores of tokens t0 + 8g + 4y + e for the lane's query rows
-            const bool edge = t0 + 31 > pfirst || (p.window && t0 <= plast - p.window && t0 + 32 > p.sinks) || __any(pv < 0);
-            uint32_t seen = 0xFF;  // tokens any row of the tiles sees (their values are read)
-            if (edge) {
-                seen = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int tok = t0 + 8 * g + e;
-                    const bool any = pv >= 0 && tok < end && (tok >= lo || tok < p.sinks);
-                    seen |= any ? 1u << e : 0u;
-                }
-                // what no row sees may hold anything: its products must not
-                if constexpr (!Q8) {
-                    u32x4 mask;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        mask[e] = (seen >> (2 * e) & 1 ? 0xFFFFu : 0u) | (seen >> (2 * e + 1) & 1 ? 0xFFFF0000u : 0u);
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) vf[d] &= mask;
-                }
-            }
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * scale;
-            if (edge) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int tok = t0 + 8 * g + e;
-                    const bool me = pv >= 0 && tok <= pos && (!p.window || tok > pos - p.window || tok < p.sinks);
-                    x[e] = me ? x[e] : -INFINITY;
-                }
-            }
-            float mx = x[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-            if (__any(mx > m + kLazy)) {
-                const float mn = fmaxf(m, groups_max(mx));
-                const float al = __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= al;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] *= al;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(x[e] - m);
-                l += x[e];
-            }
-            auto parts = [&](const float (&y)[8], bf16x8 (&pp)[NP]) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float z = y[e];
-#pragma unroll
-                    for (int a = 0; a < NP; ++a) {
-                        const __bf16 w = (__bf16)z;
-                        pp[a][e] = w;
-                        z -= (float)w;
-                    }
-                }
-            };
-            bf16x8 pp[NP];
-            if constexpr (!Q8) {
-                parts(x, pp);
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int a = NP - 1; a >= 0; --a) o[d] = mfma16(__builtin_bit_cast(bf16x8, vf[d]), pp[a], o[d]);
-            } else {
-#pragma unroll
-                for (int d = 0; d < DT / 2; ++d) {
-                    float y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float vs = as_float(e & 1 ? vsc[d][e >> 1] & 0xFFFF0000u : vsc[d][e >> 1] << 16);
-                        y[e] = x[e] * (edge && !(seen >> e & 1) ? 0.f : vs);  // codes are finite, an unseen scale may not be
-                    }
-                    parts(y, pp);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int a = NP - 1; a >= 0; --a)
-                            o[2 * d + u] = mfma16(codes8(vf[d][2 * u], vf[d][2 * u + 1]), pp[a], o[2 * d + u]);
-                }
-            }
-        }
-    }
-
-    // join the waves
-    l = groups_sum(l);
-    if (g == 0) {
-        s_m[wave][c] = m;
-        s_l[wave][c] = l;
-    }
-    __syncthreads();
-    float mt = s_m[0][c], lt = 0.f;
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) mt = fmaxf(mt, s_m[w][c]);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) lt += s_l[w][c] * __builtin_amdgcn_exp2f(s_m[w][c] - mt);
-    const float f = __builtin_amdgcn_exp2f(m - mt);
-#pragma unroll
-    for (int d = 0; d < DT; ++d) *(f32x4*)&s_o[wave][c][16 * d + 4 * g] = o[d] * f;
-    if (wave == 0 && g == 0) {
-        s_mt[c] = mt;
-        s_lt[c] = lt;
-    }
-    __syncthreads();
+    constexpr bool CUT = false;
+    constexpr int from = 0, upto = 0;
+#include "bq_attn_rows.inc"
     const size_t piece = ((size_t)seq * p.tiles + blockIdx.y) * p.nsplit + blockIdx.x;
     for (int e = tid; e < 16 * (D / 4); e += 256) {
         const int row = e / (D / 4), d = e % (D / 4) * 4, r = first + row;

@@ -154,6 +154,17 @@ size_t prefill_stage_bytes(int type, int n_seq, int rows, int q_heads, int kv_he
 hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a, size_t stage_bytes, int nsplit, int cus,
                                hipStream_t st);
 
+// attention of groups that share a prefix: row tiles (per head) and pieces of the
+// prefixes and of a sequence's own tokens
+struct SharedPlan {
+    int64_t ptiles;
+    int psplit, ttiles, tsplit;
+};
+SharedPlan shared_plan(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int max_len, int n_groups, int max_prefix, int window,
+                       int sinks, int cus);
+size_t shared_part_floats(const SharedPlan& s, int n_rows, int q_heads, int D);
+hipError_t launch_attn_shared(const KvView& kv, int type, const bq_attn_args& a, const bq_attn_prefix& x, const SharedPlan& s, hipStream_t st);
+
 size_t sample_work_bytes(int rows, int vocab);
 hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, const float* temp, const int32_t* top_k,
                          const float* top_p, const float* min_p, const float* u, int32_t* out, void* work, hipStream_t st);

@@ -156,6 +156,39 @@ int bq_attn_prefill(const bq_kv_cache* c, const bq_attn_args* args, bq_stream_t 
     return from_hip(launch_attn_prefill(kv, type, a, stage, n, device_cus(), (hipStream_t)st));
 }
 
+size_t bq_attn_shared_workspace_bytes(int n_seq, int rows, int q_heads, int kv_heads, int head_dim, int max_len, int n_groups, int max_prefix) {
+    if (n_seq <= 0 || n_seq > 65535 || rows < 1 || rows > BQ_MAX_ROWS || kv_heads <= 0 || q_heads % kv_heads != 0 || q_heads <= 0 ||
+        head_dim <= 0 || max_len < 0 || n_groups < 1 || max_prefix < 0 || device_ready() != BQ_OK)
+        return 0;
+    // of either type and any window: the pieces are the most without one, of a q8 cache's own tokens
+    max_prefix = std::min(max_prefix, max_len);
+    const SharedPlan s = shared_plan(kKvQ8, n_seq, rows, q_heads, kv_heads, head_dim, max_len, n_groups, max_prefix, 0, 0, device_cus());
+    return shared_part_floats(s, n_seq * rows, q_heads, head_dim) * sizeof(float);
+}
+
+int bq_attn_decode_shared(const bq_kv_cache* c, const bq_attn_args* args, const bq_attn_prefix* prefix, bq_stream_t st) {
+    if (int r = device_ready()) return r;
+    KvView kv;
+    int type;
+    if (int r = view_of(c, kv, type)) return r;
+    if (!args || !prefix) return BQ_EINVAL;
+    bq_attn_args a = *args;
+    bq_attn_prefix x = *prefix;
+    if (int r = attn_check(kv, a)) return r;
+    if (a.row0 || (int64_t)kv.n_seq * a.rows != a.n_rows) return BQ_EINVAL;
+    if (!x.group0 || !x.len || x.n_groups < 1 || x.max_len < 0) return BQ_EINVAL;
+    if (a.rows > BQ_MAX_ROWS) return BQ_UNSUPPORTED;
+    x.max_len = std::min(x.max_len, a.max_len);
+    const SharedPlan s = shared_plan(type, kv.n_seq, a.rows, a.q_heads, kv.heads, kv.D, a.max_len, x.n_groups, x.max_len, a.window, a.sinks,
+                                     device_cus());
+    // one grid dimension holds all workgroups, another all rows
+    if (s.ptiles * kv.heads * s.psplit + (int64_t)kv.n_seq * s.ttiles * kv.heads * s.tsplit > INT32_MAX ||
+        (int64_t)a.n_rows * a.q_heads > INT32_MAX)
+        return BQ_UNSUPPORTED;
+    if (!a.work || !al16(a.work) || a.work_bytes < shared_part_floats(s, a.n_rows, a.q_heads, kv.D) * sizeof(float)) return BQ_EINVAL;
+    return from_hip(launch_attn_shared(kv, type, a, x, s, (hipStream_t)st));
+}
+
 void bq_attn_hook(void* user, int block, bq_stream_t st) {
     bq_attn_plan* p = (bq_attn_plan*)user;
     if (!p) return;
@@ -165,7 +198,10 @@ void bq_attn_hook(void* user, int block, bq_stream_t st) {
     } else if (p->blocks[block].kv) {
         const bq_attn_block& b = p->blocks[block];
         if (b.append) r = bq_append(b.kv, b.append, st);
-        if (r == BQ_OK && b.attn) r = b.prefill ? bq_attn_prefill(b.kv, b.attn, st) : bq_attn_decode(b.kv, b.attn, st);
+        if (r == BQ_OK && b.attn && b.shared)
+            r = b.prefill ? BQ_EINVAL : bq_attn_decode_shared(b.kv, b.attn, b.shared, st);
+        else if (r == BQ_OK && b.attn)
+            r = b.prefill ? bq_attn_prefill(b.kv, b.attn, st) : bq_attn_decode(b.kv, b.attn, st);
     }
     if (p->status == BQ_OK) p->status = r;
 }

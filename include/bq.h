@@ -566,17 +566,43 @@ size_t bq_attn_prefill_workspace_bytes(int type, int n_seq, int rows, int n_rows
 int bq_attn_decode(const bq_kv_cache* kv, const bq_attn_args* a, bq_stream_t st);
 int bq_attn_prefill(const bq_kv_cache* kv, const bq_attn_args* a, bq_stream_t st);
 
+/* bq_attn_decode for sequences in groups that share their first tokens (a system
+ * prompt, a document, samples of one prompt): group g is the sequences group0[g]
+ * .. group0[g + 1] - 1 (device, [n_groups + 1], non-decreasing, within n_seq), and
+ * its first len[g] tokens (device, [n_groups], clamped to max_len) are read
+ * through the table row of its first sequence, once for the rows of all; tokens
+ * from len[g] on through each sequence's own row, of which the entries (or the part
+ * of a page) before are not read.  A sequence in no group has no shared tokens.
+ * Everything else is bq_attn_decode's: kv_len counts the shared tokens, rows see
+ * what their positions, window and sinks let them (a sequence may be shorter than
+ * the prefix), precision by the types of q, out and the cache.  work: at least
+ * bq_attn_shared_workspace_bytes (else BQ_EINVAL), max_prefix being prefix->max_len;
+ * not shared by calls that overlap.  How the work is cut follows n_seq, rows,
+ * n_groups, max_len and prefix->max_len, which a captured graph fixes; group0, len
+ * and kv_len may change between replays.  Equal calls give equal bits. */
+typedef struct bq_attn_prefix {
+    const int32_t* group0;
+    const int32_t* len;
+    int n_groups;
+    int max_len;                  /* no len is larger */
+} bq_attn_prefix;
+size_t bq_attn_shared_workspace_bytes(int n_seq, int rows, int q_heads, int kv_heads, int head_dim, int max_len, int n_groups,
+                                      int max_prefix);
+int bq_attn_decode_shared(const bq_kv_cache* kv, const bq_attn_args* a, const bq_attn_prefix* prefix, bq_stream_t st);
+
 /* The decode step's attention hook over a list of blocks: set
  * bq_decode_step.attention = bq_attn_hook and user = a bq_attn_plan whose
  * blocks[i] belongs to the step's block i (kv NULL: no attention there).  The
  * hook appends the block's rows and attends, by bq_attn_prefill where
- * `prefill` is set, else bq_attn_decode.  The hook cannot fail the step, so
+ * `prefill` is set, by bq_attn_decode_shared where `shared` is (both: BQ_EINVAL),
+ * else bq_attn_decode.  The hook cannot fail the step, so
  * the first code that is not BQ_OK stays in `status` (the caller clears it). */
 typedef struct bq_attn_block {
     const bq_kv_cache* kv;
     const bq_append_args* append;
     const bq_attn_args* attn;
     int prefill;
+    const bq_attn_prefix* shared;
 } bq_attn_block;
 typedef struct bq_attn_plan {
     int n_blocks;
