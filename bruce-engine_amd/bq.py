@@ -46,7 +46,7 @@ EXPORTS = [
     "bq_noalloc_scratch_bytes", "bq_decode_enqueue", "bq_decode_graph_create", "bq_decode_graph_launch",
     "bq_decode_graph_destroy", "bq_kv_page_bytes", "bq_append", "bq_kv_read", "bq_attn_workspace_bytes",
     "bq_attn_prefill_workspace_bytes", "bq_attn_decode", "bq_attn_prefill", "bq_attn_shared_workspace_bytes",
-    "bq_attn_decode_shared", "bq_attn_hook", "bq_sample_workspace_bytes", "bq_sample",
+    "bq_attn_decode_shared", "bq_lora_workspace_bytes", "bq_lora", "bq_lora_hook", "bq_attn_hook", "bq_sample_workspace_bytes", "bq_sample",
 ]
 
 
@@ -71,6 +71,8 @@ class GgufTensor(ctypes.Structure):
 
 BLOCK_ATTN, BLOCK_FFN = 0, 1
 ATTN_HOOK = ctypes.CFUNCTYPE(None, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p)
+PROJ_QKV, PROJ_O, PROJ_GATE_UP, PROJ_DOWN = 0, 1, 2, 3
+PROJ_HOOK = ctypes.CFUNCTYPE(None, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p)
 
 
 class DecodeBlock(ctypes.Structure):
@@ -95,7 +97,7 @@ class DecodeStep(ctypes.Structure):
                 ("head_q8s", ctypes.c_void_p), ("head_rs", ctypes.c_void_p), ("head", ctypes.POINTER(Weight)),
                 ("vocab", ctypes.c_int), ("logits", ctypes.c_void_p), ("rows", ctypes.c_int),
                 ("x_alt", ctypes.c_void_p), ("xdh", ctypes.c_void_p), ("work", ctypes.c_void_p),
-                ("work_bytes", ctypes.c_size_t)]
+                ("work_bytes", ctypes.c_size_t), ("projected", PROJ_HOOK), ("projected_user", ctypes.c_void_p)]
 
 
 class KvCacheStruct(ctypes.Structure):
@@ -138,6 +140,30 @@ class AttnBlock(ctypes.Structure):
 class AttnPlanStruct(ctypes.Structure):
     """bq_attn_plan (include/bq.h)."""
     _fields_ = [("n_blocks", ctypes.c_int), ("blocks", ctypes.POINTER(AttnBlock)), ("status", ctypes.c_int)]
+
+
+class LoraPart(ctypes.Structure):
+    """bq_lora_part (include/bq.h): one matrix' adapters."""
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("base", ctypes.c_void_p), ("y", ctypes.c_void_p),
+                ("ldbase", ctypes.c_int64), ("ldy", ctypes.c_int64), ("N", ctypes.c_int)]
+
+
+class LoraArgs(ctypes.Structure):
+    """bq_lora_args (include/bq.h)."""
+    _fields_ = [("x", ctypes.c_void_p), ("xd", ctypes.c_void_p), ("x_type", ctypes.c_int), ("ldx", ctypes.c_int64),
+                ("rows", ctypes.c_int), ("K", ctypes.c_int), ("rank", ctypes.c_int), ("n_adapters", ctypes.c_int),
+                ("n_parts", ctypes.c_int), ("parts", LoraPart * 4), ("adapter", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_size_t)]
+
+
+class LoraBlock(ctypes.Structure):
+    """bq_lora_block (include/bq.h): the adapters of one block's projections."""
+    _fields_ = [("proj", ctypes.POINTER(LoraArgs) * 4)]
+
+
+class LoraPlanStruct(ctypes.Structure):
+    """bq_lora_plan (include/bq.h)."""
+    _fields_ = [("n_blocks", ctypes.c_int), ("blocks", ctypes.POINTER(LoraBlock)), ("status", ctypes.c_int)]
 
 
 _lib = None
@@ -215,6 +241,9 @@ def load(path=LIB_PATH):
         "bq_attn_prefill": (I, [P, P, P]),
         "bq_attn_shared_workspace_bytes": (S, [I] * 8),
         "bq_attn_decode_shared": (I, [P, P, P, P]),
+        "bq_lora_workspace_bytes": (S, [I, I, I]),
+        "bq_lora": (I, [P, P]),
+        "bq_lora_hook": (None, [P, I, I, P]),
         "bq_attn_hook": (None, [P, I, P]),
         "bq_sample_workspace_bytes": (S, [I, I]),
         "bq_sample": (I, [P, ctypes.c_int64, I, I, P, P, P, P, P, P, P, S, P]),
@@ -880,6 +909,78 @@ class AttentionPlan:
     def check(self):
         code, self.struct.status = self.struct.status, BQ_OK
         return _check(code, "bq_attn_hook")
+
+
+class Lora:
+    """bq_lora over fixed buffers: x fp32 or bf16 [rows, K] (rows may be strided) or the q8 rows (xq int8 [rows, K], xd
+    fp32 [rows, K / 32]), adapter int32 [rows], parts: up to four (a bf16 [n_adapters, rank, K], b bf16 [n_adapters, N,
+    rank], y fp32 [rows, N], base fp32 [rows, N] or None; without a base the part adds to y itself), scale fp32
+    [n_adapters] or None.  work: a workspace tensor of the caller's, or None for one of the object's own."""
+
+    def __init__(self, x, adapter, parts, scale=None, work=None):
+        import torch
+        xd = None
+        if isinstance(x, (tuple, list)):
+            x, xd = x[:2]
+        rows, K = x.shape
+        n, rank = parts[0][0].shape[:2]
+        if not 1 <= len(parts) <= 4:
+            raise ValueError("parts: one to four")
+        if xd is not None:
+            _expect(x, torch.int8, (rows, K), "xq")
+            _expect(xd, torch.float32, (rows, K // 32), "xd")
+        kind = TYPE_Q8_0 if xd is not None else _type_of(x, "x")
+        _expect(adapter, torch.int32, (rows,), "adapter")
+        _expect(scale, torch.float32, (n,), "scale")
+        _one_device(x.device, xd=xd, adapter=adapter, scale=scale)
+        L = load()
+        if work is None:
+            work = torch.empty(int(L.bq_lora_workspace_bytes(rows, rank, len(parts))), dtype=torch.uint8, device=x.device)
+        _work_of(work, x.device)
+        s = self.struct = LoraArgs(_ptr(x), _ptr(xd), kind, _rows_ld(x, K, "x"), rows, K, rank, n, len(parts))
+        for i, part in enumerate(parts):
+            a, b, y = part[:3]
+            base = part[3] if len(part) > 3 else y
+            N = y.shape[1]
+            _expect(a, torch.bfloat16, (n, rank, K), "a")
+            _expect(b, torch.bfloat16, (n, N, rank), "b")
+            for t, what in ((y, "y"), (base, "base")):
+                if t is not None and (t.dtype != torch.float32 or t.shape[0] != rows):
+                    raise ValueError(f"{what}: fp32 rows, as many as x has")
+            _one_device(x.device, a=a, b=b, y=y, base=base)
+            s.parts[i] = LoraPart(_ptr(a), _ptr(b), _ptr(base), _ptr(y), 0 if base is None else _rows_ld(base, N, "base"),
+                                  _rows_ld(y, N, "y"), N)
+        s.adapter, s.scale, s.work, s.work_bytes = _ptr(adapter), _ptr(scale), _ptr(work), work.numel() * work.element_size()
+        self.work, self._keep = work, (x, xd, adapter, parts, scale)
+        self._ref, self._run, self._device = ctypes.byref(s), L.bq_lora, x.device.index
+        _bind_device()
+
+    def run(self):
+        d = self._device
+        return _check(self._run(self._ref, _raw_stream(d)) if _current() == d else _on(d, self._run, self._ref), "bq_lora")
+
+
+class LoraPlan:
+    """The decode step's projection hook over its blocks: blocks[i] a dict of PROJ_... to the Lora beside that projection
+    (or empty, or None).  install(step) sets step.projected and its user; check() raises what the hook met."""
+
+    def __init__(self, blocks):
+        self._keep = blocks
+        self._blocks = (LoraBlock * max(1, len(blocks)))()
+        for i, b in enumerate(blocks):
+            for proj, lora in (b or {}).items():
+                self._blocks[i].proj[proj] = ctypes.pointer(lora.struct)
+        self.struct = LoraPlanStruct(len(blocks), self._blocks, BQ_OK)
+
+    def install(self, step):
+        step.projected = ctypes.cast(load().bq_lora_hook, PROJ_HOOK)
+        step.projected_user = ctypes.addressof(self.struct)
+        step._lora_plan = self
+        return step
+
+    def check(self):
+        code, self.struct.status = self.struct.status, BQ_OK
+        return _check(code, "bq_lora_hook")
 
 
 class Sampler:

@@ -107,6 +107,11 @@ int parts_rows_of(float* const* ys, const bq_weight* const* ws, int n, int rows,
     return BQ_OK;
 }
 
+// the caller's part of a projection (adapters), which has just been enqueued
+void projected(const bq_decode_step* s, int block, int proj, bq_stream_t st) {
+    if (s->projected) s->projected(s->projected_user, block, proj, st);
+}
+
 // one attention block: bruce.cu:7915-7993 (QKV, attention, gate norm, O);
 // rows 2..8: :7636-7757
 int attn_block(const bq_decode_step* s, const bq_decode_block& b, int bi, int rows, Resid& rs, bq_stream_t st) {
@@ -192,6 +197,7 @@ int attn_block(const bq_decode_step* s, const bq_decode_block& b, int bi, int ro
     for (int p = 0; p < b.n_qkv; ++p)
         if (b.qkv[p].ggml_type != BQ_TYPE_Q5_K)
             if (int e = gemv_rows_of(b.qkv_out[p], &b.qkv[p], rows, s, st)) return e;
+    projected(s, bi, BQ_PROJ_QKV, st);
     if (s->attention) s->attention(s->user, bi, st);
     // gate norm -> q8, then O (k_gate_norm :7975-7978, launch_gemv :7982;
     // rows: k_gate_norm_vec4 :7740, launch_gemm_b :7757); folded: the gate
@@ -213,12 +219,14 @@ int attn_block(const bq_decode_step* s, const bq_decode_block& b, int bi, int ro
     if (int e = bq_gate_norm_q8(nullptr, b.attn_out, b.attn_gate, b.sgate, rows, b.n_attn, s->xq, s->xd, s->xsum,
                                 st))
         return e;
-    return gemv_rows_of(s->proj, b.o, rows, s, st);
+    if (int e = gemv_rows_of(s->proj, b.o, rows, s, st)) return e;
+    projected(s, bi, BQ_PROJ_O, st);
+    return BQ_OK;
 }
 
 // one FFN block: bruce.cu:7994-8012 (gate+up, silu*mul norm, down); rows
 // 2..8: :7759-7800
-int ffn_block(const bq_decode_step* s, const bq_decode_block& b, int rows, Resid& rs, bq_stream_t st) {
+int ffn_block(const bq_decode_step* s, const bq_decode_block& b, int bi, int rows, Resid& rs, bq_stream_t st) {
     if (!b.gate || !b.up || !b.down || !b.s_gate || !b.s_up || !s->ffn_g || b.n_ff <= 0 || (b.n_ff % 32) != 0)
         return BQ_EINVAL;
     if (int e = flush(s, rs, st)) return e;
@@ -234,10 +242,13 @@ int ffn_block(const bq_decode_step* s, const bq_decode_block& b, int rows, Resid
     float* y2[2] = {s->ffn_g, s->ffn_u};
     const bq_weight* p2[2] = {b.gate, b.up};
     if (int r = parts_rows_of(y2, p2, 2, rows, s, st)) return r;
+    projected(s, bi, BQ_PROJ_GATE_UP, st);
     if (int e = bq_silu_mul_norm_q8(nullptr, s->ffn_g, s->ffn_u, b.s_gate, b.s_up, rows, b.n_ff, s->xq, s->xd,
                                     s->xsum, st))
         return e;
-    return gemv_rows_of(s->proj, b.down, rows, s, st);
+    if (int e = gemv_rows_of(s->proj, b.down, rows, s, st)) return e;
+    projected(s, bi, BQ_PROJ_DOWN, st);
+    return BQ_OK;
 }
 
 }  // namespace
@@ -254,6 +265,8 @@ int bq_decode_enqueue(const bq_decode_step* s, bq_stream_t st) {
     const int n = s->n_embd, rows = rows_of(s);
     // the folded producers are one-row GEMV epilogues / prologues
     if (s->fold && rows > 1) return BQ_UNSUPPORTED;
+    // and leave no place between a projection and what reads it
+    if (s->fold && s->projected) return BQ_UNSUPPORTED;
     Resid rs;
     rs.cur = s->x;
     for (int i = 0; i < s->n_blocks; ++i) {
@@ -268,7 +281,7 @@ int bq_decode_enqueue(const bq_decode_step* s, bq_stream_t st) {
                 return e;
             }
         }
-        const int r = b.kind == BQ_BLOCK_FFN ? ffn_block(s, b, rows, rs, st) : b.kind == BQ_BLOCK_ATTN
+        const int r = b.kind == BQ_BLOCK_FFN ? ffn_block(s, b, i, rows, rs, st) : b.kind == BQ_BLOCK_ATTN
                                                                                  ? attn_block(s, b, i, rows, rs, st)
                                                                                  : BQ_EINVAL;
         if (r) return r;

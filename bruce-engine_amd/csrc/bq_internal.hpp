@@ -165,6 +165,9 @@ SharedPlan shared_plan(int type, int n_seq, int rows, int q_heads, int kv_heads,
 size_t shared_part_floats(const SharedPlan& s, int n_rows, int q_heads, int D);
 hipError_t launch_attn_shared(const KvView& kv, int type, const bq_attn_args& a, const bq_attn_prefix& x, const SharedPlan& s, hipStream_t st);
 
+size_t lora_work_bytes(int rows, int rank, int n_parts);
+hipError_t launch_lora(const bq_lora_args& a, hipStream_t st);
+
 size_t sample_work_bytes(int rows, int vocab);
 hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, const float* temp, const int32_t* top_k,
                          const float* top_p, const float* min_p, const float* u, int32_t* out, void* work, hipStream_t st);

@@ -206,6 +206,46 @@ void bq_attn_hook(void* user, int block, bq_stream_t st) {
     if (p->status == BQ_OK) p->status = r;
 }
 
+size_t bq_lora_workspace_bytes(int rows, int rank, int n_parts) {
+    return rows > 0 && rank > 0 && rank <= BQ_MAX_RANK && n_parts > 0 && n_parts <= BQ_MAX_PARTS ? lora_work_bytes(rows, rank, n_parts) : 0;
+}
+
+int bq_lora(const bq_lora_args* a, bq_stream_t st) {
+    if (int r = device_ready()) return r;
+    if (!a || a->rows < 0 || a->K <= 0 || a->rank <= 0 || a->n_adapters <= 0 || a->n_parts < 1 || a->n_parts > BQ_MAX_PARTS) return BQ_EINVAL;
+    if (a->x_type != BQ_TYPE_Q8_0 && !float_type(a->x_type)) return BQ_EINVAL;
+    if (a->K % 32 || a->rank % 8 || a->rank > BQ_MAX_RANK) return BQ_UNSUPPORTED;
+    int64_t outputs = 0;
+    for (int i = 0; i < a->n_parts; ++i) {
+        const bq_lora_part& p = a->parts[i];
+        if (p.N <= 0) return BQ_EINVAL;
+        if (p.N % 16) return BQ_UNSUPPORTED;
+        outputs += (p.N + 255) / 256;
+    }
+    if (outputs > 65535) return BQ_UNSUPPORTED;  // a grid dimension
+    if (a->rows == 0) return BQ_OK;
+    if (!a->x || !al16(a->x) || !a->adapter) return BQ_EINVAL;
+    if (a->x_type == BQ_TYPE_Q8_0 ? !a->xd : a->ldx < a->K || a->ldx % (a->x_type == BQ_TYPE_F32 ? 4 : 8)) return BQ_EINVAL;
+    for (int i = 0; i < a->n_parts; ++i) {
+        const bq_lora_part& p = a->parts[i];
+        if (!p.a || !p.b || !p.y || !al16(p.a) || !al16(p.b) || !al16(p.y) || !al16(p.base) || p.ldy < p.N || (p.ldy & 3)) return BQ_EINVAL;
+        if (p.base && (p.ldbase < p.N || (p.ldbase & 3) || (p.base == p.y && p.ldbase != p.ldy))) return BQ_EINVAL;
+    }
+    if (!a->work || !al16(a->work) || a->work_bytes < lora_work_bytes(a->rows, a->rank, a->n_parts)) return BQ_EINVAL;
+    return from_hip(launch_lora(*a, (hipStream_t)st));
+}
+
+void bq_lora_hook(void* user, int block, int proj, bq_stream_t st) {
+    bq_lora_plan* p = (bq_lora_plan*)user;
+    if (!p) return;
+    int r = BQ_OK;
+    if (block < 0 || block >= p->n_blocks || !p->blocks || proj < 0 || proj >= BQ_N_PROJ)
+        r = BQ_EINVAL;
+    else if (const bq_lora_args* a = p->blocks[block].proj[proj])
+        r = bq_lora(a, st);
+    if (p->status == BQ_OK) p->status = r;
+}
+
 size_t bq_sample_workspace_bytes(int rows, int vocab) {
     return rows > 0 && vocab > 0 && vocab <= (1 << 20) ? sample_work_bytes(rows, vocab) : 0;
 }

@@ -386,6 +386,11 @@ int bq_gguf_load(bq_gguf* g, int64_t i, void* raw, void* rep, void* rep_min, bq_
  * (needs x_alt; 1 launch fewer per layer than fold = 1).  The attention
  * kernels are the caller's: `attention(user, block, st)` must enqueue them
  * on st (and only there) and write attn_out; NULL leaves attn_out as it is.
+ * `projected(projected_user, block, proj, st)`, where it is set, is called behind
+ * each of a block's projections (BQ_PROJ_QKV, BQ_PROJ_O, BQ_PROJ_GATE_UP,
+ * BQ_PROJ_DOWN) while xq/xd/xsum still hold the rows that it read, and may add to
+ * what it wrote (qkv_out, proj, ffn_g and ffn_u, proj); fold must be 0 then
+ * (BQ_UNSUPPORTED: the folded forms have no such place).
  * Every buffer holds `rows` rows, row-major: x, input_h, proj
  * [rows][n_embd]; attn_out, attn_gate [rows][n_attn]; qkv_out[p] [rows][N_p];
  * ffn_g, ffn_u [rows][n_ff] (with fold >= 1 ffn_u, optional, is scratch: when
@@ -398,6 +403,7 @@ int bq_gguf_load(bq_gguf* g, int64_t i, void* raw, void* rep, void* rep_min, bq_
  * place.  A graph captures the pointers and the row count it is created with:
  * replays read and write the same buffers. */
 enum { BQ_BLOCK_ATTN = 0, BQ_BLOCK_FFN = 1 };
+enum { BQ_PROJ_QKV = 0, BQ_PROJ_O = 1, BQ_PROJ_GATE_UP = 2, BQ_PROJ_DOWN = 3, BQ_N_PROJ = 4 };
 typedef struct bq_decode_block {
     int kind;                     /* BQ_BLOCK_ATTN or BQ_BLOCK_FFN */
     int norm_before, norm_after;  /* loop start / end of the reference's recurrence */
@@ -437,6 +443,8 @@ typedef struct bq_decode_step {
     uint16_t* xdh;
     void* work;
     size_t work_bytes;
+    void (*projected)(void* user, int block, int proj, bq_stream_t st);  /* NULL: none */
+    void* projected_user;
 } bq_decode_step;
 /* Enqueue one token's launch sequence on st (stream-ordered, allocates nothing). */
 int bq_decode_enqueue(const bq_decode_step* s, bq_stream_t st);
@@ -610,6 +618,57 @@ typedef struct bq_attn_plan {
     int status;
 } bq_attn_plan;
 void bq_attn_hook(void* user, int block, bq_stream_t st);
+
+/* Low-rank adapters beside a projection, every row with one of its own (a batch of
+ * requests that share the base weights).  For the parts p < n_parts, which share x,
+ *   y_p[r] = base_p[r] + scale[a] * B_p[a] (A_p[a] x[r]),  a = adapter[r],
+ * with A_p bf16 [n_adapters][rank][K] and B_p bf16 [n_adapters][N][rank], the
+ * adapters of a pool of n_adapters slots (a smaller rank: zeros behind it).  An
+ * adapter outside 0..n_adapters-1 is none: y_p[r] = base_p[r].  base NULL is zeros;
+ * base may be y itself (the projection's output; rows without an adapter are then
+ * not touched), and must not overlap it otherwise.  scale NULL is 1.
+ * x: fp32 or bf16 rows (ldx apart), or the q8 rows that the projection read (xq as
+ * x, and xd, as from bq_quantize_q8; ldx is not used), finite.  fp32 precision
+ * throughout: products are exact, sums fp32.
+ * K % 32 == 0, N % 16 == 0, rank % 8 == 0 and rank <= 256, else BQ_UNSUPPORTED.
+ * Pointers 16-byte aligned (xd, adapter and scale apart); ldx a multiple of 16
+ * bytes, ldbase and ldy of 4 elements.  work: at least bq_lora_workspace_bytes (else
+ * BQ_EINVAL), not shared by calls that overlap.  Equal calls give equal bits; a row's
+ * result does not depend on the other rows' values. */
+enum { BQ_MAX_RANK = 256 };
+typedef struct bq_lora_part {
+    const uint16_t* a; const uint16_t* b;
+    const float* base; float* y;
+    int64_t ldbase, ldy;
+    int N;
+} bq_lora_part;
+typedef struct bq_lora_args {
+    const void* x; const float* xd;
+    int x_type;                   /* BQ_TYPE_F32, BQ_TYPE_BF16 or BQ_TYPE_Q8_0 */
+    int64_t ldx;
+    int rows, K, rank, n_adapters, n_parts;
+    bq_lora_part parts[BQ_MAX_PARTS];
+    const int32_t* adapter;       /* device, [rows] */
+    const float* scale;           /* device, [n_adapters] */
+    void* work;
+    size_t work_bytes;
+} bq_lora_args;
+size_t bq_lora_workspace_bytes(int rows, int rank, int n_parts);
+int bq_lora(const bq_lora_args* a, bq_stream_t st);
+
+/* The decode step's projection hook over a list of blocks: set
+ * bq_decode_step.projected = bq_lora_hook and projected_user = a bq_lora_plan whose
+ * blocks[i].proj[BQ_PROJ_...] is what is added to that projection of the step's block
+ * i (NULL: nothing).  The first code that is not BQ_OK stays in `status`. */
+typedef struct bq_lora_block {
+    const bq_lora_args* proj[BQ_N_PROJ];
+} bq_lora_block;
+typedef struct bq_lora_plan {
+    int n_blocks;
+    const bq_lora_block* blocks;
+    int status;
+} bq_lora_plan;
+void bq_lora_hook(void* user, int block, int proj, bq_stream_t st);
 
 /* One token per row of logits, from one given uniform number per row.  With
  * x_i = (logit_i - max) / temperature[r], tokens ordered by logit, ties by the
