@@ -47,6 +47,7 @@ EXPORTS = [
     "bq_decode_graph_destroy", "bq_kv_page_bytes", "bq_append", "bq_kv_read", "bq_attn_workspace_bytes",
     "bq_attn_prefill_workspace_bytes", "bq_attn_decode", "bq_attn_prefill", "bq_attn_shared_workspace_bytes",
     "bq_attn_decode_shared", "bq_lora_workspace_bytes", "bq_lora", "bq_lora_hook", "bq_attn_hook", "bq_sample_workspace_bytes", "bq_sample",
+    "bq_logprobs_workspace_bytes", "bq_logprobs",
 ]
 
 
@@ -166,6 +167,15 @@ class LoraPlanStruct(ctypes.Structure):
     _fields_ = [("n_blocks", ctypes.c_int), ("blocks", ctypes.POINTER(LoraBlock)), ("status", ctypes.c_int)]
 
 
+class LogprobsArgs(ctypes.Structure):
+    """bq_logprobs_args (include/bq.h)."""
+    _fields_ = [("logits", ctypes.c_void_p), ("ld", ctypes.c_int64), ("rows", ctypes.c_int), ("vocab", ctypes.c_int),
+                ("temperature", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("logprob", ctypes.c_void_p),
+                ("rank", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("top", ctypes.c_int),
+                ("top_tokens", ctypes.c_void_p), ("top_logprobs", ctypes.c_void_p), ("work", ctypes.c_void_p),
+                ("work_bytes", ctypes.c_size_t)]
+
+
 _lib = None
 
 
@@ -246,6 +256,8 @@ def load(path=LIB_PATH):
         "bq_lora_hook": (None, [P, I, I, P]),
         "bq_attn_hook": (None, [P, I, P]),
         "bq_sample_workspace_bytes": (S, [I, I]),
+        "bq_logprobs_workspace_bytes": (S, [I, I, I]),
+        "bq_logprobs": (I, [P, P]),
         "bq_sample": (I, [P, ctypes.c_int64, I, I, P, P, P, P, P, P, P, S, P]),
     }
     for name, (res, args) in sig.items():
@@ -1011,3 +1023,39 @@ class Sampler:
     def run(self):
         d = self._device
         return _check(self._run(*self._args, _raw_stream(d)) if _current() == d else _on(d, self._run, *self._args), "bq_sample")
+
+
+class LogProbs:
+    """bq_logprobs over fixed buffers: logits fp32 [rows, vocab] (rows may be strided), tokens int32 [rows]; of the
+    outputs those that are wanted: logprob and entropy fp32 [rows], rank int32 [rows], top_tokens int32 and top_logprobs
+    fp32 [rows, top].  temperature fp32 [rows] or None."""
+
+    def __init__(self, logits, tokens=None, logprob=None, rank=None, entropy=None, top_tokens=None, top_logprobs=None,
+                 temperature=None, work=None):
+        import torch
+        rows, vocab = logits.shape
+        if logits.dtype != torch.float32:
+            raise TypeError("logits: fp32")
+        for t, what in ((tokens, "tokens"), (rank, "rank")):
+            _expect(t, torch.int32, (rows,), what)
+        for t, what in ((logprob, "logprob"), (entropy, "entropy"), (temperature, "temperature")):
+            _expect(t, torch.float32, (rows,), what)
+        top = next((t.shape[1] for t in (top_tokens, top_logprobs) if t is not None), 0)
+        _expect(top_tokens, torch.int32, (rows, top), "top_tokens")
+        _expect(top_logprobs, torch.float32, (rows, top), "top_logprobs")
+        _one_device(logits.device, tokens=tokens, logprob=logprob, rank=rank, entropy=entropy, top_tokens=top_tokens,
+                    top_logprobs=top_logprobs, temperature=temperature)
+        L = load()
+        if work is None:
+            work = torch.empty(int(L.bq_logprobs_workspace_bytes(rows, vocab, top)), dtype=torch.uint8, device=logits.device)
+        _work_of(work, logits.device)
+        self.work, self._keep = work, (logits, tokens, logprob, rank, entropy, top_tokens, top_logprobs, temperature)
+        self.struct = LogprobsArgs(_ptr(logits), _rows_ld(logits, vocab, "logits"), rows, vocab, _ptr(temperature), _ptr(tokens),
+                                   _ptr(logprob), _ptr(rank), _ptr(entropy), top, _ptr(top_tokens), _ptr(top_logprobs),
+                                   _ptr(work), work.numel() * work.element_size())
+        self._ref, self._run, self._device = ctypes.byref(self.struct), L.bq_logprobs, logits.device.index
+        _bind_device()
+
+    def run(self):
+        d = self._device
+        return _check(self._run(self._ref, _raw_stream(d)) if _current() == d else _on(d, self._run, self._ref), "bq_logprobs")

@@ -171,5 +171,7 @@ hipError_t launch_lora(const bq_lora_args& a, hipStream_t st);
 size_t sample_work_bytes(int rows, int vocab);
 hipError_t launch_sample(const float* logits, int64_t ld, int rows, int vocab, const float* temp, const int32_t* top_k,
                          const float* top_p, const float* min_p, const float* u, int32_t* out, void* work, hipStream_t st);
+size_t logprob_work_bytes(int rows, int vocab, int top);
+hipError_t launch_logprobs(const bq_logprobs_args& a, hipStream_t st);
 
 }  // namespace bq

@@ -260,4 +260,21 @@ int bq_sample(const float* logits, int64_t ld, int rows, int vocab, const float*
     return from_hip(launch_sample(logits, ld, rows, vocab, temperature, top_k, top_p, min_p, u, out, work, (hipStream_t)st));
 }
 
+size_t bq_logprobs_workspace_bytes(int rows, int vocab, int top) {
+    return rows > 0 && vocab > 0 && vocab <= (1 << 20) && top >= 0 && top <= BQ_MAX_TOP ? logprob_work_bytes(rows, vocab, top) : 0;
+}
+
+int bq_logprobs(const bq_logprobs_args* a, bq_stream_t st) {
+    if (int r = device_ready()) return r;
+    if (!a || a->rows < 0 || a->vocab <= 0 || a->ld < a->vocab || a->top < 0) return BQ_EINVAL;
+    if (a->vocab > (1 << 20) || a->rows > 65535 || a->top > BQ_MAX_TOP) return BQ_UNSUPPORTED;
+    // what a result is of, or where it goes
+    if (!a->tokens && (a->logprob || a->rank)) return BQ_EINVAL;
+    if (!a->logprob && !a->rank && !a->entropy && !(a->top && (a->top_tokens || a->top_logprobs))) return BQ_EINVAL;
+    if (a->rows == 0) return BQ_OK;
+    if (!a->logits || ((uintptr_t)a->logits & 3) || !a->work || !al16(a->work) || a->work_bytes < logprob_work_bytes(a->rows, a->vocab, a->top))
+        return BQ_EINVAL;
+    return from_hip(launch_logprobs(*a, (hipStream_t)st));
+}
+
 }  // extern "C"

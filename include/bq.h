@@ -687,6 +687,39 @@ int bq_sample(const float* logits, int64_t ld, int rows, int vocab, const float*
               const float* top_p, const float* min_p, const float* u, int32_t* out, void* work, size_t work_bytes,
               bq_stream_t st);
 
+/* What rows of logits say of a given token each, and of the likeliest: with x_i =
+ * (logit_i - max) / temperature[r] and log p_i = x_i - log sum exp(x),
+ *   logprob[r]   log p of tokens[r] (-inf for a token outside the vocabulary)
+ *   rank[r]      the tokens before it: a larger logit, or an equal one and a lower
+ *                index (vocab for a token outside the vocabulary)
+ *   entropy[r]   -sum p log p, in nats
+ *   top_tokens, top_logprobs [rows][top]   the first `top` tokens in that order, and
+ *                log p of each (-1 and -inf behind the vocab-th)
+ * As in bq_sample a NaN logit counts as -inf, and where the temperature is not above 0
+ * (or NaN), the largest logit +inf, or none above -inf, the first token alone has
+ * probability: log p is 0 for it, -inf for the others, the entropy 0.  p of -inf is 0.
+ * fp32 precision, relative also where a row is nearly sure (log p of its first token
+ * and the entropy are then tiny; a token 2^-126 times as likely counts as 0).  Outputs that are not wanted are
+ * NULL (tokens too, with logprob and rank; BQ_EINVAL if none is wanted), temperature
+ * NULL is 1.  Rows are ld >= vocab apart, any ld; vocab <= 2^20, rows <= 65535 and top
+ * <= BQ_MAX_TOP (else BQ_UNSUPPORTED).  work: at least bq_logprobs_workspace_bytes
+ * (else BQ_EINVAL), not shared by calls that overlap.  Equal calls give equal bits. */
+enum { BQ_MAX_TOP = 64 };
+typedef struct bq_logprobs_args {
+    const float* logits;
+    int64_t ld;
+    int rows, vocab;
+    const float* temperature;     /* device, [rows] */
+    const int32_t* tokens;        /* device, [rows] */
+    float* logprob; int32_t* rank; float* entropy;
+    int top;
+    int32_t* top_tokens; float* top_logprobs;
+    void* work;
+    size_t work_bytes;
+} bq_logprobs_args;
+size_t bq_logprobs_workspace_bytes(int rows, int vocab, int top);
+int bq_logprobs(const bq_logprobs_args* a, bq_stream_t st);
+
 /* ---- tooling ---------------------------------------------------------------
  * No counterpart in the reference (its harnesses bracket launches with
  * cudaEventRecord, tools/gemvbench.cu:360-371).  Times the calling thread's
