@@ -6,14 +6,16 @@
 //   log p = x - log1p(r),  H = log1p(r) - sum exp(x) x / (1 + r)
 // so neither cancels: a row that is nearly sure keeps r, and H, to fp32's relative
 // precision.  Two launches:
-//   k_logprob_scan, one workgroup per 4096 logits: reads them once (the floor: 4 bytes
-//     a logit), and leaves the slice's largest, its two sums, its tokens that come
-//     before the given one, and, for more than one alternative, its candidates: the
-//     logits not below a threshold that at least `top` of the slice's reach, taken
-//     from the lanes' maxima.  Where these are too many (equal logits), the slice's
-//     `top` largest exactly, by bisection on the ordered bits, then on the index.
-//   k_logprob_join, one workgroup per row: joins the slices in their order, and ranks
-//     the candidates not below the largest threshold by counting.
+//   k_logprob_scan, one wave per 1024 logits: reads them once (the floor: 4 bytes a
+//     logit), and leaves the slice's largest, its two sums, its tokens that come before
+//     the given one, and, for more than one alternative, its candidates: the logits not
+//     below a threshold that at least `top` of the slice's reach, taken from the maxima
+//     of 8 logits.  Where these are too many (equal logits), the slice's `top` largest
+//     exactly, by bisection on the ordered bits, then on the index.  Waves share nothing:
+//     no barrier.
+//   k_logprob_join, one workgroup per row: joins the slices in their order.  `top` of
+//     the row's logits reach the top-th largest of its slices' maxima, which few slices
+//     and one to two times `top` candidates do; those are ranked by counting.
 #include <algorithm>
 #include <cmath>
 
@@ -23,18 +25,20 @@
 namespace bq {
 
 namespace {
-constexpr int kSlice = 4096;
-constexpr int kKeys = 1024;  // candidates that the join holds at once
-constexpr int kStep = 768;   // and looks at between two counts of them
-static_assert(kKeys - kStep >= 2 * BQ_MAX_TOP, "the likeliest so far and a step's candidates fit");
+constexpr int kSlice = 1024;
+constexpr int kMaxSlices = 1024;  // the entry point's limit on the vocabulary
+constexpr int kStep = 1024;       // candidates that the join looks at between two counts,
+constexpr int kKeys = 1280;       // and holds at once: the likeliest so far, and a step's
+static_assert(kKeys - kStep >= 2 * BQ_MAX_TOP, "");
 typedef unsigned long long u64;
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any logit
 
 struct SliceInfo {
     u64 best;        // largest key
     float sum, dot;  // of 2^y and 2^y y over the slice but its first largest, y relative to that (log2)
-    uint32_t t;      // ordered bits that at least `top` of the slice's logits reach (0: none known)
-    int before, count, pad;
+    int before, count;
+    uint32_t t, pad;    // ordered bits that at least `top` of the slice's logits reach (0: none known)
+    uint32_t group[4];  // of the largest of each 16 lanes' logits
 };
 
 struct LogprobP {
@@ -83,11 +87,13 @@ BQ_DEV float exponent(float v, float m, float T) {
 }
 BQ_DEV float temperature_of(const LogprobP& p, int row) { return p.temp ? p.temp[row] : 1.f; }
 
-BQ_DEV float wave_max(float v) {
-    v = fmaxf(v, dpp_f<0xB1, 0xF, true>(v));   // quad_perm [1,0,3,2]
-    v = fmaxf(v, dpp_f<0x4E, 0xF, true>(v));   // quad_perm [2,3,0,1]
-    v = fmaxf(v, dpp_f<0x141, 0xF, true>(v));  // row_half_mirror
-    v = fmaxf(v, dpp_f<0x140, 0xF, true>(v));  // row_mirror
+BQ_DEV float row16_max(float v) {
+    v = fmaxf(v, dpp_f<0xB1, 0xF, true>(v));          // quad_perm [1,0,3,2]
+    v = fmaxf(v, dpp_f<0x4E, 0xF, true>(v));          // quad_perm [2,3,0,1]
+    v = fmaxf(v, dpp_f<0x141, 0xF, true>(v));         // row_half_mirror
+    return fmaxf(v, dpp_f<0x140, 0xF, true>(v));      // row_mirror
+}
+BQ_DEV float rows_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16, 64));
     return fmaxf(v, __shfl_xor(v, 32, 64));
 }
@@ -97,13 +103,13 @@ BQ_DEV int wave_min(int v) {
 }
 
 __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
-    constexpr int V = kSlice / 1024;  // 16-byte loads of a thread
-    __shared__ float s_max[4], s_sum[4], s_dot[4];
-    __shared__ uint32_t s_t[4];
-    __shared__ int s_first[4], s_before[4], s_count[2][4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slice = blockIdx.x, row = blockIdx.y;
+    constexpr int V = kSlice / 256;  // 16-byte loads of a lane
+    const int lane = threadIdx.x & 63, slice = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.y;
+    if (slice >= p.slices) return;
     const float* x = p.logits + (size_t)row * p.ld;
-    auto at = [&](int k) { return slice * kSlice + (k * 256 + tid) * 4; };
+    const int token = p.tokens ? p.tokens[row] : -1;
+    const float T = temperature_of(p, row);
+    auto at = [&](int k) { return slice * kSlice + (k * 64 + lane) * 4; };
     float v[V][4];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
@@ -116,52 +122,32 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
                 if (i + e < p.vocab) a[e] = x[i + e];
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[k][e] = clean(a[e]);
+        for (int e = 0; e < 4; ++e) v[k][e] = a[e];
     }
-    const float T = temperature_of(p, row);
-    const int token = p.tokens ? p.tokens[row] : -1;
     const bool given = (unsigned)token < (unsigned)p.vocab;
-    const float given_v = given ? clean(x[token]) : INFINITY;
-
-    float mine = v[0][0];
+    const float given_v = given ? x[token] : INFINITY;  // used last: it comes behind another load
 #pragma unroll
     for (int k = 0; k < V; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mine = fmaxf(mine, v[k][e]);
-    const float wmax = wave_max(mine);
-    if (p.top > 1) {
-        // the wave's threshold: the largest 16-bit prefix of the ordered bits that `top`
-        // of its lanes' maxima reach
-        uint32_t cut = 0;
-        const uint32_t om = ordered(mine);
+        for (int e = 0; e < 4; ++e) v[k][e] = clean(v[k][e]);
+
+    float half[2];
 #pragma unroll
-        for (int bit = 31; bit >= 16; --bit) {
-            const uint32_t c = cut | 1u << bit;
-            if (__popcll(__ballot(om >= c)) >= p.top) cut = c;
-        }
-        if (lane == 0) s_t[wave] = cut;
+    for (int h = 0; h < 2; ++h) {
+        half[h] = -INFINITY;
+#pragma unroll
+        for (int k = V / 2 * h; k < V / 2 * (h + 1); ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) half[h] = fmaxf(half[h], v[k][e]);
     }
-    if (lane == 0) s_max[wave] = wmax;
-    __syncthreads();
-    const float mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    const float mine = fmaxf(half[0], half[1]), group = row16_max(mine), mx = rows_max(group);
     int first = 0x7FFFFFFF;
-    if (__any(mine == mx)) {
 #pragma unroll
-        for (int k = V - 1; k >= 0; --k)
+    for (int k = V - 1; k >= 0; --k)
 #pragma unroll
-            for (int e = 3; e >= 0; --e)
-                if (v[k][e] == mx) first = at(k) + e;
-        first = wave_min(first);
-    }
-    int before = 0;
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) before += v[k][e] > given_v || (v[k][e] == given_v && at(k) + e < token);
-    if (lane == 0) s_first[wave] = first;
-    __syncthreads();
-    first = min(min(s_first[0], s_first[1]), min(s_first[2], s_first[3]));
-
+        for (int e = 3; e >= 0; --e)
+            if (v[k][e] == mx) first = at(k) + e;
+    first = wave_min(first);
     float sum = 0.f, dot = 0.f;
     if (mx > -INFINITY && mx < INFINITY && T > 0.f) {
         const Scaled to(T);
@@ -176,28 +162,23 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
     }
     sum = wave_sum_dpp63(sum);
     dot = wave_sum_dpp63(dot);
-    for (int d = 1; d < 64; d <<= 1) before += __shfl_xor(before, d, 64);
-    if (lane == 63) {
-        s_sum[wave] = sum;
-        s_dot[wave] = dot;
-        s_before[wave] = before;
-    }
     int total = 0;
     uint32_t t = 0;
     if (p.top > 1) {
-        t = max(max(s_t[0], s_t[1]), max(s_t[2], s_t[3]));
-        int turn = 0;
-        // tokens of the slice that satisfy f, over the workgroup
+        // the largest 16-bit prefix of the ordered bits that `top` of the halves' maxima reach
+        const uint32_t h0 = ordered(half[0]), h1 = ordered(half[1]);
+#pragma unroll
+        for (int bit = 31; bit >= 16; --bit) {
+            const uint32_t c = t | 1u << bit;
+            if (__popcll(__ballot(h0 >= c)) + __popcll(__ballot(h1 >= c)) >= p.top) t = c;
+        }
         auto count = [&](auto f) {
             int n = 0;
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) n += __popcll(__ballot(at(k) + e < p.vocab && f(ordered(v[k][e]), at(k) + e)));
-            turn ^= 1;
-            if (lane == 0) s_count[turn][wave] = n;
-            __syncthreads();
-            return s_count[turn][0] + s_count[turn][1] + s_count[turn][2] + s_count[turn][3];
+            return n;
         };
         int last = 0x7FFFFFFF;  // of the logits that equal t, those up to this index
         total = count([&](uint32_t o, int) { return o >= t; });
@@ -212,10 +193,9 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
             for (int step = kSlice / 2; step > 0; step >>= 1)  // the most that hold fewer than wanted, and one more
                 if (count([&](uint32_t o, int i) { return o == t && i <= last + step; }) < want) last += step;
             ++last;
-            total = count([&](uint32_t o, int i) { return o > t || (o == t && i <= last); });
+            total = p.top;
         }
         u64* cand = p.cand + (((size_t)row * p.slices + slice) << p.cap_log);
-        for (int w = 0; w < wave; ++w) cand += s_count[turn][w];
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
@@ -229,33 +209,54 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
                 cand += __popcll(mask);
             }
     }
-    __syncthreads();
-    if (tid == 0) {
-        SliceInfo* info = p.info + (size_t)row * p.slices + slice;
+    int before = 0;
+    const float limit = clean(given_v);
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) before += __popcll(__ballot(v[k][e] > limit || (v[k][e] == limit && at(k) + e < token)));
+    SliceInfo* info = p.info + (size_t)row * p.slices + slice;
+    if ((lane & 15) == 0) info->group[lane >> 4] = ordered(group);
+    if (lane == 63) {
         info->best = key_of(mx, first);
-        info->sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-        info->dot = (s_dot[0] + s_dot[1]) + (s_dot[2] + s_dot[3]);
-        info->t = t;
-        info->before = s_before[0] + s_before[1] + s_before[2] + s_before[3];
+        info->sum = sum;
+        info->dot = dot;
+        info->before = before;
         info->count = total;
+        info->t = t;
     }
 }
 
 BQ_DEV u64 larger(u64 a, u64 b) { return a > b ? a : b; }
 
 __global__ void __launch_bounds__(256) k_logprob_join(LogprobP p) {
+    constexpr int S = kMaxSlices / 256;  // slices of a thread at most
     __shared__ u64 s_key[kKeys], s_top[BQ_MAX_TOP], s_best[4];
-    __shared__ uint32_t s_t[4];
+    __shared__ uint32_t s_t[4], s_high;
     __shared__ float s_sum[4], s_dot[4];
-    __shared__ int s_before[4], s_n;
+    __shared__ int s_before[4], s_n, s_live;
+    __shared__ uint16_t s_slice[kMaxSlices], s_count[kMaxSlices];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
     const SliceInfo* info = p.info + (size_t)row * p.slices;
-    // at most 256 slices (the entry point's limit on the vocabulary): one a thread
-    SliceInfo mine = {};
-    if (tid < p.slices) mine = info[tid];
-    u64 best = mine.best;
-    uint32_t t = mine.t;
-    int before = mine.before;
+    const float T = temperature_of(p, row);
+    const int token = p.tokens ? p.tokens[row] : -1;
+    const bool given = (unsigned)token < (unsigned)p.vocab;
+    SliceInfo mine[S];
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        mine[i] = SliceInfo{};
+        if (tid + 256 * i < p.slices) mine[i] = info[tid + 256 * i];
+    }
+    const float given_v = given ? p.logits[(size_t)row * p.ld + token] : 0.f;
+    u64 best = 0;
+    uint32_t t = 0;
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        best = larger(best, mine[i].best);
+        t = max(t, mine[i].t);
+        before += mine[i].before;
+    }
     for (int d = 1; d < 64; d <<= 1) {
         best = larger(best, (u64)__shfl_xor((uint32_t)(best >> 32), d, 64) << 32 | __shfl_xor((uint32_t)best, d, 64));
         t = max(t, (uint32_t)__shfl_xor(t, d, 64));
@@ -266,25 +267,59 @@ __global__ void __launch_bounds__(256) k_logprob_join(LogprobP p) {
         s_t[wave] = t;
         s_before[wave] = before;
     }
-    if (tid == 0) s_n = 0;
+    if (tid == 0) s_n = s_live = 0;
+    // the slices' maxima, or those of their quarters where the slices are few, to wave 0
+    const bool few = p.slices < 2 * p.top;
+    uint32_t* s_max = (uint32_t*)s_key;
+    if (p.top > 1) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int s = tid + 256 * i;
+            if (s >= p.slices) continue;
+            if (few)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) s_max[4 * s + g] = mine[i].group[g];
+            else
+                s_max[s] = (uint32_t)(mine[i].best >> 32);
+        }
+    }
     __syncthreads();
     best = larger(larger(s_best[0], s_best[1]), larger(s_best[2], s_best[3]));
-    t = max(max(s_t[0], s_t[1]), max(s_t[2], s_t[3]));
-    const float T = temperature_of(p, row), M = value_of(best);
+    const float M = value_of(best);
     // only the first token has probability: no temperature, an infinite logit, or none above -inf
     const bool sure = !(T > 0.f) || !(M > -INFINITY && M < INFINITY);
     float sum = 0.f, dot = 0.f;
-    if (!sure && tid < p.slices && value_of(mine.best) > -INFINITY) {
+    if (!sure) {
         const Scaled to(T);
-        const float y = to.y(value_of(mine.best), M), w = __builtin_amdgcn_exp2f(y), own = mine.best == best ? 0.f : 1.f;
-        sum = w * (mine.sum + own);
-        dot = w * (mine.dot + y * (mine.sum + own));
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            if (tid + 256 * i >= p.slices || value_of(mine[i].best) == -INFINITY) continue;
+            const float y = to.y(value_of(mine[i].best), M), w = __builtin_amdgcn_exp2f(y), own = mine[i].best == best ? 0.f : 1.f;
+            sum += w * (mine[i].sum + own);
+            dot += w * (mine[i].dot + y * (mine[i].sum + own));
+        }
     }
     sum = wave_sum_dpp63(sum);
     dot = wave_sum_dpp63(dot);
     if (lane == 63) {
         s_sum[wave] = sum;
         s_dot[wave] = dot;
+    }
+    if (p.top > 1 && wave == 0) {
+        constexpr int R = kMaxSlices / 64;
+        const int n = few ? 4 * p.slices : p.slices;  // < 8 top <= 512, or at most 1024
+        uint32_t v[R], high = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) v[i] = 64 * i + lane < n ? s_max[64 * i + lane] : 0;
+        for (int bit = 31; bit >= 16; --bit) {
+            const uint32_t c = high | 1u << bit;
+            int reach = 0;
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (64 * i < n) reach += __popcll(__ballot(v[i] >= c));
+            if (reach >= p.top) high = c;
+        }
+        if (lane == 0) s_high = high;
     }
     __syncthreads();
     sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
@@ -296,20 +331,26 @@ __global__ void __launch_bounds__(256) k_logprob_join(LogprobP p) {
     };
     if (tid == 0) {
         if (p.entropy) p.entropy[row] = sure ? 0.f : log_z - 0.693147180559945309f * dot / (1.f + sum);
-        if (p.tokens) {
-            const int token = p.tokens[row];
-            const bool given = (unsigned)token < (unsigned)p.vocab;
-            if (p.logprob) p.logprob[row] = given ? log_p(clean(p.logits[(size_t)row * p.ld + token]), token) : -INFINITY;
-            if (p.rank) p.rank[row] = given ? s_before[0] + s_before[1] + s_before[2] + s_before[3] : p.vocab;
-        }
+        if (p.logprob) p.logprob[row] = given ? log_p(clean(given_v), token) : -INFINITY;
+        if (p.rank) p.rank[row] = given ? s_before[0] + s_before[1] + s_before[2] + s_before[3] : p.vocab;
     }
     if (p.top == 0) return;
     int n = 1;
     if (p.top == 1) {
         if (tid == 0) s_top[0] = best;
     } else {
-        // candidates not below t into s_key; where another step's might not fit, the `top`
-        // largest of those found replace them
+        t = max(max(max(s_t[0], s_t[1]), max(s_t[2], s_t[3])), s_high);
+        // the slices that hold candidates not below t
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+            if (tid + 256 * i < p.slices && (uint32_t)(mine[i].best >> 32) >= t) {
+                const int j = atomicAdd(&s_live, 1);
+                s_slice[j] = tid + 256 * i;
+                s_count[j] = mine[i].count;
+            }
+        __syncthreads();
+        // their candidates not below t into s_key; where another step's might not fit, the
+        // `top` largest of those found replace them
         auto cut = [&] {
             n = s_n;
             for (int i = tid; i < n; i += 256) {
@@ -321,17 +362,18 @@ __global__ void __launch_bounds__(256) k_logprob_join(LogprobP p) {
             n = min(n, p.top);
             __syncthreads();
         };
-        const int slots = p.slices << p.cap_log;
+        const int slots = s_live << p.cap_log;
         const u64* cand = p.cand + ((size_t)row * p.slices << p.cap_log);
         for (int e0 = 0; e0 < slots; e0 += kStep) {
+            u64 key[kStep / 256];
 #pragma unroll
             for (int i = 0; i < kStep / 256; ++i) {
-                const int e = e0 + 256 * i + tid, s = e >> p.cap_log;
-                if (e < slots && (e & ((1 << p.cap_log) - 1)) < info[s].count) {
-                    const u64 key = cand[e];
-                    if ((uint32_t)(key >> 32) >= t) s_key[atomicAdd(&s_n, 1)] = key;
-                }
+                const int e = e0 + 256 * i + tid, j = e >> p.cap_log, at = e & ((1 << p.cap_log) - 1);
+                key[i] = e < slots && at < s_count[j] ? cand[((size_t)s_slice[j] << p.cap_log) + at] : 0;
             }
+#pragma unroll
+            for (int i = 0; i < kStep / 256; ++i)
+                if (key[i] != 0 && (uint32_t)(key[i] >> 32) >= t) s_key[atomicAdd(&s_n, 1)] = key[i];
             __syncthreads();
             if (s_n > kKeys - kStep && e0 + kStep < slots) {
                 cut();
@@ -352,11 +394,10 @@ __global__ void __launch_bounds__(256) k_logprob_join(LogprobP p) {
 }
 
 int slices_of(int vocab) { return (vocab + kSlice - 1) / kSlice; }
-// room for a slice's candidates: about 1.5 `top` of a slice of independent logits, 3 `top`
-// hardly ever
+// room for a slice's candidates: 1.1 to 1.4 `top` of a slice of independent logits
 int cap_log_of(int top) {
-    int n = 6;
-    while (1 << n < 4 * top) ++n;
+    int n = 4;
+    while (1 << n < 2 * top) ++n;
     return n;
 }
 }  // namespace
@@ -373,7 +414,7 @@ hipError_t launch_logprobs(const bq_logprobs_args& a, hipStream_t st) {
     p.top_tokens = a.top_tokens; p.top_logprobs = a.top_logprobs;
     p.info = (SliceInfo*)a.work;
     p.cand = (u64*)(p.info + (size_t)a.rows * p.slices);
-    launch_kernel(k_logprob_scan, dim3(p.slices, a.rows), dim3(256), 0, st, p);
+    launch_kernel(k_logprob_scan, dim3((p.slices + 3) / 4, a.rows), dim3(256), 0, st, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     launch_kernel(k_logprob_join, dim3(a.rows), dim3(256), 0, st, p);
