@@ -58,7 +58,7 @@ struct LogprobP {
 
 // ordered bits of a logit (-0 as 0, NaN as -inf), and the sort key: larger logits
 // first, then lower indices
-BQ_DEV float clean(float x) { return x == x ? x + 0.f : -INFINITY; }
+BQ_DEV float clean(float x) { return fmaxf(x + 0.f, -INFINITY); }
 BQ_DEV uint32_t ordered(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x);
     return b ^ (b >> 31 ? 0xFFFFFFFFu : 0x80000000u);
@@ -80,6 +80,9 @@ struct Scaled {
         mul = 1.44269504088896341f / (T * q * up);
     }
     BQ_DEV float y(float v, float m) const { return fmaxf((v * q - m * q) * up * mul, -1000.f); }
+    // whether none of that can happen: then the difference, and one product
+    static BQ_DEV bool plain(float T, float m) { return T >= 0x1p-100f && T <= 0x1p100f && m <= 0x1p126f; }
+    static BQ_DEV float plain_y(float v, float m, float mul) { return fmaxf((v - m) * mul, -1000.f); }
 };
 // x = (v - m) / T in units of 1, v <= m, m finite
 BQ_DEV float exponent(float v, float m, float T) {
@@ -111,54 +114,66 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
     const float T = temperature_of(p, row);
     auto at = [&](int k) { return slice * kSlice + (k * 64 + lane) * 4; };
     float v[V][4];
+    if ((slice + 1) * kSlice <= p.vocab) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int i = at(k);
-        f32x4 a = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (i + 4 <= p.vocab) {
-            a = *(const f32x4u*)(x + i);
-        } else {
-            for (int e = 0; e < 4; ++e)
-                if (i + e < p.vocab) a[e] = x[i + e];
+        for (int k = 0; k < V; ++k) {
+            const f32x4 a = *(const f32x4u*)(x + at(k));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[k][e] = a[e];
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[k][e] = a[e];
-    }
-    const bool given = (unsigned)token < (unsigned)p.vocab;
-    const float given_v = given ? x[token] : INFINITY;  // used last: it comes behind another load
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[k][e] = clean(v[k][e]);
-
-    float half[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        half[h] = -INFINITY;
-#pragma unroll
-        for (int k = V / 2 * h; k < V / 2 * (h + 1); ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) half[h] = fmaxf(half[h], v[k][e]);
-    }
-    const float mine = fmaxf(half[0], half[1]), group = row16_max(mine), mx = rows_max(group);
-    int first = 0x7FFFFFFF;
-#pragma unroll
-    for (int k = V - 1; k >= 0; --k)
-#pragma unroll
-        for (int e = 3; e >= 0; --e)
-            if (v[k][e] == mx) first = at(k) + e;
-    first = wave_min(first);
-    float sum = 0.f, dot = 0.f;
-    if (mx > -INFINITY && mx < INFINITY && T > 0.f) {
-        const Scaled to(T);
+    } else {
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float y = to.y(v[k][e], mx), w = at(k) + e == first ? 0.f : __builtin_amdgcn_exp2f(y);
-                sum += w;
-                dot = __builtin_fmaf(w, y, dot);
-            }
+            for (int e = 0; e < 4; ++e) v[k][e] = at(k) + e < p.vocab ? x[at(k) + e] : -INFINITY;
+    }
+    const bool given = (unsigned)token < (unsigned)p.vocab;
+    const float given_v = given ? x[token] : INFINITY;  // used last: it comes behind another load
+
+    float quad[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[k][e] = clean(v[k][e]);
+        quad[k] = fmaxf(fmaxf(v[k][0], v[k][1]), fmaxf(v[k][2], v[k][3]));
+    }
+    static_assert(V == 4, "two halves of two quads");
+    const float half[2] = {fmaxf(quad[0], quad[1]), fmaxf(quad[2], quad[3])};
+    const float mine = fmaxf(half[0], half[1]), group = row16_max(mine), mx = rows_max(group);
+    // where the first of the largest stands: the first run of 256, its first lane, its first value
+    int run = 0, first = 0;
+#pragma unroll
+    for (int k = V - 1; k >= 0; --k) {
+        const uint64_t in = __ballot(quad[k] == mx);
+        if (in == 0) continue;
+        const int l = __builtin_ctzll(in);
+        run = k;
+        first = slice * kSlice + (k * 64 + l) * 4 + 3;
+#pragma unroll
+        for (int e = 2; e >= 0; --e)
+            if (__ballot(v[k][e] == mx) >> l & 1) first = slice * kSlice + (k * 64 + l) * 4 + e;
+    }
+    float sum = 0.f, dot = 0.f;
+    if (mx > -INFINITY && mx < INFINITY && T > 0.f) {
+        const Scaled to(T);
+        auto add = [&](auto y_of) {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = y_of(v[k][e]);
+                    float w = __builtin_amdgcn_exp2f(y);
+                    if (k == run) w = at(k) + e == first ? 0.f : w;
+                    sum += w;
+                    dot = __builtin_fmaf(w, y, dot);
+                }
+        };
+        if (Scaled::plain(T, mx)) {
+            const float mul = 1.44269504088896341f / T;
+            add([&](float x) { return Scaled::plain_y(x, mx, mul); });
+        } else {
+            add([&](float x) { return to.y(x, mx); });
+        }
     }
     sum = wave_sum_dpp63(sum);
     dot = wave_sum_dpp63(dot);
@@ -172,49 +187,56 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
             const uint32_t c = t | 1u << bit;
             if (__popcll(__ballot(h0 >= c)) + __popcll(__ballot(h1 >= c)) >= p.top) t = c;
         }
-        auto count = [&](auto f) {
+        const int cap = 1 << p.cap_log;
+        u64* cand = p.cand + (((size_t)row * p.slices + slice) << p.cap_log);
+        // the logits that satisfy f to cand, as far as there is room; their number
+        auto keep = [&](auto f) {
             int n = 0;
 #pragma unroll
             for (int k = 0; k < V; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) n += __popcll(__ballot(at(k) + e < p.vocab && f(ordered(v[k][e]), at(k) + e)));
+                for (int e = 0; e < 4; ++e) {
+                    const bool in = f(v[k][e], at(k) + e);
+                    const uint64_t mask = __ballot(in);
+                    const int to = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+                    if (in && to < cap) cand[to] = key_of(v[k][e], at(k) + e);
+                    n += __popcll(mask);
+                }
             return n;
         };
-        int last = 0x7FFFFFFF;  // of the logits that equal t, those up to this index
-        total = count([&](uint32_t o, int) { return o >= t; });
-        if (total > 1 << p.cap_log) {
+        // below the lowest finite logit t stands for all of the slice, of which the last may be short
+        const float least = t <= ordered(-INFINITY) ? -INFINITY : unordered(t);
+        total = least == -INFINITY ? keep([&](float, int i) { return i < p.vocab; }) : keep([&](float x, int) { return x >= least; });
+        if (total > cap) {
+            auto count = [&](auto f) {
+                int n = 0;
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) n += __popcll(__ballot(at(k) + e < p.vocab && f(ordered(v[k][e]), at(k) + e)));
+                return n;
+            };
             t = 0;
             for (int bit = 31; bit >= 0; --bit) {
                 const uint32_t c = t | 1u << bit;
                 if (count([&](uint32_t o, int) { return o >= c; }) >= p.top) t = c;
             }
             const int want = p.top - count([&](uint32_t o, int) { return o > t; });
-            last = slice * kSlice - 1;
+            int last = slice * kSlice - 1;  // of the logits that equal t, those up to this index
             for (int step = kSlice / 2; step > 0; step >>= 1)  // the most that hold fewer than wanted, and one more
                 if (count([&](uint32_t o, int i) { return o == t && i <= last + step; }) < want) last += step;
             ++last;
-            total = p.top;
+            total = keep([&](float x, int i) { return i < p.vocab && (ordered(x) > t || (ordered(x) == t && i <= last)); });
         }
-        u64* cand = p.cand + (((size_t)row * p.slices + slice) << p.cap_log);
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t o = ordered(v[k][e]);
-                const bool in = at(k) + e < p.vocab && (o > t || (o == t && at(k) + e <= last));
-                const uint64_t mask = __ballot(in);
-                if (mask == 0) continue;
-                if (in) cand[__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] =
-                    key_of(v[k][e], at(k) + e);
-                cand += __popcll(mask);
-            }
     }
     int before = 0;
     const float limit = clean(given_v);
+    if (limit <= mx) {
 #pragma unroll
-    for (int k = 0; k < V; ++k)
+        for (int k = 0; k < V; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) before += __popcll(__ballot(v[k][e] > limit || (v[k][e] == limit && at(k) + e < token)));
+            for (int e = 0; e < 4; ++e) before += __popcll(__ballot(v[k][e] > limit || (v[k][e] == limit && at(k) + e < token)));
+    }
     SliceInfo* info = p.info + (size_t)row * p.slices + slice;
     if ((lane & 15) == 0) info->group[lane >> 4] = ordered(group);
     if (lane == 63) {
