@@ -250,6 +250,39 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
 }
 
 BQ_DEV u64 larger(u64 a, u64 b) { return a > b ? a : b; }
+// combines the wave's values by f in every lane
+template <int CTRL>
+BQ_DEV uint32_t lane_dpp(uint32_t v) { return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, false); }
+template <int CTRL>
+BQ_DEV u64 lane_dpp(u64 v) { return (u64)lane_dpp<CTRL>((uint32_t)(v >> 32)) << 32 | lane_dpp<CTRL>((uint32_t)v); }
+BQ_DEV uint32_t lane_xor(uint32_t v, int d) { return __shfl_xor(v, d, 64); }
+BQ_DEV u64 lane_xor(u64 v, int d) { return (u64)lane_xor((uint32_t)(v >> 32), d) << 32 | lane_xor((uint32_t)v, d); }
+template <typename X, typename F>
+BQ_DEV X over_wave(X v, F f) {
+    v = f(v, lane_dpp<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = f(v, lane_dpp<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = f(v, lane_dpp<0x141>(v));  // row_half_mirror
+    v = f(v, lane_dpp<0x140>(v));  // row_mirror
+    v = f(v, lane_xor(v, 16));
+    return f(v, lane_xor(v, 32));
+}
+// the largest 16-bit prefix that `top` of the n <= 64 R values reach (one wave)
+template <int R>
+BQ_DEV uint32_t reached(const uint32_t* at, int n, int top) {
+    const int lane = threadIdx.x & 63;
+    uint32_t v[R], high = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] = 64 * i + lane < n ? at[64 * i + lane] : 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t c = high | 1u << bit;
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) reach += __popcll(__ballot(v[i] >= c));
+        if (reach >= top) high = c;
+    }
+    return high;
+}
 
 __global__ void __launch_bounds__(256) k_logprob_join(LogprobP p) {
     constexpr int S = kMaxSlices / 256;  // slices of a thread at most
@@ -279,11 +312,9 @@ __global__ void __launch_bounds__(256) k_logprob_join(LogprobP p) {
         t = max(t, mine[i].t);
         before += mine[i].before;
     }
-    for (int d = 1; d < 64; d <<= 1) {
-        best = larger(best, (u64)__shfl_xor((uint32_t)(best >> 32), d, 64) << 32 | __shfl_xor((uint32_t)best, d, 64));
-        t = max(t, (uint32_t)__shfl_xor(t, d, 64));
-        before += __shfl_xor(before, d, 64);
-    }
+    best = over_wave(best, larger);
+    t = over_wave(t, [](uint32_t a, uint32_t b) { return max(a, b); });
+    before = (int)over_wave((uint32_t)before, [](uint32_t a, uint32_t b) { return a + b; });
     if (lane == 0) {
         s_best[wave] = best;
         s_t[wave] = t;
@@ -328,19 +359,8 @@ __global__ void __launch_bounds__(256) k_logprob_join(LogprobP p) {
         s_dot[wave] = dot;
     }
     if (p.top > 1 && wave == 0) {
-        constexpr int R = kMaxSlices / 64;
         const int n = few ? 4 * p.slices : p.slices;  // < 8 top <= 512, or at most 1024
-        uint32_t v[R], high = 0;
-#pragma unroll
-        for (int i = 0; i < R; ++i) v[i] = 64 * i + lane < n ? s_max[64 * i + lane] : 0;
-        for (int bit = 31; bit >= 16; --bit) {
-            const uint32_t c = high | 1u << bit;
-            int reach = 0;
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-                if (64 * i < n) reach += __popcll(__ballot(v[i] >= c));
-            if (reach >= p.top) high = c;
-        }
+        const uint32_t high = n <= 128 ? reached<2>(s_max, n, p.top) : n <= 512 ? reached<8>(s_max, n, p.top) : reached<16>(s_max, n, p.top);
         if (lane == 0) s_high = high;
     }
     __syncthreads();
@@ -375,11 +395,15 @@ __global__ void __launch_bounds__(256) k_logprob_join(LogprobP p) {
         // `top` largest of those found replace them
         auto cut = [&] {
             n = s_n;
-            for (int i = tid; i < n; i += 256) {
-                const u64 key = s_key[i];
-                int rank = 0;
-                for (int j = 0; j < n; ++j) rank += s_key[j] > key;
-                if (rank < p.top) s_top[rank] = key;
+            for (int i0 = 0; i0 < n; i0 += 64) {  // four lanes a key
+                const int i = i0 + (tid >> 2);
+                const u64 key = i < n ? s_key[i] : 0;
+                uint32_t rank = 0;
+#pragma unroll 4
+                for (int j = tid & 3; j < n; j += 4) rank += s_key[j] > key;
+                rank += lane_dpp<0xB1>(rank);
+                rank += lane_dpp<0x4E>(rank);
+                if (i < n && (tid & 3) == 0 && rank < (uint32_t)p.top) s_top[rank] = key;
             }
             n = min(n, p.top);
             __syncthreads();
