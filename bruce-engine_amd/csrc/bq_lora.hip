@@ -12,8 +12,12 @@
 //
 // Rows of one adapter are found by each workgroup itself: of up to kGather rows the
 // first that has an adapter takes all that share it, from anywhere in the batch (a
-// decode step's rows); of more, a workgroup takes 16 neighbours and their adapters
-// one after the other (prompts: nearly always one).
+// decode step's rows), 16 at a time; of more, a workgroup takes 32 neighbours and their
+// adapters one after the other (prompts: nearly always one).
+//
+// All of x, A, base and y is moved a row at a time, 256 to 1024 contiguous bytes, and
+// turned into operands or out of results in LDS: rows are often a multiple of 4 KiB
+// apart, and a load of 64 bytes from each of 16 such rows meets one memory channel.
 #include <algorithm>
 
 #include "bq_internal.hpp"
@@ -24,7 +28,9 @@ namespace bq {
 namespace {
 constexpr int kGather = 256;
 constexpr int kRankTiles = 4;  // 16-rank tiles of a workgroup of k_lora_down at most
-constexpr int kUpTiles = 4;    // 16-output tiles of a wave of k_lora_up
+constexpr int kChunk = 256;    // values of K that it stages at once
+constexpr int kPieces = 8;     // pieces that K is cut into at most
+constexpr int kRun = 256;      // outputs that a workgroup of k_lora_up has at once
 
 enum XKind { kXQ8, kXF32, kXBf16 };
 
@@ -41,7 +47,8 @@ struct LoraP {
     int64_t ldbase[kMaxParts], ldy[kMaxParts];
     int N[kMaxParts], chunk0[kMaxParts];  // first output chunk of a part
     int n_parts, rows, K, rank, n_adapters;
-    float* t;  // [rows][n_parts][rank]
+    int pieces, turns;  // of K; runs of kRun outputs that a workgroup of k_lora_up takes
+    float* t;           // [pieces][rows][n_parts][rank]
 };
 
 BQ_DEV f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -52,12 +59,12 @@ BQ_DEV int adapter_of(const LoraP& p, int r) {
     return (unsigned)a < (unsigned)p.n_adapters ? a : -1;
 }
 
-// Calls f(adapter, rows, n) for this workgroup's rows, n <= 16 of one adapter at a
+// Calls f(adapter, rows, n) for this workgroup's rows, n <= 16 RT of one adapter at a
 // time (rows in LDS).  All of the workgroup's lanes take part; f may hold barriers.
-template <typename F>
+template <int RT, typename F>
 BQ_DEV void each_adapter(const LoraP& p, int* s_rows, int* s_n, F f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (p.rows <= kGather) {
+    if constexpr (RT == 1) {  // at most kGather rows
         const int me = blockIdx.x, a = adapter_of(p, me);
         if (wave == 0) {
             int n = 0;
@@ -74,15 +81,17 @@ BQ_DEV void each_adapter(const LoraP& p, int* s_rows, int* s_n, F f) {
         const int n = *s_n;
         for (int i = 0; i < n; i += 16) f(a, s_rows + i, min(16, n - i));
     } else {
-        const int r0 = blockIdx.x * 16, n = min(16, p.rows - r0), a = adapter_of(p, r0 + min(lane & 15, n - 1));
-        uint32_t left = (1u << n) - 1;
+        constexpr int T = 16 * RT;
+        static_assert(T <= 64, "");
+        const int r0 = blockIdx.x * T, n = min(T, p.rows - r0), a = adapter_of(p, r0 + min(lane, n - 1));
+        uint64_t left = ~0ull >> (64 - n);
         while (left) {
-            const int one = __builtin_amdgcn_readlane(a, __builtin_ctz(left));
-            const uint32_t same = (uint32_t)__ballot(a == one) & left;
+            const int one = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
+            const uint64_t same = __ballot(a == one) & left;
             left &= ~same;
-            if (wave == 0 && lane < 16 && (same >> lane & 1)) s_rows[__builtin_popcount(same & ((1u << lane) - 1))] = r0 + lane;
+            if (wave == 0 && (same >> lane & 1)) s_rows[__builtin_popcountll(same & ((1ull << lane) - 1))] = r0 + lane;
             __syncthreads();
-            f(one, s_rows, __builtin_popcount(same));
+            f(one, s_rows, __builtin_popcountll(same));
             __syncthreads();
         }
     }
@@ -111,145 +120,290 @@ BQ_DEV u32x2 codes_bf16(uint32_t w) {
     return u32x2{hi2(a, b), hi2(c, d)};
 }
 
-// t: a workgroup has up to 16 TILES ranks of one part; its waves share K.  (The number of
-// tiles is fixed when it is compiled: with a branch between an MFMA and the first use of
-// its result the compiler has left out the wait that the result needs.)
-template <int X, int TILES>
+// A piece of t: a workgroup has 16 RT rows and up to TILES 16-rank tiles, of any parts,
+// so that x is read once for up to 64 ranks.  kChunk values of K at a time pass LDS; each
+// wave takes a quarter of them.  (The number of tiles is fixed when it is compiled: with a
+// branch between an MFMA and the first use of its result the compiler has left out the
+// wait that the result needs.)
+template <int X, int TILES, int RT>
 __global__ void __launch_bounds__(256) k_lora_down(LoraP p) {
-    __shared__ int s_rows[kGather], s_n;
-    __shared__ __attribute__((aligned(16))) float s_t[4][16][16 * TILES + 4];
+    constexpr int M = 16 * RT, U = X == kXF32 ? 4 : X == kXBf16 ? 2 : 1;  // bytes of a value of x
+    // rows of LDS are 16 bytes longer than their values: 16 lanes on 16 rows meet 16 bank groups
+    constexpr int PA = 2 * kChunk + 16, PX = U * kChunk + 16, PT = 16 * TILES + 4;
+    constexpr int NA = 16 * TILES * (kChunk / 8) / 256, NX = M * U * kChunk / 16 / 256;  // 16-byte units of a thread
+    constexpr int kStage = 16 * TILES * PA + M * PX, kSums = 4 * M * PT * 4;
+    __shared__ __attribute__((aligned(16))) char s_stage[kStage > kSums ? kStage : kSums];
+    __shared__ float s_d[M][kChunk / 32 + 1];  // q8: the groups' scales
+    __shared__ int s_rows[RT == 1 ? kGather : M], s_n;
+    char* s_a = s_stage;
+    char* s_x = s_stage + 16 * TILES * PA;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-    const int chunks = (p.rank + 16 * TILES - 1) / (16 * TILES), part = blockIdx.y / chunks, j0 = blockIdx.y % chunks * 16 * TILES;
-    const int nj = min(16 * TILES, p.rank - j0);
-    const int steps = p.K / 32;
-    each_adapter(p, s_rows, &s_n, [&](int a, const int* rows, int n) {
+    const int per_part = (p.rank + 15) / 16, tiles = per_part * p.n_parts, tile0 = blockIdx.y * TILES;
+    const int chunks = (p.K + kChunk - 1) / kChunk;
+    const int c0 = chunks * blockIdx.z / p.pieces, c1 = chunks * (blockIdx.z + 1) / p.pieces;
+    each_adapter<RT>(p, s_rows, &s_n, [&](int a, const int* rows, int n) {
         if (a < 0) return;
-        const int64_t row = rows[min(c, n - 1)];
-        const uint16_t* A[TILES];
+        const char* A[NA];
+        const char* Xp[NX];
 #pragma unroll
-        for (int i = 0; i < TILES; ++i)  // ranks past the last read it again; they are not stored
-            A[i] = p.a[part] + ((int64_t)a * p.rank + min(j0 + 16 * i + c, p.rank - 1)) * p.K + 8 * g;
-        f32x4 t[TILES];
+        for (int i = 0; i < NA; ++i) {  // tiles and ranks past the last read it again; they are not stored
+            const int u = tid + 256 * i, r = u / (kChunk / 8), tile = min(tile0 + r / 16, tiles - 1), part = tile / per_part;
+            A[i] = (const char*)(p.a[part] + ((int64_t)a * p.rank + min(tile % per_part * 16 + r % 16, p.rank - 1)) * p.K) + 16 * (u % (kChunk / 8));
+        }
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) t[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int s = wave; s < steps; s += 4) {
-            const int k = 32 * s;
-            bf16x8 xp[3];
-            float d = 1.f;
-            if constexpr (X == kXQ8) {
-                const u32x2 w = *(const u32x2*)((const char*)p.x + row * p.K + k + 8 * g);
-                const u32x2 lo = codes_bf16(w[0]), hi = codes_bf16(w[1]);
-                xp[0] = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
-                d = p.xd[row * steps + s];
-            } else if constexpr (X == kXF32) {
-                const float* x = (const float*)p.x + row * p.ldx + k + 8 * g;
-                parts_of(*(const f32x4*)x, *(const f32x4*)(x + 4), xp);
-            } else {
-                xp[0] = __builtin_bit_cast(bf16x8, *(const u32x4*)((const uint16_t*)p.x + row * p.ldx + k + 8 * g));
+        for (int i = 0; i < NX; ++i) {
+            const int u = tid + 256 * i, r = u / (U * kChunk / 16);
+            Xp[i] = (const char*)p.x + (int64_t)rows[min(r, n - 1)] * (X == kXQ8 ? p.K : p.ldx) * U + 16 * (u % (U * kChunk / 16));
+        }
+        const int dr = tid / (kChunk / 32), ds = tid % (kChunk / 32);
+        const float* D = X == kXQ8 ? p.xd + (int64_t)rows[min(dr, n - 1)] * (p.K / 32) : nullptr;
+        u32x4 wa[NA], wx[NX];
+        float wd = 0.f;
+        const u32x4 zero = {0, 0, 0, 0};
+        auto load = [&](int ch) {  // what lies past K counts nothing
+            const int k0 = ch * kChunk;
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                const bool in = k0 + (tid + 256 * i) % (kChunk / 8) * 8 < p.K;
+                wa[i] = in ? *(const u32x4*)(A[i] + 2 * k0) : zero;
             }
 #pragma unroll
-            for (int i = 0; i < TILES; ++i) {
-                const bf16x8 w = __builtin_bit_cast(bf16x8, *(const u32x4*)(A[i] + k));
-                if constexpr (X == kXQ8) {
-                    t[i] += mfma16(w, xp[0], f32x4{0.f, 0.f, 0.f, 0.f}) * d;
-                } else {
+            for (int i = 0; i < NX; ++i) {
+                const bool in = k0 + (tid + 256 * i) % (U * kChunk / 16) * 16 / U < p.K;
+                wx[i] = in ? *(const u32x4*)(Xp[i] + (int64_t)U * k0) : zero;
+            }
+            if (X == kXQ8 && dr < M) wd = k0 + 32 * ds < p.K ? D[k0 / 32 + ds] : 0.f;
+        };
+        f32x4 t[RT][TILES];
 #pragma unroll
-                    for (int q = X == kXF32 ? 2 : 0; q >= 0; --q) t[i] = mfma16(w, xp[q], t[i]);
+        for (int h = 0; h < RT; ++h)
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) t[h][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        load(c0);
+        for (int ch = c0; ch < c1; ++ch) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                const int u = tid + 256 * i;
+                *(u32x4*)(s_a + u / (kChunk / 8) * PA + u % (kChunk / 8) * 16) = wa[i];
+            }
+#pragma unroll
+            for (int i = 0; i < NX; ++i) {
+                const int u = tid + 256 * i;
+                *(u32x4*)(s_x + u / (U * kChunk / 16) * PX + u % (U * kChunk / 16) * 16) = wx[i];
+            }
+            if (X == kXQ8 && dr < M) s_d[dr][ds] = wd;
+            __syncthreads();
+            if (ch + 1 < c1) load(ch + 1);
+#pragma unroll
+            for (int s = 0; s < kChunk / 128; ++s) {
+                const int step = 4 * s + wave;
+                bf16x8 xp[RT][3];
+                float d[RT];
+#pragma unroll
+                for (int h = 0; h < RT; ++h) {
+                    const char* v = s_x + (16 * h + c) * PX + (32 * step + 8 * g) * U;
+                    if constexpr (X == kXQ8) {
+                        const u32x2 q = *(const u32x2*)v;
+                        const u32x2 lo = codes_bf16(q[0]), hi = codes_bf16(q[1]);
+                        xp[h][0] = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+                        d[h] = s_d[16 * h + c][step];
+                    } else if constexpr (X == kXF32) {
+                        parts_of(*(const f32x4*)v, *(const f32x4*)(v + 16), xp[h]);
+                    } else {
+                        xp[h][0] = __builtin_bit_cast(bf16x8, *(const u32x4*)v);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) {
+                    const bf16x8 w = __builtin_bit_cast(bf16x8, *(const u32x4*)(s_a + (16 * i + c) * PA + (32 * step + 8 * g) * 2));
+#pragma unroll
+                    for (int h = 0; h < RT; ++h) {
+                        if constexpr (X == kXQ8) {
+                            t[h][i] += mfma16(w, xp[h][0], f32x4{0.f, 0.f, 0.f, 0.f}) * d[h];
+                        } else {
+#pragma unroll
+                            for (int q = X == kXF32 ? 2 : 0; q >= 0; --q) t[h][i] = mfma16(w, xp[h][q], t[h][i]);
+                        }
+                    }
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) *(f32x4*)&s_t[wave][c][16 * i + 4 * g] = t[i];
         __syncthreads();
-        const float scale = p.scale ? p.scale[a] : 1.f;
-        for (int e = tid; e < n * nj; e += 256) {
-            const int r = e / nj, j = e % nj;
-            const float v = (s_t[0][r][j] + s_t[1][r][j]) + (s_t[2][r][j] + s_t[3][r][j]);
-            p.t[((int64_t)rows[r] * p.n_parts + part) * p.rank + j0 + j] = v * scale;
+        float* sums = (float*)s_stage;  // [4][M][PT]
+#pragma unroll
+        for (int h = 0; h < RT; ++h)
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) *(f32x4*)(sums + (wave * M + 16 * h + c) * PT + 16 * i + 4 * g) = t[h][i];
+        __syncthreads();
+        for (int e = tid; e < n * 16 * TILES; e += 256) {
+            const int r = e / (16 * TILES), j = e % (16 * TILES), tile = tile0 + j / 16, rank = tile % per_part * 16 + j % 16;
+            if (tile >= tiles || rank >= p.rank) continue;
+            const float* v = sums + r * PT + j;
+            p.t[(((int64_t)blockIdx.z * p.rows + rows[r]) * p.n_parts + tile / per_part) * p.rank + rank] =
+                (v[0] + v[M * PT]) + (v[2 * M * PT] + v[3 * M * PT]);
         }
         __syncthreads();
     });
 }
 
-// y: a wave has kUpTiles tiles of 16 outputs of one part
+// y: 16 RT rows and p.turns runs of kRun outputs of one part; ranks in R steps of 32
+template <int R, int RT>
 __global__ void __launch_bounds__(256) k_lora_up(LoraP p) {
-    __shared__ int s_rows[kGather], s_n;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    constexpr int M = 16 * RT, PP = 64 * R + 16, PY = kRun + 4, NR = M / 4;
+    __shared__ __attribute__((aligned(16))) char s_p[3][M * PP];  // t's bf16 parts
+    __shared__ __attribute__((aligned(16))) float s_y[M * PY];
+    __shared__ int s_rows[RT == 1 ? kGather : M], s_n;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     int part = 0;
     while (part + 1 < p.n_parts && (int)blockIdx.y >= p.chunk0[part + 1]) ++part;
-    const int n0 = (((int)blockIdx.y - p.chunk0[part]) * 4 + wave) * 16 * kUpTiles, N = p.N[part];
+    const int N = p.N[part], n0 = ((int)blockIdx.y - p.chunk0[part]) * p.turns * kRun, n1 = min(N, n0 + p.turns * kRun);
     const float* base = p.base[part];
     float* y = p.y[part];
-    each_adapter(p, s_rows, &s_n, [&](int a, const int* rows, int n) {
+    each_adapter<RT>(p, s_rows, &s_n, [&](int a, const int* rows, int n) {
         if (a < 0 && base == y) return;
-        const bool live = c < n;
-        const int64_t row = rows[min(c, n - 1)];
-        f32x4 acc[kUpTiles];
+        // wave w has rows w, w + 4, .. of base and y
+        const float* from[NR];
+        float* to[NR];
 #pragma unroll
-        for (int i = 0; i < kUpTiles; ++i) {
-            acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            const int o = n0 + 16 * i + 4 * g;
-            if (base && live && o < N) acc[i] = *(const f32x4*)(base + row * p.ldbase[part] + o);
+        for (int i = 0; i < NR; ++i) {
+            const int64_t row = rows[min(wave + 4 * i, n - 1)];
+            from[i] = base + row * p.ldbase[part] + 4 * lane;
+            to[i] = y + row * p.ldy[part] + 4 * lane;
         }
+        const uint16_t* B = p.b[part];
         if (a >= 0) {
-            const float* t = p.t + (row * p.n_parts + part) * p.rank;
-            const uint16_t* B = p.b[part] + (int64_t)a * N * p.rank;
-            for (int k = 8 * g; k < (p.rank + 31 & ~31); k += 32) {
-                const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                bf16x8 tp[3];
-                parts_of(k < p.rank ? *(const f32x4*)(t + k) : zero, k < p.rank ? *(const f32x4*)(t + k + 4) : zero, tp);
+            B += (int64_t)a * N * p.rank;
+            const float scale = p.scale ? p.scale[a] : 1.f;
+            const int64_t piece = (int64_t)p.rows * p.n_parts * p.rank;
+            for (int e = tid; e < M * 4 * R; e += 256) {
+                const int r = e / (4 * R), k = e % (4 * R) * 8;
+                const float* t = p.t + ((int64_t)rows[min(r, n - 1)] * p.n_parts + part) * p.rank + min(k, p.rank - 8);
+                f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo, u[kPieces], v[kPieces];
 #pragma unroll
-                for (int i = 0; i < kUpTiles; ++i) {
-                    const int o = n0 + 16 * i + c;
-                    const u32x4 w = k < p.rank && o < N ? *(const u32x4*)(B + (int64_t)o * p.rank + k) : u32x4{0, 0, 0, 0};
+                for (int z = 0; z < kPieces; ++z)
+                    if (z < p.pieces) {
+                        u[z] = *(const f32x4*)(t + z * piece);
+                        v[z] = *(const f32x4*)(t + z * piece + 4);
+                    }
 #pragma unroll
-                    for (int q = 2; q >= 0; --q) acc[i] = mfma16(__builtin_bit_cast(bf16x8, w), tp[q], acc[i]);
-                }
+                for (int z = 0; z < kPieces; ++z)
+                    if (z < p.pieces) {
+                        lo += u[z];
+                        hi += v[z];
+                    }
+                if (k >= p.rank) lo = hi = f32x4{0.f, 0.f, 0.f, 0.f};
+                bf16x8 parts[3];
+                parts_of(lo * scale, hi * scale, parts);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) *(bf16x8*)(s_p[q] + r * PP + 2 * k) = parts[q];
             }
+            __syncthreads();
         }
+        for (int o0 = n0; o0 < n1; o0 += kRun) {
+            const bool in = o0 + 4 * lane < N;
+            f32x4 yb[NR];
 #pragma unroll
-        for (int i = 0; i < kUpTiles; ++i) {
-            const int o = n0 + 16 * i + 4 * g;
-            if (live && o < N) *(f32x4*)(y + row * p.ldy[part] + o) = acc[i];
+            for (int i = 0; i < NR; ++i) {
+                yb[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (base && in && wave + 4 * i < n) yb[i] = *(const f32x4*)(from[i] + o0);
+            }
+            if (a >= 0) {
+                f32x4 acc[RT][4];
+#pragma unroll
+                for (int h = 0; h < RT; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[h][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const int k = 32 * r + 8 * g;
+                    u32x4 w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int o = o0 + 64 * wave + 16 * i + c;
+                        w[i] = k < p.rank && o < N ? *(const u32x4*)(B + (int64_t)o * p.rank + k) : u32x4{0, 0, 0, 0};
+                    }
+#pragma unroll
+                    for (int h = 0; h < RT; ++h)
+#pragma unroll
+                        for (int q = 2; q >= 0; --q) {
+                            const bf16x8 tp = *(const bf16x8*)(s_p[q] + (16 * h + c) * PP + 2 * k);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[h][i] = mfma16(__builtin_bit_cast(bf16x8, w[i]), tp, acc[h][i]);
+                        }
+                }
+#pragma unroll
+                for (int h = 0; h < RT; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) *(f32x4*)(s_y + (16 * h + c) * PY + 64 * wave + 16 * i + 4 * g) = acc[h][i];
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < NR; ++i) yb[i] += *(const f32x4*)(s_y + (wave + 4 * i) * PY + 4 * lane);
+            }
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+                if (in && wave + 4 * i < n) *(f32x4*)(to[i] + o0) = yb[i];
+            if (a >= 0) __syncthreads();
         }
     });
 }
-template <int X>
+
+template <int X, int RT>
 void launch_down(const LoraP& p, int tiles, dim3 grid, hipStream_t st) {
     switch (tiles) {
-        case 1: launch_kernel((k_lora_down<X, 1>), grid, dim3(256), 0, st, p); break;
-        case 2: launch_kernel((k_lora_down<X, 2>), grid, dim3(256), 0, st, p); break;
-        case 3: launch_kernel((k_lora_down<X, 3>), grid, dim3(256), 0, st, p); break;
-        default: launch_kernel((k_lora_down<X, 4>), grid, dim3(256), 0, st, p);
+        case 1: launch_kernel((k_lora_down<X, 1, RT>), grid, dim3(256), 0, st, p); break;
+        case 2: launch_kernel((k_lora_down<X, 2, RT>), grid, dim3(256), 0, st, p); break;
+        case 3: launch_kernel((k_lora_down<X, 3, RT>), grid, dim3(256), 0, st, p); break;
+        default: launch_kernel((k_lora_down<X, 4, RT>), grid, dim3(256), 0, st, p);
     }
+}
+template <int RT>
+hipError_t launch_of(const LoraP& p, int x_type, int tiles, dim3 down, dim3 up, hipStream_t st) {
+    switch (x_type) {
+        case BQ_TYPE_Q8_0: launch_down<kXQ8, RT>(p, tiles, down, st); break;
+        case BQ_TYPE_F32: launch_down<kXF32, RT>(p, tiles, down, st); break;
+        default: launch_down<kXBf16, RT>(p, tiles, down, st);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (p.rank <= 32) launch_kernel((k_lora_up<1, RT>), up, dim3(256), 0, st, p);
+    else if (p.rank <= 64) launch_kernel((k_lora_up<2, RT>), up, dim3(256), 0, st, p);
+    else if (p.rank <= 128) launch_kernel((k_lora_up<4, RT>), up, dim3(256), 0, st, p);
+    else launch_kernel((k_lora_up<8, RT>), up, dim3(256), 0, st, p);
+    return hipGetLastError();
+}
+
+int groups_of(int rows) { return rows <= kGather ? rows : (rows + 31) / 32; }
+// pieces of K: as many as fill two workgroups a CU, a chunk each at least
+int pieces_of(int rows, int rank, int n_parts, int K) {
+    const int64_t wgs = (int64_t)groups_of(rows) * ((n_parts * ((rank + 15) / 16) + kRankTiles - 1) / kRankTiles);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({((int64_t)K + kChunk - 1) / kChunk, 512 / wgs, kPieces}));
 }
 }  // namespace
 
-size_t lora_work_bytes(int rows, int rank, int n_parts) { return (size_t)rows * n_parts * rank * sizeof(float); }
+size_t lora_work_bytes(int rows, int rank, int n_parts) {
+    return (size_t)rows * n_parts * rank * pieces_of(rows, rank, n_parts, 1 << 20) * sizeof(float);
+}
 
 hipError_t launch_lora(const bq_lora_args& a, hipStream_t st) {
     LoraP p;
     p.x = a.x; p.xd = a.xd; p.ldx = a.ldx; p.adapter = a.adapter; p.scale = a.scale;
     p.n_parts = a.n_parts; p.rows = a.rows; p.K = a.K; p.rank = a.rank; p.n_adapters = a.n_adapters; p.t = (float*)a.work;
+    p.pieces = pieces_of(a.rows, a.rank, a.n_parts, a.K);
+    const int groups = groups_of(a.rows);
+    int64_t runs = 0;
+    for (int i = 0; i < a.n_parts; ++i) runs += (a.parts[i].N + kRun - 1) / kRun;
+    p.turns = groups * runs >= 4096 ? 4 : 1;
     int chunks = 0;
     for (int i = 0; i < a.n_parts; ++i) {
         const bq_lora_part& q = a.parts[i];
         p.a[i] = q.a; p.b[i] = q.b; p.base[i] = q.base; p.y[i] = q.y; p.ldbase[i] = q.ldbase; p.ldy[i] = q.ldy; p.N[i] = q.N;
         p.chunk0[i] = chunks;
-        chunks += (q.N + 64 * kUpTiles - 1) / (64 * kUpTiles);
+        chunks += (q.N + kRun * p.turns - 1) / (kRun * p.turns);
     }
-    const uint32_t groups = a.rows <= kGather ? a.rows : (a.rows + 15) / 16;
-    const int tiles = std::min((a.rank + 15) / 16, kRankTiles);
-    const dim3 down(groups, a.n_parts * ((a.rank + 16 * tiles - 1) / (16 * tiles)));
-    switch (a.x_type) {
-        case BQ_TYPE_Q8_0: launch_down<kXQ8>(p, tiles, down, st); break;
-        case BQ_TYPE_F32: launch_down<kXF32>(p, tiles, down, st); break;
-        default: launch_down<kXBf16>(p, tiles, down, st);
-    }
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    launch_kernel(k_lora_up, dim3(groups, chunks), dim3(256), 0, st, p);
-    return hipGetLastError();
+    const int tiles = a.n_parts * ((a.rank + 15) / 16), per = std::min(tiles, kRankTiles);
+    const dim3 down(groups, (tiles + per - 1) / per, p.pieces), up(groups, chunks);
+    return a.rows <= kGather ? launch_of<1>(p, a.x_type, per, down, up, st) : launch_of<2>(p, a.x_type, per, down, up, st);
 }
 
 }  // namespace bq
