@@ -10,10 +10,8 @@
 // group of a q8 row is one MFMA of its codes, scaled in fp32; fp32 rows and t are the
 // sum of three bf16 parts (all 24 bits), an MFMA each.
 //
-// Rows of one adapter are found by each workgroup itself: of up to kGather rows the
-// first that has an adapter takes all that share it, from anywhere in the batch (a
-// decode step's rows), 16 at a time; of more, a workgroup takes 32 neighbours and their
-// adapters one after the other (prompts: nearly always one).
+// Rows of one adapter are found by each workgroup itself, 16 or 32 at a time, wherever
+// in the batch (or in its window of 256 rows) they stand: see each_adapter.
 //
 // All of x, A, base and y is moved a row at a time, 256 to 1024 contiguous bytes, and
 // turned into operands or out of results in LDS: rows are often a multiple of 4 KiB
@@ -26,7 +24,7 @@
 namespace bq {
 
 namespace {
-constexpr int kGather = 256;
+constexpr int kWindow = 256;   // rows among which those of one adapter are brought together
 constexpr int kRankTiles = 4;  // 16-rank tiles of a workgroup of k_lora_down at most
 constexpr int kChunk = 256;    // values of K that it stages at once
 constexpr int kPieces = 8;     // pieces that K is cut into at most
@@ -47,7 +45,7 @@ struct LoraP {
     int64_t ldbase[kMaxParts], ldy[kMaxParts];
     int N[kMaxParts], chunk0[kMaxParts];  // first output chunk of a part
     int n_parts, rows, K, rank, n_adapters;
-    int pieces, turns;  // of K; runs of kRun outputs that a workgroup of k_lora_up takes
+    int slots, pieces, turns;  // workgroups of a window; of K; runs of kRun outputs that a workgroup of k_lora_up takes
     float* t;           // [pieces][rows][n_parts][rank]
 };
 
@@ -61,38 +59,69 @@ BQ_DEV int adapter_of(const LoraP& p, int r) {
 
 // Calls f(adapter, rows, n) for this workgroup's rows, n <= 16 RT of one adapter at a
 // time (rows in LDS).  All of the workgroup's lanes take part; f may hold barriers.
+//   RT 1, a batch of at most kWindow rows, a workgroup per row: the 16 i-th row of an
+//     adapter has that one and the next 15; the other rows' workgroups have none.
+//   RT 2, p.slots workgroups per window: the window's adapters in the order of their
+//     first rows, 32 rows at a time, are dealt to them in turn (a prompt's window has 8
+//     such runs, and one more for each border between two adapters).
 template <int RT, typename F>
-BQ_DEV void each_adapter(const LoraP& p, int* s_rows, int* s_n, F f) {
+BQ_DEV void each_adapter(const LoraP& p, int group, int* s_rows, F f) {
+    constexpr int M = 16 * RT, Q = kWindow / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if constexpr (RT == 1) {  // at most kGather rows
-        const int me = blockIdx.x, a = adapter_of(p, me);
-        if (wave == 0) {
-            int n = 0;
-            for (int r0 = 0; r0 < p.rows; r0 += 64) {
-                const int r = r0 + lane;
-                const uint64_t same = __ballot(r < p.rows && adapter_of(p, min(r, p.rows - 1)) == a);
-                if (same >> lane & 1) s_rows[n + __builtin_popcountll(same & ((1ull << lane) - 1))] = r;
-                n += __builtin_popcountll(same);
-            }
-            if (lane == 0) *s_n = n;
+    auto below = [](uint64_t mask, int l) { return (int)__builtin_popcountll(mask & ((1ull << l) - 1)); };
+    const int r0 = RT == 1 ? 0 : group / p.slots * kWindow;
+    int a[Q];
+    uint64_t left[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int r = r0 + 64 * q + lane;
+        a[q] = r < p.rows ? adapter_of(p, r) : -1;
+        left[q] = __ballot(r < p.rows);
+    }
+    // the rows of an adapter from its first-th on to LDS; how many
+    auto take = [&](const uint64_t (&same)[Q], int first) {
+        int at = -first;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const int i = at + below(same[q], lane);
+            if (wave == 0 && (same[q] >> lane & 1) && i >= 0 && i < M) s_rows[i] = r0 + 64 * q + lane;
+            at += __builtin_popcountll(same[q]);
         }
         __syncthreads();
-        if (s_rows[0] != me) return;
-        const int n = *s_n;
-        for (int i = 0; i < n; i += 16) f(a, s_rows + i, min(16, n - i));
+        return min(at, M);
+    };
+    uint64_t same[Q];
+    if constexpr (RT == 1) {
+        const int one = __builtin_amdgcn_readfirstlane(adapter_of(p, group));
+        int rank = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            same[q] = __ballot(a[q] == one) & left[q];
+            rank += group >= 64 * q + 64 ? (int)__builtin_popcountll(same[q]) : group >= 64 * q ? below(same[q], group - 64 * q) : 0;
+        }
+        if (rank % M) return;
+        const int n = take(same, rank);
+        f(one, n);
     } else {
-        constexpr int T = 16 * RT;
-        static_assert(T <= 64, "");
-        const int r0 = blockIdx.x * T, n = min(T, p.rows - r0), a = adapter_of(p, r0 + min(lane, n - 1));
-        uint64_t left = ~0ull >> (64 - n);
-        while (left) {
-            const int one = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
-            const uint64_t same = __ballot(a == one) & left;
-            left &= ~same;
-            if (wave == 0 && (same >> lane & 1)) s_rows[__builtin_popcountll(same & ((1ull << lane) - 1))] = r0 + lane;
-            __syncthreads();
-            f(one, s_rows, __builtin_popcountll(same));
-            __syncthreads();
+        int slot = group % p.slots, seen = 0;
+        while (left[0] | left[1] | left[2] | left[3]) {
+            int one = 0, count = 0;
+#pragma unroll
+            for (int q = Q - 1; q >= 0; --q)
+                if (left[q]) one = __builtin_amdgcn_readlane(a[q], __builtin_ctzll(left[q]));
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                same[q] = __ballot(a[q] == one) & left[q];
+                left[q] &= ~same[q];
+                count += __builtin_popcountll(same[q]);
+            }
+            const int runs = (count + M - 1) / M;
+            for (; slot < seen + runs; slot += p.slots) {
+                const int n = take(same, (slot - seen) * M);
+                f(one, n);
+                __syncthreads();
+            }
+            seen += runs;
         }
     }
 }
@@ -134,14 +163,14 @@ __global__ void __launch_bounds__(256) k_lora_down(LoraP p) {
     constexpr int kStage = 16 * TILES * PA + M * PX, kSums = 4 * M * PT * 4;
     __shared__ __attribute__((aligned(16))) char s_stage[kStage > kSums ? kStage : kSums];
     __shared__ float s_d[M][kChunk / 32 + 1];  // q8: the groups' scales
-    __shared__ int s_rows[RT == 1 ? kGather : M], s_n;
+    __shared__ int s_rows[M];
     char* s_a = s_stage;
     char* s_x = s_stage + 16 * TILES * PA;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const int per_part = (p.rank + 15) / 16, tiles = per_part * p.n_parts, tile0 = blockIdx.y * TILES;
     const int chunks = (p.K + kChunk - 1) / kChunk;
     const int c0 = chunks * blockIdx.z / p.pieces, c1 = chunks * (blockIdx.z + 1) / p.pieces;
-    each_adapter<RT>(p, s_rows, &s_n, [&](int a, const int* rows, int n) {
+    each_adapter<RT>(p, blockIdx.x, s_rows, [&](int a, int n) {
         if (a < 0) return;
         const char* A[NA];
         const char* Xp[NX];
@@ -153,10 +182,10 @@ __global__ void __launch_bounds__(256) k_lora_down(LoraP p) {
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
             const int u = tid + 256 * i, r = u / (U * kChunk / 16);
-            Xp[i] = (const char*)p.x + (int64_t)rows[min(r, n - 1)] * (X == kXQ8 ? p.K : p.ldx) * U + 16 * (u % (U * kChunk / 16));
+            Xp[i] = (const char*)p.x + (int64_t)s_rows[min(r, n - 1)] * (X == kXQ8 ? p.K : p.ldx) * U + 16 * (u % (U * kChunk / 16));
         }
         const int dr = tid / (kChunk / 32), ds = tid % (kChunk / 32);
-        const float* D = X == kXQ8 ? p.xd + (int64_t)rows[min(dr, n - 1)] * (p.K / 32) : nullptr;
+        const float* D = X == kXQ8 ? p.xd + (int64_t)s_rows[min(dr, n - 1)] * (p.K / 32) : nullptr;
         u32x4 wa[NA], wx[NX];
         float wd = 0.f;
         const u32x4 zero = {0, 0, 0, 0};
@@ -240,7 +269,7 @@ __global__ void __launch_bounds__(256) k_lora_down(LoraP p) {
             const int r = e / (16 * TILES), j = e % (16 * TILES), tile = tile0 + j / 16, rank = tile % per_part * 16 + j % 16;
             if (tile >= tiles || rank >= p.rank) continue;
             const float* v = sums + r * PT + j;
-            p.t[(((int64_t)blockIdx.z * p.rows + rows[r]) * p.n_parts + tile / per_part) * p.rank + rank] =
+            p.t[(((int64_t)blockIdx.z * p.rows + s_rows[r]) * p.n_parts + tile / per_part) * p.rank + rank] =
                 (v[0] + v[M * PT]) + (v[2 * M * PT] + v[3 * M * PT]);
         }
         __syncthreads();
@@ -249,28 +278,33 @@ __global__ void __launch_bounds__(256) k_lora_down(LoraP p) {
 
 // y: 16 RT rows and p.turns runs of kRun outputs of one part; ranks in R steps of 32
 template <int R, int RT>
-__global__ void __launch_bounds__(256) k_lora_up(LoraP p) {
+__global__ void __launch_bounds__(256, R <= 2 ? 3 : 2) k_lora_up(LoraP p) {
     constexpr int M = 16 * RT, PP = 64 * R + 16, PY = kRun + 4, NR = M / 4;
     __shared__ __attribute__((aligned(16))) char s_p[3][M * PP];  // t's bf16 parts
     __shared__ __attribute__((aligned(16))) float s_y[M * PY];
-    __shared__ int s_rows[RT == 1 ? kGather : M], s_n;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    __shared__ int s_rows[M];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     int part = 0;
-    while (part + 1 < p.n_parts && (int)blockIdx.y >= p.chunk0[part + 1]) ++part;
-    const int N = p.N[part], n0 = ((int)blockIdx.y - p.chunk0[part]) * p.turns * kRun, n1 = min(N, n0 + p.turns * kRun);
+    while (part + 1 < p.n_parts && (int)blockIdx.x >= p.chunk0[part + 1]) ++part;
+    const int N = p.N[part], n0 = ((int)blockIdx.x - p.chunk0[part]) * p.turns * kRun, n1 = min(N, n0 + p.turns * kRun);
     const float* base = p.base[part];
     float* y = p.y[part];
-    each_adapter<RT>(p, s_rows, &s_n, [&](int a, const int* rows, int n) {
+    const int64_t ldbase = p.ldbase[part], ldy = p.ldy[part];
+    each_adapter<RT>(p, blockIdx.y, s_rows, [&](int a, int n) {
         if (a < 0 && base == y) return;
         // wave w has rows w, w + 4, .. of base and y
-        const float* from[NR];
-        float* to[NR];
+        int row[NR];
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            const int64_t row = rows[min(wave + 4 * i, n - 1)];
-            from[i] = base + row * p.ldbase[part] + 4 * lane;
-            to[i] = y + row * p.ldy[part] + 4 * lane;
-        }
+        for (int i = 0; i < NR; ++i) row[i] = __builtin_amdgcn_readfirstlane(s_rows[min(wave + 4 * i, n - 1)]);
+        f32x4 yb[NR];
+        auto fetch = [&](int o0) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                yb[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (base && o0 + 4 * lane < N && wave + 4 * i < n) yb[i] = *(const f32x4*)(base + row[i] * ldbase + o0 + 4 * lane);
+            }
+        };
+        fetch(n0);
         const uint16_t* B = p.b[part];
         if (a >= 0) {
             B += (int64_t)a * N * p.rank;
@@ -278,20 +312,13 @@ __global__ void __launch_bounds__(256) k_lora_up(LoraP p) {
             const int64_t piece = (int64_t)p.rows * p.n_parts * p.rank;
             for (int e = tid; e < M * 4 * R; e += 256) {
                 const int r = e / (4 * R), k = e % (4 * R) * 8;
-                const float* t = p.t + ((int64_t)rows[min(r, n - 1)] * p.n_parts + part) * p.rank + min(k, p.rank - 8);
-                f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo, u[kPieces], v[kPieces];
-#pragma unroll
-                for (int z = 0; z < kPieces; ++z)
-                    if (z < p.pieces) {
-                        u[z] = *(const f32x4*)(t + z * piece);
-                        v[z] = *(const f32x4*)(t + z * piece + 4);
-                    }
-#pragma unroll
-                for (int z = 0; z < kPieces; ++z)
-                    if (z < p.pieces) {
-                        lo += u[z];
-                        hi += v[z];
-                    }
+                const float* t = p.t + ((int64_t)s_rows[min(r, n - 1)] * p.n_parts + part) * p.rank + min(k, p.rank - 8);
+                f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll 4
+                for (int z = 0; z < p.pieces; ++z) {
+                    lo += *(const f32x4*)(t + z * piece);
+                    hi += *(const f32x4*)(t + z * piece + 4);
+                }
                 if (k >= p.rank) lo = hi = f32x4{0.f, 0.f, 0.f, 0.f};
                 bf16x8 parts[3];
                 parts_of(lo * scale, hi * scale, parts);
@@ -302,12 +329,7 @@ __global__ void __launch_bounds__(256) k_lora_up(LoraP p) {
         }
         for (int o0 = n0; o0 < n1; o0 += kRun) {
             const bool in = o0 + 4 * lane < N;
-            f32x4 yb[NR];
-#pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                yb[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (base && in && wave + 4 * i < n) yb[i] = *(const f32x4*)(from[i] + o0);
-            }
+            if (o0 > n0) fetch(o0);
             if (a >= 0) {
                 f32x4 acc[RT][4];
 #pragma unroll
@@ -342,7 +364,7 @@ __global__ void __launch_bounds__(256) k_lora_up(LoraP p) {
             }
 #pragma unroll
             for (int i = 0; i < NR; ++i)
-                if (in && wave + 4 * i < n) *(f32x4*)(to[i] + o0) = yb[i];
+                if (in && wave + 4 * i < n) *(f32x4*)(y + row[i] * ldy + o0 + 4 * lane) = yb[i];
             if (a >= 0) __syncthreads();
         }
     });
@@ -373,11 +395,15 @@ hipError_t launch_of(const LoraP& p, int x_type, int tiles, dim3 down, dim3 up, 
     return hipGetLastError();
 }
 
-int groups_of(int rows) { return rows <= kGather ? rows : (rows + 31) / 32; }
-// pieces of K: as many as fill two workgroups a CU, a chunk each at least
+// Workgroups of a window, where the batch has several.  More than a prompt's 8 runs cost
+// what idle ones do (4096 rows 112 us with 12, 118 with 16), fewer make one workgroup take
+// several runs in a row (512 rows of 64 adapters 65 us with 16, 81 with 12)
+int slots_of(int rows) { return rows <= 2048 ? 16 : 12; }
+int groups_of(int rows) { return rows <= kWindow ? rows : (rows + kWindow - 1) / kWindow * slots_of(rows); }
+// pieces of K: as many as fill a workgroup a CU, a chunk each at least
 int pieces_of(int rows, int rank, int n_parts, int K) {
-    const int64_t wgs = (int64_t)groups_of(rows) * ((n_parts * ((rank + 15) / 16) + kRankTiles - 1) / kRankTiles);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({((int64_t)K + kChunk - 1) / kChunk, 512 / wgs, kPieces}));
+    const int64_t wgs = (int64_t)(rows <= kWindow ? rows : (rows + 31) / 32) * ((n_parts * ((rank + 15) / 16) + kRankTiles - 1) / kRankTiles);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({((int64_t)K + kChunk - 1) / kChunk, 256 / wgs, kPieces}));
 }
 }  // namespace
 
@@ -389,11 +415,12 @@ hipError_t launch_lora(const bq_lora_args& a, hipStream_t st) {
     LoraP p;
     p.x = a.x; p.xd = a.xd; p.ldx = a.ldx; p.adapter = a.adapter; p.scale = a.scale;
     p.n_parts = a.n_parts; p.rows = a.rows; p.K = a.K; p.rank = a.rank; p.n_adapters = a.n_adapters; p.t = (float*)a.work;
+    p.slots = slots_of(a.rows);
     p.pieces = pieces_of(a.rows, a.rank, a.n_parts, a.K);
     const int groups = groups_of(a.rows);
     int64_t runs = 0;
     for (int i = 0; i < a.n_parts; ++i) runs += (a.parts[i].N + kRun - 1) / kRun;
-    p.turns = groups * runs >= 4096 ? 4 : 1;
+    p.turns = groups * runs >= 4096 ? 2 : 1;
     int chunks = 0;
     for (int i = 0; i < a.n_parts; ++i) {
         const bq_lora_part& q = a.parts[i];
@@ -402,8 +429,8 @@ hipError_t launch_lora(const bq_lora_args& a, hipStream_t st) {
         chunks += (q.N + kRun * p.turns - 1) / (kRun * p.turns);
     }
     const int tiles = a.n_parts * ((a.rank + 15) / 16), per = std::min(tiles, kRankTiles);
-    const dim3 down(groups, (tiles + per - 1) / per, p.pieces), up(groups, chunks);
-    return a.rows <= kGather ? launch_of<1>(p, a.x_type, per, down, up, st) : launch_of<2>(p, a.x_type, per, down, up, st);
+    const dim3 down(groups, (tiles + per - 1) / per, p.pieces), up(chunks, groups);
+    return a.rows <= kWindow ? launch_of<1>(p, a.x_type, per, down, up, st) : launch_of<2>(p, a.x_type, per, down, up, st);
 }
 
 }  // namespace bq
