@@ -28,54 +28,64 @@ struct SharedP {
     int n_groups, max_prefix;
     int rows, n_rows, q_heads, G, max_len, window, sinks, q_bf16, out_bf16;
     int ptiles, psplit, ttiles, tsplit;  // row tiles per head and pieces: of the prefixes, of a sequence's own tokens
+    int punits;       // workgroups of the prefixes
     float scale;      // scale * log2(e)
 };
 
 BQ_DEV int length_of(const SharedP& p, int seq) {
     return min(max(p.kv_len[seq], 0), min(p.max_len, p.kv.max_pages << p.kv.plog));
 }
-BQ_DEV int prefix_of(const SharedP& p, int g) {
-    return min(max(p.prefix[g], 0), min(p.max_prefix, p.kv.max_pages << p.kv.plog));
+struct Group {
+    int s0, s1, prefix;  // its sequences [s0, s1), inside the batch whatever group0 holds, and shared tokens
+};
+BQ_DEV Group group_of(const SharedP& p, int g) {
+    Group r;
+    const int a = p.group0[g], b = p.group0[g + 1], n = p.prefix[g];
+    r.s0 = min(max(a, 0), p.kv.n_seq);
+    r.s1 = min(max(b, r.s0), p.kv.n_seq);
+    r.prefix = min(max(n, 0), min(p.max_prefix, p.kv.max_pages << p.kv.plog));
+    return r;
 }
-// sequences [s0, s1) of a group, inside the batch whatever group0 holds
-BQ_DEV void group_of(const SharedP& p, int g, int& s0, int& s1) {
-    s0 = min(max(p.group0[g], 0), p.kv.n_seq);
-    s1 = min(max(p.group0[g + 1], s0), p.kv.n_seq);
+BQ_DEV Group from_lane(const Group& g, int lane) {
+    return Group{__builtin_amdgcn_readlane(g.s0, lane), __builtin_amdgcn_readlane(g.s1, lane), __builtin_amdgcn_readlane(g.prefix, lane)};
 }
-// the group that holds a sequence, -1: none (the same in every lane of a wave)
-BQ_DEV int group_with(const SharedP& p, int seq) {
+// the group that holds a sequence (the same in every lane of a wave)
+BQ_DEV bool group_with(const SharedP& p, int seq, Group& found) {
     const int lane = threadIdx.x & 63;
     for (int g0 = 0; g0 < p.n_groups; g0 += 64) {
-        int s0 = 0, s1 = 0;
-        if (g0 + lane < p.n_groups) group_of(p, g0 + lane, s0, s1);
-        const uint64_t in = __ballot(seq >= s0 && seq < s1);
-        if (in) return g0 + __builtin_ctzll(in);
+        const Group g = g0 + lane < p.n_groups ? group_of(p, g0 + lane) : Group{0, 0, 0};
+        const uint64_t in = __ballot(seq >= g.s0 && seq < g.s1);
+        if (in) {
+            found = from_lane(g, __builtin_ctzll(in));
+            return true;
+        }
     }
-    return -1;
+    return false;
 }
 // the group whose row tiles (of T query rows) include the tile-th of all, and its
-// number among them; -1: there are fewer
+// number among them; false: there are fewer
 template <int T>
-BQ_DEV int tile_group(const SharedP& p, int& tile) {
+BQ_DEV bool tile_group(const SharedP& p, int& tile, Group& found) {
     const int lane = threadIdx.x & 63, per = p.rows * p.G;
     for (int g0 = 0; g0 < p.n_groups; g0 += 64) {
-        int s0 = 0, s1 = 0;
-        if (g0 + lane < p.n_groups) group_of(p, g0 + lane, s0, s1);
-        const int n = ((s1 - s0) * per + T - 1) / T;
+        const Group g = g0 + lane < p.n_groups ? group_of(p, g0 + lane) : Group{0, 0, 0};
+        const int n = ((g.s1 - g.s0) * per + T - 1) / T;
         int upto = n;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int below = __shfl_up(upto, d, 64);
-            if (lane >= d) upto += below;
-        }
+        if (p.n_groups > 1)
+            for (int d = 1; d < 64; d <<= 1) {
+                const int below = __shfl_up(upto, d, 64);
+                if (lane >= d) upto += below;
+            }
         const uint64_t past = __ballot(upto > tile);
         if (past) {
             const int at = __builtin_ctzll(past);
+            found = from_lane(g, at);
             tile -= __builtin_amdgcn_readlane(upto - n, at);
-            return g0 + at;
+            return true;
         }
         tile -= __builtin_amdgcn_readlane(upto, 63);
     }
-    return -1;
+    return false;
 }
 
 // the steps of tokens from .. upto - 1 that rows at positions pfirst..plast see
@@ -90,6 +100,17 @@ BQ_DEV Steps steps_of(const SharedP& p, int pfirst, int plast, int from, int upt
     return s;
 }
 
+// A workgroup's row tile, head and piece of the prefixes.  The tiles of one head and
+// piece read the same tokens: they follow each other on one XCD (workgroups are dealt to
+// the 8 XCDs in turn), whose L2 then holds them.
+BQ_DEV bool prefix_unit(const SharedP& p, int u, int& tile, int& h, int& split) {
+    const int at = u / (8 * p.ptiles) * 8 + u % 8;
+    tile = u / 8 % p.ptiles;
+    h = at % p.kv.heads;
+    split = at / p.kv.heads;
+    return split < p.psplit;
+}
+
 BQ_DEV void store4(const SharedP& p, size_t at, f32x4 a) {
     if (p.out_bf16)
         *(u32x2*)((uint16_t*)p.out + at) = u32x2{f2bf2(a[0], a[1]), f2bf2(a[2], a[3])};
@@ -97,69 +118,376 @@ BQ_DEV void store4(const SharedP& p, size_t at, f32x4 a) {
         *(f32x4*)((float*)p.out + at) = a;
 }
 
-// NQ parts of q, NP of a softmax weight
-template <int D, int KV, int NQ, int NP>
-__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_shared(SharedP p) {
-    constexpr int KS = D / 32, DT = D / 16;
-    constexpr bool CUT = true;
-    __shared__ int s_page[kRound * 2];
-    __shared__ __attribute__((aligned(16))) float s_o[kWaves][16][D + 4];
-    __shared__ float s_m[kWaves][16], s_l[kWaves][16], s_mt[16], s_lt[16];
+// 8 floats rounded to bf16, two to a word; what that leaves of them stays in x
+BQ_DEV u32x4 bf16_part(float (&x)[8]) {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        w[e] = f2bf2(x[2 * e], x[2 * e + 1]);
+        x[2 * e] -= as_float(w[e] << 16);
+        x[2 * e + 1] -= as_float(w[e] & 0xFFFF0000u);
+    }
+    return w;
+}
+
+// One workgroup's 16 QT query rows over a piece of their group's prefix.  As in
+// bq_attn_rows.inc a wave takes 32 tokens at a time; here it holds their K and V for QT
+// row tiles, whose queries wait in LDS.
+template <int D, int KV, int NQ, int NP, int QT>
+BQ_DEV void attend_prefix(const SharedP& p, char* lds, int* s_page, float (&s_m)[kWaves][16], float (&s_l)[kWaves][16], float (&s_scale)[16 * QT]) {
+    constexpr int KS = D / 32, DT = D / 16, M = 16 * QT, PQ = 2 * D + 16, L = D / 8;
+    constexpr bool Q8 = KV == kKvQ8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const KvView& kv = p.kv;
-    // the prefixes' workgroups first, then the sequences' own
-    int u = blockIdx.x, seq, h, tile, split, nsplit, from, upto, M, piece0;
-    const bool shared = u < p.ptiles * kv.heads * p.psplit;
-    if (shared) {
-        tile = u % p.ptiles;
-        h = u / p.ptiles % kv.heads;
-        split = u / (p.ptiles * kv.heads);
-        nsplit = p.psplit;
-        piece0 = 0;
-        const int gr = tile_group<16>(p, tile);
-        if (gr < 0) return;
-        int s1;
-        group_of(p, gr, seq, s1);
-        M = (s1 - seq) * p.rows * p.G;
-        from = 0;
-        upto = prefix_of(p, gr);
-        if (tile < 0 || tile > (M - 1) / 16) return;  // group0 is not what it should be
-    } else {
-        u -= p.ptiles * kv.heads * p.psplit;
-        split = u % p.tsplit;
-        u /= p.tsplit;
-        h = u % kv.heads;
-        tile = u / kv.heads % p.ttiles;
-        seq = u / (kv.heads * p.ttiles);
-        nsplit = p.tsplit;
-        piece0 = p.psplit;
-        M = p.rows * p.G;
-        const int gr = group_with(p, seq);
-        from = gr < 0 ? 0 : prefix_of(p, gr);
-        upto = 0x7FFFFFFF;
+    int tile, h, split;
+    if (!prefix_unit(p, blockIdx.x, tile, h, split)) return;
+    Group gr;
+    if (!tile_group<M>(p, tile, gr)) return;
+    const int seq = gr.s0, upto = gr.prefix, per_seq = p.rows * p.G, rows = (gr.s1 - gr.s0) * per_seq, tiles = (rows + M - 1) / M;
+    const int first = tile * M, last = min(rows, first + M) - 1;
+    if (tile < 0 || tile >= tiles) return;  // group0 is not what it should be
+
+    // the queries, L lanes a row, and the lanes' positions: these loads first
+    constexpr int NU = (M * L + 255) / 256;
+    u32x4 raw[NU][2];
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        const int u = min(tid + 256 * i, M * L - 1), row = u / L, d = u % L * 8, r = min(first + row, last);
+        const size_t at = (size_t)(seq * p.rows + r / p.G) * p.ldq + (size_t)(h * p.G + r % p.G) * D + d;
+        if (p.q_bf16) {
+            raw[i][0] = *(const u32x4*)((const uint16_t*)p.q + at);
+        } else {
+            raw[i][0] = *(const u32x4*)((const float*)p.q + at);
+            raw[i][1] = *(const u32x4*)((const float*)p.q + at + 4);
+        }
     }
-    // the lane's query row: of sequence seq + rs its new token i, head r % G of the group
-    const int first = tile * 16, last = min(M, first + 16) - 1, r = min(first + c, last);
-    const int rs = r / (p.rows * p.G), i = r / p.G % p.rows;
-    const int pos = length_of(p, seq + rs) - p.rows + i;
-    int pfirst = pos, plast = pos;
+    int pos[QT], pfirst = 0x7FFFFFFF, plast = -0x7FFFFFFF;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int r = min(first + 16 * t + c, last);
+        pos[t] = length_of(p, seq + r / per_seq) - p.rows + r / p.G % p.rows;
+        pfirst = min(pfirst, pos[t]);
+        plast = max(plast, pos[t]);
+    }
     for (int d = 1; d < 16; d <<= 1) {
         pfirst = min(pfirst, __shfl_xor(pfirst, d, 64));
         plast = max(plast, __shfl_xor(plast, d, 64));
     }
     pfirst = __builtin_amdgcn_readfirstlane(pfirst);
     plast = __builtin_amdgcn_readfirstlane(plast);
-    const size_t qat = (size_t)(seq * p.rows + r / p.G) * p.ldq + (size_t)(h * p.G + r % p.G) * D;
+    const Steps st = steps_of(p, pfirst, plast, 0, upto);
+    const int end = min(plast + 1, upto), lo = st.lo, n = st.n;
+    const int per = (n + p.psplit - 1) / p.psplit;
+    const int v0 = min(n, split * per), v1 = min(n, v0 + per);
+    const bool half_pages = kv.plog == 4;  // a step spans two 16-token pages
+    const int P = kv.P;
+    auto step_at = [&](int v) { return v < st.ns ? v : v - st.ns + st.lo_step; };
+    auto stage_pages = [&](int vr) {
+        const int cnt = min(kRound, v1 - vr);
+        for (int e = tid; e < cnt << (half_pages ? 1 : 0); e += 256)
+            s_page[e] = kv_page(kv, seq, step_at(vr + (half_pages ? e >> 1 : e)) * 32 + (half_pages ? (e & 1) * 16 : 0));
+    };
+    stage_pages(v0);
+
+    // their parts to LDS
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        const int u = tid + 256 * i, row = u / L, d = u % L * 8;
+        if (M * L % 256 != 0 && u >= M * L) break;  // whole rows: L lanes in step
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            x[e] = p.q_bf16 ? as_float(e & 1 ? raw[i][0][e >> 1] & 0xFFFF0000u : raw[i][0][e >> 1] << 16) : as_float(raw[i][e >> 2][e & 3]);
+        float scale = p.scale;
+        if constexpr (Q8) {  // the row's largest value to [16, 32), but for rows of 2^-122 and less
+            float amax = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+            for (int y = 1; y < L; y <<= 1) amax = fmaxf(amax, __shfl_xor(amax, y, 64));
+            const int ex = max(-126, min(126, ilogb2(amax) - 4));
+            scale *= pow2(ex);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= pow2(-ex);
+        }
+        if (d == 0) s_scale[row] = scale;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            if constexpr (Q8) {
+                f16x8 y;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    y[e] = (_Float16)x[e];
+                    x[e] -= (float)y[e];
+                }
+                *(f16x8*)(lds + (n * M + row) * PQ + 2 * d) = y;
+            } else {
+                *(u32x4*)(lds + (n * M + row) * PQ + 2 * d) = bf16_part(x);
+            }
+        }
+    }
+
+    f32x4 o[QT][DT];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        m[t] = kNone;
+        l[t] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int vr = v0; vr < v1; vr += kRound) {
+        const int cnt = min(kRound, v1 - vr);
+        if (vr > v0) {
+            __syncthreads();
+            stage_pages(vr);
+        }
+        __syncthreads();
+        // a step's K and V, as they lie in the cache
+        u32x4 kf[2][Q8 ? KS / 2 : KS], vf[Q8 ? DT / 2 : DT], ksc[Q8 ? KS : 1], vsc[Q8 ? KS : 1];
+        auto load_k = [&](int w) {
+            const int t0 = step_at(vr + w) * 32, ib = t0 & (P - 1);  // 0 with 16-token pages
+            // lane row c holds token 8 (c / 4) + c % 4 (+ 4 in the second tile)
+            const int gk = c >> 2, pk = half_pages ? s_page[2 * w + (gk >> 1)] : s_page[w], tk = ib + 8 * (half_pages ? gk & 1 : gk) + (c & 3);
+            const char* bk = kv.pages + (size_t)max(pk, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
+#pragma unroll
+            for (int k = 0; k < (Q8 ? KS / 2 : KS); ++k)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                    kf[y][k] = *(const u32x4*)(bk + (Q8 ? kv_kq_unit(P, k, g, tk + 4 * y) : kv_k_unit(P, 4 * k + g, tk + 4 * y)));
+            if constexpr (Q8) {
+                const int pv = half_pages ? s_page[2 * w + (g >> 1)] : s_page[w], tv = ib + 8 * (half_pages ? g & 1 : g);
+                const char* bv = kv.pages + (size_t)max(pv, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) ksc[k] = *(const u32x4*)(bv + kv_ks_off(P, D, k, tv));
+            }
+        };
+        auto load_v = [&](int w) {  // tokens 8g..
+            const int t0 = step_at(vr + w) * 32, ib = t0 & (P - 1);
+            const int pv = half_pages ? s_page[2 * w + (g >> 1)] : s_page[w], tv = ib + 8 * (half_pages ? g & 1 : g);
+            const char* bv = kv.pages + (size_t)max(pv, 0) * kv.page_bytes + (size_t)h * kv.head_bytes;
+#pragma unroll
+            for (int d = 0; d < (Q8 ? DT / 2 : DT); ++d)
+                vf[d] = *(const u32x4*)(bv + (Q8 ? kv_vq_unit(P, D, tv >> 3, d, c) : kv_v_unit(P, D, tv >> 3, 16 * d + c)));
+            if constexpr (Q8)
+#pragma unroll
+                for (int d = 0; d < KS; ++d) vsc[d] = *(const u32x4*)(bv + kv_vs_off(P, D, d, tv));
+        };
+        // the wave's steps, every row tile from another one on: tiles that went over the
+        // piece side by side would all wait for the same few loads from memory; like this
+        // each brings a part of the piece into the L2 for the others
+        const int mine = (cnt - wave + kWaves - 1) / kWaves, from = (int)((int64_t)mine * tile / tiles);
+        auto turn = [&](int i) { return wave + kWaves * (i + from < mine ? i + from : i + from - mine); };
+        if (mine > 0) {
+            load_k(turn(0));
+            load_v(turn(0));
+        }
+        for (int i = 0; i < mine; ++i) {
+            const int w = turn(i), t0 = step_at(vr + w) * 32, next = i + 1 < mine ? turn(i + 1) : w;
+            const int pv = half_pages ? s_page[2 * w + (g >> 1)] : s_page[w];
+            // the scores of all tiles: then the keys' registers take the next step's, which
+            // arrive during the second products, and the values' after those
+            f32x4 s[QT][2];
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                // the queries are read anew in every step: kept over the loop they would need
+                // more registers than there are
+                int qo = (16 * t + c) * PQ + 16 * g;
+                asm volatile("" : "+v"(qo));
+                const char* ql = lds + qo;
+                __builtin_amdgcn_sched_barrier(0);
+                s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    u32x4 q[NQ];
+#pragma unroll
+                    for (int a = 0; a < NQ; ++a) q[a] = *(const u32x4*)(ql + a * M * PQ + 64 * k);
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        if constexpr (!Q8) {
+#pragma unroll
+                            for (int a = NQ - 1; a >= 0; --a)
+                                s[t][y] = mfma16(__builtin_bit_cast(bf16x8, kf[y][k]), __builtin_bit_cast(bf16x8, q[a]), s[t][y]);
+                        } else {
+                            const uint32_t a0 = ksc[k][2 * y], a1 = ksc[k][2 * y + 1];
+                            const f32x4 sc = {as_float(a0 << 16), as_float(a0 & 0xFFFF0000u), as_float(a1 << 16), as_float(a1 & 0xFFFF0000u)};
+                            const f16x8 kb = codes8h(kf[y][k / 2][2 * (k & 1)], kf[y][k / 2][2 * (k & 1) + 1]);
+                            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int a = NQ - 1; a >= 0; --a) x = mfma16h(kb, __builtin_bit_cast(f16x8, q[a]), x);
+                            s[t][y] += x * sc;
+                        }
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_k(next);
+            __builtin_amdgcn_sched_barrier(0);
+            const bool edge = t0 + 31 > pfirst || (p.window && t0 <= plast - p.window && t0 + 32 > p.sinks) || __any(pv < 0) || t0 + 32 > upto;
+            if (edge) {  // what no row sees may hold anything: its products must not
+                uint32_t seen = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int tok = t0 + 8 * g + e;
+                    seen |= pv >= 0 && tok < end && (tok >= lo || tok < p.sinks) ? 1u << e : 0u;
+                }
+                u32x4 mask;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mask[e] = (seen >> (2 * e) & 1 ? 0xFFFFu : 0u) | (seen >> (2 * e + 1) & 1 ? 0xFFFF0000u : 0u);
+                if constexpr (!Q8) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) vf[d] &= mask;
+                } else {  // codes are finite, an unseen scale may not be
+#pragma unroll
+                    for (int d = 0; d < KS; ++d) vsc[d] &= mask;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                // scores of tokens t0 + 8g + 4y + e for the lane's query row
+                const float scale = Q8 ? s_scale[16 * t + c] : p.scale;
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[t][e >> 2][e & 3] * scale;
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int tok = t0 + 8 * g + e;
+                        const bool me = pv >= 0 && tok <= pos[t] && tok < upto && (!p.window || tok > pos[t] - p.window || tok < p.sinks);
+                        x[e] = me ? x[e] : -INFINITY;
+                    }
+                }
+                float mx = x[0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+                if (__any(mx > m[t] + kLazy)) {
+                    const float mn = fmaxf(m[t], groups_max(mx));
+                    const float al = __builtin_amdgcn_exp2f(m[t] - mn);
+                    m[t] = mn;
+                    l[t] *= al;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[t][d] *= al;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(x[e] - m[t]);
+                    l[t] += x[e];
+                }
+                auto parts = [&](float (&y)[8], bf16x8 (&pp)[NP]) {
+#pragma unroll
+                    for (int a = 0; a < NP; ++a) pp[a] = __builtin_bit_cast(bf16x8, bf16_part(y));
+                };
+                bf16x8 pp[NP];
+                if constexpr (!Q8) {
+                    parts(x, pp);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int a = NP - 1; a >= 0; --a) o[t][d] = mfma16(__builtin_bit_cast(bf16x8, vf[d]), pp[a], o[t][d]);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < DT / 2; ++d) {
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = x[e] * as_float(e & 1 ? vsc[d][e >> 1] & 0xFFFF0000u : vsc[d][e >> 1] << 16);
+                        parts(y, pp);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int a = NP - 1; a >= 0; --a)
+                                o[t][2 * d + u] = mfma16(codes8(vf[d][2 * u], vf[d][2 * u + 1]), pp[a], o[t][2 * d + u]);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            load_v(next);
+        }
+    }
+
+    // join the waves, a tile at a time, through the queries' LDS
+    constexpr int PO = D + 4;
+    float* s_o = (float*)lds;  // [kWaves][16][PO]
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        l[t] = groups_sum(l[t]);
+        __syncthreads();
+        if (g == 0) {
+            s_m[wave][c] = m[t];
+            s_l[wave][c] = l[t];
+        }
+        __syncthreads();
+        float mt = s_m[0][c];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) mt = fmaxf(mt, s_m[w][c]);
+        const float f = __builtin_amdgcn_exp2f(m[t] - mt);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *(f32x4*)(s_o + (wave * 16 + c) * PO + 16 * d + 4 * g) = o[t][d] * f;
+        __syncthreads();
+        for (int e = tid; e < 16 * (D / 4); e += 256) {
+            const int row = e / (D / 4), d = e % (D / 4) * 4, r = first + 16 * t + row;
+            if (r > last) continue;
+            const size_t at = ((size_t)split * p.n_rows + seq * p.rows + r / p.G) * p.q_heads + h * p.G + r % p.G;
+            if (d == 0) {
+                float mt = s_m[0][row], lt = 0.f;
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) mt = fmaxf(mt, s_m[w][row]);
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) lt += s_l[w][row] * __builtin_amdgcn_exp2f(s_m[w][row] - mt);
+                *(u32x2*)(p.part + p.ml + at * 2) = u32x2{__builtin_bit_cast(uint32_t, mt), __builtin_bit_cast(uint32_t, lt)};
+            }
+            if (v0 >= v1) continue;  // l is 0: the row is not read
+            f32x4 a = *(const f32x4*)(s_o + row * PO + d);
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) a += *(const f32x4*)(s_o + (w * 16 + row) * PO + d);
+            *(f32x4*)(p.part + at * D + d) = a;
+        }
+    }
+}
+
+// NQ parts of q, NP of a softmax weight, QT row tiles of a workgroup over a prefix
+template <int D, int KV, int NQ, int NP, int QT>
+__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_shared(SharedP p) {
+    constexpr int kPrefixParts = NP < 2 ? NP : 2;  // of a weight over the prefix: 2^-17 of it
+    constexpr int KS = D / 32, DT = D / 16;
+    constexpr bool CUT = true;
+    constexpr int kQueries = NQ * 16 * QT * (2 * D + 16), kSums = kWaves * 16 * (D + 4) * 4;
+    __shared__ __attribute__((aligned(16))) char lds[kQueries > kSums ? kQueries : kSums];
+    __shared__ int s_page[kRound * 2];
+    __shared__ float s_m[kWaves][16], s_l[kWaves][16], s_mt[16], s_lt[16], s_scale[16 * QT];
+    // the prefixes' workgroups first, then the sequences' own
+    if ((int)blockIdx.x < p.punits) {
+        attend_prefix<D, KV, NQ, kPrefixParts, QT>(p, lds, s_page, s_m, s_l, s_scale);
+        return;
+    }
+    float(&s_o)[kWaves][16][D + 4] = *(float(*)[kWaves][16][D + 4])lds;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const KvView& kv = p.kv;
+    int u = blockIdx.x - p.punits;
+    const int split = u % p.tsplit;
+    u /= p.tsplit;
+    const int h = u % kv.heads, tile = u / kv.heads % p.ttiles, seq = u / (kv.heads * p.ttiles);
+    Group gr;
+    const bool grouped = group_with(p, seq, gr);
+    const int from = grouped ? gr.prefix : 0, upto = 0x7FFFFFFF;
+    // the lane's query row: new token i, head r % G of the group
+    const int len = length_of(p, seq), M = p.rows * p.G, first = tile * 16, last = min(M, first + 16) - 1;
+    const int pfirst = len - p.rows + first / p.G, plast = len - p.rows + last / p.G;
+    const int r = min(first + c, last), i = r / p.G, pos = len - p.rows + i;
+    const size_t qat = (size_t)(seq * p.rows + i) * p.ldq + (size_t)(h * p.G + r % p.G) * D;
     const Steps st = steps_of(p, pfirst, plast, from, upto);
     const int end = plast + 1, lo = st.lo, n = st.n;
-    const int per = (n + nsplit - 1) / nsplit;
+    const int per = (n + p.tsplit - 1) / p.tsplit;
     const int v0 = min(n, split * per), v1 = min(n, v0 + per);
 #include "bq_attn_rows.inc"
     for (int e = tid; e < 16 * (D / 4); e += 256) {
         const int row = e / (D / 4), d = e % (D / 4) * 4, r = first + row;
         if (r > last) continue;
-        const size_t at = ((size_t)(piece0 + split) * p.n_rows + seq * p.rows + r / p.G) * p.q_heads + h * p.G + r % p.G;
+        const size_t at = ((size_t)(p.psplit + split) * p.n_rows + seq * p.rows + r / p.G) * p.q_heads + h * p.G + r % p.G;
         if (d == 0) *(u32x2*)(p.part + p.ml + at * 2) = u32x2{__builtin_bit_cast(uint32_t, s_mt[row]), __builtin_bit_cast(uint32_t, s_lt[row])};
+        // a sequence of no group has no prefix pieces
+        if (!grouped && split == 0)
+            for (int s = d / 4; s < p.psplit; s += D / 4)
+                *(u32x2*)(p.part + p.ml + (at + ((size_t)s - p.psplit) * p.n_rows * p.q_heads) * 2) = u32x2{0, 0};
         if (v0 >= v1) continue;  // l is 0: the row is not read
         f32x4 a = *(const f32x4*)&s_o[0][row][d];
 #pragma unroll
@@ -168,53 +496,72 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_shared(SharedP p
     }
 }
 
-// joins the pieces of one query row: D / 4 lanes per piece, the pieces dealt over the
-// rest of the workgroup's lanes, in a fixed order
+// joins the pieces of one query row and head: D / 4 lanes per piece, the pieces dealt over
+// the rest of the workgroup's lanes, in a fixed order, each in one pass with a running m
 template <int D>
 __global__ void __launch_bounds__(256) k_attn_shared_join(SharedP p) {
     constexpr int T = 256, L = D / 4, S = T / L;
     __shared__ __attribute__((aligned(16))) float s_o[S][D];
-    __shared__ float s_l[S], s_mx[T / 64];
-    const int tid = threadIdx.x, row = blockIdx.x / p.q_heads, head = blockIdx.x % p.q_heads;
+    __shared__ float s_m[S], s_l[S];
+    const int tid = threadIdx.x, row = blockIdx.x / p.q_heads, head = blockIdx.x % p.q_heads, at = tid / L, d = tid % L * 4;
     const int64_t rows = (int64_t)p.n_rows * p.q_heads;
-    // a sequence of no group has no prefix pieces
-    const int first = group_with(p, row / p.rows) < 0 ? p.psplit : 0, n = p.psplit + p.tsplit;
     const float* ml = p.part + p.ml + (int64_t)blockIdx.x * 2;
-    float mt = kNone;
-    for (int s = first + tid; s < n; s += T) mt = fmaxf(mt, ml[s * rows * 2]);
-    for (int d = 1; d < 64; d <<= 1) mt = fmaxf(mt, __shfl_xor(mt, d, 64));
-    if ((tid & 63) == 0) s_mx[tid >> 6] = mt;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < T / 64; ++w) mt = fmaxf(mt, s_mx[w]);
+    const float* part = p.part + (int64_t)blockIdx.x * D + d;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
-    float lt = 0.f;
+    float mt = kNone, lt = 0.f;
 #pragma unroll 4
-    for (int s = first + tid / L; s < n; s += S) {
-        const float l = ml[s * rows * 2 + 1];
+    for (int s = at; s < p.psplit + p.tsplit; s += S) {
+        const u32x2 b = *(const u32x2*)(ml + s * rows * 2);
+        const f32x4 o = *(const f32x4*)(part + s * rows * D);
+        const float m = as_float(b[0]), l = as_float(b[1]);
         if (l == 0.f) continue;  // nothing was stored
-        const float f = __builtin_amdgcn_exp2f(ml[s * rows * 2] - mt);
-        a += *(const f32x4*)(p.part + (s * rows + blockIdx.x) * D + tid % L * 4) * f;
-        lt += l * f;
+        const float mn = fmaxf(mt, m), f = __builtin_amdgcn_exp2f(mt - mn), g = __builtin_amdgcn_exp2f(m - mn);
+        a = a * f + o * g;
+        lt = lt * f + l * g;
+        mt = mn;
     }
-    *(f32x4*)&s_o[tid / L][tid % L * 4] = a;
-    if (tid % L == 0) s_l[tid / L] = lt;
+    *(f32x4*)&s_o[at][d] = a;
+    if (d == 0) {
+        s_m[at] = mt;
+        s_l[at] = lt;
+    }
     __syncthreads();
     if (tid >= L) return;
-    for (int s = 1; s < S; ++s) {
-        a += *(const f32x4*)&s_o[s][tid * 4];
-        lt += s_l[s];
+    float m = s_m[0], l = 0.f;
+#pragma unroll
+    for (int s = 1; s < S; ++s) m = fmaxf(m, s_m[s]);
+    a = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const float f = __builtin_amdgcn_exp2f(s_m[s] - m);
+        a += *(const f32x4*)&s_o[s][d] * f;
+        l += s_l[s] * f;
     }
-    store4(p, (size_t)row * p.ldo + (size_t)head * D + tid * 4, lt == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a * (1.f / lt));
+    store4(p, (size_t)row * p.ldo + (size_t)head * D + d, l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a * (1.f / l));
 }
 
+// Row tiles of a workgroup over a prefix at most: with two of 256 dims over a q8 cache
+// the registers do not hold what one step needs
 template <int D, int KV>
-hipError_t launch_of(const SharedP& p, hipStream_t st) {
-    const uint32_t units = (uint32_t)(p.ptiles * p.kv.heads * p.psplit + p.kv.n_seq * p.ttiles * p.kv.heads * p.tsplit);
+constexpr int kMostTiles = D == 256 && KV == kKvQ8 ? 1 : 2;
+
+template <int D, int KV, int NQ, int NP>
+void launch_tiles(const SharedP& p, int qt, uint32_t units, hipStream_t st) {
+    if constexpr (kMostTiles<D, KV> == 2) {
+        if (qt == 2) {
+            launch_kernel((k_attn_shared<D, KV, NQ, NP, 2>), dim3(units), dim3(256), 0, st, p);
+            return;
+        }
+    }
+    launch_kernel((k_attn_shared<D, KV, NQ, NP, 1>), dim3(units), dim3(256), 0, st, p);
+}
+template <int D, int KV>
+hipError_t launch_of(const SharedP& p, int qt, hipStream_t st) {
+    const uint32_t units = (uint32_t)(p.punits + p.kv.n_seq * p.ttiles * p.kv.heads * p.tsplit);
     if (p.q_bf16 && p.out_bf16)
-        launch_kernel((k_attn_shared<D, KV, 1, 1>), dim3(units), dim3(256), 0, st, p);
+        launch_tiles<D, KV, 1, 1>(p, qt, units, st);
     else
-        launch_kernel((k_attn_shared<D, KV, KV == kKvQ8 ? 2 : 3, KV == kKvQ8 ? 2 : 3>), dim3(units), dim3(256), 0, st, p);
+        launch_tiles<D, KV, KV == kKvQ8 ? 2 : 3, KV == kKvQ8 ? 2 : 3>(p, qt, units, st);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     launch_kernel((k_attn_shared_join<D>), dim3((uint32_t)(p.n_rows * p.q_heads)), dim3(256), 0, st, p);
@@ -222,21 +569,25 @@ hipError_t launch_of(const SharedP& p, hipStream_t st) {
 }
 }  // namespace
 
-// Row tiles of all groups together, per head: every group may end with a broken one.
-static int64_t shared_tiles(int n_seq, int rows, int G, int n_groups) {
-    return ((int64_t)n_seq * rows * G + 15) / 16 + std::min(n_groups, n_seq) - 1;
-}
-
-SharedPlan shared_plan(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int max_len, int n_groups, int max_prefix, int window,
-                       int sinks, int cus) {
+SharedPlan shared_plan(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int max_len, int n_groups, int max_prefix,
+                       int window, int sinks, int cus) {
     SharedPlan s;
-    const int G = q_heads / kv_heads;
-    const int64_t tiles = shared_tiles(n_seq, rows, G, n_groups);
+    const int G = q_heads / kv_heads, groups = std::min(n_groups, n_seq);
+    const int64_t all = (int64_t)n_seq * rows * G, each_group = all / groups;
     const int64_t prefix = std::min<int64_t>(decode_reach(rows, window, sinks, max_len), max_prefix);
     const int64_t own = std::min<int64_t>(decode_reach(rows, window, sinks, max_len), std::max(max_len - max_prefix, 1));
-    const int64_t each = ((prefix + 31) / 32 + kWaves - 1) / kWaves;
-    s.ptiles = tiles;
-    s.psplit = (int)std::max<int64_t>(1, std::min<int64_t>(each, 2 * cus / (tiles * kv_heads)));
+    const int64_t each = ((prefix + 31) / 32 + kWaves - 1) / kWaves;  // steps of a wave
+    // two row tiles share a step's K and V where single ones would more than fill the chip
+    // (16 sequences of 8 heads behind 8192 tokens 24.5 us with one, 22.5 with two; four
+    // behind 600 tokens 11.3 and 12.9)
+    const bool many = (all + 15) / 16 * kv_heads * each > cus && each_group > 16;
+    s.qt = many ? D == 256 && type == kKvQ8 ? kMostTiles<256, kKvQ8> : 2 : 1;
+    // row tiles of all groups together, per head: every group may end with a broken one
+    s.ptiles = (all + 16 * s.qt - 1) / (16 * s.qt) + groups - 1;
+    // pieces: one workgroup a CU, which leaves room for one of the sequences' own tokens
+    // beside it (64 sequences of up to 2048 own tokens behind 8192 50 us, 60 with two)
+    s.psplit = (int)std::max<int64_t>(1, std::min<int64_t>(each, cus / (s.ptiles * kv_heads)));
+    s.punits = (s.psplit * kv_heads + 7) / 8 * 8 * s.ptiles;
     s.ttiles = (rows * G + 15) / 16;
     s.tsplit = decode_splits(type, n_seq, rows, q_heads, kv_heads, D, own, cus);
     return s;
@@ -254,14 +605,14 @@ hipError_t launch_attn_shared(const KvView& kv, int type, const bq_attn_args& a,
     p.max_len = a.max_len; p.window = a.window; p.sinks = a.sinks;
     p.q_bf16 = a.q_type == BQ_TYPE_BF16; p.out_bf16 = a.out_type == BQ_TYPE_BF16;
     p.scale = a.scale * 1.44269504088896341f;
-    p.ptiles = (int)s.ptiles; p.psplit = s.psplit; p.ttiles = s.ttiles; p.tsplit = s.tsplit;
+    p.ptiles = (int)s.ptiles; p.punits = (int)s.punits; p.psplit = s.psplit; p.ttiles = s.ttiles; p.tsplit = s.tsplit;
     p.part = (float*)a.work;
     p.ml = (int64_t)(s.psplit + s.tsplit) * a.n_rows * a.q_heads * kv.D;
     const bool q8 = type == kKvQ8;
     switch (kv.D) {
-        case 64: return q8 ? launch_of<64, kKvQ8>(p, st) : launch_of<64, kKvBf16>(p, st);
-        case 128: return q8 ? launch_of<128, kKvQ8>(p, st) : launch_of<128, kKvBf16>(p, st);
-        default: return q8 ? launch_of<256, kKvQ8>(p, st) : launch_of<256, kKvBf16>(p, st);
+        case 64: return q8 ? launch_of<64, kKvQ8>(p, s.qt, st) : launch_of<64, kKvBf16>(p, s.qt, st);
+        case 128: return q8 ? launch_of<128, kKvQ8>(p, s.qt, st) : launch_of<128, kKvBf16>(p, s.qt, st);
+        default: return q8 ? launch_of<256, kKvQ8>(p, s.qt, st) : launch_of<256, kKvBf16>(p, s.qt, st);
     }
 }
 

@@ -157,11 +157,12 @@ hipError_t launch_attn_prefill(const KvView& kv, int type, const bq_attn_args& a
 // attention of groups that share a prefix: row tiles (per head) and pieces of the
 // prefixes and of a sequence's own tokens
 struct SharedPlan {
-    int64_t ptiles;
-    int psplit, ttiles, tsplit;
+    int64_t ptiles, punits;   // of the prefixes: row tiles, workgroups
+    int qt, psplit;           // 16-row tiles of a workgroup there
+    int ttiles, tsplit;
 };
-SharedPlan shared_plan(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int max_len, int n_groups, int max_prefix, int window,
-                       int sinks, int cus);
+SharedPlan shared_plan(int type, int n_seq, int rows, int q_heads, int kv_heads, int D, int max_len, int n_groups, int max_prefix,
+                       int window, int sinks, int cus);
 size_t shared_part_floats(const SharedPlan& s, int n_rows, int q_heads, int D);
 hipError_t launch_attn_shared(const KvView& kv, int type, const bq_attn_args& a, const bq_attn_prefix& x, const SharedPlan& s, hipStream_t st);
 

@@ -160,10 +160,13 @@ size_t bq_attn_shared_workspace_bytes(int n_seq, int rows, int q_heads, int kv_h
     if (n_seq <= 0 || n_seq > 65535 || rows < 1 || rows > BQ_MAX_ROWS || kv_heads <= 0 || q_heads % kv_heads != 0 || q_heads <= 0 ||
         head_dim <= 0 || max_len < 0 || n_groups < 1 || max_prefix < 0 || device_ready() != BQ_OK)
         return 0;
-    // of either type and any window: the pieces are the most without one, of a q8 cache's own tokens
+    // of either type and any window: the pieces are the most without one
     max_prefix = std::min(max_prefix, max_len);
-    const SharedPlan s = shared_plan(kKvQ8, n_seq, rows, q_heads, kv_heads, head_dim, max_len, n_groups, max_prefix, 0, 0, device_cus());
-    return shared_part_floats(s, n_seq * rows, q_heads, head_dim) * sizeof(float);
+    size_t most = 0;
+    for (int type : {kKvBf16, kKvQ8})
+        most = std::max(most, shared_part_floats(shared_plan(type, n_seq, rows, q_heads, kv_heads, head_dim, max_len, n_groups, max_prefix, 0, 0,
+                                                             device_cus()), n_seq * rows, q_heads, head_dim));
+    return most * sizeof(float);
 }
 
 int bq_attn_decode_shared(const bq_kv_cache* c, const bq_attn_args* args, const bq_attn_prefix* prefix, bq_stream_t st) {
@@ -182,7 +185,7 @@ int bq_attn_decode_shared(const bq_kv_cache* c, const bq_attn_args* args, const 
     const SharedPlan s = shared_plan(type, kv.n_seq, a.rows, a.q_heads, kv.heads, kv.D, a.max_len, x.n_groups, x.max_len, a.window, a.sinks,
                                      device_cus());
     // one grid dimension holds all workgroups, another all rows
-    if (s.ptiles * kv.heads * s.psplit + (int64_t)kv.n_seq * s.ttiles * kv.heads * s.tsplit > INT32_MAX ||
+    if (s.punits + (int64_t)kv.n_seq * s.ttiles * kv.heads * s.tsplit > INT32_MAX ||
         (int64_t)a.n_rows * a.q_heads > INT32_MAX)
         return BQ_UNSUPPORTED;
     if (!a.work || !al16(a.work) || a.work_bytes < shared_part_floats(s, a.n_rows, a.q_heads, kv.D) * sizeof(float)) return BQ_EINVAL;

@@ -159,6 +159,15 @@ def test_long_prefixes(bq, kv, D, Hq, H, P):
     _shared(bq, kv, [(2, 1500), (7, 700)], [1300, 3, 800, 1, 2, 40, 5, 77, 600], 3, Hq, H, D, P, "f32", "f32", 1000, 5, seed=D + 1)
 
 
+@pytest.mark.parametrize("kv", ["bf16", "q8"])
+@pytest.mark.parametrize("D,Hq,H", [(64, 64, 8), (128, 32, 4), (256, 24, 3)])
+def test_rows_that_fill_the_chip(bq, kv, D, Hq, H):
+    """Enough rows and tokens that two row tiles share a step, with a broken tile at the end of each group."""
+    for rows, types, window, sinks in ((1, ("f32", "f32"), 0, 0), (2, ("bf16", "bf16"), 0, 0), (1, ("f32", "f32"), 1500, 40)):
+        _shared(bq, kv, [(9, 2100), (2, 1900), (6, 800)], [1 + 7 * i % 40 for i in range(17)], rows, Hq, H, D, 64, *types, window, sinks,
+                seed=D + rows)
+
+
 def test_sequences_before_the_first_group(bq):
     _shared(bq, "bf16", [(3, 60)], [100, 33, 5, 6, 70, 2], 1, 8, 2, 128, 16, "f32", "f32", seed=11, lead=2)
 
