@@ -946,9 +946,6 @@ class Lora:
         _expect(scale, torch.float32, (n,), "scale")
         _one_device(x.device, xd=xd, adapter=adapter, scale=scale)
         L = load()
-        if work is None:
-            work = torch.empty(int(L.bq_lora_workspace_bytes(rows, rank, len(parts))), dtype=torch.uint8, device=x.device)
-        _work_of(work, x.device)
         s = self.struct = LoraArgs(_ptr(x), _ptr(xd), kind, _rows_ld(x, K, "x"), rows, K, rank, n, len(parts))
         for i, part in enumerate(parts):
             a, b, y = part[:3]
@@ -962,6 +959,9 @@ class Lora:
             _one_device(x.device, a=a, b=b, y=y, base=base)
             s.parts[i] = LoraPart(_ptr(a), _ptr(b), _ptr(base), _ptr(y), 0 if base is None else _rows_ld(base, N, "base"),
                                   _rows_ld(y, N, "y"), N)
+        if work is None:
+            work = torch.empty(int(L.bq_lora_workspace_bytes(rows, rank, len(parts))), dtype=torch.uint8, device=x.device)
+        _work_of(work, x.device)
         s.adapter, s.scale, s.work, s.work_bytes = _ptr(adapter), _ptr(scale), _ptr(work), work.numel() * work.element_size()
         self.work, self._keep = work, (x, xd, adapter, parts, scale)
         self._ref, self._run, self._device = ctypes.byref(s), L.bq_lora, x.device.index

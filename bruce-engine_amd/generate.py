@@ -1,7 +1,7 @@
 """Token generation through libbq: prompt chunks, then decoded tokens, with the
 library's own attention and sampling around its matmuls.
 
-    python bruce-engine_amd/generate.py [--kv q8] [--tokens 32] [--batch 4] ...
+    python bruce-engine_amd/generate.py [--kv q8] [--tokens 32] [--batch 4] [--shared 2000] [--adapters 3] [--logprobs 5] ...
 
 Random weights of a small architecture (or larger, by the options), random
 prompts.  What it shows is the wiring a serving program needs:
@@ -12,7 +12,12 @@ prompts.  What it shows is the wiring a serving program needs:
 * prompts in chunks (BQ rows of one sequence, prefill attention), then all
   sequences together, one token each, as one captured graph replayed per token
   (positions and lengths are device memory, so one graph serves them all);
-* Sampler on the logits; its tokens feed the next step without leaving the GPU.
+* Sampler on the logits; its tokens feed the next step without leaving the GPU;
+* a prompt that all sequences begin with (--shared): prefilled once, its pages in
+  every row of the block table, and SharedAttention in the decode step;
+* low-rank adapters (--adapters): one per sequence, a Lora beside every
+  projection of every layer, by the step's projection hook (LoraPlan);
+* log probabilities of the drawn tokens and their alternatives (--logprobs).
 """
 import argparse
 import ctypes
@@ -42,9 +47,10 @@ class Model:
     """Random weights: per layer q, k, gate and v (Q5_K, with the W144 repack the prefill GEMMs use), o, gate, up
     (Q5_K), down (Q6_K, W160), the norm weights of q and k, and a Q8_0 head."""
 
-    def __init__(self, c, seed=0):
+    def __init__(self, c, seed=0, adapters=0, rank=16):
+        """adapters: slots of low-rank adapters beside every projection, random as the weights are."""
         import torch
-        self.c = c
+        self.c, self.adapters, self.rank = c, adapters, rank
         g = torch.Generator().manual_seed(seed)
         self.rng = np.random.default_rng(seed)
         vec = lambda n, mean=1.0, std=0.2: (mean + std * torch.randn(n, generator=g)).cuda()
@@ -61,6 +67,12 @@ class Model:
         self.head = bq.quantize_q8s((torch.randn((c.vocab, c.n_embd), generator=g) * 0.3).bfloat16().view(torch.int16).cuda(),
                                     c.n_embd, c.vocab)
         self.scale = vec(c.vocab, 8.0, 0.5)
+        # [layer][projection]: (a, b) of its parts, in the order of the step's outputs
+        rand = lambda *shape: torch.randn(shape, generator=g)
+        pair = lambda K, N: ((rand(adapters, rank, K) * K ** -0.5).bfloat16().cuda(), (rand(adapters, N, rank) * 0.02).bfloat16().cuda())
+        self.lora = [{bq.PROJ_QKV: [pair(c.n_embd, n) for n in (c.n_attn, c.n_kv, c.n_attn, c.n_kv)],
+                      bq.PROJ_O: [pair(c.n_attn, c.n_embd)], bq.PROJ_GATE_UP: [pair(c.n_embd, c.n_ff) for _ in range(2)],
+                      bq.PROJ_DOWN: [pair(c.n_ff, c.n_embd)]} for _ in range(c.layers)] if adapters else None
 
     def _raw(self, quantize, K, N):
         import torch
@@ -79,9 +91,11 @@ class Model:
 class Step:
     """A decode step over `rows` rows of the model: buffers, the attention plan over `caches`, and run().  decode:
     row r is the next token of sequence r; otherwise the rows are a chunk of the only sequence of the caches.
-    max_len: the most tokens a sequence has in any run (it sizes the attention's workspace and its pieces)."""
+    max_len: the most tokens a sequence has in any run (it sizes the attention's workspace and its pieces).
+    prefix: (group0, prefix_len, most tokens) of the groups that share a prefix, for a decode step.  adapter: int32
+    [rows], each row's adapter, where the model has some."""
 
-    def __init__(self, model, caches, rope, rows, pos, kv_len, max_len, decode):
+    def __init__(self, model, caches, rope, rows, pos, kv_len, max_len, decode, prefix=None, adapter=None):
         import torch
         c, self.model, self.rows = model.c, model, rows
         f32 = lambda *s: torch.zeros(s, device="cuda")
@@ -112,8 +126,11 @@ class Step:
             blocks.append(b)
             append = bq.Append(cache, self.qkv[0], self.qkv[1], self.qkv[3], pos, self.q, seq=seq, q_weight=L["q_weight"],
                                k_weight=L["k_weight"], rope=rope)
-            attention = bq.Attention(cache, self.q, self.attn_out, kv_len, window=c.window, sinks=c.sinks, max_len=max_len,
-                                     work=attn_work)
+            common = dict(window=c.window, sinks=c.sinks, max_len=max_len, work=attn_work)
+            if prefix is None:
+                attention = bq.Attention(cache, self.q, self.attn_out, kv_len, **common)
+            else:
+                attention = bq.SharedAttention(cache, self.q, self.attn_out, kv_len, *prefix[:2], max_prefix=prefix[2], **common)
             attn_work = attention.work
             plan.append((append, attention))
             b = bq.DecodeBlock()
@@ -131,12 +148,37 @@ class Step:
         st.xdh, st.work, st.work_bytes = ptr(xdh), ptr(work), work.numel() * 4
         self.plan = bq.AttentionPlan(plan, prefill=not decode)
         self.plan.install(st)
+        self.adapters = self._adapters(adapter, ffn) if adapter is not None and model.lora else None
+        if self.adapters:
+            self.adapters.install(st)
         self._keep = (blocks, keep, ffn, xdh, work, caches, rope, seq)
         self.graph = None
 
+    def _adapters(self, adapter, ffn):
+        """The projection hook's plan: an attention block's projections, then an FFN block's, layer by layer."""
+        import torch
+        c, rows = self.model.c, self.rows
+        # the calls, of one, two and four parts, run one after another: one workspace serves all
+        size = max(bq.load().bq_lora_workspace_bytes(rows, self.model.rank, parts) for parts in (1, 2, 4))
+        work = torch.empty(int(size), dtype=torch.uint8, device="cuda")
+
+        def lora(K, weights, outputs):
+            x = (self.q8[0][: rows * K].view(rows, K), self.q8[1][: rows * K // 32].view(rows, K // 32))
+            return bq.Lora(x, adapter, [(a, b, y) for (a, b), y in zip(weights, outputs)], work=work)
+        blocks = []
+        for L in self.model.lora:
+            blocks.append({bq.PROJ_QKV: lora(c.n_embd, L[bq.PROJ_QKV], self.qkv), bq.PROJ_O: lora(c.n_attn, L[bq.PROJ_O], [self.proj])})
+            blocks.append({bq.PROJ_GATE_UP: lora(c.n_embd, L[bq.PROJ_GATE_UP], ffn), bq.PROJ_DOWN: lora(c.n_ff, L[bq.PROJ_DOWN], [self.proj])})
+        return bq.LoraPlan(blocks)
+
+    def check(self):
+        self.plan.check()
+        if self.adapters:
+            self.adapters.check()
+
     def capture(self):
         self.graph = bq.DecodeGraph(self.struct)
-        self.plan.check()
+        self.check()
 
     def run(self, tokens):
         """Embeds tokens [rows] (device) and runs the step; the logits are in self.logits."""
@@ -148,14 +190,15 @@ class Step:
             self.graph.launch()
         else:
             bq.decode_enqueue(self.struct)
-            self.plan.check()
+            self.check()
         return self.logits
 
 
 class Generator:
-    """Sequences over one paged cache per layer: prefill(s, tokens), then decode() rounds over all of them."""
+    """Sequences over one paged cache per layer: prefill(s, tokens), then decode() rounds over all of them.  shared:
+    the sequences may begin with a prompt that is prefilled once: share(tokens) before any prefill."""
 
-    def __init__(self, model, n_seq, max_len, seed=1):
+    def __init__(self, model, n_seq, max_len, seed=1, shared=False):
         import torch
         c, self.model, self.n_seq, self.max_len = model.c, model, n_seq, max_len
         per = (max_len + c.page_tokens - 1) // c.page_tokens
@@ -167,7 +210,13 @@ class Generator:
         self.length = torch.zeros(n_seq, dtype=torch.int32, device="cuda")   # tokens cached per sequence
         self.pos = torch.zeros(n_seq, dtype=torch.int32, device="cuda")      # of the decode step's rows
         self.kv_len = torch.zeros(n_seq, dtype=torch.int32, device="cuda")
-        self.step = Step(model, self.caches, self.rope, n_seq, self.pos, self.kv_len, max_len, True)
+        # each sequence's adapter (-1: none)
+        self.adapter = torch.full((n_seq,), -1, dtype=torch.int32, device="cuda")
+        self.prefix_len = torch.zeros(1, dtype=torch.int32, device="cuda")
+        self.shared = 0                                                      # tokens that all sequences begin with
+        group0 = torch.tensor([0, n_seq], dtype=torch.int32, device="cuda")
+        self.step = Step(model, self.caches, self.rope, n_seq, self.pos, self.kv_len, max_len, True,
+                         prefix=(group0, self.prefix_len, max_len) if shared else None, adapter=self.adapter)
         self.used = [0] * n_seq                                              # of max_len tokens, on the host
         self.tokens = torch.zeros(n_seq, dtype=torch.int32, device="cuda")
         self.u = torch.zeros(n_seq, device="cuda")
@@ -177,27 +226,55 @@ class Generator:
         """Runs prompt (int32 device tensor) of sequence s in even chunks of at most `chunk` tokens; returns the last
         token's logits [vocab].  (Even, as a few tokens left over would take the decode path, which rounds otherwise.)"""
         import torch
-        c, done = self.model.c, 0
-        if len(prompt) > self.max_len:
-            raise ValueError(f"a prompt of {len(prompt)} tokens: the caches have room for {self.max_len}")
+        c, done, first = self.model.c, 0, self.shared
+        if first + len(prompt) > self.max_len:
+            raise ValueError(f"a prompt of {first + len(prompt)} tokens: the caches have room for {self.max_len}")
         row = self.table[s: s + 1].contiguous()
         views = [bq.KvCache(k.pages, row, c.kv_type, c.kv_heads, c.head_dim, c.page_tokens) for k in self.caches]
         while done < len(prompt):
             left = len(prompt) - done
             n = -(-left // -(-left // chunk))
-            pos = torch.arange(done, done + n, dtype=torch.int32, device="cuda")
-            step = Step(self.model, views, self.rope, n, pos, torch.tensor([done + n], dtype=torch.int32, device="cuda"),
-                        done + n, False)
+            pos = torch.arange(first + done, first + done + n, dtype=torch.int32, device="cuda")
+            step = Step(self.model, views, self.rope, n, pos, torch.tensor([first + done + n], dtype=torch.int32, device="cuda"),
+                        first + done + n, False, adapter=self.adapter[s: s + 1].expand(n).contiguous())
             logits = step.run(prompt[done: done + n])
             done += n
-        self.length[s] = self.used[s] = len(prompt)
+        self.length[s] = self.used[s] = first + len(prompt)
         return logits[-1]
 
-    def set_sampling(self, temperature=0.8, top_k=40, top_p=0.95, min_p=0.0):
+    def share(self, prompt, chunk=512):
+        """Runs the prompt that every sequence begins with, once, for the base model (sequence 0, which must have no
+        adapter yet); prefill(s, ..) then goes on behind it.  Its whole pages enter every row of the table; where it
+        ends inside a page each sequence has a copy of that one, as its own tokens follow there."""
+        if self.shared or any(self.used):
+            raise ValueError("share: before any prefill")
+        if int(self.adapter[0]) >= 0:
+            raise ValueError("share: the prompt is the base model's, so sequence 0 must have no adapter yet")
+        self.prefill(0, prompt, chunk)
+        whole = len(prompt) // self.model.c.page_tokens
+        self.table[1:, :whole] = self.table[0, :whole]
+        if len(prompt) % self.model.c.page_tokens:
+            ids = self.table[:, whole].long()
+            for cache in self.caches:
+                cache.pages[ids[1:]] = cache.pages[ids[0]].clone()
+        self.shared = len(prompt)
+        self.prefix_len.fill_(self.shared)
+        self.length.fill_(self.shared)
+        self.used = [self.shared] * self.n_seq
+
+    def set_sampling(self, temperature=0.8, top_k=40, top_p=0.95, min_p=0.0, logprobs=0):
+        """logprobs: alternatives beside each drawn token's log probability, rank and entropy, which decode() then
+        leaves in self.logprobs (a dict of device tensors)."""
         import torch
         n, f = self.n_seq, lambda v, dt=torch.float32: torch.full((self.n_seq,), v, dtype=dt, device="cuda")
         self.rules = dict(temperature=f(temperature), top_k=f(top_k, torch.int32), top_p=f(top_p), min_p=f(min_p))
         self.sampler = bq.Sampler(self.step.logits[:n], self.tokens, self.u, **self.rules)
+        self.logprobs = self.scorer = None
+        if logprobs:
+            i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")
+            self.logprobs = dict(logprob=f(0.0), rank=i32(n), entropy=f(0.0), top_tokens=i32(n, logprobs),
+                                 top_logprobs=torch.zeros((n, logprobs), device="cuda"))
+            self.scorer = bq.LogProbs(self.step.logits[:n], tokens=self.tokens, temperature=self.rules["temperature"], **self.logprobs)
 
     def first(self, s, logits):
         """The first token of sequence s from its prompt's last logits."""
@@ -216,6 +293,8 @@ class Generator:
         self.step.run(self.tokens)
         self.u.uniform_(0, 1, generator=self.gen)
         self.sampler.run()
+        if self.scorer:
+            self.scorer.run()
         return self.tokens
 
 
@@ -225,7 +304,8 @@ def main():
     import torch
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     for name, value in (("batch", 4), ("prompt", 300), ("tokens", 32), ("layers", 2), ("n-embd", 1024), ("q-heads", 8),
-                        ("kv-heads", 2), ("n-ff", 2048), ("vocab", 4096), ("window", 0), ("sinks", 0), ("seed", 0)):
+                        ("kv-heads", 2), ("n-ff", 2048), ("vocab", 4096), ("window", 0), ("sinks", 0), ("seed", 0),
+                        ("shared", 0), ("adapters", 0), ("rank", 16), ("logprobs", 0)):
         ap.add_argument("--" + name, type=int, default=value)
     ap.add_argument("--kv", choices=("bf16", "q8"), default="bf16")
     a = ap.parse_args()
@@ -233,12 +313,16 @@ def main():
         ap.error("--batch: 1 to 8 sequences")
     c = Config(n_embd=a.n_embd, q_heads=a.q_heads, kv_heads=a.kv_heads, n_ff=a.n_ff, layers=a.layers, vocab=a.vocab,
                kv_type=a.kv, window=a.window, sinks=a.sinks)
-    g = Generator(Model(c, a.seed), a.batch, a.prompt + a.tokens + 1)
-    g.set_sampling()
+    g = Generator(Model(c, a.seed, a.adapters, a.rank), a.batch, a.shared + a.prompt + a.tokens + 1, shared=a.shared > 0)
+    g.set_sampling(logprobs=a.logprobs)
     rng = torch.Generator(device="cuda").manual_seed(a.seed)
+    tokens = lambda n: torch.randint(0, c.vocab, (n,), generator=rng, device="cuda", dtype=torch.int32)
+    if a.shared:
+        g.share(tokens(a.shared))
+    if a.adapters:
+        g.adapter.copy_(torch.arange(a.batch) % a.adapters)
     for s in range(a.batch):
-        prompt = torch.randint(0, c.vocab, (max(1, a.prompt - 17 * s),), generator=rng, device="cuda", dtype=torch.int32)
-        g.first(s, g.prefill(s, prompt))
+        g.first(s, g.prefill(s, tokens(max(1, a.prompt - 17 * s))))
     g.step.capture()
     out = [g.tokens.clone(), g.decode().clone()]
     torch.cuda.synchronize()
@@ -249,6 +333,11 @@ def main():
     spent = time.perf_counter() - began
     for s, row in enumerate(torch.stack(out, 1).tolist()):
         print(f"sequence {s}: {row}")
+    if g.logprobs:
+        for s in range(a.batch):
+            row = {k: v[s].tolist() for k, v in g.logprobs.items()}
+            print(f"sequence {s}, last token {out[-1][s]}: log p {row['logprob']:.3f}, rank {row['rank']}, entropy {row['entropy']:.3f}; "
+                  + ", ".join(f"{t} {p:.3f}" for t, p in zip(row["top_tokens"], row["top_logprobs"])))
     print(f"{a.tokens - 1} steps of {a.batch} sequences: {spent / max(1, a.tokens - 1) * 1e6:.0f} us a step")
 
 
