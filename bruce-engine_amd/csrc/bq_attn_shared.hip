@@ -447,7 +447,6 @@ BQ_DEV void attend_prefix(const SharedP& p, char* lds, int* s_page, float (&s_m)
 // NQ parts of q, NP of a softmax weight, QT row tiles of a workgroup over a prefix
 template <int D, int KV, int NQ, int NP, int QT>
 __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_shared(SharedP p) {
-    constexpr int kPrefixParts = NP < 2 ? NP : 2;  // of a weight over the prefix: 2^-17 of it
     constexpr int KS = D / 32, DT = D / 16;
     constexpr bool CUT = true;
     constexpr int kQueries = NQ * 16 * QT * (2 * D + 16), kSums = kWaves * 16 * (D + 4) * 4;
@@ -456,7 +455,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_shared(SharedP p
     __shared__ float s_m[kWaves][16], s_l[kWaves][16], s_mt[16], s_lt[16], s_scale[16 * QT];
     // the prefixes' workgroups first, then the sequences' own
     if ((int)blockIdx.x < p.punits) {
-        attend_prefix<D, KV, NQ, kPrefixParts, QT>(p, lds, s_page, s_m, s_l, s_scale);
+        attend_prefix<D, KV, NQ, NP, QT>(p, lds, s_page, s_m, s_l, s_scale);
         return;
     }
     float(&s_o)[kWaves][16][D + 4] = *(float(*)[kWaves][16][D + 4])lds;
@@ -561,7 +560,10 @@ hipError_t launch_of(const SharedP& p, int qt, hipStream_t st) {
     if (p.q_bf16 && p.out_bf16)
         launch_tiles<D, KV, 1, 1>(p, qt, units, st);
     else
-        launch_tiles<D, KV, KV == kKvQ8 ? 2 : 3, KV == kKvQ8 ? 2 : 3>(p, qt, units, st);
+        // all 24 bits of a weight (of its product with a value's scale) over q8 too, where the
+        // decode attention takes two parts: those move an output by 2.2e-6 of its length,
+        // more than fp32 sums in any order do (1.4e-6), for 5% of the time here
+        launch_tiles<D, KV, KV == kKvQ8 ? 2 : 3, 3>(p, qt, units, st);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     launch_kernel((k_attn_shared_join<D>), dim3((uint32_t)(p.n_rows * p.q_heads)), dim3(256), 0, st, p);
