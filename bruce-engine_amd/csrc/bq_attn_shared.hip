@@ -497,19 +497,22 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_attn_shared(SharedP p
 
 // joins the pieces of one query row and head: D / 4 lanes per piece, the pieces dealt over
 // the rest of the workgroup's lanes, in a fixed order, each in one pass with a running m
-template <int D>
+// (few pieces: a row for each D / 4 lanes, which take its pieces one after another)
+template <int D, bool FEW>
 __global__ void __launch_bounds__(256) k_attn_shared_join(SharedP p) {
     constexpr int T = 256, L = D / 4, S = T / L;
     __shared__ __attribute__((aligned(16))) float s_o[S][D];
     __shared__ float s_m[S], s_l[S];
-    const int tid = threadIdx.x, row = blockIdx.x / p.q_heads, head = blockIdx.x % p.q_heads, at = tid / L, d = tid % L * 4;
-    const int64_t rows = (int64_t)p.n_rows * p.q_heads;
-    const float* ml = p.part + p.ml + (int64_t)blockIdx.x * 2;
-    const float* part = p.part + (int64_t)blockIdx.x * D + d;
+    const int tid = threadIdx.x, at = FEW ? 0 : tid / L, d = tid % L * 4;
+    const int64_t rows = (int64_t)p.n_rows * p.q_heads, which = FEW ? (int64_t)blockIdx.x * S + tid / L : blockIdx.x;
+    if (which >= rows) return;
+    const int row = (int)(which / p.q_heads), head = (int)(which % p.q_heads);
+    const float* ml = p.part + p.ml + which * 2;
+    const float* part = p.part + which * D + d;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
     float mt = kNone, lt = 0.f;
 #pragma unroll 4
-    for (int s = at; s < p.psplit + p.tsplit; s += S) {
+    for (int s = at; s < p.psplit + p.tsplit; s += FEW ? 1 : S) {
         const u32x2 b = *(const u32x2*)(ml + s * rows * 2);
         const f32x4 o = *(const f32x4*)(part + s * rows * D);
         const float m = as_float(b[0]), l = as_float(b[1]);
@@ -518,6 +521,10 @@ __global__ void __launch_bounds__(256) k_attn_shared_join(SharedP p) {
         a = a * f + o * g;
         lt = lt * f + l * g;
         mt = mn;
+    }
+    if constexpr (FEW) {
+        store4(p, (size_t)row * p.ldo + (size_t)head * D + d, lt == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a * (1.f / lt));
+        return;
     }
     *(f32x4*)&s_o[at][d] = a;
     if (d == 0) {
@@ -566,7 +573,12 @@ hipError_t launch_of(const SharedP& p, int qt, hipStream_t st) {
         launch_tiles<D, KV, KV == kKvQ8 ? 2 : 3, 3>(p, qt, units, st);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    launch_kernel((k_attn_shared_join<D>), dim3((uint32_t)(p.n_rows * p.q_heads)), dim3(256), 0, st, p);
+    constexpr int S = 1024 / D;
+    const int64_t rows = (int64_t)p.n_rows * p.q_heads;
+    if (p.psplit + p.tsplit <= 4)
+        launch_kernel((k_attn_shared_join<D, true>), dim3((uint32_t)((rows + S - 1) / S)), dim3(256), 0, st, p);
+    else
+        launch_kernel((k_attn_shared_join<D, false>), dim3((uint32_t)rows), dim3(256), 0, st, p);
     return hipGetLastError();
 }
 }  // namespace

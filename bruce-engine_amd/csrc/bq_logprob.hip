@@ -25,10 +25,10 @@
 namespace bq {
 
 namespace {
-constexpr int kSlice = 1024;
+constexpr int kSlice = 1024;      // logits of a slice at most
 constexpr int kMaxSlices = 1024;  // the entry point's limit on the vocabulary
-constexpr int kStep = 1024;       // candidates that the join looks at between two counts,
-constexpr int kKeys = 1280;       // and holds at once: the likeliest so far, and a step's
+constexpr int kStep = 4096;       // places that the join looks at between two counts of what it found,
+constexpr int kKeys = 4352;       // and candidates that it holds at once: the likeliest so far, and a step's
 static_assert(kKeys - kStep >= 2 * BQ_MAX_TOP, "");
 typedef unsigned long long u64;
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any logit
@@ -44,7 +44,7 @@ struct SliceInfo {
 struct LogprobP {
     const float* logits;
     int64_t ld;
-    int vocab, slices, cap_log, top;  // a slice has room for 2^cap_log candidates (top > 1)
+    int vocab, slices, len, cap_log, top;  // a slice has len logits, and room for 2^cap_log candidates (top > 1)
     const float* temp;
     const int32_t* tokens;
     float* logprob;
@@ -112,9 +112,10 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
     const float* x = p.logits + (size_t)row * p.ld;
     const int token = p.tokens ? p.tokens[row] : -1;
     const float T = temperature_of(p, row);
-    auto at = [&](int k) { return slice * kSlice + (k * 64 + lane) * 4; };
+    const int begin = slice * p.len, end = min(p.vocab, begin + p.len);
+    auto at = [&](int k) { return begin + (k * 64 + lane) * 4; };
     float v[V][4];
-    if ((slice + 1) * kSlice <= p.vocab) {
+    if (end - begin == kSlice) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const f32x4 a = *(const f32x4u*)(x + at(k));
@@ -123,9 +124,17 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < V; ++k)
+        for (int k = 0; k < V; ++k) {
+            f32x4 a = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (at(k) + 4 <= end) {
+                a = *(const f32x4u*)(x + at(k));
+            } else {
+                for (int e = 0; e < 4; ++e)
+                    if (at(k) + e < end) a[e] = x[at(k) + e];
+            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[k][e] = at(k) + e < p.vocab ? x[at(k) + e] : -INFINITY;
+            for (int e = 0; e < 4; ++e) v[k][e] = a[e];
+        }
     }
     const bool given = (unsigned)token < (unsigned)p.vocab;
     const float given_v = given ? x[token] : INFINITY;  // used last: it comes behind another load
@@ -148,10 +157,10 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
         if (in == 0) continue;
         const int l = __builtin_ctzll(in);
         run = k;
-        first = slice * kSlice + (k * 64 + l) * 4 + 3;
+        first = begin + (k * 64 + l) * 4 + 3;
 #pragma unroll
         for (int e = 2; e >= 0; --e)
-            if (__ballot(v[k][e] == mx) >> l & 1) first = slice * kSlice + (k * 64 + l) * 4 + e;
+            if (__ballot(v[k][e] == mx) >> l & 1) first = begin + (k * 64 + l) * 4 + e;
     }
     float sum = 0.f, dot = 0.f;
     if (mx > -INFINITY && mx < INFINITY && T > 0.f) {
@@ -204,16 +213,16 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
                 }
             return n;
         };
-        // below the lowest finite logit t stands for all of the slice, of which the last may be short
+        // below the lowest finite logit t stands for all of the slice, which may be short
         const float least = t <= ordered(-INFINITY) ? -INFINITY : unordered(t);
-        total = least == -INFINITY ? keep([&](float, int i) { return i < p.vocab; }) : keep([&](float x, int) { return x >= least; });
+        total = least == -INFINITY ? keep([&](float, int i) { return i < end; }) : keep([&](float x, int) { return x >= least; });
         if (total > cap) {
             auto count = [&](auto f) {
                 int n = 0;
 #pragma unroll
                 for (int k = 0; k < V; ++k)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) n += __popcll(__ballot(at(k) + e < p.vocab && f(ordered(v[k][e]), at(k) + e)));
+                    for (int e = 0; e < 4; ++e) n += __popcll(__ballot(at(k) + e < end && f(ordered(v[k][e]), at(k) + e)));
                 return n;
             };
             t = 0;
@@ -222,20 +231,21 @@ __global__ void __launch_bounds__(256) k_logprob_scan(LogprobP p) {
                 if (count([&](uint32_t o, int) { return o >= c; }) >= p.top) t = c;
             }
             const int want = p.top - count([&](uint32_t o, int) { return o > t; });
-            int last = slice * kSlice - 1;  // of the logits that equal t, those up to this index
+            int last = begin - 1;  // of the logits that equal t, those up to this index
             for (int step = kSlice / 2; step > 0; step >>= 1)  // the most that hold fewer than wanted, and one more
                 if (count([&](uint32_t o, int i) { return o == t && i <= last + step; }) < want) last += step;
             ++last;
-            total = keep([&](float x, int i) { return i < p.vocab && (ordered(x) > t || (ordered(x) == t && i <= last)); });
+            total = keep([&](float x, int i) { return i < end && (ordered(x) > t || (ordered(x) == t && i <= last)); });
         }
     }
     int before = 0;
     const float limit = clean(given_v);
+    const int upto = min(token, end);  // what stands behind the slice's end is none of its logits
     if (limit <= mx) {
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) before += __popcll(__ballot(v[k][e] > limit || (v[k][e] == limit && at(k) + e < token)));
+            for (int e = 0; e < 4; ++e) before += __popcll(__ballot(v[k][e] > limit || (v[k][e] == limit && at(k) + e < upto)));
     }
     SliceInfo* info = p.info + (size_t)row * p.slices + slice;
     if ((lane & 15) == 0) info->group[lane >> 4] = ordered(group);
@@ -440,6 +450,8 @@ __global__ void __launch_bounds__(256) k_logprob_join(LogprobP p) {
 }
 
 int slices_of(int vocab) { return (vocab + kSlice - 1) / kSlice; }
+// slices of one length: a short last one would have to find its `top` largest by bisection
+int length_of(int vocab) { return ((vocab + slices_of(vocab) - 1) / slices_of(vocab) + 3) / 4 * 4; }
 // room for a slice's candidates: 1.1 to 1.4 `top` of a slice of independent logits
 int cap_log_of(int top) {
     int n = 4;
@@ -455,7 +467,7 @@ size_t logprob_work_bytes(int rows, int vocab, int top) {
 
 hipError_t launch_logprobs(const bq_logprobs_args& a, hipStream_t st) {
     LogprobP p;
-    p.logits = a.logits; p.ld = a.ld; p.vocab = a.vocab; p.slices = slices_of(a.vocab); p.top = a.top; p.cap_log = cap_log_of(a.top);
+    p.logits = a.logits; p.ld = a.ld; p.vocab = a.vocab; p.slices = slices_of(a.vocab); p.len = length_of(a.vocab); p.top = a.top; p.cap_log = cap_log_of(a.top);
     p.temp = a.temperature; p.tokens = a.tokens; p.logprob = a.logprob; p.rank = a.rank; p.entropy = a.entropy;
     p.top_tokens = a.top_tokens; p.top_logprobs = a.top_logprobs;
     p.info = (SliceInfo*)a.work;

@@ -400,10 +400,10 @@ hipError_t launch_of(const LoraP& p, int x_type, int tiles, dim3 down, dim3 up, 
 // several runs in a row (512 rows of 64 adapters 65 us with 16, 81 with 12)
 int slots_of(int rows) { return rows <= 2048 ? 16 : 12; }
 int groups_of(int rows) { return rows <= kWindow ? rows : (rows + kWindow - 1) / kWindow * slots_of(rows); }
-// pieces of K: as many as fill a workgroup a CU, a chunk each at least
+// pieces of K: as many as give every CU a workgroup, a chunk each at least
 int pieces_of(int rows, int rank, int n_parts, int K) {
     const int64_t wgs = (int64_t)(rows <= kWindow ? rows : (rows + 31) / 32) * ((n_parts * ((rank + 15) / 16) + kRankTiles - 1) / kRankTiles);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({((int64_t)K + kChunk - 1) / kChunk, 256 / wgs, kPieces}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({((int64_t)K + kChunk - 1) / kChunk, (255 + wgs) / wgs, kPieces}));
 }
 }  // namespace
 
