@@ -184,10 +184,9 @@ int bq_attn_decode_shared(const bq_kv_cache* c, const bq_attn_args* args, const 
     x.max_len = std::min(x.max_len, a.max_len);
     const SharedPlan s = shared_plan(type, kv.n_seq, a.rows, a.q_heads, kv.heads, kv.D, a.max_len, x.n_groups, x.max_len, a.window, a.sinks,
                                      device_cus());
-    // one grid dimension holds all workgroups, another all rows
-    if (s.punits + (int64_t)kv.n_seq * s.ttiles * kv.heads * s.tsplit > INT32_MAX ||
-        (int64_t)a.n_rows * a.q_heads > INT32_MAX)
-        return BQ_UNSUPPORTED;
+    // a grid has at most 2^32 - 1 lanes, 256 a workgroup: of all pieces, and of all rows
+    constexpr int64_t kGroups = (1 << 24) - 1;
+    if (s.punits + (int64_t)kv.n_seq * s.ttiles * kv.heads * s.tsplit > kGroups || (int64_t)a.n_rows * a.q_heads > kGroups) return BQ_UNSUPPORTED;
     if (!a.work || !al16(a.work) || a.work_bytes < shared_part_floats(s, a.n_rows, a.q_heads, kv.D) * sizeof(float)) return BQ_EINVAL;
     return from_hip(launch_attn_shared(kv, type, a, x, s, (hipStream_t)st));
 }
@@ -225,13 +224,16 @@ int bq_lora(const bq_lora_args* a, bq_stream_t st) {
         if (p.N % 16) return BQ_UNSUPPORTED;
         outputs += (p.N + 255) / 256;
     }
-    if (outputs > 65535) return BQ_UNSUPPORTED;  // a grid dimension
+    // grid dimensions: outputs and rows of one launch
+    if (outputs > 65535 || a->rows > BQ_MAX_LORA_ROWS) return BQ_UNSUPPORTED;
     if (a->rows == 0) return BQ_OK;
     if (!a->x || !al16(a->x) || !a->adapter) return BQ_EINVAL;
     if (a->x_type == BQ_TYPE_Q8_0 ? !a->xd : a->ldx < a->K || a->ldx % (a->x_type == BQ_TYPE_F32 ? 4 : 8)) return BQ_EINVAL;
     for (int i = 0; i < a->n_parts; ++i) {
         const bq_lora_part& p = a->parts[i];
         if (!p.a || !p.b || !p.y || !al16(p.a) || !al16(p.b) || !al16(p.y) || !al16(p.base) || p.ldy < p.N || (p.ldy & 3)) return BQ_EINVAL;
+        for (int j = 0; j < i; ++j)
+            if (a->parts[j].y == p.y) return BQ_EINVAL;  // the parts run side by side
         if (p.base && (p.ldbase < p.N || (p.ldbase & 3) || (p.base == p.y && p.ldbase != p.ldy))) return BQ_EINVAL;
     }
     if (!a->work || !al16(a->work) || a->work_bytes < lora_work_bytes(a->rows, a->rank, a->n_parts)) return BQ_EINVAL;

@@ -583,7 +583,9 @@ int bq_attn_prefill(const bq_kv_cache* kv, const bq_attn_args* a, bq_stream_t st
  * of a page) before are not read.  A sequence in no group has no shared tokens.
  * Everything else is bq_attn_decode's: kv_len counts the shared tokens, rows see
  * what their positions, window and sinks let them (a sequence may be shorter than
- * the prefix), precision by the types of q, out and the cache.  work: at least
+ * the prefix), precision by the types of q, out and the cache, but that unless q and
+ * out are both bf16 a weight times a value's scale has three bf16 parts over a q8
+ * cache too.  work: at least
  * bq_attn_shared_workspace_bytes (else BQ_EINVAL), max_prefix being prefix->max_len;
  * not shared by calls that overlap.  How the work is cut follows n_seq, rows,
  * n_groups, max_len and prefix->max_len, which a captured graph fixes; group0, len
@@ -626,16 +628,18 @@ void bq_attn_hook(void* user, int block, bq_stream_t st);
  * adapters of a pool of n_adapters slots (a smaller rank: zeros behind it).  An
  * adapter outside 0..n_adapters-1 is none: y_p[r] = base_p[r].  base NULL is zeros;
  * base may be y itself (the projection's output; rows without an adapter are then
- * not touched), and must not overlap it otherwise.  scale NULL is 1.
+ * not touched), and must not overlap it otherwise; nor may one part's y overlap
+ * another's y or base (columns of one buffer side by side do not).  scale NULL is 1.
  * x: fp32 or bf16 rows (ldx apart), or the q8 rows that the projection read (xq as
  * x, and xd, as from bq_quantize_q8; ldx is not used), finite.  fp32 precision
  * throughout: products are exact, sums fp32.
- * K % 32 == 0, N % 16 == 0, rank % 8 == 0 and rank <= 256, else BQ_UNSUPPORTED.
+ * K % 32 == 0, N % 16 == 0, rank % 8 == 0, rank <= BQ_MAX_RANK and rows <=
+ * BQ_MAX_LORA_ROWS, else BQ_UNSUPPORTED.
  * Pointers 16-byte aligned (xd, adapter and scale apart); ldx a multiple of 16
  * bytes, ldbase and ldy of 4 elements.  work: at least bq_lora_workspace_bytes (else
  * BQ_EINVAL), not shared by calls that overlap.  Equal calls give equal bits; a row's
  * result does not depend on the other rows' values. */
-enum { BQ_MAX_RANK = 256 };
+enum { BQ_MAX_RANK = 256, BQ_MAX_LORA_ROWS = 1 << 20 };
 typedef struct bq_lora_part {
     const uint16_t* a; const uint16_t* b;
     const float* base; float* y;

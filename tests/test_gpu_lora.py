@@ -248,6 +248,9 @@ def test_refusals(bq):
         refused(E, p, **f)
     refused(U, p, N=24)
     refused(U, p, N=1 << 26, ldy=1 << 26, ldbase=1 << 26)
+    refused(U, s, rows=(1 << 20) + 1)
+    s.parts[1] = p
+    refused(E, s, n_parts=2)   # two parts that add to the same y
     assert L.bq_lora(None, None) == E
     s.rows = 0
     assert call() == bq.BQ_OK

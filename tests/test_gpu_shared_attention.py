@@ -304,6 +304,11 @@ def test_refusals(bq):
         refused(E, att.struct, **fields)
     refused(U, att.struct, q_heads=3)
     refused(U, att.struct, rows=9, n_rows=27)
+    big = bq.KvCacheStruct.from_buffer_copy(cache.struct)
+    big.n_seq, big.kv_heads = 65535, 64
+    wide = bq.AttnArgs.from_buffer_copy(att.struct)
+    wide.rows, wide.n_rows, wide.q_heads, wide.ldq, wide.ldo = 8, 8 * 65535, 64, 64 * D, 64 * D
+    assert L.bq_attn_decode_shared(ctypes.byref(big), ctypes.byref(wide), ctypes.byref(att.prefix), None) == U   # more rows than a grid has
     assert L.bq_attn_decode_shared(None, ctypes.byref(att.struct), ctypes.byref(att.prefix), None) == E
     assert L.bq_attn_decode_shared(cache.ref, None, ctypes.byref(att.prefix), None) == E
     assert L.bq_attn_decode_shared(cache.ref, ctypes.byref(att.struct), None, None) == E

@@ -28,7 +28,7 @@ def test_ctypes_structs_match_header(tmp_path):
         src.append('printf("%s size %%zu\\n", sizeof(%s));' % (cname, cname))
         for f, _ in getattr(bq, pyname)._fields_:
             src.append('printf("%s %s %%zu\\n", offsetof(%s, %s));' % (cname, f, cname, f))
-    src.append('printf("max top %d\\nmax rank %d\\nparts %d\\nprojections %d %d %d %d %d\\n", BQ_MAX_TOP, BQ_MAX_RANK, BQ_MAX_PARTS, BQ_PROJ_QKV, '
+    src.append('printf("max top %d\\nmax rows %d\\nmax rank %d\\nparts %d\\nprojections %d %d %d %d %d\\n", BQ_MAX_TOP, BQ_MAX_LORA_ROWS, BQ_MAX_RANK, BQ_MAX_PARTS, BQ_PROJ_QKV, '
                'BQ_PROJ_O, BQ_PROJ_GATE_UP, BQ_PROJ_DOWN, BQ_N_PROJ);')
     src.append("return 0; }")
     (tmp_path / "off.c").write_text("\n".join(src))
@@ -40,7 +40,7 @@ def test_ctypes_structs_match_header(tmp_path):
         assert int(got[f"{cname} size"]) == ctypes.sizeof(S), cname
         for f, _ in S._fields_:
             assert int(got[f"{cname} {f}"]) == getattr(S, f).offset, (cname, f)
-    assert got["max top"] == "64" and got["max rank"] == "256" and got["parts"] == "4"
+    assert got["max top"] == "64" and got["max rows"] == str(1 << 20) and got["max rank"] == "256" and got["parts"] == "4"
     assert [bq.PROJ_QKV, bq.PROJ_O, bq.PROJ_GATE_UP, bq.PROJ_DOWN] == [0, 1, 2, 3] and got["projections 0 1 2 3"] == "4"
     for cname, pyname in STRUCTS[:2] + STRUCTS[5:]:
         assert [f[0] for f in getattr(bq, pyname)._fields_][: len(header_fields(cname))] == header_fields(cname), cname
