@@ -3,10 +3,23 @@
 //
 //   o = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),  x_j = scale log2(e) q.k_j
 // The sum over a group's prefix is taken for the query rows of all its sequences
-// together, so the prefix' K and V are read once per row tile instead of once per
+// together, so the prefix' K and V are read once per 32 query rows instead of once per
 // sequence; the sum over a sequence's own tokens for its rows alone (bq_attn.hip's
 // scheme in both).  Sums and maxima of the two, and of the pieces that each is cut
 // into, go to the workspace; a second launch joins them in their order.
+//
+// What bounds it: a prefix behind many rows the products (4 D flops per row and token,
+// three times that for fp32 queries, six MFMAs of bf16 parts for two) and the
+// exponentials beside them, a sequence's own tokens their bytes; so a CU has one
+// workgroup of each.  A step (32 tokens of a wave, for two row tiles) takes 1.6 us of a
+// SIMD: 0.8 of MFMA, the rest vector work and loads, which a second wave on the SIMD
+// covers by a fifth only, less than a second start costs; launches, start (group, length,
+// queries, page, K and V are a chain of loads) and join take some 11 us of a call, the
+// first step's reading from memory 6 more.
+// Measured (32 heads of 128 over 4, bf16 cache unless said otherwise): 32 sequences
+// behind 16384 tokens with up to 512 of their own 41 us with fp32 queries;
+// 64 behind 8192 with up to 2048 own in bf16 49 us, where the bytes alone are 31; 48 in
+// three groups behind 6001 over q8 (8 key-value heads) 58 us; four behind 600 10 us.
 #include <algorithm>
 
 #include "bq_attn_dev.hpp"

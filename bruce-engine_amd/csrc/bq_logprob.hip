@@ -16,6 +16,10 @@
 //   k_logprob_join, one workgroup per row: joins the slices in their order.  `top` of
 //     the row's logits reach the top-th largest of its slices' maxima, which few slices
 //     and one to two times `top` candidates do; those are ranked by counting.
+// Measured (131072 logits): 512 rows with the likeliest token 51 us, 5.3 TB/s, the
+// reading; 64 rows with 20 alternatives 19.8 us, 14 of them the scan, which the vector
+// work of finding and keeping candidates bounds there; one row 10.9 us, two launches of a
+// chain each (token, its logit; infos, threshold, candidates, ranks).
 #include <algorithm>
 #include <cmath>
 

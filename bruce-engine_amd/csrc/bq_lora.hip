@@ -6,6 +6,14 @@
 // rows as the A operand and 16 rows of one adapter as the B operand, so a lane holds
 // one row's results, four neighbours at a time.
 //
+// What bounds it: prompts the reading of base and writing of y (4096 rows of 2 x 7168
+// outputs at rank 32: 111 us, 94 to 97 of them k_lora_up at 4.8 to 5.0 TB/s, where a
+// large copy reaches 5.1; t 17 us); a token's rows two launches and, in the first, a chain of loads
+// (adapters, x and A), which pieces of K shorten (one row of 4096 to 2560 at rank 16
+// 8.6 us; 32 rows of 12 adapters at q, k, gate and v 11.4).  777 fp32
+// rows of 7168 at rank 64: 32.6 us, t 19: at least 25 runs of rows in 8 pieces, each three and a
+// half chunks of x and A one after another.
+//
 // fp32 precision on bf16 operands: the adapters and int8 codes are exact; a 32-value
 // group of a q8 row is one MFMA of its codes, scaled in fp32; fp32 rows and t are the
 // sum of three bf16 parts (all 24 bits), an MFMA each.
