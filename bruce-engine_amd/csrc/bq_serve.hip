@@ -232,8 +232,8 @@ int bq_lora(const bq_lora_args* a, bq_stream_t st) {
     for (int i = 0; i < a->n_parts; ++i) {
         const bq_lora_part& p = a->parts[i];
         if (!p.a || !p.b || !p.y || !al16(p.a) || !al16(p.b) || !al16(p.y) || !al16(p.base) || p.ldy < p.N || (p.ldy & 3)) return BQ_EINVAL;
-        for (int j = 0; j < i; ++j)
-            if (a->parts[j].y == p.y) return BQ_EINVAL;  // the parts run side by side
+        for (int j = 0; j < a->n_parts; ++j)  // the parts run side by side
+            if (j != i && (a->parts[j].y == p.y || a->parts[j].y == p.base)) return BQ_EINVAL;
         if (p.base && (p.ldbase < p.N || (p.ldbase & 3) || (p.base == p.y && p.ldbase != p.ldy))) return BQ_EINVAL;
     }
     if (!a->work || !al16(a->work) || a->work_bytes < lora_work_bytes(a->rows, a->rank, a->n_parts)) return BQ_EINVAL;

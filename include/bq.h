@@ -629,7 +629,8 @@ void bq_attn_hook(void* user, int block, bq_stream_t st);
  * adapter outside 0..n_adapters-1 is none: y_p[r] = base_p[r].  base NULL is zeros;
  * base may be y itself (the projection's output; rows without an adapter are then
  * not touched), and must not overlap it otherwise; nor may one part's y overlap
- * another's y or base (columns of one buffer side by side do not).  scale NULL is 1.
+ * another's y or base (columns of one buffer side by side do not; where two begin
+ * at one address BQ_EINVAL).  scale NULL is 1.
  * x: fp32 or bf16 rows (ldx apart), or the q8 rows that the projection read (xq as
  * x, and xd, as from bq_quantize_q8; ldx is not used), finite.  fp32 precision
  * throughout: products are exact, sums fp32.

@@ -260,6 +260,23 @@ def test_refusals(bq):
     assert W(rows, rank, 1) == s.work_bytes and W(0, 8, 1) == W(1, 0, 1) == W(1, 264, 1) == W(1, 8, 5) == W(1, 8, 0) == 0
 
 
+@pytest.mark.parametrize("reader", [0, 1])
+def test_base_that_another_part_writes(bq, reader):
+    """The parts run side by side: one whose base is another's output would read it before or after it was written."""
+    rows, K, N, rank, n = 3, 64, 32, 8, 2
+    x, a = torch.zeros((rows, K), device="cuda"), torch.zeros((n, rank, K), dtype=torch.bfloat16, device="cuda")
+    b = torch.zeros((n, N, rank), dtype=torch.bfloat16, device="cuda")
+    ys = [torch.full((rows, N), 7.0, device="cuda") for _ in range(2)]
+    op = bq.Lora(x, torch.zeros(rows, dtype=torch.int32, device="cuda"), [(a, b, ys[0]), (a, b, ys[1])])
+    call = lambda: bq.load().bq_lora(ctypes.byref(op.struct), None)
+    part, own = op.struct.parts[reader], op.struct.parts[reader].base
+    part.base = op.struct.parts[1 - reader].y
+    assert call() == bq.BQ_EINVAL
+    part.base = own
+    assert call() == bq.BQ_OK
+    torch.cuda.synchronize()
+
+
 def _q5(bq, seed, K, N):
     import synth
     raw = torch.from_numpy(synth.quantize_q5k(_rand(seed, N, K).numpy() * 0.05)).cuda()
